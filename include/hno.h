@@ -32,6 +32,13 @@ extern "C" {
 #define HNO_ACT_ELU 2
 #define HNO_ACT_SIGMOID 3 /* hno_act_fwd / hno_act_bwd only (output activation of the models); the fused conv / transform
                              epilogues take NONE, SELU or ELU */
+/* the token entry points only (hno_linear_*, hno_gncl_*), beside NONE, SELU and ELU */
+#define HNO_ACT_RELU 4
+#define HNO_ACT_GELU 5 /* z Phi(z), the exact form */
+#define HNO_ACT_SILU 6
+/* element types of the token entry points */
+#define HNO_F32 0
+#define HNO_BF16 1
 /* ORed into the `act` argument of hno_pwconv_fwd / hno_pwconv_bwd / hno_pwconv_fwd_branch / hno_pwconv_bwd_branch: run the channel
  * contraction on the bf16 matrix cores (v_mfma_f32_32x32x16_bf16, fp32 accumulation) with the operands rounded to bf16 and the
  * convolution output rounded to bf16 -- what torch.autocast(bfloat16) makes of nn.Conv3d (reference experiments/train_test.py:154-160).
@@ -594,6 +601,48 @@ int hno_zscore_modalities(const float *x, float *out, float *mean_std, void *wor
                           int has_mask, float mask_val, int has_clip, float clip_lo, float clip_hi, void *stream);
 int hno_affine_nearest(const float *x, float *out, const double *matrix12, float cval, int flip_mask, int C, int D,
                        int H, int W, void *stream);
+
+/* ------------------------------------------------------------------ token operators
+ * Tokens lie row by row, channels last; dtype HNO_F32 or HNO_BF16 names the type of every tensor that is a `void *` here, sums and statistics are
+ * fp32 or wider.  Workspaces: caller-allocated, 16-byte aligned, any contents; *_workspace_bytes say how large (0 is possible).
+ * Results do not depend on the run: no atomics, fixed orders of summation.
+ *
+ * hno_attn_fwd: out (B, Tq, H, Dv) = softmax(scale q k^T) v per head over the visible keys; a row without any is zero.
+ *   q (B, Tq, H, Dk), k (B, Tk, Hk, Dk), v (B, Tk, Hk, Dv) with element strides of (batch, token, head) and unit stride of the last axis; query head h
+ *   reads key head h / (H / Hk).  Head sizes 1 ... 128.  With L = kv_lens[b] (clamped to 0 ... Tk; NULL: Tk), key j is visible to query i when
+ *   j < L, and j <= i + L - Tq if causal (the last query is aligned with the last key), and mask[b, h, i, j] != 0 (NULL: all; strides of 0 broadcast).
+ *   Rows of k and v from L on, and those that a mask without query and head axis hides, are not looked at: they may hold anything.  Value rows that
+ *   only some queries may see have to be finite.
+ *   For the backward pass: lse (B, Tq, H) fp32, +inf for an empty row, and out_res (bf16 only), the rounding error of out; both NULL otherwise.
+ * hno_attn_bwd: dq, dk, dv (contiguous; dq or both of dk, dv may be NULL) from out, out_res, lse and dout (contiguous). */
+typedef struct hno_attn {
+    int dtype, B, Tq, Tk, H, Hk, Dk, Dv, causal;
+    float scale;
+    const void *q, *k, *v;
+    const unsigned char *mask;
+    const int *kv_lens;
+    long long q_stride[3], k_stride[3], v_stride[3], mask_stride[4];
+} hno_attn_t;
+size_t hno_attn_workspace_bytes(const hno_attn_t *p, int backward);
+int hno_attn_fwd(const hno_attn_t *p, void *out, void *out_res, float *lse, void *workspace, size_t workspace_bytes, void *stream);
+int hno_attn_bwd(const hno_attn_t *p, const void *out, const void *out_res, const float *lse, const void *dout, void *dq, void *dk, void *dv,
+                 void *workspace, size_t workspace_bytes, void *stream);
+/* hno_linear_fwd: y (M, N) = act(x w^T + bias) + residual, x (M, K) with row stride ldx, w (N, K); bias (N) of bias_dtype and residual (M, N) may be
+ *   NULL.  z (M, N), if not NULL, receives the argument of the activation, which hno_linear_bwd reads (act != NONE).
+ * hno_linear_bwd: dx (M, K), dw (N, K) of dw_dtype, db (N) of db_dtype from dy (M, N); any of them may be NULL.  (The residual's gradient is dy.) */
+size_t hno_linear_workspace_bytes(int dtype, int M, int N, int K, int act, int backward);
+int hno_linear_fwd(int dtype, const void *x, long long ldx, const void *w, const void *bias, int bias_dtype, const void *residual, void *z, void *y, int M,
+                   int N, int K, int act, void *workspace, size_t workspace_bytes, void *stream);
+int hno_linear_bwd(int dtype, const void *dy, const void *z, const void *x, long long ldx, const void *w, void *dx, void *dw, int dw_dtype, void *db,
+                   int db_dtype, int M, int N, int K, int act, void *workspace, size_t workspace_bytes, void *stream);
+/* hno_gncl_fwd: y = act(gamma xh + beta), xh = (x - mean) / sqrt(var + eps) over the V rows and C / G neighbouring channels of each group;
+ *   x, y (B, V, C); gamma, beta (C) fp32 or NULL; mean_rstd (B, G, 2) receives the statistics.
+ * hno_gncl_bwd: dx (B, V, C), dgamma, dbeta (C); any of them may be NULL.  Workspace of both: hno_gncl_workspace_bytes. */
+size_t hno_gncl_workspace_bytes(int B, long long V, int C, int G);
+int hno_gncl_fwd(int dtype, const void *x, const float *gamma, const float *beta, void *y, float *mean_rstd, void *workspace, size_t workspace_bytes,
+                 int B, long long V, int C, int G, float eps, int act, void *stream);
+int hno_gncl_bwd(int dtype, const void *dy, const void *x, const float *gamma, const float *beta, const float *mean_rstd, void *dx, float *dgamma,
+                 float *dbeta, void *workspace, size_t workspace_bytes, int B, long long V, int C, int G, int act, void *stream);
 
 /* ------------------------------------------------------------------ deferred weight-gradient reduction
  * Every *_bwd entry point that produces a weight gradient writes per-workgroup partial slabs into its workspace and then

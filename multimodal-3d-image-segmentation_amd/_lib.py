@@ -17,8 +17,26 @@ _lib = None
 
 c_void_p, c_int, c_float, c_ll, c_size_t = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_size_t
 
+
+
+class AttnArgs(ctypes.Structure):
+    """hno_attn_t of include/hno.h"""
+    _fields_ = ([(n, c_int) for n in ('dtype', 'B', 'Tq', 'Tk', 'H', 'Hk', 'Dk', 'Dv', 'causal')] + [('scale', c_float)] +
+                [(n, c_void_p) for n in ('q', 'k', 'v', 'mask', 'kv_lens')] +
+                [(n, c_ll * k) for n, k in (('q_stride', 3), ('k_stride', 3), ('v_stride', 3), ('mask_stride', 4))])
+
+
 # name -> (restype, argtypes); must list every symbol include/hno.h declares
 SIGNATURES = {
+    'hno_attn_workspace_bytes': (c_size_t, [ctypes.POINTER(AttnArgs), c_int]),
+    'hno_attn_fwd': (c_int, [ctypes.POINTER(AttnArgs)] + [c_void_p] * 4 + [c_size_t, c_void_p]),
+    'hno_attn_bwd': (c_int, [ctypes.POINTER(AttnArgs)] + [c_void_p] * 8 + [c_size_t, c_void_p]),
+    'hno_linear_workspace_bytes': (c_size_t, [c_int] * 6),
+    'hno_linear_fwd': (c_int, [c_int, c_void_p, c_ll, c_void_p, c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 4 + [c_void_p, c_size_t, c_void_p]),
+    'hno_linear_bwd': (c_int, [c_int] + [c_void_p] * 3 + [c_ll] + [c_void_p] * 3 + [c_int, c_void_p] + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
+    'hno_gncl_workspace_bytes': (c_size_t, [c_int, c_ll, c_int, c_int]),
+    'hno_gncl_fwd': (c_int, [c_int] + [c_void_p] * 6 + [c_size_t, c_int, c_ll, c_int, c_int, c_float, c_int, c_void_p]),
+    'hno_gncl_bwd': (c_int, [c_int] + [c_void_p] * 9 + [c_size_t, c_int, c_ll, c_int, c_int, c_int, c_void_p]),
     'hno_version': (c_int, []),
     'hno_last_error': (ctypes.c_char_p, []),
     'hno_dht3_workspace_bytes': (c_size_t, [c_int] * 7),

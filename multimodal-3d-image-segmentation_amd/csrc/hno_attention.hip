@@ -1,0 +1,578 @@
+// Softmax attention on (B, T, H, D) tokens, forward and backward (hno_attn_fwd, hno_attn_bwd).
+//
+//   s_ij = scale q_i . k_j,  p_ij = exp(s_ij) / sum_j exp(s_ij) over the visible keys,  o_i = sum_j p_ij v_j
+//   D_i = sum_c do_ic o_ic,  ds_ij = p_ij (do_i . v_j - D_i),  dq = scale ds k,  dk = scale ds^T q,  dv = p^T do
+//
+// Neither p nor ds is written to memory.  The forward pass keeps the running maximum and sum of each row and leaves
+// lse_i = log2 sum_j exp(s_ij); the backward kernels recompute p_ij = 2^(s_ij log2(e) - lse_i).  They are two: one walks the keys for a
+// tile of queries (dq), one walks the queries (of all heads that share the keys) for a tile of keys (dk, dv) -- 7 products where one
+// kernel with atomic sums would need 5, but every sum has one owner and a fixed order, so results do not change from run to run.
+//
+// A wave owns 32 rows of its side as the COLUMNS of its products (lane & 31): the softmax statistics are then one value per lane, and the
+// registers of a product are the operand of the next (hno_tokens.h).  The other side comes through LDS, row by row as in memory; its
+// transposed reads are ds_read_b64_tr_b16 (bf16) or single words (fp32).
+#include "hno_tokens.h"
+
+namespace hno {
+
+struct AttnArgs {
+    const void *q, *k, *v, *g, *o, *ores;
+    void *out, *outres, *dq, *dk, *dv;
+    float *lse, *delta, *part, *part2;
+    const unsigned char *mask;
+    const int *lens;
+    long long qs[3], ks[3], vs[3], ms[4];     // element strides of (batch, token, head); the mask's of (batch, head, query, key)
+    int B, Tq, Tk, H, Hk, Dk, Dv, causal, nsplit, pack, vq, vk, vv, vo, keymask;
+    float scale2, scale;                       // scale log2(e), scale
+};
+
+constexpr int AT_WAVES = 4, AT_ROWS = 32 * AT_WAVES;
+template <typename T> constexpr int at_tile() { return sizeof(T) == 2 ? 64 : 32; }     // rows of the streamed side per step
+
+__device__ __forceinline__ int at_length(const AttnArgs &a, int b) {
+    if (!a.lens) return a.Tk;
+    const int n = a.lens[b];
+    return n < 0 ? 0 : (n > a.Tk ? a.Tk : n);
+}
+__device__ __forceinline__ float at_other_half(float x) { return __shfl_xor(x, 32); }
+__device__ __forceinline__ int at_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }   // result register -> row of the tile
+
+// rows [t0, t0 + n) of one head of a token tensor -> LDS tile; rows from `end` on, and rows that `dead` names, are zeroed
+template <typename T, int DP, int ROWS, typename Dead>
+__device__ __forceinline__ void at_stage(T *tile, const T *base, long long st, int t0, int end, int D, bool vec, int tid, Dead dead) {
+    constexpr int CH = DP / 8, S = DP + tk_pad<T>();
+    for (int c = tid; c < ROWS * CH; c += 64 * AT_WAVES) {
+        const int row = c / CH, d = (c - row * CH) * 8, t = t0 + row;
+        TkFrag<T> f;
+        if (t < end && !dead(t)) {
+            f = tk_load8(base + (long long)t * st, d, D, vec);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f.set(j, 0.f);
+        }
+        tk_store8(tile + row * S + d, f);
+    }
+}
+
+// acc(32 rows of the tile x 32 own columns) = tile rows . own fragments
+template <typename T, int DP>
+__device__ __forceinline__ tk16 at_product(const T *tile, int row0, const TkFrag<T> (&own)[DP / 16], int lane) {
+    constexpr int S = DP + tk_pad<T>();
+    const T *p = tile + (row0 + (lane & 31)) * S + 8 * (lane >> 5);
+    tk16 acc = {};
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) acc = tk_mma(tk_row(p + 16 * kk), own[kk], acc);
+    return acc;
+}
+// acc[dt] += (tile rows row0 .. row0 + 31)^T . w, w being a result over the same rows
+template <typename T, int DP>
+__device__ __forceinline__ void at_accumulate(tk16 (&acc)[DP / 32], const T *tile, int row0, const tk16 &w, int lane) {
+    constexpr int S = DP + tk_pad<T>();
+    const int h = lane >> 5;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        TkFrag<T> f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f.set(j, w[8 * t + j]);
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+            acc[dt] = tk_mma(tk_col(tile, S, 32 * dt, row0 + 16 * t + 4 * h, row0 + 16 * t + 8 + 4 * h, lane), f, acc[dt]);
+    }
+}
+
+// store a transposed accumulator (register = channel, lane = row) as row `dst` of a contiguous tensor
+template <typename T, int DP, typename F>
+__device__ __forceinline__ void at_store(T *dst, const tk16 (&acc)[DP / 32], int D, bool vec, int h, F value) {
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int d = 32 * dt + 8 * u + 4 * h;
+            float x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = value(acc[dt][4 * u + j]);
+            if (vec && d < D) {
+                if constexpr (sizeof(T) == 2) {
+                    tks4 w;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[j] = (short)tk_down<T>(x[j]);
+                    *reinterpret_cast<tks4 *>(dst + d) = w;
+                } else {
+                    *reinterpret_cast<tkf4 *>(dst + d) = tkf4{x[0], x[1], x[2], x[3]};
+                }
+            } else if (!vec) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (d + j < D) dst[d + j] = tk_down<T>(x[j]);
+            }
+        }
+}
+
+// ------------------------------------------------------------------ rows of the query side
+// Workgroup (tile, head, batch x split).  Where few new tokens share a key head (pack), the rows of all its query heads form one list, so
+// the keys are read once: row r stands for query r % Tq of head hb + r / Tq.
+struct AtRow {
+    int head, i, lim;       // query head, query, and the first key that it does not see
+    bool valid;
+};
+__device__ __forceinline__ AtRow at_query_row(const AttnArgs &a, int r, int hb, int nrows, int L) {
+    AtRow w;
+    w.valid = r < nrows;
+    const int rr = w.valid ? r : nrows - 1, gi = rr / a.Tq;
+    w.head = hb + gi;
+    w.i = rr - gi * a.Tq;
+    const int lim = a.causal ? w.i + L - a.Tq + 1 : L;
+    w.lim = !w.valid ? 0 : (lim < L ? lim : L);
+    return w;
+}
+// keys [j0, j1) of this workgroup's split: whole tiles, the same number in each split but the last
+__device__ __forceinline__ void at_key_range(const AttnArgs &a, int L, int last_row, int nrows, int sp, int tile, int &j0, int &j1) {
+    int end = L;
+    if (a.causal && nrows <= a.Tq) {          // (a packed list holds the last query of every head)
+        const int e = last_row + L - a.Tq + 1;
+        end = e < 0 ? 0 : (e < L ? e : L);
+    }
+    const int nt = (end + tile - 1) / tile, per = (nt + a.nsplit - 1) / a.nsplit;
+    j0 = sp * per * tile;
+    j1 = j0 + per * tile;
+    if (j1 > end) j1 = end;
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * AT_WAVES) void attn_fwd_kernel(AttnArgs a) {
+    constexpr int KT = at_tile<T>(), S = DP + tk_pad<T>();
+    __shared__ __attribute__((aligned(16))) T Ks[KT * S];
+    __shared__ __attribute__((aligned(16))) T Vs[KT * S];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int b = blockIdx.z / a.nsplit, sp = blockIdx.z - b * a.nsplit, grp = a.H / a.Hk;
+    const int hb = blockIdx.y * (a.pack ? grp : 1), hk = hb / grp, nrows = a.pack ? grp * a.Tq : a.Tq;
+    const int L = at_length(a, b), r0 = blockIdx.x * AT_ROWS, r = r0 + wave * 32 + (lane & 31);
+    const AtRow w = at_query_row(a, r, hb, nrows, L);
+    int j0, j1;
+    at_key_range(a, L, (r0 + AT_ROWS < nrows ? r0 + AT_ROWS : nrows) - 1, nrows, sp, KT, j0, j1);
+
+    TkFrag<T> qf[DP / 16];
+    const T *qrow = (const T *)a.q + b * a.qs[0] + (long long)w.i * a.qs[1] + w.head * a.qs[2];
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) qf[kk] = tk_load8(qrow, 16 * kk + 8 * h, a.Dk, a.vq);
+    const T *kb = (const T *)a.k + b * a.ks[0] + hk * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + hk * a.vs[2];
+    const unsigned char *mrow = a.mask ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
+    // a mask that hides a key from every query of this workgroup takes the value row out too: 0 x NaN would be NaN
+    const unsigned char *mkey = a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
+
+    tk16 acc[DP / 32] = {};
+    float m = -INFINITY, l = 0.f;
+    for (int j = j0; j < j1; j += KT) {
+        __syncthreads();
+        at_stage<T, DP, KT>(Ks, kb, a.ks[1], j, j1, a.Dk, a.vk, tid, [](int) { return false; });
+        at_stage<T, DP, KT>(Vs, vb, a.vs[1], j, j1, a.Dv, a.vv, tid, [&](int t) { return mkey && !mkey[t * a.ms[3]]; });
+        __syncthreads();
+        tk16 s[KT / 32];
+        float top = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < KT / 32; ++n) {
+            s[n] = at_product<T, DP>(Ks, 32 * n, qf, lane);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int key = j + 32 * n + at_row(e, h);
+                bool on = key < w.lim;
+                if (mrow && on) on = mrow[key * a.ms[3]];
+                s[n][e] = on ? s[n][e] : -INFINITY;
+                top = fmaxf(top, s[n][e]);
+            }
+        }
+        top = fmaxf(m, fmaxf(top, at_other_half(top)));
+        const float shift = top == -INFINITY ? 0.f : top * a.scale2, old = __builtin_amdgcn_exp2f(m * a.scale2 - shift);
+        m = top;
+        l *= old;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= old;
+#pragma unroll
+        for (int n = 0; n < KT / 32; ++n) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                // the sum takes the weight as the product takes it, so the weights of a row add up to one whatever they were rounded to
+                const float p = tk_up(tk_down<T>(__builtin_amdgcn_exp2f(fmaf(s[n][e], a.scale2, -shift))));
+                s[n][e] = p;
+                l += p;
+            }
+            at_accumulate<T, DP>(acc, Vs, 32 * n, s[n], lane);
+        }
+    }
+    l += at_other_half(l);
+    if (!w.valid) return;
+    const long long row = ((long long)b * a.Tq + w.i) * a.H + w.head;
+    if (a.nsplit > 1) {
+        const long long rows = (long long)a.B * a.Tq * a.H, at = sp * rows + row;
+        at_store<float, DP>(a.part + at * a.Dv, acc, a.Dv, a.Dv % 4 == 0, h, [](float x) { return x; });
+        if (h == 0) {
+            a.part2[2 * at] = m == -INFINITY ? m : m * a.scale2;
+            a.part2[2 * at + 1] = l;
+        }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    at_store<T, DP>((T *)a.out + row * a.Dv, acc, a.Dv, a.vo, h, [&](float x) { return x * inv; });
+    if (sizeof(T) == 2 && a.outres)     // what the rounding of o lost: the backward pass needs D_i = do . o to more than 8 bits
+        at_store<T, DP>((T *)a.outres + row * a.Dv, acc, a.Dv, a.vo, h,
+                        [&](float x) { const float y = x * inv; return y - tk_up(tk_down<T>(y)); });
+    if (a.lse && h == 0) a.lse[row] = m == -INFINITY ? INFINITY : m * a.scale2 + __builtin_amdgcn_logf(l);   // +inf: an empty row
+}
+
+// joins the splits of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  One wave per row.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(const float *__restrict__ part, const float *__restrict__ ml, T *__restrict__ out,
+                                                        T *__restrict__ outres, float *__restrict__ lse, long long rows, int Dv, int nsplit) {
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    float m = -INFINITY, l = 0.f;
+    for (int s = 0; s < nsplit; ++s) m = fmaxf(m, ml[2 * (s * rows + row)]);
+    const float shift = m == -INFINITY ? 0.f : m;
+    float x[2] = {0.f, 0.f};
+    for (int s = 0; s < nsplit; ++s) {
+        const long long at = s * rows + row;
+        const float f = __builtin_amdgcn_exp2f(ml[2 * at] - shift);
+        l += f * ml[2 * at + 1];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (lane + 64 * u < Dv) x[u] += f * part[at * Dv + lane + 64 * u];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+        if (lane + 64 * u < Dv) {
+            const float y = x[u] * inv;
+            const T t = tk_down<T>(y);
+            out[row * Dv + lane + 64 * u] = t;
+            if (sizeof(T) == 2 && outres) outres[row * Dv + lane + 64 * u] = tk_down<T>(y - tk_up(t));
+        }
+    if (lse && lane == 0) lse[row] = m == -INFINITY ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// D_i = sum_c do_ic o_ic.  16 lanes per row.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_delta_kernel(const T *__restrict__ g, const T *__restrict__ o, const T *__restrict__ ores,
+                                                         const float *__restrict__ lse, float *__restrict__ delta, long long rows, int D, int vec) {
+    const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int c = threadIdx.x & 15;
+    float s = 0.f;
+    if (row < rows && lse[row] != INFINITY)
+        for (int d = 8 * c; d < D; d += 128) {
+            const TkFrag<T> x = tk_load8(g + row * D, d, D, vec), y = tk_load8(o + row * D, d, D, vec);
+            TkFrag<T> z = y;
+            if (ores) z = tk_load8(ores + row * D, d, D, vec);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s = fmaf((float)x.v[j], ores ? (float)y.v[j] + (float)z.v[j] : (float)y.v[j], s);
+        }
+#pragma unroll
+    for (int k = 8; k; k >>= 1) s += __shfl_xor(s, k);
+    if (row < rows && c == 0) delta[row] = s;
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * AT_WAVES) void attn_dq_kernel(AttnArgs a) {
+    constexpr int KT = at_tile<T>(), S = DP + tk_pad<T>();
+    __shared__ __attribute__((aligned(16))) T Ks[KT * S];
+    __shared__ __attribute__((aligned(16))) T Vs[KT * S];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int b = blockIdx.z / a.nsplit, sp = blockIdx.z - b * a.nsplit, grp = a.H / a.Hk;
+    const int hb = blockIdx.y * (a.pack ? grp : 1), hk = hb / grp, nrows = a.pack ? grp * a.Tq : a.Tq;
+    const int L = at_length(a, b), r0 = blockIdx.x * AT_ROWS, r = r0 + wave * 32 + (lane & 31);
+    const AtRow w = at_query_row(a, r, hb, nrows, L);
+    int j0, j1;
+    at_key_range(a, L, (r0 + AT_ROWS < nrows ? r0 + AT_ROWS : nrows) - 1, nrows, sp, KT, j0, j1);
+    const long long row = ((long long)b * a.Tq + w.i) * a.H + w.head;
+    TkFrag<T> qf[DP / 16], gf[DP / 16];
+    const T *qrow = (const T *)a.q + b * a.qs[0] + (long long)w.i * a.qs[1] + w.head * a.qs[2], *grow = (const T *)a.g + row * a.Dv;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+        qf[kk] = tk_load8(qrow, 16 * kk + 8 * h, a.Dk, a.vq);
+        gf[kk] = tk_load8(grow, 16 * kk + 8 * h, a.Dv, a.vo);
+    }
+    const float lse = a.lse[row], delta = a.delta[row];
+    const T *kb = (const T *)a.k + b * a.ks[0] + hk * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + hk * a.vs[2];
+    const unsigned char *mrow = a.mask ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
+    const unsigned char *mkey = a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
+    tk16 acc[DP / 32] = {};
+    for (int j = j0; j < j1; j += KT) {
+        __syncthreads();
+        at_stage<T, DP, KT>(Ks, kb, a.ks[1], j, j1, a.Dk, a.vk, tid, [&](int t) { return mkey && !mkey[t * a.ms[3]]; });
+        at_stage<T, DP, KT>(Vs, vb, a.vs[1], j, j1, a.Dv, a.vv, tid, [](int) { return false; });
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < KT / 32; ++n) {
+            tk16 s = at_product<T, DP>(Ks, 32 * n, qf, lane);
+            const tk16 dp = at_product<T, DP>(Vs, 32 * n, gf, lane);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int key = j + 32 * n + at_row(e, h);
+                bool on = key < w.lim;
+                if (mrow && on) on = mrow[key * a.ms[3]];
+                s[e] = on ? __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse)) * (dp[e] - delta) : 0.f;
+            }
+            at_accumulate<T, DP>(acc, Ks, 32 * n, s, lane);
+        }
+    }
+    if (!w.valid) return;
+    if (a.nsplit > 1) {
+        const long long rows = (long long)a.B * a.Tq * a.H;
+        at_store<float, DP>(a.part + (sp * rows + row) * a.Dk, acc, a.Dk, a.Dk % 4 == 0, h, [&](float x) { return x * a.scale; });
+        return;
+    }
+    at_store<T, DP>((T *)a.dq + row * a.Dk, acc, a.Dk, a.Dk % 8 == 0, h, [&](float x) { return x * a.scale; });
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
+    constexpr int QT = at_tile<T>(), S = DP + tk_pad<T>();
+    __shared__ __attribute__((aligned(16))) T Qs[QT * S];
+    __shared__ __attribute__((aligned(16))) T Gs[QT * S];
+    __shared__ __attribute__((aligned(16))) float lse[QT], delta[QT];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int b = blockIdx.z / a.nsplit, sp = blockIdx.z - b * a.nsplit, grp = a.H / a.Hk, hk = blockIdx.y;
+    const int L = at_length(a, b), off = L - a.Tq, key0 = blockIdx.x * AT_ROWS, key = key0 + wave * 32 + (lane & 31);
+    const bool valid = key < a.Tk;
+    const int kc = valid ? key : a.Tk - 1;
+    // queries that see this key: [first, Tq)
+    const int first = key >= L ? 0x7fffffff : (a.causal ? key - off : 0);
+    TkFrag<T> kf[DP / 16], vf[DP / 16];
+    const T *krow = (const T *)a.k + b * a.ks[0] + (long long)kc * a.ks[1] + hk * a.ks[2];
+    const T *vrow = (const T *)a.v + b * a.vs[0] + (long long)kc * a.vs[1] + hk * a.vs[2];
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+        kf[kk] = tk_load8(krow, 16 * kk + 8 * h, a.Dk, a.vk);
+        vf[kk] = tk_load8(vrow, 16 * kk + 8 * h, a.Dv, a.vv);
+    }
+    tk16 acck[DP / 32] = {}, accv[DP / 32] = {};
+    // the list of (head of the group, query tile) that sees any key of this tile, cut into nsplit runs
+    int qt0 = a.causal && key0 - off > 0 ? (key0 - off) / QT : 0;
+    const int nqt = (a.Tq + QT - 1) / QT;
+    if (key0 >= L || qt0 > nqt) qt0 = nqt;
+    const int each = nqt - qt0, total = each * grp, per = (total + a.nsplit - 1) / a.nsplit;
+    const int it1 = (sp + 1) * per < total ? (sp + 1) * per : total;
+    for (int it = sp * per; it < it1; ++it) {
+        const int gi = it / each, i0 = (qt0 + it - gi * each) * QT, head = hk * grp + gi;
+        const long long row0 = ((long long)b * a.Tq) * a.H + head;
+        __syncthreads();
+        for (int t = tid; t < QT; t += 64 * AT_WAVES) {
+            const bool in = i0 + t < a.Tq;
+            lse[t] = in ? a.lse[row0 + (long long)(i0 + t) * a.H] : INFINITY;
+            delta[t] = in ? a.delta[row0 + (long long)(i0 + t) * a.H] : 0.f;
+        }
+        // rows that see nothing are zeroed: whatever stands in them stays out of the sums
+        const auto dead = [&](int t) { return a.lse[row0 + (long long)t * a.H] == INFINITY; };
+        at_stage<T, DP, QT>(Qs, (const T *)a.q + b * a.qs[0] + head * a.qs[2], a.qs[1], i0, a.Tq, a.Dk, a.vq, tid, dead);
+        at_stage<T, DP, QT>(Gs, (const T *)a.g + row0 * a.Dv, (long long)a.H * a.Dv, i0, a.Tq, a.Dv, a.vo, tid, dead);
+        __syncthreads();
+        const unsigned char *mcol = a.mask ? a.mask + b * a.ms[0] + head * a.ms[1] + kc * a.ms[3] : nullptr;
+#pragma unroll
+        for (int n = 0; n < QT / 32; ++n) {
+            tk16 s = at_product<T, DP>(Qs, 32 * n, kf, lane);
+            tk16 dp = at_product<T, DP>(Gs, 32 * n, vf, lane);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int t = 32 * n + at_row(e, h), i = i0 + t;
+                bool on = i >= first && i < a.Tq;
+                if (mcol && on) on = mcol[i * a.ms[2]];
+                const float p = on ? __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse[t])) : 0.f;
+                dp[e] = on ? p * (dp[e] - delta[t]) : 0.f;
+                s[e] = p;
+            }
+            at_accumulate<T, DP>(accv, Gs, 32 * n, s, lane);
+            at_accumulate<T, DP>(acck, Qs, 32 * n, dp, lane);
+        }
+    }
+    if (!valid) return;
+    const long long row = ((long long)b * a.Tk + key) * a.Hk + hk;
+    if (a.nsplit > 1) {
+        const long long at = sp * ((long long)a.B * a.Tk * a.Hk) + row;
+        at_store<float, DP>(a.part + at * a.Dk, acck, a.Dk, a.Dk % 4 == 0, h, [&](float x) { return x * a.scale; });
+        at_store<float, DP>(a.part2 + at * a.Dv, accv, a.Dv, a.Dv % 4 == 0, h, [](float x) { return x; });
+        return;
+    }
+    at_store<T, DP>((T *)a.dk + row * a.Dk, acck, a.Dk, a.Dk % 8 == 0, h, [&](float x) { return x * a.scale; });
+    at_store<T, DP>((T *)a.dv + row * a.Dv, accv, a.Dv, a.Dv % 8 == 0, h, [](float x) { return x; });
+}
+
+// out = sum over splits, in split order
+template <typename T>
+__global__ __launch_bounds__(256) void attn_sum_kernel(const float *__restrict__ part, T *__restrict__ out, long long n, int nsplit) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        float s = part[i];
+        for (int k = 1; k < nsplit; ++k) s += part[k * n + i];
+        out[i] = tk_down<T>(s);
+    }
+}
+
+}  // namespace hno
+
+using namespace hno;
+
+// how many runs the streamed side is cut into: enough workgroups for the chip (two per CU), no run shorter than two tiles
+static int at_splits(long long groups, long long steps) {
+    if (groups < 1) return 1;                                  // no keys at all
+    long long n = groups >= 512 ? 1 : (512 + groups - 1) / groups;
+    if (n > steps / 2) n = steps / 2;
+    if (n > 64) n = 64;
+    return n < 1 ? 1 : (int)n;
+}
+struct AtPlan {
+    int pack, q_tiles, q_heads, q_split, k_tiles, k_split;
+};
+static AtPlan at_plan(const hno_attn_t *p) {
+    AtPlan n;
+    const int grp = p->H / p->Hk, KT = p->dtype == HNO_BF16 ? 64 : 32;
+    n.pack = grp > 1 && p->Tq < AT_ROWS;
+    n.q_tiles = ceil_div(n.pack ? grp * p->Tq : p->Tq, AT_ROWS);
+    n.q_heads = n.pack ? p->Hk : p->H;
+    n.q_split = at_splits((long long)n.q_tiles * n.q_heads * p->B, ceil_div(p->Tk, KT));
+    n.k_tiles = ceil_div(p->Tk, AT_ROWS);
+    n.k_split = at_splits((long long)n.k_tiles * p->Hk * p->B, (long long)ceil_div(p->Tq, KT) * grp);
+    return n;
+}
+static size_t at_pad(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+static int at_check(const hno_attn_t *p, const char *what) {
+    HNO_REQUIRE(p, "%s: null argument", what);
+    HNO_REQUIRE(p->dtype == HNO_F32 || p->dtype == HNO_BF16, "%s: dtype %d is neither HNO_F32 nor HNO_BF16", what, p->dtype);
+    HNO_REQUIRE(p->B > 0 && p->Tq > 0 && p->Tk >= 0 && p->H > 0 && p->Hk > 0 && p->Dk > 0 && p->Dv > 0, "%s: bad size", what);
+    HNO_REQUIRE(p->H % p->Hk == 0, "%s: %d query heads do not share %d key heads evenly", what, p->H, p->Hk);
+    HNO_REQUIRE(p->scale > 0.f && p->scale < 3e38f, "%s: scale must be positive and finite", what);
+    if (p->Dk > 128 || p->Dv > 128) return fail(HNO_ELIMIT, "%s: head sizes %d, %d exceed 128", what, p->Dk, p->Dv);
+    if (p->H > 65535 || p->B > 64000) return fail(HNO_ELIMIT, "%s: %d heads or a batch of %d exceed the grid", what, p->H, p->B);
+    if (p->Tq > (1 << 28) || p->Tk > (1 << 28) || (long long)(p->H / p->Hk) * p->Tq > (1ll << 30)) return fail(HNO_ELIMIT, "%s: too many tokens", what);
+    HNO_REQUIRE(p->q && (p->Tk == 0 || (p->k && p->v)), "%s: null pointer", what);
+    return HNO_OK;
+}
+static AttnArgs at_args(const hno_attn_t *p) {
+    AttnArgs a = {};
+    const int esz = p->dtype == HNO_BF16 ? 2 : 4;
+    const auto aligned = [&](const void *ptr, const long long *st, int D) {
+        bool ok = D % 8 == 0 && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0;
+        for (int i = 0; i < 3; ++i) ok = ok && st[i] * esz % 16 == 0;
+        return ok ? 1 : 0;
+    };
+    a.q = p->q; a.k = p->k; a.v = p->v; a.mask = p->mask; a.lens = p->kv_lens;
+    for (int i = 0; i < 3; ++i) a.qs[i] = p->q_stride[i], a.ks[i] = p->k_stride[i], a.vs[i] = p->v_stride[i];
+    for (int i = 0; i < 4; ++i) a.ms[i] = p->mask_stride[i];
+    a.B = p->B; a.Tq = p->Tq; a.Tk = p->Tk; a.H = p->H; a.Hk = p->Hk; a.Dk = p->Dk; a.Dv = p->Dv; a.causal = p->causal != 0;
+    a.vq = aligned(p->q, p->q_stride, p->Dk);
+    a.vk = aligned(p->k, p->k_stride, p->Dk);
+    a.vv = aligned(p->v, p->v_stride, p->Dv);
+    a.vo = p->Dv % 8 == 0;                        // outputs and their gradients are contiguous (16-byte aligned, checked by the entries)
+    a.keymask = p->mask && p->mask_stride[2] == 0 && p->mask_stride[1] == 0;
+    a.scale = p->scale;
+    a.scale2 = p->scale * 1.4426950408889634f;
+    return a;
+}
+static bool at_aligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static double at_bytes(const hno_attn_t *p, int q_tensors, int k_tensors) {
+    return (p->dtype == HNO_BF16 ? 2.0 : 4.0) * ((double)p->B * p->Tq * p->H * p->Dk * q_tensors + (double)p->B * p->Tk * p->Hk * p->Dk * k_tensors);
+}
+
+// the kernel of one type for the padded head size
+#define AT_DISPATCH(KERNEL, grid, s, a)                                                                       \
+    do {                                                                                                      \
+        const int dp_ = round_up(a.Dk > a.Dv ? a.Dk : a.Dv, 32);                                              \
+        if (dp_ == 32) hipLaunchKernelGGL((KERNEL<T, 32>), grid, dim3(64 * AT_WAVES), 0, s, a);               \
+        else if (dp_ == 64) hipLaunchKernelGGL((KERNEL<T, 64>), grid, dim3(64 * AT_WAVES), 0, s, a);          \
+        else if (dp_ == 96) hipLaunchKernelGGL((KERNEL<T, 96>), grid, dim3(64 * AT_WAVES), 0, s, a);          \
+        else hipLaunchKernelGGL((KERNEL<T, 128>), grid, dim3(64 * AT_WAVES), 0, s, a);                        \
+    } while (0)
+
+template <typename T>
+static int at_forward(const hno_attn_t *p, void *out, void *out_res, float *lse, void *workspace, hipStream_t s) {
+    const AtPlan n = at_plan(p);
+    AttnArgs a = at_args(p);
+    const long long rows = (long long)p->B * p->Tq * p->H;
+    a.out = out; a.outres = out_res; a.lse = lse; a.pack = n.pack; a.nsplit = n.q_split;
+    a.part = (float *)workspace;
+    a.part2 = (float *)((char *)workspace + at_pad((size_t)n.q_split * rows * p->Dv * sizeof(float)));
+    ProfScope _ps(KID_ATTN, s, at_bytes(p, 2, 2));
+    AT_DISPATCH(attn_fwd_kernel, dim3(n.q_tiles, n.q_heads, p->B * n.q_split), s, a);
+    HNO_CHECK_LAUNCH();
+    if (n.q_split > 1) {
+        hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, (const float *)a.part, (const float *)a.part2,
+                           (T *)out, (T *)out_res, lse, rows, p->Dv, n.q_split);
+        HNO_CHECK_LAUNCH();
+    }
+    return HNO_OK;
+}
+
+template <typename T>
+static int at_sum(const float *part, T *out, long long n, int nsplit, hipStream_t s) {
+    const long long blocks = (n + 255) / 256;
+    hipLaunchKernelGGL((attn_sum_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, part, out, n, nsplit);
+    HNO_CHECK_LAUNCH();
+    return HNO_OK;
+}
+
+template <typename T>
+static int at_backward(const hno_attn_t *p, const void *out, const void *out_res, const float *lse, const void *dout, void *dq, void *dk, void *dv,
+                       void *workspace, hipStream_t s) {
+    const AtPlan n = at_plan(p);
+    AttnArgs a = at_args(p);
+    const long long rows = (long long)p->B * p->Tq * p->H, krows = (long long)p->B * p->Tk * p->Hk;
+    a.g = dout; a.lse = const_cast<float *>(lse); a.delta = (float *)workspace;
+    a.dq = dq; a.dk = dk; a.dv = dv;
+    a.part = (float *)((char *)workspace + at_pad(rows * sizeof(float)));
+    {
+        ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 2, 0));
+        hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, (const T *)dout, (const T *)out,
+                           (const T *)out_res, lse, a.delta, rows, p->Dv, a.vo);
+        HNO_CHECK_LAUNCH();
+    }
+    if (dq) {
+        ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 3, 2));
+        a.pack = n.pack;
+        a.nsplit = n.q_split;
+        AT_DISPATCH(attn_dq_kernel, dim3(n.q_tiles, n.q_heads, p->B * n.q_split), s, a);
+        HNO_CHECK_LAUNCH();
+        if (n.q_split > 1)
+            if (int rc = at_sum(a.part, (T *)dq, rows * p->Dk, n.q_split, s)) return rc;
+    }
+    if (dk && p->Tk > 0) {
+        ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 2, 4));
+        a.nsplit = n.k_split;
+        a.part2 = (float *)((char *)a.part + at_pad((size_t)n.k_split * krows * p->Dk * sizeof(float)));
+        AT_DISPATCH(attn_dkv_kernel, dim3(n.k_tiles, p->Hk, p->B * n.k_split), s, a);
+        HNO_CHECK_LAUNCH();
+        if (n.k_split > 1) {
+            if (int rc = at_sum(a.part, (T *)dk, krows * p->Dk, n.k_split, s)) return rc;
+            if (int rc = at_sum(a.part2, (T *)dv, krows * p->Dv, n.k_split, s)) return rc;
+        }
+    }
+    return HNO_OK;
+}
+
+extern "C" size_t hno_attn_workspace_bytes(const hno_attn_t *p, int backward) {
+    if (at_check(p, "hno_attn_workspace_bytes") != HNO_OK) return 0;
+    const AtPlan n = at_plan(p);
+    const size_t rows = (size_t)p->B * p->Tq * p->H, krows = (size_t)p->B * p->Tk * p->Hk, f = sizeof(float);
+    if (!backward) return n.q_split > 1 ? at_pad(n.q_split * rows * p->Dv * f) + n.q_split * rows * 2 * f : 0;
+    const size_t q = n.q_split > 1 ? n.q_split * rows * p->Dk * f : 0, k = n.k_split > 1 ? at_pad(n.k_split * krows * p->Dk * f) + n.k_split * krows * p->Dv * f : 0;
+    return at_pad(rows * f) + (q > k ? q : k);
+}
+
+extern "C" int hno_attn_fwd(const hno_attn_t *p, void *out, void *out_res, float *lse, void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = at_check(p, "hno_attn_fwd")) return rc;
+    HNO_REQUIRE(out && at_aligned(out) && at_aligned(out_res), "hno_attn_fwd: out must be a 16-byte aligned tensor");
+    const size_t need = hno_attn_workspace_bytes(p, 0);
+    HNO_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && at_aligned(workspace))), "hno_attn_fwd: workspace of %zu bytes, %zu needed",
+                workspace_bytes, need);
+    if (p->dtype == HNO_BF16) return at_forward<tkh>(p, out, out_res, lse, workspace, (hipStream_t)stream);
+    return at_forward<float>(p, out, nullptr, lse, workspace, (hipStream_t)stream);
+}
+
+extern "C" int hno_attn_bwd(const hno_attn_t *p, const void *out, const void *out_res, const float *lse, const void *dout, void *dq, void *dk, void *dv,
+                            void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = at_check(p, "hno_attn_bwd")) return rc;
+    HNO_REQUIRE(out && lse && dout && (dq || dk) && !dk == !dv, "hno_attn_bwd: null pointer");
+    HNO_REQUIRE(at_aligned(out) && at_aligned(out_res) && at_aligned(dout) && at_aligned(dq) && at_aligned(dk) && at_aligned(dv),
+                "hno_attn_bwd: tensors must be 16-byte aligned");
+    const size_t need = hno_attn_workspace_bytes(p, 1);
+    HNO_REQUIRE(workspace_bytes >= need && workspace && at_aligned(workspace), "hno_attn_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (p->dtype == HNO_BF16) return at_backward<tkh>(p, out, out_res, lse, dout, dq, dk, dv, workspace, (hipStream_t)stream);
+    return at_backward<float>(p, out, nullptr, lse, dout, dq, dk, dv, workspace, (hipStream_t)stream);
+}

@@ -1,0 +1,355 @@
+"""Token operators over the ``hno_attn_*`` / ``hno_linear_*`` / ``hno_gncl_*`` entry points of include/hno.h: softmax attention, the matrix
+product with bias, activation and residual in its epilogue, and group norm with an activation -- on channels-last tokens, in fp32 or bf16, with
+their backward passes.
+
+Tensors are torch containers; nothing computes through ATen and there is no CPU path (meta tensors get shape inference only).  Parameters may
+stay fp32 next to bf16 activations: the matrix product then rounds its weight to bf16, as the bf16 convolutions do, and returns an fp32 gradient.
+Gradients of gradients are refused (``once_differentiable``).
+"""
+import contextlib
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, ops
+from ._lib import check, stream_ptr
+from .ops import _HnoFunction, _m
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}                     # HNO_F32, HNO_BF16
+_ACTS = {None: 0, 'none': 0, 'selu': 1, 'elu': 2, 'relu': 4, 'gelu': 5, 'silu': 6}
+MAX_HEAD = 128
+
+
+def act_id(act):
+    """id of an activation of the token operators: None, 'none', 'selu', 'elu', 'relu', 'gelu' (exact), 'silu', or the torch function of that name"""
+    if callable(act):
+        act = getattr(act, '__name__', act)
+    if act not in _ACTS:
+        raise ValueError(f'activation {act!r} is not supported by the token operators ({", ".join(k for k in _ACTS if k)})')
+    return _ACTS[act]
+
+
+def _dtype(t, what):
+    if t.dtype not in _DTYPES:
+        raise ValueError(f'{what}: dtype {t.dtype} is not provided by the HIP path (torch.float32 or torch.bfloat16)')
+    return _DTYPES[t.dtype]
+
+
+def _same_device(what, first, *others):
+    if not first.is_cuda:
+        raise _lib.HnoError('the HIP path needs CUDA/HIP tensors; there is no CPU fallback (use oracle/ for CPU checks)')
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f'{what}: tensors on {first.device} and {t.device}')
+
+
+def _on(t):
+    """the tensor's device as the current one (launches and workspaces go by the current device and its current stream)"""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _ws(nbytes, device):
+    return torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
+
+
+# ----------------------------------------------------------------------------------------------- attention
+def _attn_args(q, k, v, mask, kv_lens, causal, scale):
+    a = _lib.AttnArgs()
+    B, Tq, H, Dk = q.shape
+    a.dtype, a.B, a.Tq, a.Tk, a.H, a.Hk, a.Dk, a.Dv = _DTYPES[q.dtype], B, Tq, k.shape[1], H, k.shape[2], Dk, v.shape[3]
+    a.causal, a.scale = int(causal), scale
+    a.q, a.k, a.v, a.mask, a.kv_lens = _p(q), _p(k), _p(v), _p(mask), _p(kv_lens)
+    a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    if mask is not None:
+        a.mask_stride[:] = [0 if n == 1 else s for n, s in zip(mask.shape, mask.stride())]
+    return a
+
+
+class AttentionFn(_HnoFunction):
+    """out = softmax(scale q k^T) v over the visible keys; the backward pass recomputes the probabilities from lse (``attention`` has the
+    contract)."""
+
+    @staticmethod
+    def meta(q, k, v, mask, kv_lens, causal, scale):
+        return _m(tuple(q.shape[:3]) + (v.shape[3],), q.dtype)
+
+    @staticmethod
+    def forward(ctx, q, k, v, mask, kv_lens, causal, scale):
+        train = ops.backward_wanted(ctx)
+        q, k, v = (t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous() for t in (q, k, v))
+        B, Tq, H, _ = q.shape
+        out = torch.empty((B, Tq, H, v.shape[3]), device=q.device, dtype=q.dtype)
+        lse = torch.empty((B, Tq, H), device=q.device, dtype=torch.float32) if train else None
+        res = torch.empty_like(out) if train and q.dtype == torch.bfloat16 else None
+        if out.numel():
+            L = _lib.lib()
+            a = _attn_args(q, k, v, mask, kv_lens, causal, scale)
+            n = L.hno_attn_workspace_bytes(ctypes.byref(a), 0)
+            ws = _ws(n, q.device)
+            check(L.hno_attn_fwd(ctypes.byref(a), _p(out), _p(res), _p(lse), _p(ws), n, stream_ptr()), 'hno_attn_fwd')
+        if train:
+            ctx.save_for_backward(q, k, v, mask, kv_lens, out, res, lse)
+            ctx.cfg = (causal, scale)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        q, k, v, mask, kv_lens, out, res, lse = ctx.saved_tensors
+        causal, scale = ctx.cfg
+        need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        new = torch.empty if out.numel() else torch.zeros
+        dq = new(q.shape, device=q.device, dtype=q.dtype) if need_q else None
+        dk, dv = (new(t.shape, device=q.device, dtype=q.dtype) if need_kv else None for t in (k, v))
+        if out.numel():
+            with _on(q):
+                L = _lib.lib()
+                g = _aligned(g)
+                a = _attn_args(q, k, v, mask, kv_lens, causal, scale)
+                n = L.hno_attn_workspace_bytes(ctypes.byref(a), 1)
+                ws = _ws(n, q.device)
+                check(L.hno_attn_bwd(ctypes.byref(a), _p(out), _p(res), _p(lse), _p(g), _p(dq), _p(dk), _p(dv), _p(ws), n, stream_ptr()),
+                      'hno_attn_bwd')
+        return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None, None
+
+
+def _aligned(t):
+    """contiguous and 16-byte aligned (an upstream gradient can be any view)"""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def attention(q, k, v, *, causal=False, mask=None, kv_lens=None, scale=None):
+    """Softmax attention on tokens: q (B, Tq, H, Dk), k (B, Tk, Hk, Dk), v (B, Tk, Hk, Dv) -> (B, Tq, H, Dv); all fp32 or all bf16.
+
+    H is a multiple of Hk: query head h reads key head h // (H // Hk).  Head sizes 1 ... 128.  Any strides; a last axis that is not contiguous is
+    copied.  ``scale`` (positive, default Dk ** -0.5) multiplies the scores.
+    Visible to query i are the keys j < L with L = ``kv_lens[b]`` (integers (B,) on the device, clamped to 0 ... Tk; default Tk);
+    with ``causal`` those with j <= i + L - Tq (the last query is aligned with the last key);
+    with ``mask`` (bool, broadcastable to (B, H, Tq, Tk)) those that it marks True.  A query that sees no key gives zeros and has no gradient.
+    Keys and values from L on, and those that a mask of shape (B, 1, 1, Tk) hides, may hold anything (inf, NaN); a value that some
+    queries see and others do not has to be finite.  Additive (floating) masks are refused.
+    Differentiable in q, k, v; the probabilities are recomputed in the backward pass, memory grows with Tq + Tk only."""
+    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
+        raise ValueError('attention: q, k, v must be (batch, tokens, heads, channels)')
+    B, Tq, H, Dk = q.shape
+    _, Tk, Hk, Dv = v.shape
+    if tuple(k.shape) != (B, Tk, Hk, Dk) or v.shape[0] != B:
+        raise ValueError(f'attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not belong together')
+    if Hk == 0 or H % Hk or H == 0:
+        raise ValueError(f'attention: {H} query heads do not share {Hk} key heads evenly')
+    if not 1 <= Dk <= MAX_HEAD or not 1 <= Dv <= MAX_HEAD:
+        raise ValueError(f'attention: head sizes {Dk}, {Dv} are outside 1 ... {MAX_HEAD}')
+    _dtype(q, 'attention')
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f'attention: q, k, v are {q.dtype}, {k.dtype}, {v.dtype}: one type is needed')
+    scale = 1.0 / math.sqrt(Dk) if scale is None else float(scale)
+    if not 0.0 < scale < 3e38:
+        raise ValueError('attention: scale must be positive and finite')
+    if mask is not None:
+        if mask.dtype != torch.bool:
+            raise ValueError('attention: mask must be bool (True: visible); additive masks are not provided')
+        if mask.ndim > 4 or any(m not in (1, n) for m, n in zip(reversed(mask.shape), (Tk, Tq, H, B))):
+            raise ValueError(f'attention: mask {tuple(mask.shape)} does not broadcast to {(B, H, Tq, Tk)}')
+        mask = mask[(None,) * (4 - mask.ndim)]
+    if kv_lens is not None:
+        if tuple(kv_lens.shape) != (B,) or kv_lens.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f'attention: kv_lens must be {B} integers')
+    if q.is_meta:
+        return AttentionFn.apply(q, k, v, mask, kv_lens, bool(causal), scale)
+    _same_device('attention', q, k, v, mask, kv_lens)
+    with _on(q):
+        if kv_lens is not None and (kv_lens.dtype != torch.int32 or not kv_lens.is_contiguous()):
+            kv_lens = kv_lens.clamp(0, Tk).to(torch.int32).contiguous()
+        return AttentionFn.apply(q, k, v, mask, kv_lens, bool(causal), scale)
+
+
+# ----------------------------------------------------------------------------------------------- linear
+def _rows(x):
+    """x (..., K) as (M, K) with unit stride along K -> (view or copy, row stride)"""
+    x2 = x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1 and x2.shape[1] != 1:
+        x2 = x2.contiguous()
+    ld = x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
+    if ld < x2.shape[1]:          # rows that share memory (expanded views)
+        x2 = x2.contiguous()
+        ld = x2.shape[1]
+    return x2, ld
+
+
+def _bf16_weight(w):
+    out = torch.empty(w.shape, device=w.device, dtype=torch.bfloat16)
+    check(_lib.lib().hno_cast_f32_bf16(_p(w), _p(out), w.numel(), stream_ptr()), 'hno_cast_f32_bf16')
+    return out
+
+
+class LinearFn(_HnoFunction):
+    """y = act(x W^T + b) + r with the whole epilogue in the product's kernel (``linear`` has the contract)."""
+
+    @staticmethod
+    def meta(x, weight, bias, residual, act):
+        return _m(tuple(x.shape[:-1]) + (weight.shape[0],), x.dtype)
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        train = ops.backward_wanted(ctx)
+        N, K = weight.shape
+        y = torch.empty(tuple(x.shape[:-1]) + (N,), device=x.device, dtype=x.dtype)
+        z, w, x2 = None, weight.contiguous(), x
+        if y.numel():
+            L = _lib.lib()
+            x2, ldx = _rows(x)
+            M = x2.shape[0]
+            if w.dtype != x.dtype:
+                w = _bf16_weight(w)
+            b = None if bias is None else bias.contiguous()
+            r = None if residual is None else residual.contiguous()
+            z = torch.empty((M, N), device=x.device, dtype=x.dtype) if train and act else None
+            dt = _DTYPES[x.dtype]
+            n = L.hno_linear_workspace_bytes(dt, M, N, K, act, 0)
+            ws = _ws(n, x.device)
+            check(L.hno_linear_fwd(dt, _p(x2), ldx, _p(w), _p(b), 0 if b is None else _DTYPES[b.dtype], _p(r), _p(z), _p(y), M, N, K, act, _p(ws), n,
+                                   stream_ptr()), 'hno_linear_fwd')
+        if train:
+            ctx.save_for_backward(x2, w, z, weight)
+            ctx.cfg = (act, tuple(x.shape), None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, w, z, weight = ctx.saved_tensors
+        act, xshape, bias_dtype = ctx.cfg
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        N, K = w.shape
+        if not g.numel():
+            zeros = lambda shape, dt: torch.zeros(shape, device=g.device, dtype=dt)  # noqa: E731
+            return (zeros(xshape, g.dtype) if need_x else None, zeros((N, K), weight.dtype) if need_w else None,
+                    zeros((N,), bias_dtype) if need_b else None, g if need_r else None, None)
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            with _on(g):
+                L = _lib.lib()
+                gc = g.contiguous()
+                x2, ldx = _rows(x)
+                M = x2.shape[0]
+                if need_x:
+                    dx = torch.empty(xshape, device=g.device, dtype=g.dtype)
+                if need_w:
+                    own = weight.is_leaf and weight.dtype == torch.float32 and weight.is_contiguous()
+                    dw = ops._grad_buffer(weight) if own else torch.empty((N, K), device=g.device, dtype=weight.dtype)
+                if need_b:
+                    db = torch.empty(N, device=g.device, dtype=bias_dtype)
+                dt = _DTYPES[g.dtype]
+                n = L.hno_linear_workspace_bytes(dt, M, N, K, act, 1)
+                ws = _ws(n, g.device)
+                check(L.hno_linear_bwd(dt, _p(gc), _p(z), _p(x2), ldx, _p(w), _p(dx), _p(dw), 0 if dw is None else _DTYPES[dw.dtype], _p(db),
+                                       0 if db is None else _DTYPES[db.dtype], M, N, K, act, _p(ws), n, stream_ptr()), 'hno_linear_bwd')
+        return dx, dw, db, g if need_r else None, None
+
+
+def linear(x, weight, bias=None, *, act=None, residual=None):
+    """act(x W^T + bias) + residual: x (..., K), weight (N, K), bias (N,), residual (..., N) -> (..., N), in x's type (fp32 or bf16).
+
+    ``act``: see ``act_id``.  weight is of x's type, or fp32 next to a bf16 x (rounded to bf16 for the product; its gradient is fp32); bias is of either
+    type.  residual has the result's shape and type.  x may be any view; rows of equal stride are read where they lie.
+    fp32 products are formed from three bf16 terms per value, so an infinity in x or weight comes out as NaN.
+    Differentiable in all four; with an activation the backward pass keeps the product's result, in x's type."""
+    a = act_id(act)
+    if x.ndim < 1 or weight.ndim != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f'linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not belong together')
+    N, K = weight.shape
+    if N == 0 or K == 0:
+        raise ValueError('linear: empty weight')
+    _dtype(x, 'linear')
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f'linear: weight is {weight.dtype}, x is {x.dtype}')
+    if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype not in (x.dtype, torch.float32)):
+        raise ValueError(f'linear: bias must be ({N},) of {x.dtype} or fp32')
+    if residual is not None and (tuple(residual.shape) != tuple(x.shape[:-1]) + (N,) or residual.dtype != x.dtype):
+        raise ValueError(f'linear: residual must have the shape and type of the result, {tuple(x.shape[:-1]) + (N,)} {x.dtype}')
+    if x.is_meta:
+        return LinearFn.apply(x, weight, bias, residual, a)
+    _same_device('linear', x, weight, bias, residual)
+    with _on(x):
+        return LinearFn.apply(x, weight, bias, residual, a)
+
+
+# ----------------------------------------------------------------------------------------------- group norm
+class GroupNormClFn(_HnoFunction):
+    """act(GroupNorm(G, C)(x)) on channels-last tokens (``group_norm`` has the contract)."""
+
+    @staticmethod
+    def meta(x, weight, bias, groups, eps, act):
+        return _m(x.shape, x.dtype)
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act):
+        x = x.contiguous()
+        y = torch.empty_like(x)
+        B, C = x.shape[0], x.shape[-1]
+        w, b = (None if t is None else (t if t.dtype == torch.float32 else t.float()).contiguous() for t in (weight, bias))
+        mr = torch.empty((B, groups, 2), device=x.device, dtype=torch.float32)
+        if x.numel():
+            L = _lib.lib()
+            V = x.numel() // (B * C)
+            n = L.hno_gncl_workspace_bytes(B, V, C, groups)
+            ws = _ws(n, x.device)
+            check(L.hno_gncl_fwd(_DTYPES[x.dtype], _p(x), _p(w), _p(b), _p(y), _p(mr), _p(ws), n, B, V, C, groups, eps, act, stream_ptr()), 'hno_gncl_fwd')
+        if ops.backward_wanted(ctx):
+            ctx.save_for_backward(x, w, b, mr)
+            ctx.cfg = (groups, act, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, w, b, mr = ctx.saved_tensors
+        groups, act, wt, bt = ctx.cfg
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        B, C = x.shape[0], x.shape[-1]
+        new = torch.empty if x.numel() else torch.zeros
+        dx = torch.empty_like(x) if need_x else None
+        dw, db = (new(C, device=x.device, dtype=torch.float32) if n else None for n in (need_w, need_b))
+        if x.numel():
+            with _on(x):
+                L = _lib.lib()
+                g = g.contiguous()
+                V = x.numel() // (B * C)
+                n = L.hno_gncl_workspace_bytes(B, V, C, groups)
+                ws = _ws(n, x.device)
+                check(L.hno_gncl_bwd(_DTYPES[x.dtype], _p(g), _p(x), _p(w), _p(b), _p(mr), _p(dx), _p(dw), _p(db), _p(ws), n, B, V, C, groups, act,
+                                     stream_ptr()), 'hno_gncl_bwd')
+        return dx, dw if wt in (None, torch.float32) or dw is None else dw.to(wt), db if bt in (None, torch.float32) or db is None else db.to(bt), None, None, None
+
+
+def group_norm(x, num_groups, weight=None, bias=None, *, eps=1e-5, act=None):
+    """act(gamma (x - mean) / sqrt(var + eps) + beta) on channels-last x (B, ..., C), fp32 or bf16, statistics per sample and group of
+    C / num_groups neighbouring channels over all positions; weight, bias (C,) fp32 or x's type.  ``act``: see ``act_id``.
+    Statistics are joined in 64 bits.  Differentiable in x, weight, bias; the backward pass keeps x and the statistics."""
+    a = act_id(act)
+    num_groups, eps = int(num_groups), float(eps)
+    if x.ndim < 2:
+        raise ValueError('group_norm: x must be (batch, ..., channels)')
+    C = x.shape[-1]
+    if num_groups < 1 or C == 0 or C % num_groups:
+        raise ValueError(f'group_norm: {C} channels do not fall into {num_groups} groups')
+    if not eps >= 0.0:
+        raise ValueError('group_norm: eps must not be negative')
+    _dtype(x, 'group_norm')
+    for t in (weight, bias):
+        if t is not None and (tuple(t.shape) != (C,) or t.dtype not in (x.dtype, torch.float32)):
+            raise ValueError(f'group_norm: weight and bias must be ({C},) of {x.dtype} or fp32')
+    if x.is_meta:
+        return GroupNormClFn.apply(x, weight, bias, num_groups, eps, a)
+    _same_device('group_norm', x, weight, bias)
+    with _on(x):
+        return GroupNormClFn.apply(x, weight, bias, num_groups, eps, a)
