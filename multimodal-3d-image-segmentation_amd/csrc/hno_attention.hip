@@ -37,22 +37,34 @@ __device__ __forceinline__ int at_length(const AttnArgs &a, int b) {
 __device__ __forceinline__ float at_other_half(float x) { return __shfl_xor(x, 32); }
 __device__ __forceinline__ int at_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }   // result register -> row of the tile
 
-// rows [t0, t0 + n) of one head of a token tensor -> LDS tile; rows from `end` on, and rows that `dead` names, are zeroed
-template <typename T, int DP, int ROWS, typename Dead>
-__device__ __forceinline__ void at_stage(T *tile, const T *base, long long st, int t0, int end, int D, bool vec, int tid, Dead dead) {
-    constexpr int CH = DP / 8, S = DP + tk_pad<T>();
-    for (int c = tid; c < ROWS * CH; c += 64 * AT_WAVES) {
-        const int row = c / CH, d = (c - row * CH) * 8, t = t0 + row;
-        TkFrag<T> f;
-        if (t < end && !dead(t)) {
-            f = tk_load8(base + (long long)t * st, d, D, vec);
-        } else {
+// A workgroup's share of one tile of the streamed side on its way to LDS: loaded into registers one tile ahead of its use, stored
+// when the buffer is free.  Rows from `end` on, and rows that `dead` names, are zeros.
+template <typename T, int DP, int ROWS>
+struct AtStage {
+    static constexpr int CH = DP / 8, S = DP + tk_pad<T>(), N = (ROWS * CH + 64 * AT_WAVES - 1) / (64 * AT_WAVES);
+    static constexpr bool EVEN = ROWS * CH % (64 * AT_WAVES) == 0;
+    TkFrag<T> r[N];
+    template <typename Dead>
+    __device__ __forceinline__ void load(const T *base, long long st, int t0, int end, int D, bool vec, int tid, Dead dead) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f.set(j, 0.f);
+        for (int i = 0; i < N; ++i) {
+            const int c = tid + 64 * AT_WAVES * i, row = c / CH, d = (c - row * CH) * 8, t = t0 + row;
+            if ((EVEN || row < ROWS) && t < end && !dead(t)) {
+                r[i] = tk_load8(base + (long long)t * st, d, D, vec);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[i].set(j, 0.f);
+            }
         }
-        tk_store8(tile + row * S + d, f);
     }
-}
+    __device__ __forceinline__ void store(T *tile, int tid) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = tid + 64 * AT_WAVES * i, row = c / CH, d = (c - row * CH) * 8;
+            if (EVEN || row < ROWS) tk_store8(tile + row * S + d, r[i]);
+        }
+    }
+};
 
 // acc(32 rows of the tile x 32 own columns) = tile rows . own fragments
 template <typename T, int DP>
@@ -138,11 +150,37 @@ __device__ __forceinline__ void at_key_range(const AttnArgs &a, int L, int last_
     if (j1 > end) j1 = end;
 }
 
+// the smallest limit of the wave's rows: tiles that end before it need no comparison
+__device__ __forceinline__ int at_wave_min(int x) {
+#pragma unroll
+    for (int k = 16; k; k >>= 1) x = min(x, __shfl_xor(x, k));
+    return __builtin_amdgcn_readfirstlane(x);
+}
+// the weights of 8 keys as an operand, and their sum as the product takes them: the weights of a row then add up to one whatever they
+// were rounded to
+__device__ __forceinline__ void at_weights(TkFrag<tkh> &f, const tk16 &s, int t, float &l) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const b2 one = {(__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        f.set(j, s[8 * t + j]);
+        f.set(j + 1, s[8 * t + j + 1]);
+        l = __builtin_amdgcn_fdot2_f32_bf16(b2{f.v[j], f.v[j + 1]}, one, l, false);
+    }
+}
+__device__ __forceinline__ void at_weights(TkFrag<float> &f, const tk16 &s, int t, float &l) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        f.v[j] = s[8 * t + j];
+        l += f.v[j];
+    }
+}
+
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * AT_WAVES) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * AT_WAVES, 2) void attn_fwd_kernel(AttnArgs a) {
     constexpr int KT = at_tile<T>(), S = DP + tk_pad<T>();
-    __shared__ __attribute__((aligned(16))) T Ks[KT * S];
-    __shared__ __attribute__((aligned(16))) T Vs[KT * S];
+    __shared__ __attribute__((aligned(16))) T Ks[2][KT * S];
+    __shared__ __attribute__((aligned(16))) T Vs[2][KT * S];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int b = blockIdx.z / a.nsplit, sp = blockIdx.z - b * a.nsplit, grp = a.H / a.Hk;
     const int hb = blockIdx.y * (a.pack ? grp : 1), hk = hb / grp, nrows = a.pack ? grp * a.Tq : a.Tq;
@@ -150,6 +188,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_fwd_kernel(AttnArgs a) {
     const AtRow w = at_query_row(a, r, hb, nrows, L);
     int j0, j1;
     at_key_range(a, L, (r0 + AT_ROWS < nrows ? r0 + AT_ROWS : nrows) - 1, nrows, sp, KT, j0, j1);
+    const int lim_all = a.mask ? 0 : at_wave_min(w.lim);
 
     TkFrag<T> qf[DP / 16];
     const T *qrow = (const T *)a.q + b * a.qs[0] + (long long)w.i * a.qs[1] + w.head * a.qs[2];
@@ -159,45 +198,71 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_fwd_kernel(AttnArgs a) {
     const unsigned char *mrow = a.mask ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
     // a mask that hides a key from every query of this workgroup takes the value row out too: 0 x NaN would be NaN
     const unsigned char *mkey = a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
+    AtStage<T, DP, KT> ks, vs;
+    const auto load = [&](int j) {
+        ks.load(kb, a.ks[1], j, j1, a.Dk, a.vk, tid, [](int) { return false; });
+        vs.load(vb, a.vs[1], j, j1, a.Dv, a.vv, tid, [&](int t) { return mkey && !mkey[t * a.ms[3]]; });
+    };
 
     tk16 acc[DP / 32] = {};
-    float m = -INFINITY, l = 0.f;
-    for (int j = j0; j < j1; j += KT) {
+    float m = -INFINITY, l = 0.f, shift = 0.f;
+    const float slack = 8.f / a.scale2;           // the maximum is raised, and the sums rescaled, only where weights would exceed 2^8
+    int buf = 0;
+    if (j0 < j1) {
+        load(j0);
+        ks.store(Ks[0], tid);
+        vs.store(Vs[0], tid);
+        if (j0 + KT < j1) load(j0 + KT);
+    }
+    for (int j = j0; j < j1; j += KT, buf ^= 1) {
         __syncthreads();
-        at_stage<T, DP, KT>(Ks, kb, a.ks[1], j, j1, a.Dk, a.vk, tid, [](int) { return false; });
-        at_stage<T, DP, KT>(Vs, vb, a.vs[1], j, j1, a.Dv, a.vv, tid, [&](int t) { return mkey && !mkey[t * a.ms[3]]; });
-        __syncthreads();
+        if (j + KT < j1) {
+            ks.store(Ks[buf ^ 1], tid);
+            vs.store(Vs[buf ^ 1], tid);
+            if (j + 2 * KT < j1) load(j + 2 * KT);
+        }
         tk16 s[KT / 32];
+#pragma unroll
+        for (int n = 0; n < KT / 32; ++n) s[n] = at_product<T, DP>(Ks[buf], 32 * n, qf, lane);
+        if (j + KT > lim_all) {
+#pragma unroll
+            for (int n = 0; n < KT / 32; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int key = j + 32 * n + at_row(e, h);
+                    bool on = key < w.lim;
+                    if (mrow && on) on = mrow[key * a.ms[3]];
+                    s[n][e] = on ? s[n][e] : -INFINITY;
+                }
+        }
         float top = -INFINITY;
 #pragma unroll
-        for (int n = 0; n < KT / 32; ++n) {
-            s[n] = at_product<T, DP>(Ks, 32 * n, qf, lane);
+        for (int n = 0; n < KT / 32; ++n)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int key = j + 32 * n + at_row(e, h);
-                bool on = key < w.lim;
-                if (mrow && on) on = mrow[key * a.ms[3]];
-                s[n][e] = on ? s[n][e] : -INFINITY;
-                top = fmaxf(top, s[n][e]);
-            }
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, s[n][e]);
+        top = fmaxf(top, at_other_half(top));
+        if (__any(top > m + slack)) {
+            const float up = fmaxf(m, top), old = __builtin_amdgcn_exp2f((m - (up == -INFINITY ? 0.f : up)) * a.scale2);
+            m = up;
+            shift = up == -INFINITY ? 0.f : up * a.scale2;
+            l *= old;
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= old;
         }
-        top = fmaxf(m, fmaxf(top, at_other_half(top)));
-        const float shift = top == -INFINITY ? 0.f : top * a.scale2, old = __builtin_amdgcn_exp2f(m * a.scale2 - shift);
-        m = top;
-        l *= old;
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= old;
+        for (int n = 0; n < KT / 32; ++n)
 #pragma unroll
-        for (int n = 0; n < KT / 32; ++n) {
+            for (int e = 0; e < 16; ++e) s[n][e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], a.scale2, -shift));
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                // the sum takes the weight as the product takes it, so the weights of a row add up to one whatever they were rounded to
-                const float p = tk_up(tk_down<T>(__builtin_amdgcn_exp2f(fmaf(s[n][e], a.scale2, -shift))));
-                s[n][e] = p;
-                l += p;
+        for (int n = 0; n < KT / 32; ++n)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                TkFrag<T> f;
+                at_weights(f, s[n], t, l);
+                const int row = 32 * n + 16 * t + 4 * h;
+#pragma unroll
+                for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = tk_mma(tk_col(Vs[buf], S, 32 * dt, row, row + 8, lane), f, acc[dt]);
             }
-            at_accumulate<T, DP>(acc, Vs, 32 * n, s[n], lane);
-        }
     }
     l += at_other_half(l);
     if (!w.valid) return;
@@ -271,10 +336,10 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const T *__restrict__ g
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(64 * AT_WAVES) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(AttnArgs a) {
     constexpr int KT = at_tile<T>(), S = DP + tk_pad<T>();
-    __shared__ __attribute__((aligned(16))) T Ks[KT * S];
-    __shared__ __attribute__((aligned(16))) T Vs[KT * S];
+    __shared__ __attribute__((aligned(16))) T Ks[2][KT * S];
+    __shared__ __attribute__((aligned(16))) T Vs[2][KT * S];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int b = blockIdx.z / a.nsplit, sp = blockIdx.z - b * a.nsplit, grp = a.H / a.Hk;
     const int hb = blockIdx.y * (a.pack ? grp : 1), hk = hb / grp, nrows = a.pack ? grp * a.Tq : a.Tq;
@@ -294,24 +359,43 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dq_kernel(AttnArgs a) {
     const T *kb = (const T *)a.k + b * a.ks[0] + hk * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + hk * a.vs[2];
     const unsigned char *mrow = a.mask ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
     const unsigned char *mkey = a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
+    const int lim_all = a.mask ? 0 : at_wave_min(w.lim);
+    AtStage<T, DP, KT> ks, vs;
+    const auto load = [&](int j) {
+        ks.load(kb, a.ks[1], j, j1, a.Dk, a.vk, tid, [&](int t) { return mkey && !mkey[t * a.ms[3]]; });
+        vs.load(vb, a.vs[1], j, j1, a.Dv, a.vv, tid, [](int) { return false; });
+    };
     tk16 acc[DP / 32] = {};
-    for (int j = j0; j < j1; j += KT) {
+    int buf = 0;
+    if (j0 < j1) {
+        load(j0);
+        ks.store(Ks[0], tid);
+        vs.store(Vs[0], tid);
+        if (j0 + KT < j1) load(j0 + KT);
+    }
+    for (int j = j0; j < j1; j += KT, buf ^= 1) {
         __syncthreads();
-        at_stage<T, DP, KT>(Ks, kb, a.ks[1], j, j1, a.Dk, a.vk, tid, [&](int t) { return mkey && !mkey[t * a.ms[3]]; });
-        at_stage<T, DP, KT>(Vs, vb, a.vs[1], j, j1, a.Dv, a.vv, tid, [](int) { return false; });
-        __syncthreads();
+        if (j + KT < j1) {
+            ks.store(Ks[buf ^ 1], tid);
+            vs.store(Vs[buf ^ 1], tid);
+            if (j + 2 * KT < j1) load(j + 2 * KT);
+        }
+        const bool whole = j + KT <= lim_all;
 #pragma unroll
         for (int n = 0; n < KT / 32; ++n) {
-            tk16 s = at_product<T, DP>(Ks, 32 * n, qf, lane);
-            const tk16 dp = at_product<T, DP>(Vs, 32 * n, gf, lane);
+            tk16 s = at_product<T, DP>(Ks[buf], 32 * n, qf, lane);
+            const tk16 dp = at_product<T, DP>(Vs[buf], 32 * n, gf, lane);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int key = j + 32 * n + at_row(e, h);
-                bool on = key < w.lim;
-                if (mrow && on) on = mrow[key * a.ms[3]];
-                s[e] = on ? __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse)) * (dp[e] - delta) : 0.f;
-            }
-            at_accumulate<T, DP>(acc, Ks, 32 * n, s, lane);
+            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse)) * (dp[e] - delta);
+            if (!whole)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int key = j + 32 * n + at_row(e, h);
+                    bool on = key < w.lim;
+                    if (mrow && on) on = mrow[key * a.ms[3]];
+                    s[e] = on ? s[e] : 0.f;
+                }
+            at_accumulate<T, DP>(acc, Ks[buf], 32 * n, s, lane);
         }
     }
     if (!w.valid) return;
@@ -326,9 +410,9 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dq_kernel(AttnArgs a) {
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
     constexpr int QT = at_tile<T>(), S = DP + tk_pad<T>();
-    __shared__ __attribute__((aligned(16))) T Qs[QT * S];
-    __shared__ __attribute__((aligned(16))) T Gs[QT * S];
-    __shared__ __attribute__((aligned(16))) float lse[QT], delta[QT];
+    __shared__ __attribute__((aligned(16))) T Qs[2][QT * S];
+    __shared__ __attribute__((aligned(16))) T Gs[2][QT * S];
+    __shared__ __attribute__((aligned(16))) float lses[2][QT], deltas[2][QT];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int b = blockIdx.z / a.nsplit, sp = blockIdx.z - b * a.nsplit, grp = a.H / a.Hk, hk = blockIdx.y;
     const int L = at_length(a, b), off = L - a.Tq, key0 = blockIdx.x * AT_ROWS, key = key0 + wave * 32 + (lane & 31);
@@ -351,36 +435,68 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
     if (key0 >= L || qt0 > nqt) qt0 = nqt;
     const int each = nqt - qt0, total = each * grp, per = (total + a.nsplit - 1) / a.nsplit;
     const int it1 = (sp + 1) * per < total ? (sp + 1) * per : total;
-    for (int it = sp * per; it < it1; ++it) {
+    // queries from here on are seen by every key of the wave
+    const int first_all = a.mask || key0 + wave * 32 + 32 > L ? 0x7fffffff : (a.causal ? key0 + wave * 32 + 31 - off : 0);
+    AtStage<T, DP, QT> qs, gs;
+    float nlse = 0.f, ndelta = 0.f;               // row tid of the tile
+    const auto load = [&](int it) {
         const int gi = it / each, i0 = (qt0 + it - gi * each) * QT, head = hk * grp + gi;
         const long long row0 = ((long long)b * a.Tq) * a.H + head;
-        __syncthreads();
-        for (int t = tid; t < QT; t += 64 * AT_WAVES) {
-            const bool in = i0 + t < a.Tq;
-            lse[t] = in ? a.lse[row0 + (long long)(i0 + t) * a.H] : INFINITY;
-            delta[t] = in ? a.delta[row0 + (long long)(i0 + t) * a.H] : 0.f;
-        }
         // rows that see nothing are zeroed: whatever stands in them stays out of the sums
         const auto dead = [&](int t) { return a.lse[row0 + (long long)t * a.H] == INFINITY; };
-        at_stage<T, DP, QT>(Qs, (const T *)a.q + b * a.qs[0] + head * a.qs[2], a.qs[1], i0, a.Tq, a.Dk, a.vq, tid, dead);
-        at_stage<T, DP, QT>(Gs, (const T *)a.g + row0 * a.Dv, (long long)a.H * a.Dv, i0, a.Tq, a.Dv, a.vo, tid, dead);
+        qs.load((const T *)a.q + b * a.qs[0] + head * a.qs[2], a.qs[1], i0, a.Tq, a.Dk, a.vq, tid, dead);
+        gs.load((const T *)a.g + row0 * a.Dv, (long long)a.H * a.Dv, i0, a.Tq, a.Dv, a.vo, tid, dead);
+        if (tid < QT) {
+            const bool in = i0 + tid < a.Tq;
+            nlse = in ? a.lse[row0 + (long long)(i0 + tid) * a.H] : INFINITY;
+            ndelta = in ? a.delta[row0 + (long long)(i0 + tid) * a.H] : 0.f;
+        }
+    };
+    const auto store = [&](int to) {
+        qs.store(Qs[to], tid);
+        gs.store(Gs[to], tid);
+        if (tid < QT) lses[to][tid] = nlse, deltas[to][tid] = ndelta;
+    };
+    int buf = 0;
+    if (sp * per < it1) {
+        load(sp * per);
+        store(0);
+        if (sp * per + 1 < it1) load(sp * per + 1);
+    }
+    for (int it = sp * per; it < it1; ++it, buf ^= 1) {
         __syncthreads();
+        if (it + 1 < it1) {
+            store(buf ^ 1);
+            if (it + 2 < it1) load(it + 2);
+        }
+        const int gi = it / each, i0 = (qt0 + it - gi * each) * QT, head = hk * grp + gi;
+        const bool whole = i0 >= first_all && i0 + QT <= a.Tq;
         const unsigned char *mcol = a.mask ? a.mask + b * a.ms[0] + head * a.ms[1] + kc * a.ms[3] : nullptr;
 #pragma unroll
         for (int n = 0; n < QT / 32; ++n) {
-            tk16 s = at_product<T, DP>(Qs, 32 * n, kf, lane);
-            tk16 dp = at_product<T, DP>(Gs, 32 * n, vf, lane);
+            tk16 s = at_product<T, DP>(Qs[buf], 32 * n, kf, lane);
+            tk16 dp = at_product<T, DP>(Gs[buf], 32 * n, vf, lane);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int t = 32 * n + at_row(e, h), i = i0 + t;
-                bool on = i >= first && i < a.Tq;
-                if (mcol && on) on = mcol[i * a.ms[2]];
-                const float p = on ? __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse[t])) : 0.f;
-                dp[e] = on ? p * (dp[e] - delta[t]) : 0.f;
-                s[e] = p;
+            for (int u = 0; u < 4; ++u) {
+                const tkf4 le = *reinterpret_cast<const tkf4 *>(&lses[buf][32 * n + 8 * u + 4 * h]), de = *reinterpret_cast<const tkf4 *>(&deltas[buf][32 * n + 8 * u + 4 * h]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = 4 * u + j;
+                    s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -le[j]));
+                    dp[e] = s[e] * (dp[e] - de[j]);
+                }
             }
-            at_accumulate<T, DP>(accv, Gs, 32 * n, s, lane);
-            at_accumulate<T, DP>(acck, Qs, 32 * n, dp, lane);
+            if (!whole)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int i = i0 + 32 * n + at_row(e, h);
+                    bool on = i >= first && i < a.Tq;
+                    if (mcol && on) on = mcol[i * a.ms[2]];
+                    s[e] = on ? s[e] : 0.f;
+                    dp[e] = on ? dp[e] : 0.f;
+                }
+            at_accumulate<T, DP>(accv, Gs[buf], 32 * n, s, lane);
+            at_accumulate<T, DP>(acck, Qs[buf], 32 * n, dp, lane);
         }
     }
     if (!valid) return;
