@@ -38,33 +38,60 @@ __device__ __forceinline__ float at_other_half(float x) { return __shfl_xor(x, 3
 __device__ __forceinline__ int at_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }   // result register -> row of the tile
 
 // A workgroup's share of one tile of the streamed side on its way to LDS: loaded into registers one tile ahead of its use, stored
-// when the buffer is free.  Rows from `end` on, and rows that `dead` names, are zeros.
-template <typename T, int DP, int ROWS>
+// when the buffer is free.  Rows from `end` on are zeros; so are rows whose flag (loaded beside them, looked at when they are stored, so that no load
+// waits for another) says that nobody looks at them.
+template <typename T, int DP, int ROWS, typename Flag>
 struct AtStage {
     static constexpr int CH = DP / 8, S = DP + tk_pad<T>(), N = (ROWS * CH + 64 * AT_WAVES - 1) / (64 * AT_WAVES);
     static constexpr bool EVEN = ROWS * CH % (64 * AT_WAVES) == 0;
     TkFrag<T> r[N];
-    template <typename Dead>
-    __device__ __forceinline__ void load(const T *base, long long st, int t0, int end, int D, bool vec, int tid, Dead dead) {
+    Flag flag[N];
+    template <typename F>
+    __device__ __forceinline__ void load(const T *base, long long st, int t0, int end, int D, bool vec, int tid, F flag_of) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + 64 * AT_WAVES * i, row = c / CH, d = (c - row * CH) * 8, t = t0 + row;
-            if ((EVEN || row < ROWS) && t < end && !dead(t)) {
+            if ((EVEN || row < ROWS) && t < end) {
                 r[i] = tk_load8(base + (long long)t * st, d, D, vec);
+                flag[i] = flag_of(t);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[i].set(j, 0.f);
             }
         }
     }
-    __device__ __forceinline__ void store(T *tile, int tid) const {
+    template <typename P>
+    __device__ __forceinline__ void store(T *tile, int tid, P dead) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + 64 * AT_WAVES * i, row = c / CH, d = (c - row * CH) * 8;
+            if (dead(flag[i]))
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[i].set(j, 0.f);
             if (EVEN || row < ROWS) tk_store8(tile + row * S + d, r[i]);
         }
     }
 };
+
+// mask bytes of one row for the 4 x 4 keys of a result (j0 = first key of the 32): word u holds keys j0 + 8 u + 4 h + {0..3}.
+// The row is read inside [0, Tk) only; keys beyond it are hidden by the row's limit.
+struct AtMask { unsigned w[4]; };
+__device__ __forceinline__ AtMask at_mask_row(const AttnArgs &a, const unsigned char *row, int j0, int h) {
+    AtMask m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int key = j0 + 8 * u + 4 * h;
+        if (a.ms[3] == 1 && key + 3 < a.Tk) {
+            __builtin_memcpy(&m.w[u], row + key, 4);
+        } else {
+            m.w[u] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m.w[u] |= key + j < a.Tk ? (unsigned)row[(key + j) * a.ms[3]] << (8 * j) : 0u;
+        }
+    }
+    return m;
+}
+__device__ __forceinline__ bool at_mask_on(const AtMask &m, int e) { return (m.w[e >> 2] >> (8 * (e & 3))) & 0xffu; }
 
 // acc(32 rows of the tile x 32 own columns) = tile rows . own fragments
 template <typename T, int DP>
@@ -198,10 +225,14 @@ __global__ __launch_bounds__(64 * AT_WAVES, 2) void attn_fwd_kernel(AttnArgs a) 
     const unsigned char *mrow = a.mask ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
     // a mask that hides a key from every query of this workgroup takes the value row out too: 0 x NaN would be NaN
     const unsigned char *mkey = a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
-    AtStage<T, DP, KT> ks, vs;
+    AtStage<T, DP, KT, unsigned char> ks, vs;
     const auto load = [&](int j) {
-        ks.load(kb, a.ks[1], j, j1, a.Dk, a.vk, tid, [](int) { return false; });
-        vs.load(vb, a.vs[1], j, j1, a.Dv, a.vv, tid, [&](int t) { return mkey && !mkey[t * a.ms[3]]; });
+        ks.load(kb, a.ks[1], j, j1, a.Dk, a.vk, tid, [](int) { return (unsigned char)1; });
+        vs.load(vb, a.vs[1], j, j1, a.Dv, a.vv, tid, [&](int t) { return mkey ? mkey[t * a.ms[3]] : (unsigned char)1; });
+    };
+    const auto store = [&](int to) {
+        ks.store(Ks[to], tid, [](unsigned char) { return false; });
+        vs.store(Vs[to], tid, [&](unsigned char f) { return mkey && !f; });
     };
 
     tk16 acc[DP / 32] = {};
@@ -210,18 +241,20 @@ __global__ __launch_bounds__(64 * AT_WAVES, 2) void attn_fwd_kernel(AttnArgs a) 
     int buf = 0;
     if (j0 < j1) {
         load(j0);
-        ks.store(Ks[0], tid);
-        vs.store(Vs[0], tid);
+        store(0);
         if (j0 + KT < j1) load(j0 + KT);
     }
     for (int j = j0; j < j1; j += KT, buf ^= 1) {
         __syncthreads();
         if (j + KT < j1) {
-            ks.store(Ks[buf ^ 1], tid);
-            vs.store(Vs[buf ^ 1], tid);
+            store(buf ^ 1);
             if (j + 2 * KT < j1) load(j + 2 * KT);
         }
         tk16 s[KT / 32];
+        AtMask mk[KT / 32];
+        if (mrow)
+#pragma unroll
+            for (int n = 0; n < KT / 32; ++n) mk[n] = at_mask_row(a, mrow, j + 32 * n, h);
 #pragma unroll
         for (int n = 0; n < KT / 32; ++n) s[n] = at_product<T, DP>(Ks[buf], 32 * n, qf, lane);
         if (j + KT > lim_all) {
@@ -229,9 +262,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, 2) void attn_fwd_kernel(AttnArgs a) 
             for (int n = 0; n < KT / 32; ++n)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const int key = j + 32 * n + at_row(e, h);
-                    bool on = key < w.lim;
-                    if (mrow && on) on = mrow[key * a.ms[3]];
+                    const bool on = j + 32 * n + at_row(e, h) < w.lim && (!mrow || at_mask_on(mk[n], e));
                     s[n][e] = on ? s[n][e] : -INFINITY;
                 }
         }
@@ -360,29 +391,33 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
     const unsigned char *mrow = a.mask ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
     const unsigned char *mkey = a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
     const int lim_all = a.mask ? 0 : at_wave_min(w.lim);
-    AtStage<T, DP, KT> ks, vs;
+    AtStage<T, DP, KT, unsigned char> ks, vs;
     const auto load = [&](int j) {
-        ks.load(kb, a.ks[1], j, j1, a.Dk, a.vk, tid, [&](int t) { return mkey && !mkey[t * a.ms[3]]; });
-        vs.load(vb, a.vs[1], j, j1, a.Dv, a.vv, tid, [](int) { return false; });
+        ks.load(kb, a.ks[1], j, j1, a.Dk, a.vk, tid, [&](int t) { return mkey ? mkey[t * a.ms[3]] : (unsigned char)1; });
+        vs.load(vb, a.vs[1], j, j1, a.Dv, a.vv, tid, [](int) { return (unsigned char)1; });
+    };
+    const auto store = [&](int to) {
+        ks.store(Ks[to], tid, [&](unsigned char f) { return mkey && !f; });
+        vs.store(Vs[to], tid, [](unsigned char) { return false; });
     };
     tk16 acc[DP / 32] = {};
     int buf = 0;
     if (j0 < j1) {
         load(j0);
-        ks.store(Ks[0], tid);
-        vs.store(Vs[0], tid);
+        store(0);
         if (j0 + KT < j1) load(j0 + KT);
     }
     for (int j = j0; j < j1; j += KT, buf ^= 1) {
         __syncthreads();
         if (j + KT < j1) {
-            ks.store(Ks[buf ^ 1], tid);
-            vs.store(Vs[buf ^ 1], tid);
+            store(buf ^ 1);
             if (j + 2 * KT < j1) load(j + 2 * KT);
         }
         const bool whole = j + KT <= lim_all;
 #pragma unroll
         for (int n = 0; n < KT / 32; ++n) {
+            AtMask mk;
+            if (mrow) mk = at_mask_row(a, mrow, j + 32 * n, h);
             tk16 s = at_product<T, DP>(Ks[buf], 32 * n, qf, lane);
             const tk16 dp = at_product<T, DP>(Vs[buf], 32 * n, gf, lane);
 #pragma unroll
@@ -390,9 +425,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
             if (!whole)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const int key = j + 32 * n + at_row(e, h);
-                    bool on = key < w.lim;
-                    if (mrow && on) on = mrow[key * a.ms[3]];
+                    const bool on = j + 32 * n + at_row(e, h) < w.lim && (!mrow || at_mask_on(mk, e));
                     s[e] = on ? s[e] : 0.f;
                 }
             at_accumulate<T, DP>(acc, Ks[buf], 32 * n, s, lane);
@@ -437,15 +470,14 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
     const int it1 = (sp + 1) * per < total ? (sp + 1) * per : total;
     // queries from here on are seen by every key of the wave
     const int first_all = a.mask || key0 + wave * 32 + 32 > L ? 0x7fffffff : (a.causal ? key0 + wave * 32 + 31 - off : 0);
-    AtStage<T, DP, QT> qs, gs;
+    AtStage<T, DP, QT, float> qs, gs;
     float nlse = 0.f, ndelta = 0.f;               // row tid of the tile
     const auto load = [&](int it) {
         const int gi = it / each, i0 = (qt0 + it - gi * each) * QT, head = hk * grp + gi;
         const long long row0 = ((long long)b * a.Tq) * a.H + head;
-        // rows that see nothing are zeroed: whatever stands in them stays out of the sums
-        const auto dead = [&](int t) { return a.lse[row0 + (long long)t * a.H] == INFINITY; };
-        qs.load((const T *)a.q + b * a.qs[0] + head * a.qs[2], a.qs[1], i0, a.Tq, a.Dk, a.vq, tid, dead);
-        gs.load((const T *)a.g + row0 * a.Dv, (long long)a.H * a.Dv, i0, a.Tq, a.Dv, a.vo, tid, dead);
+        const auto flag = [&](int t) { return a.lse[row0 + (long long)t * a.H]; };
+        qs.load((const T *)a.q + b * a.qs[0] + head * a.qs[2], a.qs[1], i0, a.Tq, a.Dk, a.vq, tid, flag);
+        gs.load((const T *)a.g + row0 * a.Dv, (long long)a.H * a.Dv, i0, a.Tq, a.Dv, a.vo, tid, flag);
         if (tid < QT) {
             const bool in = i0 + tid < a.Tq;
             nlse = in ? a.lse[row0 + (long long)(i0 + tid) * a.H] : INFINITY;
@@ -453,8 +485,10 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
         }
     };
     const auto store = [&](int to) {
-        qs.store(Qs[to], tid);
-        gs.store(Gs[to], tid);
+        // rows that see nothing are zeroed: whatever stands in them stays out of the sums
+        const auto dead = [](float f) { return f == INFINITY; };
+        qs.store(Qs[to], tid, dead);
+        gs.store(Gs[to], tid, dead);
         if (tid < QT) lses[to][tid] = nlse, deltas[to][tid] = ndelta;
     };
     int buf = 0;
@@ -474,6 +508,10 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
         const unsigned char *mcol = a.mask ? a.mask + b * a.ms[0] + head * a.ms[1] + kc * a.ms[3] : nullptr;
 #pragma unroll
         for (int n = 0; n < QT / 32; ++n) {
+            unsigned char mk[16];
+            if (mcol)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mk[e] = mcol[min(i0 + 32 * n + at_row(e, h), a.Tq - 1) * a.ms[2]];
             tk16 s = at_product<T, DP>(Qs[buf], 32 * n, kf, lane);
             tk16 dp = at_product<T, DP>(Gs[buf], 32 * n, vf, lane);
 #pragma unroll
@@ -490,8 +528,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int i = i0 + 32 * n + at_row(e, h);
-                    bool on = i >= first && i < a.Tq;
-                    if (mcol && on) on = mcol[i * a.ms[2]];
+                    const bool on = i >= first && i < a.Tq && (!mcol || mk[e]);
                     s[e] = on ? s[e] : 0.f;
                     dp[e] = on ? dp[e] : 0.f;
                 }
