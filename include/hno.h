@@ -609,7 +609,7 @@ int hno_affine_nearest(const float *x, float *out, const double *matrix12, float
  *
  * hno_attn_fwd: out (B, Tq, H, Dv) = softmax(scale q k^T) v per head over the visible keys; a row without any is zero.
  *   q (B, Tq, H, Dk), k (B, Tk, Hk, Dk), v (B, Tk, Hk, Dv) with element strides of (batch, token, head) and unit stride of the last axis; query head h
- *   reads key head h / (H / Hk).  Head sizes 1 ... 128.  With L = kv_lens[b] (clamped to 0 ... Tk; NULL: Tk), key j is visible to query i when
+ *   reads key head h / (H / Hk).  Head sizes: multiples of 8 up to 128; every row starts on 16 bytes.  With L = kv_lens[b] (clamped to 0 ... Tk; NULL: Tk), key j is visible to query i when
  *   j < L, and j <= i + L - Tq if causal (the last query is aligned with the last key), and mask[b, h, i, j] != 0 (NULL: all; strides of 0 broadcast).
  *   Rows of k and v from L on, and those that a mask without query and head axis hides, are not looked at: they may hold anything.  Value rows that
  *   only some queries may see have to be finite.

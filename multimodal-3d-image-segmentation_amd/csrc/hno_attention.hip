@@ -22,7 +22,7 @@ struct AttnArgs {
     const unsigned char *mask;
     const int *lens;
     long long qs[3], ks[3], vs[3], ms[4];     // element strides of (batch, token, head); the mask's of (batch, head, query, key)
-    int B, Tq, Tk, H, Hk, Dk, Dv, causal, nsplit, pack, vq, vk, vv, vo, keymask;
+    int B, Tq, Tk, H, Hk, Dk, Dv, causal, nsplit, tiles, pack, keymask;
     float scale2, scale;                       // scale log2(e), scale
 };
 
@@ -37,22 +37,63 @@ __device__ __forceinline__ int at_length(const AttnArgs &a, int b) {
 __device__ __forceinline__ float at_other_half(float x) { return __shfl_xor(x, 32); }
 __device__ __forceinline__ int at_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }   // result register -> row of the tile
 
+// Where element d (a multiple of 4) of row `row` stands in an LDS tile of DP channels.  bf16: rows without padding whose 16-byte chunks change places, so
+// that 16 consecutive rows read at one chunk (row reads) and 4 consecutive rows read at four neighbouring chunks (transposed reads)
+// touch 64 different banks each; with padded rows the transposed reads met 4-way conflicts (dk / dv of 2x16x4096x128: XX us).
+// DP = 96: a row is 3/4 of the banks, rows shift by themselves and the chunks rotate by row / 4; else an exclusive or.
+template <int DP>
+__device__ __forceinline__ int at_at(const tkh *, int row, int d) {
+    const int c = d >> 3;
+    int slot;
+    if constexpr (DP == 128) slot = c ^ (((row & 3) << 2) | ((row >> 2) & 3));
+    else if constexpr (DP == 64) slot = c ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3));
+    else if constexpr (DP == 32) slot = c ^ ((row >> 2) & 3);
+    else slot = c + ((row >> 2) & 3) - (c + ((row >> 2) & 3) >= 12 ? 12 : 0);
+    return row * DP + slot * 8 + (d & 7);
+}
+template <int DP>
+__device__ __forceinline__ int at_at(const float *, int row, int d) { return row * (DP + 4) + d; }
+template <typename T, int DP> constexpr int at_stride() { return sizeof(T) == 2 ? DP : DP + 4; }
+// the fragment of the transposed tile: channel 32 dt + (lane & 31), rows r0 .. r0 + 3 and r0 + 8 .. r0 + 11
+template <int DP>
+__device__ __forceinline__ TkFrag<tkh> at_col(const tkh *tile, int dt, int r0, int lane) {
+    typedef __attribute__((address_space(3))) tks4 *lds4;
+    const int row = r0 + ((lane & 15) >> 2), d = 32 * dt + (lane & 16) + 4 * (lane & 3);
+    const tks4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(tile + at_at<DP>(tile, row, d)));
+    const tks4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(tile + at_at<DP>(tile, row + 8, d)));
+    return {__builtin_bit_cast(tkb8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7))};
+}
+template <int DP>
+__device__ __forceinline__ TkFrag<float> at_col(const float *tile, int dt, int r0, int lane) {
+    return tk_col(tile, DP + 4, 32 * dt, r0, r0 + 8, lane);
+}
+
+// 8 channels of a row (D % 8 == 0, 16-byte aligned: checked by the entry points); channels from D on are zeros
+template <typename T>
+__device__ __forceinline__ TkFrag<T> at_load8(const T *row, int d, int D) {
+    if (d < D) return tk_row(row + d);
+    TkFrag<T> f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f.set(j, 0.f);
+    return f;
+}
+
 // A workgroup's share of one tile of the streamed side on its way to LDS: loaded into registers one tile ahead of its use, stored
 // when the buffer is free.  Rows from `end` on are zeros; so are rows whose flag (loaded beside them, looked at when they are stored, so that no load
 // waits for another) says that nobody looks at them.
 template <typename T, int DP, int ROWS, typename Flag>
 struct AtStage {
-    static constexpr int CH = DP / 8, S = DP + tk_pad<T>(), N = (ROWS * CH + 64 * AT_WAVES - 1) / (64 * AT_WAVES);
+    static constexpr int CH = DP / 8, N = (ROWS * CH + 64 * AT_WAVES - 1) / (64 * AT_WAVES);
     static constexpr bool EVEN = ROWS * CH % (64 * AT_WAVES) == 0;
     TkFrag<T> r[N];
     Flag flag[N];
     template <typename F>
-    __device__ __forceinline__ void load(const T *base, long long st, int t0, int end, int D, bool vec, int tid, F flag_of) {
+    __device__ __forceinline__ void load(const T *base, long long st, int t0, int end, int D, int tid, F flag_of) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int c = tid + 64 * AT_WAVES * i, row = c / CH, d = (c - row * CH) * 8, t = t0 + row;
             if ((EVEN || row < ROWS) && t < end) {
-                r[i] = tk_load8(base + (long long)t * st, d, D, vec);
+                r[i] = at_load8(base + (long long)t * st, d, D);
                 flag[i] = flag_of(t);
             } else {
 #pragma unroll
@@ -68,7 +109,7 @@ struct AtStage {
             if (dead(flag[i]))
 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[i].set(j, 0.f);
-            if (EVEN || row < ROWS) tk_store8(tile + row * S + d, r[i]);
+            if (EVEN || row < ROWS) tk_store8(tile + at_at<DP>(tile, row, d), r[i]);
         }
     }
 };
@@ -96,59 +137,66 @@ __device__ __forceinline__ bool at_mask_on(const AtMask &m, int e) { return (m.w
 // acc(32 rows of the tile x 32 own columns) = tile rows . own fragments
 template <typename T, int DP>
 __device__ __forceinline__ tk16 at_product(const T *tile, int row0, const TkFrag<T> (&own)[DP / 16], int lane) {
-    constexpr int S = DP + tk_pad<T>();
-    const T *p = tile + (row0 + (lane & 31)) * S + 8 * (lane >> 5);
     tk16 acc = {};
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) acc = tk_mma(tk_row(p + 16 * kk), own[kk], acc);
+    for (int kk = 0; kk < DP / 16; ++kk) acc = tk_mma(tk_row(tile + at_at<DP>(tile, row0 + (lane & 31), 16 * kk + 8 * (lane >> 5))), own[kk], acc);
     return acc;
 }
 // acc[dt] += (tile rows row0 .. row0 + 31)^T . w, w being a result over the same rows
 template <typename T, int DP>
 __device__ __forceinline__ void at_accumulate(tk16 (&acc)[DP / 32], const T *tile, int row0, const tk16 &w, int lane) {
-    constexpr int S = DP + tk_pad<T>();
-    const int h = lane >> 5;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         TkFrag<T> f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) f.set(j, w[8 * t + j]);
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt)
-            acc[dt] = tk_mma(tk_col(tile, S, 32 * dt, row0 + 16 * t + 4 * h, row0 + 16 * t + 8 + 4 * h, lane), f, acc[dt]);
+        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = tk_mma(at_col<DP>(tile, dt, row0 + 16 * t + 4 * (lane >> 5), lane), f, acc[dt]);
     }
 }
 
 // store a transposed accumulator (register = channel, lane = row) as row `dst` of a contiguous tensor
 template <typename T, int DP, typename F>
-__device__ __forceinline__ void at_store(T *dst, const tk16 (&acc)[DP / 32], int D, bool vec, int h, F value) {
+__device__ __forceinline__ void at_store(T *dst, const tk16 (&acc)[DP / 32], int D, int h, F value) {
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int d = 32 * dt + 8 * u + 4 * h;
-            float x[4];
+            if (d >= D) continue;
+            if constexpr (sizeof(T) == 2) {
+                tks4 w;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = value(acc[dt][4 * u + j]);
-            if (vec && d < D) {
-                if constexpr (sizeof(T) == 2) {
-                    tks4 w;
+                for (int j = 0; j < 4; ++j) w[j] = (short)tk_down<T>(value(acc[dt][4 * u + j]));
+                *reinterpret_cast<tks4 *>(dst + d) = w;
+            } else {
+                tkf4 w;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) w[j] = (short)tk_down<T>(x[j]);
-                    *reinterpret_cast<tks4 *>(dst + d) = w;
-                } else {
-                    *reinterpret_cast<tkf4 *>(dst + d) = tkf4{x[0], x[1], x[2], x[3]};
-                }
-            } else if (!vec) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (d + j < D) dst[d + j] = tk_down<T>(x[j]);
+                for (int j = 0; j < 4; ++j) w[j] = value(acc[dt][4 * u + j]);
+                *reinterpret_cast<tkf4 *>(dst + d) = w;
             }
         }
 }
 
+// Workgroup -> work.  The 8 XCDs take workgroups in turn and each has its own L2: every XCD gets one run of the list
+// key head x batch x tile x (head of the group, split), so the workgroups that stream the same keys (or queries) share an L2, and an XCD
+// meets batch entries of several lengths.  The tiles that see most come first, where a causal mask makes them unequal.
+struct AtBlock {
+    int b, hk, tile, gi, sp;
+};
+__device__ __forceinline__ AtBlock at_block(const AttnArgs &a, int grp) {
+    const int n = gridDim.x, xcd = blockIdx.x & 7, each = n >> 3, more = n & 7;
+    int at = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
+    AtBlock w;
+    w.sp = at % a.nsplit, at /= a.nsplit;
+    w.gi = at % grp, at /= grp;
+    w.tile = at % a.tiles, at /= a.tiles;
+    w.b = at % a.B;
+    w.hk = at / a.B;
+    return w;
+}
 // ------------------------------------------------------------------ rows of the query side
-// Workgroup (tile, head, batch x split).  Where few new tokens share a key head (pack), the rows of all its query heads form one list, so
+// Where few new tokens share a key head (pack), the rows of all its query heads form one list, so
 // the keys are read once: row r stands for query r % Tq of head hb + r / Tq.
 struct AtRow {
     int head, i, lim;       // query head, query, and the first key that it does not see
@@ -203,36 +251,36 @@ __device__ __forceinline__ void at_weights(TkFrag<float> &f, const tk16 &s, int 
     }
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(64 * AT_WAVES, 2) void attn_fwd_kernel(AttnArgs a) {
-    constexpr int KT = at_tile<T>(), S = DP + tk_pad<T>();
+template <typename T, int DP, bool MASK>
+__global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void attn_fwd_kernel(AttnArgs a) {
+    constexpr int KT = at_tile<T>(), S = at_stride<T, DP>();
     __shared__ __attribute__((aligned(16))) T Ks[2][KT * S];
     __shared__ __attribute__((aligned(16))) T Vs[2][KT * S];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const int b = blockIdx.z / a.nsplit, sp = blockIdx.z - b * a.nsplit, grp = a.H / a.Hk;
-    const int hb = blockIdx.y * (a.pack ? grp : 1), hk = hb / grp, nrows = a.pack ? grp * a.Tq : a.Tq;
-    const int L = at_length(a, b), r0 = blockIdx.x * AT_ROWS, r = r0 + wave * 32 + (lane & 31);
+    const AtBlock w0 = at_block(a, a.pack ? 1 : a.H / a.Hk);
+    const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk, hb = hk * grp + w0.gi, nrows = a.pack ? grp * a.Tq : a.Tq;
+    const int L = at_length(a, b), r0 = (a.causal ? a.tiles - 1 - w0.tile : w0.tile) * AT_ROWS, r = r0 + wave * 32 + (lane & 31);
     const AtRow w = at_query_row(a, r, hb, nrows, L);
     int j0, j1;
     at_key_range(a, L, (r0 + AT_ROWS < nrows ? r0 + AT_ROWS : nrows) - 1, nrows, sp, KT, j0, j1);
-    const int lim_all = a.mask ? 0 : at_wave_min(w.lim);
+    const int lim_all = MASK ? 0 : at_wave_min(w.lim);
 
     TkFrag<T> qf[DP / 16];
     const T *qrow = (const T *)a.q + b * a.qs[0] + (long long)w.i * a.qs[1] + w.head * a.qs[2];
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) qf[kk] = tk_load8(qrow, 16 * kk + 8 * h, a.Dk, a.vq);
+    for (int kk = 0; kk < DP / 16; ++kk) qf[kk] = at_load8(qrow, 16 * kk + 8 * h, a.Dk);
     const T *kb = (const T *)a.k + b * a.ks[0] + hk * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + hk * a.vs[2];
-    const unsigned char *mrow = a.mask ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
+    const unsigned char *mrow = MASK ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
     // a mask that hides a key from every query of this workgroup takes the value row out too: 0 x NaN would be NaN
-    const unsigned char *mkey = a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
+    const unsigned char *mkey = MASK && a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
     AtStage<T, DP, KT, unsigned char> ks, vs;
     const auto load = [&](int j) {
-        ks.load(kb, a.ks[1], j, j1, a.Dk, a.vk, tid, [](int) { return (unsigned char)1; });
-        vs.load(vb, a.vs[1], j, j1, a.Dv, a.vv, tid, [&](int t) { return mkey ? mkey[t * a.ms[3]] : (unsigned char)1; });
+        ks.load(kb, a.ks[1], j, j1, a.Dk, tid, [](int) { return (unsigned char)1; });
+        vs.load(vb, a.vs[1], j, j1, a.Dv, tid, [&](int t) { return MASK && mkey ? mkey[t * a.ms[3]] : (unsigned char)1; });
     };
     const auto store = [&](int to) {
         ks.store(Ks[to], tid, [](unsigned char) { return false; });
-        vs.store(Vs[to], tid, [&](unsigned char f) { return mkey && !f; });
+        vs.store(Vs[to], tid, [&](unsigned char f) { return MASK && mkey && !f; });
     };
 
     tk16 acc[DP / 32] = {};
@@ -252,7 +300,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, 2) void attn_fwd_kernel(AttnArgs a) 
         }
         tk16 s[KT / 32];
         AtMask mk[KT / 32];
-        if (mrow)
+        if (MASK)
 #pragma unroll
             for (int n = 0; n < KT / 32; ++n) mk[n] = at_mask_row(a, mrow, j + 32 * n, h);
 #pragma unroll
@@ -262,7 +310,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, 2) void attn_fwd_kernel(AttnArgs a) 
             for (int n = 0; n < KT / 32; ++n)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const bool on = j + 32 * n + at_row(e, h) < w.lim && (!mrow || at_mask_on(mk[n], e));
+                    const bool on = j + 32 * n + at_row(e, h) < w.lim && (!MASK || at_mask_on(mk[n], e));
                     s[n][e] = on ? s[n][e] : -INFINITY;
                 }
         }
@@ -292,7 +340,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, 2) void attn_fwd_kernel(AttnArgs a) 
                 at_weights(f, s[n], t, l);
                 const int row = 32 * n + 16 * t + 4 * h;
 #pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = tk_mma(tk_col(Vs[buf], S, 32 * dt, row, row + 8, lane), f, acc[dt]);
+                for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = tk_mma(at_col<DP>(Vs[buf], dt, row, lane), f, acc[dt]);
             }
     }
     l += at_other_half(l);
@@ -300,7 +348,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, 2) void attn_fwd_kernel(AttnArgs a) 
     const long long row = ((long long)b * a.Tq + w.i) * a.H + w.head;
     if (a.nsplit > 1) {
         const long long rows = (long long)a.B * a.Tq * a.H, at = sp * rows + row;
-        at_store<float, DP>(a.part + at * a.Dv, acc, a.Dv, a.Dv % 4 == 0, h, [](float x) { return x; });
+        at_store<float, DP>(a.part + at * a.Dv, acc, a.Dv, h, [](float x) { return x; });
         if (h == 0) {
             a.part2[2 * at] = m == -INFINITY ? m : m * a.scale2;
             a.part2[2 * at + 1] = l;
@@ -308,9 +356,9 @@ __global__ __launch_bounds__(64 * AT_WAVES, 2) void attn_fwd_kernel(AttnArgs a) 
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    at_store<T, DP>((T *)a.out + row * a.Dv, acc, a.Dv, a.vo, h, [&](float x) { return x * inv; });
+    at_store<T, DP>((T *)a.out + row * a.Dv, acc, a.Dv, h, [&](float x) { return x * inv; });
     if (sizeof(T) == 2 && a.outres)     // what the rounding of o lost: the backward pass needs D_i = do . o to more than 8 bits
-        at_store<T, DP>((T *)a.outres + row * a.Dv, acc, a.Dv, a.vo, h,
+        at_store<T, DP>((T *)a.outres + row * a.Dv, acc, a.Dv, h,
                         [&](float x) { const float y = x * inv; return y - tk_up(tk_down<T>(y)); });
     if (a.lse && h == 0) a.lse[row] = m == -INFINITY ? INFINITY : m * a.scale2 + __builtin_amdgcn_logf(l);   // +inf: an empty row
 }
@@ -349,15 +397,15 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float *__restrict_
 // D_i = sum_c do_ic o_ic.  16 lanes per row.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_delta_kernel(const T *__restrict__ g, const T *__restrict__ o, const T *__restrict__ ores,
-                                                         const float *__restrict__ lse, float *__restrict__ delta, long long rows, int D, int vec) {
+                                                         const float *__restrict__ lse, float *__restrict__ delta, long long rows, int D) {
     const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
     const int c = threadIdx.x & 15;
     float s = 0.f;
     if (row < rows && lse[row] != INFINITY)
-        for (int d = 8 * c; d < D; d += 128) {
-            const TkFrag<T> x = tk_load8(g + row * D, d, D, vec), y = tk_load8(o + row * D, d, D, vec);
+        if (const int d = 8 * c; d < D) {
+            const TkFrag<T> x = tk_row(g + row * D + d), y = tk_row(o + row * D + d);
             TkFrag<T> z = y;
-            if (ores) z = tk_load8(ores + row * D, d, D, vec);
+            if (ores) z = tk_row(ores + row * D + d);
 #pragma unroll
             for (int j = 0; j < 8; ++j) s = fmaf((float)x.v[j], ores ? (float)y.v[j] + (float)z.v[j] : (float)y.v[j], s);
         }
@@ -366,15 +414,15 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const T *__restrict__ g
     if (row < rows && c == 0) delta[row] = s;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(AttnArgs a) {
-    constexpr int KT = at_tile<T>(), S = DP + tk_pad<T>();
+    constexpr int KT = at_tile<T>(), S = at_stride<T, DP>();
     __shared__ __attribute__((aligned(16))) T Ks[2][KT * S];
     __shared__ __attribute__((aligned(16))) T Vs[2][KT * S];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const int b = blockIdx.z / a.nsplit, sp = blockIdx.z - b * a.nsplit, grp = a.H / a.Hk;
-    const int hb = blockIdx.y * (a.pack ? grp : 1), hk = hb / grp, nrows = a.pack ? grp * a.Tq : a.Tq;
-    const int L = at_length(a, b), r0 = blockIdx.x * AT_ROWS, r = r0 + wave * 32 + (lane & 31);
+    const AtBlock w0 = at_block(a, a.pack ? 1 : a.H / a.Hk);
+    const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk, hb = hk * grp + w0.gi, nrows = a.pack ? grp * a.Tq : a.Tq;
+    const int L = at_length(a, b), r0 = (a.causal ? a.tiles - 1 - w0.tile : w0.tile) * AT_ROWS, r = r0 + wave * 32 + (lane & 31);
     const AtRow w = at_query_row(a, r, hb, nrows, L);
     int j0, j1;
     at_key_range(a, L, (r0 + AT_ROWS < nrows ? r0 + AT_ROWS : nrows) - 1, nrows, sp, KT, j0, j1);
@@ -383,21 +431,21 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
     const T *qrow = (const T *)a.q + b * a.qs[0] + (long long)w.i * a.qs[1] + w.head * a.qs[2], *grow = (const T *)a.g + row * a.Dv;
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
-        qf[kk] = tk_load8(qrow, 16 * kk + 8 * h, a.Dk, a.vq);
-        gf[kk] = tk_load8(grow, 16 * kk + 8 * h, a.Dv, a.vo);
+        qf[kk] = at_load8(qrow, 16 * kk + 8 * h, a.Dk);
+        gf[kk] = at_load8(grow, 16 * kk + 8 * h, a.Dv);
     }
     const float lse = a.lse[row], delta = a.delta[row];
     const T *kb = (const T *)a.k + b * a.ks[0] + hk * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + hk * a.vs[2];
-    const unsigned char *mrow = a.mask ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
-    const unsigned char *mkey = a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
-    const int lim_all = a.mask ? 0 : at_wave_min(w.lim);
+    const unsigned char *mrow = MASK ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
+    const unsigned char *mkey = MASK && a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
+    const int lim_all = MASK ? 0 : at_wave_min(w.lim);
     AtStage<T, DP, KT, unsigned char> ks, vs;
     const auto load = [&](int j) {
-        ks.load(kb, a.ks[1], j, j1, a.Dk, a.vk, tid, [&](int t) { return mkey ? mkey[t * a.ms[3]] : (unsigned char)1; });
-        vs.load(vb, a.vs[1], j, j1, a.Dv, a.vv, tid, [](int) { return (unsigned char)1; });
+        ks.load(kb, a.ks[1], j, j1, a.Dk, tid, [&](int t) { return MASK && mkey ? mkey[t * a.ms[3]] : (unsigned char)1; });
+        vs.load(vb, a.vs[1], j, j1, a.Dv, tid, [](int) { return (unsigned char)1; });
     };
     const auto store = [&](int to) {
-        ks.store(Ks[to], tid, [&](unsigned char f) { return mkey && !f; });
+        ks.store(Ks[to], tid, [&](unsigned char f) { return MASK && mkey && !f; });
         vs.store(Vs[to], tid, [](unsigned char) { return false; });
     };
     tk16 acc[DP / 32] = {};
@@ -417,7 +465,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
 #pragma unroll
         for (int n = 0; n < KT / 32; ++n) {
             AtMask mk;
-            if (mrow) mk = at_mask_row(a, mrow, j + 32 * n, h);
+            if (MASK) mk = at_mask_row(a, mrow, j + 32 * n, h);
             tk16 s = at_product<T, DP>(Ks[buf], 32 * n, qf, lane);
             const tk16 dp = at_product<T, DP>(Vs[buf], 32 * n, gf, lane);
 #pragma unroll
@@ -425,7 +473,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
             if (!whole)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const bool on = j + 32 * n + at_row(e, h) < w.lim && (!mrow || at_mask_on(mk, e));
+                    const bool on = j + 32 * n + at_row(e, h) < w.lim && (!MASK || at_mask_on(mk, e));
                     s[e] = on ? s[e] : 0.f;
                 }
             at_accumulate<T, DP>(acc, Ks[buf], 32 * n, s, lane);
@@ -434,21 +482,22 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
     if (!w.valid) return;
     if (a.nsplit > 1) {
         const long long rows = (long long)a.B * a.Tq * a.H;
-        at_store<float, DP>(a.part + (sp * rows + row) * a.Dk, acc, a.Dk, a.Dk % 4 == 0, h, [&](float x) { return x * a.scale; });
+        at_store<float, DP>(a.part + (sp * rows + row) * a.Dk, acc, a.Dk, h, [&](float x) { return x * a.scale; });
         return;
     }
-    at_store<T, DP>((T *)a.dq + row * a.Dk, acc, a.Dk, a.Dk % 8 == 0, h, [&](float x) { return x * a.scale; });
+    at_store<T, DP>((T *)a.dq + row * a.Dk, acc, a.Dk, h, [&](float x) { return x * a.scale; });
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
-    constexpr int QT = at_tile<T>(), S = DP + tk_pad<T>();
+    constexpr int QT = at_tile<T>(), S = at_stride<T, DP>();
     __shared__ __attribute__((aligned(16))) T Qs[2][QT * S];
     __shared__ __attribute__((aligned(16))) T Gs[2][QT * S];
     __shared__ __attribute__((aligned(16))) float lses[2][QT], deltas[2][QT];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const int b = blockIdx.z / a.nsplit, sp = blockIdx.z - b * a.nsplit, grp = a.H / a.Hk, hk = blockIdx.y;
-    const int L = at_length(a, b), off = L - a.Tq, key0 = blockIdx.x * AT_ROWS, key = key0 + wave * 32 + (lane & 31);
+    const AtBlock w0 = at_block(a, 1);
+    const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk;
+    const int L = at_length(a, b), off = L - a.Tq, key0 = w0.tile * AT_ROWS, key = key0 + wave * 32 + (lane & 31);
     const bool valid = key < a.Tk;
     const int kc = valid ? key : a.Tk - 1;
     // queries that see this key: [first, Tq)
@@ -458,8 +507,8 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
     const T *vrow = (const T *)a.v + b * a.vs[0] + (long long)kc * a.vs[1] + hk * a.vs[2];
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
-        kf[kk] = tk_load8(krow, 16 * kk + 8 * h, a.Dk, a.vk);
-        vf[kk] = tk_load8(vrow, 16 * kk + 8 * h, a.Dv, a.vv);
+        kf[kk] = at_load8(krow, 16 * kk + 8 * h, a.Dk);
+        vf[kk] = at_load8(vrow, 16 * kk + 8 * h, a.Dv);
     }
     tk16 acck[DP / 32] = {}, accv[DP / 32] = {};
     // the list of (head of the group, query tile) that sees any key of this tile, cut into nsplit runs
@@ -469,15 +518,15 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
     const int each = nqt - qt0, total = each * grp, per = (total + a.nsplit - 1) / a.nsplit;
     const int it1 = (sp + 1) * per < total ? (sp + 1) * per : total;
     // queries from here on are seen by every key of the wave
-    const int first_all = a.mask || key0 + wave * 32 + 32 > L ? 0x7fffffff : (a.causal ? key0 + wave * 32 + 31 - off : 0);
+    const int first_all = MASK || key0 + wave * 32 + 32 > L ? 0x7fffffff : (a.causal ? key0 + wave * 32 + 31 - off : 0);
     AtStage<T, DP, QT, float> qs, gs;
     float nlse = 0.f, ndelta = 0.f;               // row tid of the tile
     const auto load = [&](int it) {
         const int gi = it / each, i0 = (qt0 + it - gi * each) * QT, head = hk * grp + gi;
         const long long row0 = ((long long)b * a.Tq) * a.H + head;
         const auto flag = [&](int t) { return a.lse[row0 + (long long)t * a.H]; };
-        qs.load((const T *)a.q + b * a.qs[0] + head * a.qs[2], a.qs[1], i0, a.Tq, a.Dk, a.vq, tid, flag);
-        gs.load((const T *)a.g + row0 * a.Dv, (long long)a.H * a.Dv, i0, a.Tq, a.Dv, a.vo, tid, flag);
+        qs.load((const T *)a.q + b * a.qs[0] + head * a.qs[2], a.qs[1], i0, a.Tq, a.Dk, tid, flag);
+        gs.load((const T *)a.g + row0 * a.Dv, (long long)a.H * a.Dv, i0, a.Tq, a.Dv, tid, flag);
         if (tid < QT) {
             const bool in = i0 + tid < a.Tq;
             nlse = in ? a.lse[row0 + (long long)(i0 + tid) * a.H] : INFINITY;
@@ -505,11 +554,11 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
         }
         const int gi = it / each, i0 = (qt0 + it - gi * each) * QT, head = hk * grp + gi;
         const bool whole = i0 >= first_all && i0 + QT <= a.Tq;
-        const unsigned char *mcol = a.mask ? a.mask + b * a.ms[0] + head * a.ms[1] + kc * a.ms[3] : nullptr;
+        const unsigned char *mcol = MASK ? a.mask + b * a.ms[0] + head * a.ms[1] + kc * a.ms[3] : nullptr;
 #pragma unroll
         for (int n = 0; n < QT / 32; ++n) {
             unsigned char mk[16];
-            if (mcol)
+            if (MASK)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) mk[e] = mcol[min(i0 + 32 * n + at_row(e, h), a.Tq - 1) * a.ms[2]];
             tk16 s = at_product<T, DP>(Qs[buf], 32 * n, kf, lane);
@@ -528,7 +577,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int i = i0 + 32 * n + at_row(e, h);
-                    const bool on = i >= first && i < a.Tq && (!mcol || mk[e]);
+                    const bool on = i >= first && i < a.Tq && (!MASK || mk[e]);
                     s[e] = on ? s[e] : 0.f;
                     dp[e] = on ? dp[e] : 0.f;
                 }
@@ -540,12 +589,12 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
     const long long row = ((long long)b * a.Tk + key) * a.Hk + hk;
     if (a.nsplit > 1) {
         const long long at = sp * ((long long)a.B * a.Tk * a.Hk) + row;
-        at_store<float, DP>(a.part + at * a.Dk, acck, a.Dk, a.Dk % 4 == 0, h, [&](float x) { return x * a.scale; });
-        at_store<float, DP>(a.part2 + at * a.Dv, accv, a.Dv, a.Dv % 4 == 0, h, [](float x) { return x; });
+        at_store<float, DP>(a.part + at * a.Dk, acck, a.Dk, h, [&](float x) { return x * a.scale; });
+        at_store<float, DP>(a.part2 + at * a.Dv, accv, a.Dv, h, [](float x) { return x; });
         return;
     }
-    at_store<T, DP>((T *)a.dk + row * a.Dk, acck, a.Dk, a.Dk % 8 == 0, h, [&](float x) { return x * a.scale; });
-    at_store<T, DP>((T *)a.dv + row * a.Dv, accv, a.Dv, a.Dv % 8 == 0, h, [](float x) { return x; });
+    at_store<T, DP>((T *)a.dk + row * a.Dk, acck, a.Dk, h, [&](float x) { return x * a.scale; });
+    at_store<T, DP>((T *)a.dv + row * a.Dv, accv, a.Dv, h, [](float x) { return x; });
 }
 
 // out = sum over splits, in split order
@@ -586,6 +635,7 @@ static AtPlan at_plan(const hno_attn_t *p) {
 }
 static size_t at_pad(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
+static bool at_aligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static int at_check(const hno_attn_t *p, const char *what) {
     HNO_REQUIRE(p, "%s: null argument", what);
     HNO_REQUIRE(p->dtype == HNO_F32 || p->dtype == HNO_BF16, "%s: dtype %d is neither HNO_F32 nor HNO_BF16", what, p->dtype);
@@ -593,45 +643,44 @@ static int at_check(const hno_attn_t *p, const char *what) {
     HNO_REQUIRE(p->H % p->Hk == 0, "%s: %d query heads do not share %d key heads evenly", what, p->H, p->Hk);
     HNO_REQUIRE(p->scale > 0.f && p->scale < 3e38f, "%s: scale must be positive and finite", what);
     if (p->Dk > 128 || p->Dv > 128) return fail(HNO_ELIMIT, "%s: head sizes %d, %d exceed 128", what, p->Dk, p->Dv);
-    if (p->H > 65535 || p->B > 64000) return fail(HNO_ELIMIT, "%s: %d heads or a batch of %d exceed the grid", what, p->H, p->B);
+    if ((double)p->B * p->H * (ceil_div(p->Tq, AT_ROWS) + ceil_div(p->Tk, AT_ROWS)) > 1e8) return fail(HNO_ELIMIT, "%s: the grid is too large", what);
     if (p->Tq > (1 << 28) || p->Tk > (1 << 28) || (long long)(p->H / p->Hk) * p->Tq > (1ll << 30)) return fail(HNO_ELIMIT, "%s: too many tokens", what);
     HNO_REQUIRE(p->q && (p->Tk == 0 || (p->k && p->v)), "%s: null pointer", what);
+    const int esz = p->dtype == HNO_BF16 ? 2 : 4;
+    bool ok = p->Dk % 8 == 0 && p->Dv % 8 == 0 && at_aligned(p->q) && at_aligned(p->k) && at_aligned(p->v);
+    for (int i = 0; i < 3; ++i) ok = ok && p->q_stride[i] * esz % 16 == 0 && p->k_stride[i] * esz % 16 == 0 && p->v_stride[i] * esz % 16 == 0;
+    HNO_REQUIRE(ok, "%s: head sizes must be multiples of 8 and rows 16-byte aligned", what);
     return HNO_OK;
 }
 static AttnArgs at_args(const hno_attn_t *p) {
     AttnArgs a = {};
-    const int esz = p->dtype == HNO_BF16 ? 2 : 4;
-    const auto aligned = [&](const void *ptr, const long long *st, int D) {
-        bool ok = D % 8 == 0 && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0;
-        for (int i = 0; i < 3; ++i) ok = ok && st[i] * esz % 16 == 0;
-        return ok ? 1 : 0;
-    };
     a.q = p->q; a.k = p->k; a.v = p->v; a.mask = p->mask; a.lens = p->kv_lens;
     for (int i = 0; i < 3; ++i) a.qs[i] = p->q_stride[i], a.ks[i] = p->k_stride[i], a.vs[i] = p->v_stride[i];
     for (int i = 0; i < 4; ++i) a.ms[i] = p->mask_stride[i];
     a.B = p->B; a.Tq = p->Tq; a.Tk = p->Tk; a.H = p->H; a.Hk = p->Hk; a.Dk = p->Dk; a.Dv = p->Dv; a.causal = p->causal != 0;
-    a.vq = aligned(p->q, p->q_stride, p->Dk);
-    a.vk = aligned(p->k, p->k_stride, p->Dk);
-    a.vv = aligned(p->v, p->v_stride, p->Dv);
-    a.vo = p->Dv % 8 == 0;                        // outputs and their gradients are contiguous (16-byte aligned, checked by the entries)
     a.keymask = p->mask && p->mask_stride[2] == 0 && p->mask_stride[1] == 0;
     a.scale = p->scale;
     a.scale2 = p->scale * 1.4426950408889634f;
     return a;
 }
-static bool at_aligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static double at_bytes(const hno_attn_t *p, int q_tensors, int k_tensors) {
     return (p->dtype == HNO_BF16 ? 2.0 : 4.0) * ((double)p->B * p->Tq * p->H * p->Dk * q_tensors + (double)p->B * p->Tk * p->Hk * p->Dk * k_tensors);
 }
 
-// the kernel of one type for the padded head size
-#define AT_DISPATCH(KERNEL, grid, s, a)                                                                       \
-    do {                                                                                                      \
-        const int dp_ = round_up(a.Dk > a.Dv ? a.Dk : a.Dv, 32);                                              \
-        if (dp_ == 32) hipLaunchKernelGGL((KERNEL<T, 32>), grid, dim3(64 * AT_WAVES), 0, s, a);               \
-        else if (dp_ == 64) hipLaunchKernelGGL((KERNEL<T, 64>), grid, dim3(64 * AT_WAVES), 0, s, a);          \
-        else if (dp_ == 96) hipLaunchKernelGGL((KERNEL<T, 96>), grid, dim3(64 * AT_WAVES), 0, s, a);          \
-        else hipLaunchKernelGGL((KERNEL<T, 128>), grid, dim3(64 * AT_WAVES), 0, s, a);                        \
+// the kernel of one type for the padded head size, with or without a mask
+#define AT_LAUNCH(KERNEL, DP)                                                                                      \
+    do {                                                                                                           \
+        if (a.mask) hipLaunchKernelGGL((KERNEL<T, DP, true>), dim3(n_), dim3(64 * AT_WAVES), 0, s, a);             \
+        else hipLaunchKernelGGL((KERNEL<T, DP, false>), dim3(n_), dim3(64 * AT_WAVES), 0, s, a);                   \
+    } while (0)
+#define AT_DISPATCH(KERNEL, blocks, s, a)                                                                          \
+    do {                                                                                                           \
+        const int dp_ = round_up(a.Dk > a.Dv ? a.Dk : a.Dv, 32);                                                   \
+        const unsigned n_ = (unsigned)(blocks);                                                                    \
+        if (dp_ == 32) AT_LAUNCH(KERNEL, 32);                                                                      \
+        else if (dp_ == 64) AT_LAUNCH(KERNEL, 64);                                                                 \
+        else if (dp_ == 96) AT_LAUNCH(KERNEL, 96);                                                                 \
+        else AT_LAUNCH(KERNEL, 128);                                                                               \
     } while (0)
 
 template <typename T>
@@ -639,11 +688,11 @@ static int at_forward(const hno_attn_t *p, void *out, void *out_res, float *lse,
     const AtPlan n = at_plan(p);
     AttnArgs a = at_args(p);
     const long long rows = (long long)p->B * p->Tq * p->H;
-    a.out = out; a.outres = out_res; a.lse = lse; a.pack = n.pack; a.nsplit = n.q_split;
+    a.out = out; a.outres = out_res; a.lse = lse; a.pack = n.pack; a.nsplit = n.q_split; a.tiles = n.q_tiles;
     a.part = (float *)workspace;
     a.part2 = (float *)((char *)workspace + at_pad((size_t)n.q_split * rows * p->Dv * sizeof(float)));
     ProfScope _ps(KID_ATTN, s, at_bytes(p, 2, 2));
-    AT_DISPATCH(attn_fwd_kernel, dim3(n.q_tiles, n.q_heads, p->B * n.q_split), s, a);
+    AT_DISPATCH(attn_fwd_kernel, (long long)n.q_tiles * n.q_heads * p->B * n.q_split, s, a);
     HNO_CHECK_LAUNCH();
     if (n.q_split > 1) {
         hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, (const float *)a.part, (const float *)a.part2,
@@ -673,14 +722,15 @@ static int at_backward(const hno_attn_t *p, const void *out, const void *out_res
     {
         ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 2, 0));
         hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, (const T *)dout, (const T *)out,
-                           (const T *)out_res, lse, a.delta, rows, p->Dv, a.vo);
+                           (const T *)out_res, lse, a.delta, rows, p->Dv);
         HNO_CHECK_LAUNCH();
     }
     if (dq) {
         ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 3, 2));
         a.pack = n.pack;
         a.nsplit = n.q_split;
-        AT_DISPATCH(attn_dq_kernel, dim3(n.q_tiles, n.q_heads, p->B * n.q_split), s, a);
+        a.tiles = n.q_tiles;
+        AT_DISPATCH(attn_dq_kernel, (long long)n.q_tiles * n.q_heads * p->B * n.q_split, s, a);
         HNO_CHECK_LAUNCH();
         if (n.q_split > 1)
             if (int rc = at_sum(a.part, (T *)dq, rows * p->Dk, n.q_split, s)) return rc;
@@ -688,8 +738,9 @@ static int at_backward(const hno_attn_t *p, const void *out, const void *out_res
     if (dk && p->Tk > 0) {
         ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 2, 4));
         a.nsplit = n.k_split;
+        a.tiles = n.k_tiles;
         a.part2 = (float *)((char *)a.part + at_pad((size_t)n.k_split * krows * p->Dk * sizeof(float)));
-        AT_DISPATCH(attn_dkv_kernel, dim3(n.k_tiles, p->Hk, p->B * n.k_split), s, a);
+        AT_DISPATCH(attn_dkv_kernel, (long long)n.k_tiles * p->Hk * p->B * n.k_split, s, a);
         HNO_CHECK_LAUNCH();
         if (n.k_split > 1) {
             if (int rc = at_sum(a.part, (T *)dk, krows * p->Dk, n.k_split, s)) return rc;

@@ -61,6 +61,17 @@ def _ws(nbytes, device):
 
 
 # ----------------------------------------------------------------------------------------------- attention
+def _heads(t, esize):
+    """a (B, T, H, D) operand as the kernels take it: unit stride along D, D a multiple of 8, rows 16-byte aligned -- the tensor itself where it is so,
+    else a copy padded with zeros (which change no score; padded channels of the result are cut off)"""
+    D, step = t.shape[3], 16 // esize
+    if D % 8 == 0 and (t.stride(3) == 1) and t.data_ptr() % 16 == 0 and all(s % step == 0 for s in t.stride()[:3]):
+        return t
+    if D % 8 == 0:
+        return t.clone(memory_format=torch.contiguous_format)
+    return torch.nn.functional.pad(t, (0, -D % 8))
+
+
 def _attn_args(q, k, v, mask, kv_lens, causal, scale):
     a = _lib.AttnArgs()
     B, Tq, H, Dk = q.shape
@@ -84,7 +95,8 @@ class AttentionFn(_HnoFunction):
     @staticmethod
     def forward(ctx, q, k, v, mask, kv_lens, causal, scale):
         train = ops.backward_wanted(ctx)
-        q, k, v = (t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous() for t in (q, k, v))
+        Dk, Dv = q.shape[3], v.shape[3]
+        q, k, v = (_heads(t, t.element_size()) for t in (q, k, v))
         B, Tq, H, _ = q.shape
         out = torch.empty((B, Tq, H, v.shape[3]), device=q.device, dtype=q.dtype)
         lse = torch.empty((B, Tq, H), device=q.device, dtype=torch.float32) if train else None
@@ -97,14 +109,14 @@ class AttentionFn(_HnoFunction):
             check(L.hno_attn_fwd(ctypes.byref(a), _p(out), _p(res), _p(lse), _p(ws), n, stream_ptr()), 'hno_attn_fwd')
         if train:
             ctx.save_for_backward(q, k, v, mask, kv_lens, out, res, lse)
-            ctx.cfg = (causal, scale)
-        return out
+            ctx.cfg = (causal, scale, Dk, Dv)
+        return out if out.shape[3] == Dv else out[..., :Dv].contiguous()
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         q, k, v, mask, kv_lens, out, res, lse = ctx.saved_tensors
-        causal, scale = ctx.cfg
+        causal, scale, Dk, Dv = ctx.cfg
         need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         new = torch.empty if out.numel() else torch.zeros
         dq = new(q.shape, device=q.device, dtype=q.dtype) if need_q else None
@@ -112,26 +124,21 @@ class AttentionFn(_HnoFunction):
         if out.numel():
             with _on(q):
                 L = _lib.lib()
-                g = _aligned(g)
+                g = _heads(g, g.element_size()).contiguous()
                 a = _attn_args(q, k, v, mask, kv_lens, causal, scale)
                 n = L.hno_attn_workspace_bytes(ctypes.byref(a), 1)
                 ws = _ws(n, q.device)
                 check(L.hno_attn_bwd(ctypes.byref(a), _p(out), _p(res), _p(lse), _p(g), _p(dq), _p(dk), _p(dv), _p(ws), n, stream_ptr()),
                       'hno_attn_bwd')
+        dq, dk, dv = (t if t is None or t.shape[3] == D else t[..., :D] for t, D in ((dq, Dk), (dk, Dk), (dv, Dv)))
         return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None, None
-
-
-def _aligned(t):
-    """contiguous and 16-byte aligned (an upstream gradient can be any view)"""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def attention(q, k, v, *, causal=False, mask=None, kv_lens=None, scale=None):
     """Softmax attention on tokens: q (B, Tq, H, Dk), k (B, Tk, Hk, Dk), v (B, Tk, Hk, Dv) -> (B, Tq, H, Dv); all fp32 or all bf16.
 
-    H is a multiple of Hk: query head h reads key head h // (H // Hk).  Head sizes 1 ... 128.  Any strides; a last axis that is not contiguous is
-    copied.  ``scale`` (positive, default Dk ** -0.5) multiplies the scores.
+    H is a multiple of Hk: query head h reads key head h // (H // Hk).  Head sizes 1 ... 128.  Any strides; rows that are not
+    16-byte aligned or contiguous, and head sizes that are no multiple of 8, are copied.  ``scale`` (positive, default Dk ** -0.5) multiplies the scores.
     Visible to query i are the keys j < L with L = ``kv_lens[b]`` (integers (B,) on the device, clamped to 0 ... Tk; default Tk);
     with ``causal`` those with j <= i + L - Tq (the last query is aligned with the last key);
     with ``mask`` (bool, broadcastable to (B, H, Tq, Tk)) those that it marks True.  A query that sees no key gives zeros and has no gradient.

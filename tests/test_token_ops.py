@@ -615,7 +615,8 @@ def test_entry_points_check_before_any_launch():
         return L.hno_attn_fwd(ctypes.byref(a), out, None, None, None, ws, None)
     for kw in ({'dtype': 2}, {'Tq': 0}, {'Tk': -1}, {'H': 3, 'Hk': 2}, {'scale': 0.0}, {'scale': float('nan')}, {'q': None}, {'k': None}, {'out': None}, {'out': 4098}):
         assert attn(**kw) == -1, kw
-    assert attn(Dk=129) == -2 and attn(B=70000) == -2
+    assert attn(Dk=36) == -1 and attn(q=4100) == -1
+    assert attn(Dk=136) == -2 and attn(B=70000000) == -2
     assert L.hno_attn_fwd(None, None, None, None, None, 0, None) == -1
     assert attn(Tk=100000, Tq=1) == -1 and b'workspace' in L.hno_last_error()
     assert L.hno_attn_bwd(ctypes.byref(a), 4096, None, 4096, 4096, None, 4096, None, 4096, 1 << 40, None) == -1      # dk without dv
