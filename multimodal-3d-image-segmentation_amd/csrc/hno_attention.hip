@@ -22,7 +22,7 @@ struct AttnArgs {
     const unsigned char *mask;
     const int *lens;
     long long qs[3], ks[3], vs[3], ms[4];     // element strides of (batch, token, head); the mask's of (batch, head, query, key)
-    int B, Tq, Tk, H, Hk, Dk, Dv, causal, nsplit, tiles, pack, keymask;
+    int B, Tq, Tk, H, Hk, Dk, Dv, causal, nsplit, tiles, pack, fold, keymask;
     float scale2, scale;                       // scale log2(e), scale
 };
 
@@ -78,38 +78,104 @@ __device__ __forceinline__ TkFrag<T> at_load8(const T *row, int d, int D) {
     return f;
 }
 
-// A workgroup's share of one tile of the streamed side on its way to LDS: loaded into registers one tile ahead of its use, stored
-// when the buffer is free.  Rows from `end` on are zeros; so are rows whose flag (loaded beside them, looked at when they are stored, so that no load
-// waits for another) says that nobody looks at them.
-template <typename T, int DP, int ROWS, typename Flag>
-struct AtStage {
-    static constexpr int CH = DP / 8, N = (ROWS * CH + 64 * AT_WAVES - 1) / (64 * AT_WAVES);
-    static constexpr bool EVEN = ROWS * CH % (64 * AT_WAVES) == 0;
-    TkFrag<T> r[N];
-    Flag flag[N];
-    template <typename F>
-    __device__ __forceinline__ void load(const T *base, long long st, int t0, int end, int D, int tid, F flag_of) {
+// A workgroup's share of one tile (ROWS rows of a head) of the streamed side on its way to LDS.  Thread t moves the 16-byte (fp32: 32-byte) slots
+// t, t + 256, ...  Use: fetch(tile) -> settle(tile) -> barrier -> read it, with the next fetch behind the barrier.
+// Rows from `end` on may hold any row of the tensor: their scores are hidden.  Rows whose flag is set in settle() are zeroed: nobody looks at
+// them, so they may hold NaN, and 0 x NaN must not reach a sum.
+//
+// bf16: LDS-DMA (global_load_lds_dwordx4), which needs no registers: with tiles staged through registers dk / dv of 128 channels took 357 of them and
+// spilled 25 when held to two waves per SIMD.  The DMA writes its slots in lane order, so the slot permutation of at_at is applied to the source.
+template <typename T, int DP, int ROWS>
+struct AtTile;
+template <int DP, int ROWS>
+struct AtTile<tkh, DP, ROWS> {
+    static constexpr int CH = DP / 8, N = ROWS * CH / (64 * AT_WAVES);
+    static_assert(ROWS * CH % (64 * AT_WAVES) == 0, "whole slots per thread");    
+    unsigned off[N];          // byte offset of the slot's source from the tile's first row
+    long long st;
+    int D;
+    __device__ __forceinline__ static int row(int i, int tid) { return (tid + 64 * AT_WAVES * i) / CH; }
+    __device__ __forceinline__ static int chunk(int i, int tid) {
+        const int s = tid + 64 * AT_WAVES * i, r = s / CH, slot = s - r * CH;
+        if constexpr (DP == 128) return slot ^ (((r & 3) << 2) | ((r >> 2) & 3));
+        else if constexpr (DP == 64) return slot ^ ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
+        else if constexpr (DP == 32) return slot ^ ((r >> 2) & 3);
+        else return slot - ((r >> 2) & 3) + (slot < ((r >> 2) & 3) ? 12 : 0);
+    }
+    __device__ __forceinline__ void init(long long st_, int D_, int tid) {
+        st = st_, D = D_;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = tid + 64 * AT_WAVES * i, row = c / CH, d = (c - row * CH) * 8, t = t0 + row;
-            if ((EVEN || row < ROWS) && t < end) {
-                r[i] = at_load8(base + (long long)t * st, d, D);
-                flag[i] = flag_of(t);
-            } else {
+            const int c = chunk(i, tid) * 8;
+            off[i] = (unsigned)(row(i, tid) * st + (c < D ? c : 0)) * 2;      // (channels from D on: multiplied by zeros, or never stored)
+        }
+    }
+    __device__ __forceinline__ void fetch(tkh *tile, const tkh *base, int t0, int end, int tid) {
+        typedef __attribute__((address_space(3))) tkh *ldsp;
+        const tkh *src = base + (long long)t0 * st;
+        const unsigned dst = (unsigned)(uintptr_t)(ldsp)tile + (tid >> 6) * 1024;
+        if (t0 + ROWS <= end) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) r[i].set(j, 0.f);
+            for (int i = 0; i < N; ++i) dma(src, off[i], dst + i * 4096);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int r = row(i, tid), c = chunk(i, tid) * 8, last = end - 1 - t0;
+                dma(src, (unsigned)((r < last ? r : last) * st + (c < D ? c : 0)) * 2, dst + i * 4096);
             }
         }
     }
+    // 64 lanes x 16 bytes to 1024 consecutive LDS bytes; M0 holds the destination
+    __device__ __forceinline__ static void dma(const tkh *src, unsigned off, unsigned dst) {
+        unsigned keep;
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep) : "v"(off), "s"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory");
+    }
     template <typename P>
-    __device__ __forceinline__ void store(T *tile, int tid, P dead) {
+    __device__ __forceinline__ void settle(tkh *tile, int tid, P dead) const {
+        dma_wait<0>();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (dead(i)) *reinterpret_cast<tku4 *>(tile + (tid + 64 * AT_WAVES * i) * 8) = tku4{0, 0, 0, 0};
+    }
+};
+template <int DP, int ROWS>
+struct AtTile<float, DP, ROWS> {
+    static constexpr int CH = DP / 8, N = (ROWS * CH + 64 * AT_WAVES - 1) / (64 * AT_WAVES);
+    TkFrag<float> r[N];
+    long long st;
+    int D;
+    __device__ __forceinline__ static int row(int i, int tid) { return (tid + 64 * AT_WAVES * i) / CH; }
+    __device__ __forceinline__ void init(long long st_, int D_, int) { st = st_, D = D_; }
+    __device__ __forceinline__ void fetch(float *, const float *base, int t0, int end, int tid) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = tid + 64 * AT_WAVES * i, row = c / CH, d = (c - row * CH) * 8;
-            if (dead(flag[i]))
+            const int k = row(i, tid), d = (tid + 64 * AT_WAVES * i - k * CH) * 8, t = t0 + k;
+            r[i] = at_load8(base + (long long)(t < end ? t : end - 1) * st, d, D);
+        }
+    }
+    template <typename P>
+    __device__ __forceinline__ void settle(float *tile, int tid, P dead) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int k = row(i, tid), d = (tid + 64 * AT_WAVES * i - k * CH) * 8;
+            if (dead(i))
 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[i].set(j, 0.f);
-            if (EVEN || row < ROWS) tk_store8(tile + at_at<DP>(tile, row, d), r[i]);
+            if (k < ROWS) tk_store8(tile + at_at<DP>(tile, k, d), r[i]);
+        }
+    }
+};
+// flags of the rows a thread moves, loaded with them
+template <typename T, int DP, int ROWS, typename F>
+struct AtFlags {
+    F f[AtTile<T, DP, ROWS>::N];
+    template <typename G>
+    __device__ __forceinline__ void load(int t0, int end, int tid, G get) {
+#pragma unroll
+        for (int i = 0; i < AtTile<T, DP, ROWS>::N; ++i) {
+            const int t = t0 + AtTile<T, DP, ROWS>::row(i, tid);
+            f[i] = get(t < end ? t : end - 1);
         }
     }
 };
@@ -186,7 +252,10 @@ struct AtBlock {
 };
 __device__ __forceinline__ AtBlock at_block(const AttnArgs &a, int grp) {
     const int n = gridDim.x, xcd = blockIdx.x & 7, each = n >> 3, more = n & 7;
-    int at = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
+    int i = blockIdx.x >> 3;
+    // all resident at once, two on a CU: the second half of the run backwards, so that a CU gets one of the long and one of the short
+    if (a.fold && 2 * i >= each) i = i < each ? each - 1 - (i - (each + 1) / 2) : i;
+    int at = xcd * each + min(xcd, more) + i;
     AtBlock w;
     w.sp = at % a.nsplit, at /= a.nsplit;
     w.gi = at % grp, at /= grp;
@@ -273,31 +342,29 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) 
     const unsigned char *mrow = MASK ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
     // a mask that hides a key from every query of this workgroup takes the value row out too: 0 x NaN would be NaN
     const unsigned char *mkey = MASK && a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
-    AtStage<T, DP, KT, unsigned char> ks, vs;
-    const auto load = [&](int j) {
-        ks.load(kb, a.ks[1], j, j1, a.Dk, tid, [](int) { return (unsigned char)1; });
-        vs.load(vb, a.vs[1], j, j1, a.Dv, tid, [&](int t) { return MASK && mkey ? mkey[t * a.ms[3]] : (unsigned char)1; });
+    AtTile<T, DP, KT> ks, vs;
+    AtFlags<T, DP, KT, unsigned char> flag;
+    ks.init(a.ks[1], a.Dk, tid);
+    vs.init(a.vs[1], a.Dv, tid);
+    const auto fetch = [&](int to, int j) {
+        ks.fetch(Ks[to], kb, j, j1, tid);
+        vs.fetch(Vs[to], vb, j, j1, tid);
+        if (MASK && mkey) flag.load(j, j1, tid, [&](int t) { return mkey[t * a.ms[3]]; });
     };
-    const auto store = [&](int to) {
-        ks.store(Ks[to], tid, [](unsigned char) { return false; });
-        vs.store(Vs[to], tid, [&](unsigned char f) { return MASK && mkey && !f; });
+    const auto settle = [&](int to) {
+        ks.settle(Ks[to], tid, [](int) { return false; });
+        vs.settle(Vs[to], tid, [&](int i) { return MASK && mkey && !flag.f[i]; });
     };
 
     tk16 acc[DP / 32] = {};
     float m = -INFINITY, l = 0.f, shift = 0.f;
     const float slack = 8.f / a.scale2;           // the maximum is raised, and the sums rescaled, only where weights would exceed 2^8
     int buf = 0;
-    if (j0 < j1) {
-        load(j0);
-        store(0);
-        if (j0 + KT < j1) load(j0 + KT);
-    }
+    if (j0 < j1) fetch(0, j0);
     for (int j = j0; j < j1; j += KT, buf ^= 1) {
+        settle(buf);
         __syncthreads();
-        if (j + KT < j1) {
-            store(buf ^ 1);
-            if (j + 2 * KT < j1) load(j + 2 * KT);
-        }
+        if (j + KT < j1) fetch(buf ^ 1, j + KT);
         tk16 s[KT / 32];
         AtMask mk[KT / 32];
         if (MASK)
@@ -439,28 +506,26 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
     const unsigned char *mrow = MASK ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
     const unsigned char *mkey = MASK && a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
     const int lim_all = MASK ? 0 : at_wave_min(w.lim);
-    AtStage<T, DP, KT, unsigned char> ks, vs;
-    const auto load = [&](int j) {
-        ks.load(kb, a.ks[1], j, j1, a.Dk, tid, [&](int t) { return MASK && mkey ? mkey[t * a.ms[3]] : (unsigned char)1; });
-        vs.load(vb, a.vs[1], j, j1, a.Dv, tid, [](int) { return (unsigned char)1; });
+    AtTile<T, DP, KT> ks, vs;
+    AtFlags<T, DP, KT, unsigned char> flag;
+    ks.init(a.ks[1], a.Dk, tid);
+    vs.init(a.vs[1], a.Dv, tid);
+    const auto fetch = [&](int to, int j) {
+        ks.fetch(Ks[to], kb, j, j1, tid);
+        vs.fetch(Vs[to], vb, j, j1, tid);
+        if (MASK && mkey) flag.load(j, j1, tid, [&](int t) { return mkey[t * a.ms[3]]; });
     };
-    const auto store = [&](int to) {
-        ks.store(Ks[to], tid, [&](unsigned char f) { return MASK && mkey && !f; });
-        vs.store(Vs[to], tid, [](unsigned char) { return false; });
+    const auto settle = [&](int to) {
+        ks.settle(Ks[to], tid, [&](int i) { return MASK && mkey && !flag.f[i]; });
+        vs.settle(Vs[to], tid, [](int) { return false; });
     };
     tk16 acc[DP / 32] = {};
     int buf = 0;
-    if (j0 < j1) {
-        load(j0);
-        store(0);
-        if (j0 + KT < j1) load(j0 + KT);
-    }
+    if (j0 < j1) fetch(0, j0);
     for (int j = j0; j < j1; j += KT, buf ^= 1) {
+        settle(buf);
         __syncthreads();
-        if (j + KT < j1) {
-            store(buf ^ 1);
-            if (j + 2 * KT < j1) load(j + 2 * KT);
-        }
+        if (j + KT < j1) fetch(buf ^ 1, j + KT);
         const bool whole = j + KT <= lim_all;
 #pragma unroll
         for (int n = 0; n < KT / 32; ++n) {
@@ -488,8 +553,8 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
     at_store<T, DP>((T *)a.dq + row * a.Dk, acc, a.Dk, h, [&](float x) { return x * a.scale; });
 }
 
-template <typename T, int DP, bool MASK>
-__global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
+template <typename T, int DP, bool MASK, int WHAT>
+__global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
     constexpr int QT = at_tile<T>(), S = at_stride<T, DP>();
     __shared__ __attribute__((aligned(16))) T Qs[2][QT * S];
     __shared__ __attribute__((aligned(16))) T Gs[2][QT * S];
@@ -502,15 +567,16 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
     const int kc = valid ? key : a.Tk - 1;
     // queries that see this key: [first, Tq)
     const int first = key >= L ? 0x7fffffff : (a.causal ? key - off : 0);
+    constexpr bool DK = WHAT & 1, DV = WHAT & 2;
     TkFrag<T> kf[DP / 16], vf[DP / 16];
     const T *krow = (const T *)a.k + b * a.ks[0] + (long long)kc * a.ks[1] + hk * a.ks[2];
     const T *vrow = (const T *)a.v + b * a.vs[0] + (long long)kc * a.vs[1] + hk * a.vs[2];
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
         kf[kk] = at_load8(krow, 16 * kk + 8 * h, a.Dk);
-        vf[kk] = at_load8(vrow, 16 * kk + 8 * h, a.Dv);
+        if (DK) vf[kk] = at_load8(vrow, 16 * kk + 8 * h, a.Dv);
     }
-    tk16 acck[DP / 32] = {}, accv[DP / 32] = {};
+    tk16 acck[DK ? DP / 32 : 1] = {}, accv[DV ? DP / 32 : 1] = {};
     // the list of (head of the group, query tile) that sees any key of this tile, cut into nsplit runs
     int qt0 = a.causal && key0 - off > 0 ? (key0 - off) / QT : 0;
     const int nqt = (a.Tq + QT - 1) / QT;
@@ -519,39 +585,39 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
     const int it1 = (sp + 1) * per < total ? (sp + 1) * per : total;
     // queries from here on are seen by every key of the wave
     const int first_all = MASK || key0 + wave * 32 + 32 > L ? 0x7fffffff : (a.causal ? key0 + wave * 32 + 31 - off : 0);
-    AtStage<T, DP, QT, float> qs, gs;
+    AtTile<T, DP, QT> qs, gs;
+    AtFlags<T, DP, QT, float> flag;
+    qs.init(a.qs[1], a.Dk, tid);
+    gs.init((long long)a.H * a.Dv, a.Dv, tid);
     float nlse = 0.f, ndelta = 0.f;               // row tid of the tile
-    const auto load = [&](int it) {
+    const int empty = a.causal ? -off : 0;        // queries before it see nothing
+    int i_next = 0;
+    const auto fetch = [&](int to, int it) {
         const int gi = it / each, i0 = (qt0 + it - gi * each) * QT, head = hk * grp + gi;
         const long long row0 = ((long long)b * a.Tq) * a.H + head;
-        const auto flag = [&](int t) { return a.lse[row0 + (long long)t * a.H]; };
-        qs.load((const T *)a.q + b * a.qs[0] + head * a.qs[2], a.qs[1], i0, a.Tq, a.Dk, tid, flag);
-        gs.load((const T *)a.g + row0 * a.Dv, (long long)a.H * a.Dv, i0, a.Tq, a.Dv, tid, flag);
+        i_next = i0;
+        qs.fetch(Qs[to], (const T *)a.q + b * a.qs[0] + head * a.qs[2], i0, a.Tq, tid);
+        gs.fetch(Gs[to], (const T *)a.g + row0 * a.Dv, i0, a.Tq, tid);
+        if (MASK) flag.load(i0, a.Tq, tid, [&](int t) { return a.lse[row0 + (long long)t * a.H]; });
         if (tid < QT) {
-            const bool in = i0 + tid < a.Tq;
-            nlse = in ? a.lse[row0 + (long long)(i0 + tid) * a.H] : INFINITY;
-            ndelta = in ? a.delta[row0 + (long long)(i0 + tid) * a.H] : 0.f;
+            const int i = i0 + tid < a.Tq ? i0 + tid : a.Tq - 1;
+            nlse = a.lse[row0 + (long long)i * a.H];
+            ndelta = a.delta[row0 + (long long)i * a.H];
         }
     };
-    const auto store = [&](int to) {
-        // rows that see nothing are zeroed: whatever stands in them stays out of the sums
-        const auto dead = [](float f) { return f == INFINITY; };
-        qs.store(Qs[to], tid, dead);
-        gs.store(Gs[to], tid, dead);
+    const auto settle = [&](int to) {
+        // queries that see nothing, by their position or by the mask
+        const auto dead = [&](int i) { return i_next + AtTile<T, DP, QT>::row(i, tid) < empty || (MASK && flag.f[i] == INFINITY); };
+        qs.settle(Qs[to], tid, dead);
+        gs.settle(Gs[to], tid, dead);
         if (tid < QT) lses[to][tid] = nlse, deltas[to][tid] = ndelta;
     };
     int buf = 0;
-    if (sp * per < it1) {
-        load(sp * per);
-        store(0);
-        if (sp * per + 1 < it1) load(sp * per + 1);
-    }
+    if (sp * per < it1) fetch(0, sp * per);
     for (int it = sp * per; it < it1; ++it, buf ^= 1) {
+        settle(buf);
         __syncthreads();
-        if (it + 1 < it1) {
-            store(buf ^ 1);
-            if (it + 2 < it1) load(it + 2);
-        }
+        if (it + 1 < it1) fetch(buf ^ 1, it + 1);
         const int gi = it / each, i0 = (qt0 + it - gi * each) * QT, head = hk * grp + gi;
         const bool whole = i0 >= first_all && i0 + QT <= a.Tq;
         const unsigned char *mcol = MASK ? a.mask + b * a.ms[0] + head * a.ms[1] + kc * a.ms[3] : nullptr;
@@ -562,7 +628,8 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) mk[e] = mcol[min(i0 + 32 * n + at_row(e, h), a.Tq - 1) * a.ms[2]];
             tk16 s = at_product<T, DP>(Qs[buf], 32 * n, kf, lane);
-            tk16 dp = at_product<T, DP>(Gs[buf], 32 * n, vf, lane);
+            tk16 dp = {};
+            if (DK) dp = at_product<T, DP>(Gs[buf], 32 * n, vf, lane);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const tkf4 le = *reinterpret_cast<const tkf4 *>(&lses[buf][32 * n + 8 * u + 4 * h]), de = *reinterpret_cast<const tkf4 *>(&deltas[buf][32 * n + 8 * u + 4 * h]);
@@ -581,20 +648,20 @@ __global__ __launch_bounds__(64 * AT_WAVES) void attn_dkv_kernel(AttnArgs a) {
                     s[e] = on ? s[e] : 0.f;
                     dp[e] = on ? dp[e] : 0.f;
                 }
-            at_accumulate<T, DP>(accv, Gs[buf], 32 * n, s, lane);
-            at_accumulate<T, DP>(acck, Qs[buf], 32 * n, dp, lane);
+            if constexpr (DV) at_accumulate<T, DP>(accv, Gs[buf], 32 * n, s, lane);
+            if constexpr (DK) at_accumulate<T, DP>(acck, Qs[buf], 32 * n, dp, lane);
         }
     }
     if (!valid) return;
     const long long row = ((long long)b * a.Tk + key) * a.Hk + hk;
     if (a.nsplit > 1) {
         const long long at = sp * ((long long)a.B * a.Tk * a.Hk) + row;
-        at_store<float, DP>(a.part + at * a.Dk, acck, a.Dk, h, [&](float x) { return x * a.scale; });
-        at_store<float, DP>(a.part2 + at * a.Dv, accv, a.Dv, h, [](float x) { return x; });
+        if constexpr (DK) at_store<float, DP>(a.part + at * a.Dk, acck, a.Dk, h, [&](float x) { return x * a.scale; });
+        if constexpr (DV) at_store<float, DP>(a.part2 + at * a.Dv, accv, a.Dv, h, [](float x) { return x; });
         return;
     }
-    at_store<T, DP>((T *)a.dk + row * a.Dk, acck, a.Dk, h, [&](float x) { return x * a.scale; });
-    at_store<T, DP>((T *)a.dv + row * a.Dv, accv, a.Dv, h, [](float x) { return x; });
+    if constexpr (DK) at_store<T, DP>((T *)a.dk + row * a.Dk, acck, a.Dk, h, [&](float x) { return x * a.scale; });
+    if constexpr (DV) at_store<T, DP>((T *)a.dv + row * a.Dv, accv, a.Dv, h, [](float x) { return x; });
 }
 
 // out = sum over splits, in split order
@@ -650,6 +717,8 @@ static int at_check(const hno_attn_t *p, const char *what) {
     bool ok = p->Dk % 8 == 0 && p->Dv % 8 == 0 && at_aligned(p->q) && at_aligned(p->k) && at_aligned(p->v);
     for (int i = 0; i < 3; ++i) ok = ok && p->q_stride[i] * esz % 16 == 0 && p->k_stride[i] * esz % 16 == 0 && p->v_stride[i] * esz % 16 == 0;
     HNO_REQUIRE(ok, "%s: head sizes must be multiples of 8 and rows 16-byte aligned", what);
+    for (const long long st : {p->q_stride[1], p->k_stride[1], p->v_stride[1], (long long)p->H * p->Dv})     // offsets inside a tile take 32 bits
+        HNO_REQUIRE(st >= 0 && st < (1 << 24), "%s: a token stride of %lld elements", what, st);
     return HNO_OK;
 }
 static AttnArgs at_args(const hno_attn_t *p) {
@@ -668,19 +737,19 @@ static double at_bytes(const hno_attn_t *p, int q_tensors, int k_tensors) {
 }
 
 // the kernel of one type for the padded head size, with or without a mask
-#define AT_LAUNCH(KERNEL, DP)                                                                                      \
+#define AT_LAUNCH(KERNEL, DP, ...)                                                                                      \
     do {                                                                                                           \
-        if (a.mask) hipLaunchKernelGGL((KERNEL<T, DP, true>), dim3(n_), dim3(64 * AT_WAVES), 0, s, a);             \
-        else hipLaunchKernelGGL((KERNEL<T, DP, false>), dim3(n_), dim3(64 * AT_WAVES), 0, s, a);                   \
+        if (a.mask) hipLaunchKernelGGL((KERNEL<T, DP, true __VA_ARGS__>), dim3(n_), dim3(64 * AT_WAVES), 0, s, a);             \
+        else hipLaunchKernelGGL((KERNEL<T, DP, false __VA_ARGS__>), dim3(n_), dim3(64 * AT_WAVES), 0, s, a);                   \
     } while (0)
 #define AT_DISPATCH(KERNEL, blocks, s, a)                                                                          \
     do {                                                                                                           \
         const int dp_ = round_up(a.Dk > a.Dv ? a.Dk : a.Dv, 32);                                                   \
         const unsigned n_ = (unsigned)(blocks);                                                                    \
-        if (dp_ == 32) AT_LAUNCH(KERNEL, 32);                                                                      \
-        else if (dp_ == 64) AT_LAUNCH(KERNEL, 64);                                                                 \
-        else if (dp_ == 96) AT_LAUNCH(KERNEL, 96);                                                                 \
-        else AT_LAUNCH(KERNEL, 128);                                                                               \
+        if (dp_ == 32) AT_LAUNCH(KERNEL, 32, );                                                                      \
+        else if (dp_ == 64) AT_LAUNCH(KERNEL, 64, );                                                                 \
+        else if (dp_ == 96) AT_LAUNCH(KERNEL, 96, );                                                                 \
+        else AT_LAUNCH(KERNEL, 128, );                                                                               \
     } while (0)
 
 template <typename T>
@@ -699,6 +768,27 @@ static int at_forward(const hno_attn_t *p, void *out, void *out_res, float *lse,
                            (T *)out, (T *)out_res, lse, rows, p->Dv, n.q_split);
         HNO_CHECK_LAUNCH();
     }
+    return HNO_OK;
+}
+
+// dk and dv in one kernel, or each in its own (where one kernel would not leave registers for two waves per SIMD)
+template <typename T>
+static int at_launch_dkv(AttnArgs a, unsigned n_, hipStream_t s) {
+    a.fold = a.causal && n_ <= 512;
+    const int dp = round_up(a.Dk > a.Dv ? a.Dk : a.Dv, 32);
+    if (dp == 32) AT_LAUNCH(attn_dkv_kernel, 32, , 3);
+    else if (dp == 64) AT_LAUNCH(attn_dkv_kernel, 64, , 3);
+    else if constexpr (sizeof(T) == 4) {
+        if (dp == 96) AT_LAUNCH(attn_dkv_kernel, 96, , 3);
+        else AT_LAUNCH(attn_dkv_kernel, 128, , 3);
+    } else if (dp == 96) {
+        AT_LAUNCH(attn_dkv_kernel, 96, , 1);
+        AT_LAUNCH(attn_dkv_kernel, 96, , 2);
+    } else {
+        AT_LAUNCH(attn_dkv_kernel, 128, , 1);
+        AT_LAUNCH(attn_dkv_kernel, 128, , 2);
+    }
+    HNO_CHECK_LAUNCH();
     return HNO_OK;
 }
 
@@ -740,7 +830,7 @@ static int at_backward(const hno_attn_t *p, const void *out, const void *out_res
         a.nsplit = n.k_split;
         a.tiles = n.k_tiles;
         a.part2 = (float *)((char *)a.part + at_pad((size_t)n.k_split * krows * p->Dk * sizeof(float)));
-        AT_DISPATCH(attn_dkv_kernel, (long long)n.k_tiles * p->Hk * p->B * n.k_split, s, a);
+        if (int rc = at_launch_dkv<T>(a, (unsigned)((long long)n.k_tiles * p->Hk * p->B * n.k_split), s)) return rc;
         HNO_CHECK_LAUNCH();
         if (n.k_split > 1) {
             if (int rc = at_sum(a.part, (T *)dk, krows * p->Dk, n.k_split, s)) return rc;

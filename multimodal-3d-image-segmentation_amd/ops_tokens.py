@@ -62,10 +62,11 @@ def _ws(nbytes, device):
 
 # ----------------------------------------------------------------------------------------------- attention
 def _heads(t, esize):
-    """a (B, T, H, D) operand as the kernels take it: unit stride along D, D a multiple of 8, rows 16-byte aligned -- the tensor itself where it is so,
+    """a (B, T, H, D) operand as the kernels take it: unit stride along D, D a multiple of 8, rows 16-byte aligned and
+    less than 2^24 elements apart -- the tensor itself where it is so,
     else a copy padded with zeros (which change no score; padded channels of the result are cut off)"""
     D, step = t.shape[3], 16 // esize
-    if D % 8 == 0 and (t.stride(3) == 1) and t.data_ptr() % 16 == 0 and all(s % step == 0 for s in t.stride()[:3]):
+    if D % 8 == 0 and (t.stride(3) == 1) and t.data_ptr() % 16 == 0 and all(s % step == 0 for s in t.stride()[:3]) and t.stride(1) < 1 << 24:
         return t
     if D % 8 == 0:
         return t.clone(memory_format=torch.contiguous_format)
