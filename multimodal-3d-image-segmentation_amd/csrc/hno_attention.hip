@@ -22,7 +22,7 @@ struct AttnArgs {
     const unsigned char *mask;
     const int *lens;
     long long qs[3], ks[3], vs[3], ms[4];     // element strides of (batch, token, head); the mask's of (batch, head, query, key)
-    int B, Tq, Tk, H, Hk, Dk, Dv, causal, nsplit, tiles, pack, fold, keymask;
+    int B, Tq, Tk, H, Hk, Dk, Dv, causal, nsplit, tiles, pack, pair, keymask;
     float scale2, scale;                       // scale log2(e), scale
 };
 
@@ -246,23 +246,27 @@ __device__ __forceinline__ void at_store(T *dst, const tk16 (&acc)[DP / 32], int
 
 // Workgroup -> work.  The 8 XCDs take workgroups in turn and each has its own L2: every XCD gets one run of the list
 // key head x batch x tile x (head of the group, split), so the workgroups that stream the same keys (or queries) share an L2, and an XCD
-// meets batch entries of several lengths.  The tiles that see most come first, where a causal mask makes them unequal.
+// meets batch entries of several lengths.  A causal mask makes tiles unequal: those that see most come first, or, where all workgroups are resident at
+// once (pair), each takes a long one and its short counterpart one after the other.
 struct AtBlock {
     int b, hk, tile, gi, sp;
 };
 __device__ __forceinline__ AtBlock at_block(const AttnArgs &a, int grp) {
     const int n = gridDim.x, xcd = blockIdx.x & 7, each = n >> 3, more = n & 7;
-    int i = blockIdx.x >> 3;
-    // all resident at once, two on a CU: the second half of the run backwards, so that a CU gets one of the long and one of the short
-    if (a.fold && 2 * i >= each) i = i < each ? each - 1 - (i - (each + 1) / 2) : i;
-    int at = xcd * each + min(xcd, more) + i;
+    int at = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
     AtBlock w;
     w.sp = at % a.nsplit, at /= a.nsplit;
     w.gi = at % grp, at /= grp;
-    w.tile = at % a.tiles, at /= a.tiles;
+    const int tiles = a.pair ? (a.tiles + 1) >> 1 : a.tiles;
+    w.tile = at % tiles, at /= tiles;
     w.b = at % a.B;
     w.hk = at / a.B;
     return w;
+}
+// the tile of pass `half` (0, 1) of a workgroup; -1: none.  `back`: the last tile is the one that sees most
+__device__ __forceinline__ int at_tile_of(const AttnArgs &a, int t, int half, bool back) {
+    if (half && (!a.pair || 2 * t == a.tiles - 1)) return -1;
+    return (half != 0) != back ? a.tiles - 1 - t : t;
 }
 // ------------------------------------------------------------------ rows of the query side
 // Where few new tokens share a key head (pack), the rows of all its query heads form one list, so
@@ -328,7 +332,12 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const AtBlock w0 = at_block(a, a.pack ? 1 : a.H / a.Hk);
     const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk, hb = hk * grp + w0.gi, nrows = a.pack ? grp * a.Tq : a.Tq;
-    const int L = at_length(a, b), r0 = (a.causal ? a.tiles - 1 - w0.tile : w0.tile) * AT_ROWS, r = r0 + wave * 32 + (lane & 31);
+    const int L = at_length(a, b);
+    for (int half = 0; half < 2; ++half) {
+    const int tile = at_tile_of(a, w0.tile, half, a.causal);
+    if (tile < 0) break;
+    if (half) __syncthreads();
+    const int r0 = tile * AT_ROWS, r = r0 + wave * 32 + (lane & 31);
     const AtRow w = at_query_row(a, r, hb, nrows, L);
     int j0, j1;
     at_key_range(a, L, (r0 + AT_ROWS < nrows ? r0 + AT_ROWS : nrows) - 1, nrows, sp, KT, j0, j1);
@@ -411,7 +420,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) 
             }
     }
     l += at_other_half(l);
-    if (!w.valid) return;
+    if (!w.valid) continue;
     const long long row = ((long long)b * a.Tq + w.i) * a.H + w.head;
     if (a.nsplit > 1) {
         const long long rows = (long long)a.B * a.Tq * a.H, at = sp * rows + row;
@@ -420,7 +429,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) 
             a.part2[2 * at] = m == -INFINITY ? m : m * a.scale2;
             a.part2[2 * at + 1] = l;
         }
-        return;
+        continue;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     at_store<T, DP>((T *)a.out + row * a.Dv, acc, a.Dv, h, [&](float x) { return x * inv; });
@@ -428,6 +437,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) 
         at_store<T, DP>((T *)a.outres + row * a.Dv, acc, a.Dv, h,
                         [&](float x) { const float y = x * inv; return y - tk_up(tk_down<T>(y)); });
     if (a.lse && h == 0) a.lse[row] = m == -INFINITY ? INFINITY : m * a.scale2 + __builtin_amdgcn_logf(l);   // +inf: an empty row
+    }
 }
 
 // joins the splits of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  One wave per row.
@@ -489,7 +499,12 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const AtBlock w0 = at_block(a, a.pack ? 1 : a.H / a.Hk);
     const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk, hb = hk * grp + w0.gi, nrows = a.pack ? grp * a.Tq : a.Tq;
-    const int L = at_length(a, b), r0 = (a.causal ? a.tiles - 1 - w0.tile : w0.tile) * AT_ROWS, r = r0 + wave * 32 + (lane & 31);
+    const int L = at_length(a, b);
+    for (int half = 0; half < 2; ++half) {
+    const int tile = at_tile_of(a, w0.tile, half, a.causal);
+    if (tile < 0) break;
+    if (half) __syncthreads();
+    const int r0 = tile * AT_ROWS, r = r0 + wave * 32 + (lane & 31);
     const AtRow w = at_query_row(a, r, hb, nrows, L);
     int j0, j1;
     at_key_range(a, L, (r0 + AT_ROWS < nrows ? r0 + AT_ROWS : nrows) - 1, nrows, sp, KT, j0, j1);
@@ -544,13 +559,14 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
             at_accumulate<T, DP>(acc, Ks[buf], 32 * n, s, lane);
         }
     }
-    if (!w.valid) return;
+    if (!w.valid) continue;
     if (a.nsplit > 1) {
         const long long rows = (long long)a.B * a.Tq * a.H;
         at_store<float, DP>(a.part + (sp * rows + row) * a.Dk, acc, a.Dk, h, [&](float x) { return x * a.scale; });
-        return;
+        continue;
     }
     at_store<T, DP>((T *)a.dq + row * a.Dk, acc, a.Dk, h, [&](float x) { return x * a.scale; });
+    }
 }
 
 template <typename T, int DP, bool MASK, int WHAT>
@@ -562,7 +578,12 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const AtBlock w0 = at_block(a, 1);
     const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk;
-    const int L = at_length(a, b), off = L - a.Tq, key0 = w0.tile * AT_ROWS, key = key0 + wave * 32 + (lane & 31);
+    const int L = at_length(a, b), off = L - a.Tq;
+    for (int half = 0; half < 2; ++half) {
+    const int ktile = at_tile_of(a, w0.tile, half, false);
+    if (ktile < 0) break;
+    if (half) __syncthreads();
+    const int key0 = ktile * AT_ROWS, key = key0 + wave * 32 + (lane & 31);
     const bool valid = key < a.Tk;
     const int kc = valid ? key : a.Tk - 1;
     // queries that see this key: [first, Tq)
@@ -652,16 +673,17 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
             if constexpr (DK) at_accumulate<T, DP>(acck, Qs[buf], 32 * n, dp, lane);
         }
     }
-    if (!valid) return;
+    if (!valid) continue;
     const long long row = ((long long)b * a.Tk + key) * a.Hk + hk;
     if (a.nsplit > 1) {
         const long long at = sp * ((long long)a.B * a.Tk * a.Hk) + row;
         if constexpr (DK) at_store<float, DP>(a.part + at * a.Dk, acck, a.Dk, h, [&](float x) { return x * a.scale; });
         if constexpr (DV) at_store<float, DP>(a.part2 + at * a.Dv, accv, a.Dv, h, [](float x) { return x; });
-        return;
+        continue;
     }
     if constexpr (DK) at_store<T, DP>((T *)a.dk + row * a.Dk, acck, a.Dk, h, [&](float x) { return x * a.scale; });
     if constexpr (DV) at_store<T, DP>((T *)a.dv + row * a.Dv, accv, a.Dv, h, [](float x) { return x; });
+    }
 }
 
 // out = sum over splits, in split order
@@ -687,7 +709,8 @@ static int at_splits(long long groups, long long steps) {
     return n < 1 ? 1 : (int)n;
 }
 struct AtPlan {
-    int pack, q_tiles, q_heads, q_split, k_tiles, k_split;
+    int pack, q_tiles, q_heads, q_split, q_pair, k_tiles, k_split, k_pair;
+    long long q_blocks, k_blocks;
 };
 static AtPlan at_plan(const hno_attn_t *p) {
     AtPlan n;
@@ -695,9 +718,16 @@ static AtPlan at_plan(const hno_attn_t *p) {
     n.pack = grp > 1 && p->Tq < AT_ROWS;
     n.q_tiles = ceil_div(n.pack ? grp * p->Tq : p->Tq, AT_ROWS);
     n.q_heads = n.pack ? p->Hk : p->H;
-    n.q_split = at_splits((long long)n.q_tiles * n.q_heads * p->B, ceil_div(p->Tk, KT));
     n.k_tiles = ceil_div(p->Tk, AT_ROWS);
-    n.k_split = at_splits((long long)n.k_tiles * p->Hk * p->B, (long long)ceil_div(p->Tq, KT) * grp);
+    long long q = (long long)n.q_heads * p->B, k = (long long)p->Hk * p->B;
+    n.q_pair = p->causal && q * n.q_tiles <= 1024;
+    n.k_pair = p->causal && k * n.k_tiles <= 1024;
+    q *= n.q_pair ? (n.q_tiles + 1) / 2 : n.q_tiles;
+    k *= n.k_pair ? (n.k_tiles + 1) / 2 : n.k_tiles;
+    n.q_split = at_splits(q, ceil_div(p->Tk, KT));
+    n.k_split = at_splits(k, (long long)ceil_div(p->Tq, KT) * grp);
+    n.q_blocks = q * n.q_split;
+    n.k_blocks = k * n.k_split;
     return n;
 }
 static size_t at_pad(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -757,11 +787,11 @@ static int at_forward(const hno_attn_t *p, void *out, void *out_res, float *lse,
     const AtPlan n = at_plan(p);
     AttnArgs a = at_args(p);
     const long long rows = (long long)p->B * p->Tq * p->H;
-    a.out = out; a.outres = out_res; a.lse = lse; a.pack = n.pack; a.nsplit = n.q_split; a.tiles = n.q_tiles;
+    a.out = out; a.outres = out_res; a.lse = lse; a.pack = n.pack; a.nsplit = n.q_split; a.tiles = n.q_tiles, a.pair = n.q_pair;
     a.part = (float *)workspace;
     a.part2 = (float *)((char *)workspace + at_pad((size_t)n.q_split * rows * p->Dv * sizeof(float)));
     ProfScope _ps(KID_ATTN, s, at_bytes(p, 2, 2));
-    AT_DISPATCH(attn_fwd_kernel, (long long)n.q_tiles * n.q_heads * p->B * n.q_split, s, a);
+    AT_DISPATCH(attn_fwd_kernel, n.q_blocks, s, a);
     HNO_CHECK_LAUNCH();
     if (n.q_split > 1) {
         hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, (const float *)a.part, (const float *)a.part2,
@@ -773,8 +803,7 @@ static int at_forward(const hno_attn_t *p, void *out, void *out_res, float *lse,
 
 // dk and dv in one kernel, or each in its own (where one kernel would not leave registers for two waves per SIMD)
 template <typename T>
-static int at_launch_dkv(AttnArgs a, unsigned n_, hipStream_t s) {
-    a.fold = a.causal && n_ <= 512;
+static int at_launch_dkv(const AttnArgs &a, unsigned n_, hipStream_t s) {
     const int dp = round_up(a.Dk > a.Dv ? a.Dk : a.Dv, 32);
     if (dp == 32) AT_LAUNCH(attn_dkv_kernel, 32, , 3);
     else if (dp == 64) AT_LAUNCH(attn_dkv_kernel, 64, , 3);
@@ -819,8 +848,8 @@ static int at_backward(const hno_attn_t *p, const void *out, const void *out_res
         ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 3, 2));
         a.pack = n.pack;
         a.nsplit = n.q_split;
-        a.tiles = n.q_tiles;
-        AT_DISPATCH(attn_dq_kernel, (long long)n.q_tiles * n.q_heads * p->B * n.q_split, s, a);
+        a.tiles = n.q_tiles, a.pair = n.q_pair;
+        AT_DISPATCH(attn_dq_kernel, n.q_blocks, s, a);
         HNO_CHECK_LAUNCH();
         if (n.q_split > 1)
             if (int rc = at_sum(a.part, (T *)dq, rows * p->Dk, n.q_split, s)) return rc;
@@ -828,9 +857,9 @@ static int at_backward(const hno_attn_t *p, const void *out, const void *out_res
     if (dk && p->Tk > 0) {
         ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 2, 4));
         a.nsplit = n.k_split;
-        a.tiles = n.k_tiles;
+        a.tiles = n.k_tiles, a.pair = n.k_pair;
         a.part2 = (float *)((char *)a.part + at_pad((size_t)n.k_split * krows * p->Dk * sizeof(float)));
-        if (int rc = at_launch_dkv<T>(a, (unsigned)((long long)n.k_tiles * p->Hk * p->B * n.k_split), s)) return rc;
+        if (int rc = at_launch_dkv<T>(a, (unsigned)n.k_blocks, s)) return rc;
         HNO_CHECK_LAUNCH();
         if (n.k_split > 1) {
             if (int rc = at_sum(a.part, (T *)dk, krows * p->Dk, n.k_split, s)) return rc;
