@@ -116,20 +116,14 @@ struct AtTile<tkh, DP, ROWS> {
         const unsigned dst = (unsigned)(uintptr_t)(ldsp)tile + (tid >> 6) * 1024;
         if (t0 + ROWS <= end) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) dma(src, off[i], dst + i * 4096);
+            for (int i = 0; i < N; ++i) tk_dma16(src, off[i], dst + i * 4096);
         } else {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int r = row(i, tid), c = chunk(i, tid) * 8, last = end - 1 - t0;
-                dma(src, (unsigned)((r < last ? r : last) * st + (c < D ? c : 0)) * 2, dst + i * 4096);
+                tk_dma16(src, (unsigned)((r < last ? r : last) * st + (c < D ? c : 0)) * 2, dst + i * 4096);
             }
         }
-    }
-    // 64 lanes x 16 bytes to 1024 consecutive LDS bytes; M0 holds the destination
-    __device__ __forceinline__ static void dma(const tkh *src, unsigned off, unsigned dst) {
-        unsigned keep;
-        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-                     : "=&s"(keep) : "v"(off), "s"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory");
     }
     template <typename P>
     __device__ __forceinline__ void settle(tkh *tile, int tid, P dead) const {
@@ -341,7 +335,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) 
     const AtRow w = at_query_row(a, r, hb, nrows, L);
     int j0, j1;
     at_key_range(a, L, (r0 + AT_ROWS < nrows ? r0 + AT_ROWS : nrows) - 1, nrows, sp, KT, j0, j1);
-    const int lim_all = MASK ? 0 : at_wave_min(w.lim);
+    const int lim_all = MASK ? 0 : at_wave_min(w.lim), lim_any = -at_wave_min(-w.lim);
 
     TkFrag<T> qf[DP / 16];
     const T *qrow = (const T *)a.q + b * a.qs[0] + (long long)w.i * a.qs[1] + w.head * a.qs[2];
@@ -374,6 +368,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) 
         settle(buf);
         __syncthreads();
         if (j + KT < j1) fetch(buf ^ 1, j + KT);
+        if (j >= lim_any) continue;             // none of this wave's rows sees the tile
         tk16 s[KT / 32];
         AtMask mk[KT / 32];
         if (MASK)
@@ -440,35 +435,67 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) 
     }
 }
 
-// joins the splits of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  One wave per row.
+// joins the splits of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  32 lanes of 4 channels; the 8 groups of lanes share the splits of one
+// row (many splits, few rows: 32 splits of 64 rows took 35 us with one wave per row) or take a row each.  Each lane loads its (at most 8)
+// splits at once.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_join_kernel(const float *__restrict__ part, const float *__restrict__ ml, T *__restrict__ out,
                                                         T *__restrict__ outres, float *__restrict__ lse, long long rows, int Dv, int nsplit) {
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (row >= rows) return;
-    float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < nsplit; ++s) m = fmaxf(m, ml[2 * (s * rows + row)]);
-    const float shift = m == -INFINITY ? 0.f : m;
-    float x[2] = {0.f, 0.f};
-    for (int s = 0; s < nsplit; ++s) {
+    __shared__ tkf4 sum[8][32];
+    __shared__ float wsum[8][32], top[8][32];
+    const int c = threadIdx.x & 31, y = threadIdx.x >> 5, ys = nsplit >= 8 ? 8 : 1, s0 = ys > 1 ? y : 0;
+    const long long row = ys > 1 ? blockIdx.x : (long long)blockIdx.x * 8 + y;
+    const bool on = row < rows, in = on && 4 * c < Dv;
+    float ms[8], ls[8], m = -INFINITY, l = 0.f;
+    tkf4 xs[8], x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int s = s0 + k * ys;
         const long long at = s * rows + row;
-        const float f = __builtin_amdgcn_exp2f(ml[2 * at] - shift);
-        l += f * ml[2 * at + 1];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-            if (lane + 64 * u < Dv) x[u] += f * part[at * Dv + lane + 64 * u];
+        ms[k] = on && s < nsplit ? ml[2 * at] : -INFINITY;
+        ls[k] = on && s < nsplit ? ml[2 * at + 1] : 0.f;
+        xs[k] = in && s < nsplit ? *reinterpret_cast<const tkf4 *>(part + at * Dv + 4 * c) : tkf4{0.f, 0.f, 0.f, 0.f};
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-        if (lane + 64 * u < Dv) {
-            const float y = x[u] * inv;
-            const T t = tk_down<T>(y);
-            out[row * Dv + lane + 64 * u] = t;
-            if (sizeof(T) == 2 && outres) outres[row * Dv + lane + 64 * u] = tk_down<T>(y - tk_up(t));
+    for (int k = 0; k < 8; ++k) m = fmaxf(m, ms[k]);
+    const float shift = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float f = __builtin_amdgcn_exp2f(ms[k] - shift);
+        l = fmaf(f, ls[k], l);
+        x += f * xs[k];
+    }
+    if (ys > 1) {
+        sum[y][c] = x, wsum[y][c] = l, top[y][c] = m;
+        __syncthreads();
+        if (y) return;
+        float all = m;
+        for (int k = 1; k < 8; ++k) all = fmaxf(all, top[k][c]);
+        const float base = all == -INFINITY ? 0.f : all;
+        x = tkf4{0.f, 0.f, 0.f, 0.f}, l = 0.f;
+        for (int k = 0; k < 8; ++k) {
+            const float f = __builtin_amdgcn_exp2f(top[k][c] - base);
+            l = fmaf(f, wsum[k][c], l);
+            x += f * sum[k][c];
         }
-    if (lse && lane == 0) lse[row] = m == -INFINITY ? INFINITY : m + __builtin_amdgcn_logf(l);
+        m = all;
+    }
+    if (!on) return;
+    if (lse && c == 0) lse[row] = m == -INFINITY ? INFINITY : m + __builtin_amdgcn_logf(l);
+    if (!in) return;
+    x *= l == 0.f ? 0.f : 1.f / l;
+    if constexpr (sizeof(T) == 2) {
+        tks4 t, r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            t[j] = (short)tk_down<T>(x[j]);
+            r[j] = (short)tk_down<T>(x[j] - tk_up((T)t[j]));
+        }
+        *reinterpret_cast<tks4 *>(out + row * Dv + 4 * c) = t;
+        if (outres) *reinterpret_cast<tks4 *>(outres + row * Dv + 4 * c) = r;
+    } else {
+        *reinterpret_cast<tkf4 *>(out + row * Dv + 4 * c) = x;
+    }
 }
 
 // D_i = sum_c do_ic o_ic.  16 lanes per row.
@@ -520,7 +547,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
     const T *kb = (const T *)a.k + b * a.ks[0] + hk * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + hk * a.vs[2];
     const unsigned char *mrow = MASK ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
     const unsigned char *mkey = MASK && a.keymask ? a.mask + b * a.ms[0] + hb * a.ms[1] : nullptr;
-    const int lim_all = MASK ? 0 : at_wave_min(w.lim);
+    const int lim_all = MASK ? 0 : at_wave_min(w.lim), lim_any = -at_wave_min(-w.lim);
     AtTile<T, DP, KT> ks, vs;
     AtFlags<T, DP, KT, unsigned char> flag;
     ks.init(a.ks[1], a.Dk, tid);
@@ -541,6 +568,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
         settle(buf);
         __syncthreads();
         if (j + KT < j1) fetch(buf ^ 1, j + KT);
+        if (j >= lim_any) continue;             // none of this wave's rows sees the tile
         const bool whole = j + KT <= lim_all;
 #pragma unroll
         for (int n = 0; n < KT / 32; ++n) {
@@ -686,13 +714,30 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
     }
 }
 
-// out = sum over splits, in split order
+// out = sum over splits, in split order, of one or two tensors (4 elements a thread; n is a multiple of 8)
+struct AtSum {
+    const float *part[2];
+    void *out[2];
+    long long n[2];
+};
 template <typename T>
-__global__ __launch_bounds__(256) void attn_sum_kernel(const float *__restrict__ part, T *__restrict__ out, long long n, int nsplit) {
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-        float s = part[i];
-        for (int k = 1; k < nsplit; ++k) s += part[k * n + i];
-        out[i] = tk_down<T>(s);
+__global__ __launch_bounds__(256) void attn_sum_kernel(AtSum a, int nsplit) {
+    long long i = 4 * ((long long)blockIdx.x * 256 + threadIdx.x);
+    const int k = i >= a.n[0];
+    if (k) i -= a.n[0];
+    const long long n = a.n[k];
+    if (i >= n) return;
+    const float *p = a.part[k] + i;
+    tkf4 x = *reinterpret_cast<const tkf4 *>(p);
+#pragma unroll 4
+    for (int s = 1; s < nsplit; ++s) x += *reinterpret_cast<const tkf4 *>(p + s * n);
+    if constexpr (sizeof(T) == 2) {
+        tks4 t;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = (short)tk_down<T>(x[j]);
+        *reinterpret_cast<tks4 *>((T *)a.out[k] + i) = t;
+    } else {
+        *reinterpret_cast<tkf4 *>((T *)a.out[k] + i) = x;
     }
 }
 
@@ -794,7 +839,7 @@ static int at_forward(const hno_attn_t *p, void *out, void *out_res, float *lse,
     AT_DISPATCH(attn_fwd_kernel, n.q_blocks, s, a);
     HNO_CHECK_LAUNCH();
     if (n.q_split > 1) {
-        hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, (const float *)a.part, (const float *)a.part2,
+        hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)(n.q_split >= 8 ? rows : (rows + 7) / 8)), dim3(256), 0, s, (const float *)a.part, (const float *)a.part2,
                            (T *)out, (T *)out_res, lse, rows, p->Dv, n.q_split);
         HNO_CHECK_LAUNCH();
     }
@@ -822,9 +867,8 @@ static int at_launch_dkv(const AttnArgs &a, unsigned n_, hipStream_t s) {
 }
 
 template <typename T>
-static int at_sum(const float *part, T *out, long long n, int nsplit, hipStream_t s) {
-    const long long blocks = (n + 255) / 256;
-    hipLaunchKernelGGL((attn_sum_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, part, out, n, nsplit);
+static int at_sum(const AtSum &a, int nsplit, hipStream_t s) {
+    hipLaunchKernelGGL((attn_sum_kernel<T>), dim3((unsigned)((a.n[0] + a.n[1] + 1023) / 1024)), dim3(256), 0, s, a, nsplit);
     HNO_CHECK_LAUNCH();
     return HNO_OK;
 }
@@ -852,7 +896,7 @@ static int at_backward(const hno_attn_t *p, const void *out, const void *out_res
         AT_DISPATCH(attn_dq_kernel, n.q_blocks, s, a);
         HNO_CHECK_LAUNCH();
         if (n.q_split > 1)
-            if (int rc = at_sum(a.part, (T *)dq, rows * p->Dk, n.q_split, s)) return rc;
+            if (int rc = at_sum<T>({{a.part, nullptr}, {dq, nullptr}, {rows * p->Dk, 0}}, n.q_split, s)) return rc;
     }
     if (dk && p->Tk > 0) {
         ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 2, 4));
@@ -861,10 +905,8 @@ static int at_backward(const hno_attn_t *p, const void *out, const void *out_res
         a.part2 = (float *)((char *)a.part + at_pad((size_t)n.k_split * krows * p->Dk * sizeof(float)));
         if (int rc = at_launch_dkv<T>(a, (unsigned)n.k_blocks, s)) return rc;
         HNO_CHECK_LAUNCH();
-        if (n.k_split > 1) {
-            if (int rc = at_sum(a.part, (T *)dk, krows * p->Dk, n.k_split, s)) return rc;
-            if (int rc = at_sum(a.part2, (T *)dv, krows * p->Dv, n.k_split, s)) return rc;
-        }
+        if (n.k_split > 1)
+            if (int rc = at_sum<T>({{a.part, a.part2}, {dk, dv}, {krows * p->Dk, krows * p->Dv}}, n.k_split, s)) return rc;
     }
     return HNO_OK;
 }

@@ -15,164 +15,265 @@ struct LinArgs {
     void *z, *y;
     float *part;
     long long lda, ldb;
-    int M, N, K, va, vb, vc, act, bias32, out32, nsplit;
+    int M, N, K, act, bias32, out32, nsplit;
 };
 
-constexpr int LN_T = 128;                                   // tile: 128 x 128, four waves of 64 x 64
+// Tiles: 256 x 256 by 8 waves of 128 x 64, or 128 x 128 by 4 waves of 64 x 64 (small results); KB contraction elements a step.  With 64 x 64 per wave the
+// LDS reads of a step take as long as its matrix instructions, with 128 x 64 three quarters.
+template <int TILE> struct LnTile;
+template <> struct LnTile<256> { static constexpr int WAVES = 8, WM = 128, WN = 64; };
+template <> struct LnTile<128> { static constexpr int WAVES = 4, WM = 64, WN = 64; };
+
+// fp32: a value is three bf16 terms, its leading 8 bits, the next 8 and the last 8 (cut, not rounded: their sum is the value), and a product is the six products
+// of terms down to 2^-16 on the bf16 matrix instruction -- the two dropped ones are 2^-22 at most, 2^-25 on average, of the product.
+// An fp32 matrix instruction takes 1.3 times as long for the same work (and more than twice counting that six need one set of operands).
+template <typename T> constexpr int ln_planes() { return sizeof(T) == 2 ? 1 : 3; }
 template <typename T> constexpr int ln_kb() { return sizeof(T) == 2 ? 64 : 32; }
 
-// tile of one operand: `along` k: LN_T rows of KB; across: KB rows of LN_T
-template <typename T, bool ACROSS> constexpr int ln_stride() { return (ACROSS ? LN_T : ln_kb<T>()) + tk_pad<T>(); }
-template <typename T, bool ACROSS> constexpr int ln_tile() { return (ACROSS ? ln_kb<T>() : LN_T) * ln_stride<T, ACROSS>(); }
-
-template <typename T, bool ACROSS>
-__device__ __forceinline__ void ln_stage(T *tile, const T *base, long long ld, int m0, int M, int k0, int K, bool vec, int tid) {
-    constexpr int KB = ln_kb<T>(), S = ln_stride<T, ACROSS>(), W = ACROSS ? LN_T : KB, R = ACROSS ? KB : LN_T, CH = W / 8;
-    const int row0 = ACROSS ? k0 : m0, rows = ACROSS ? K : M, col0 = ACROSS ? m0 : k0, cols = ACROSS ? M : K;
-#pragma unroll
-    for (int c = tid; c < R * CH; c += 256) {
-        const int row = c / CH, d = (c - row * CH) * 8;
-        TkFrag<T> f;
-        if (row0 + row < rows) {
-            f = tk_load8(base + (long long)(row0 + row) * ld, col0 + d, cols, vec);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f.set(j, 0.f);
-        }
-        tk_store8(tile + row * S + d, f);
-    }
-}
-template <typename T, bool ACROSS>
-__device__ __forceinline__ TkFrag<T> ln_frag(const T *tile, int m0, int kk, int lane) {
-    constexpr int S = ln_stride<T, ACROSS>();
-    const int k = 16 * kk + 8 * (lane >> 5);
-    if constexpr (ACROSS) return tk_col(tile, S, m0, k, k + 4, lane);
-    else return tk_row(tile + (m0 + (lane & 31)) * S + k);
+// Where 8 elements (chunk c of row r) of an operand's LDS tile stand.  Along k: TILE rows of KB; 16 consecutive rows at one chunk touch all banks.
+// Across: KB rows of TILE; 4 consecutive rows at four neighbouring chunks touch all banks (the transposed reads).
+template <int TILE, int KB, bool ACROSS>
+__device__ __forceinline__ int ln_at(int r, int c) {
+    if constexpr (ACROSS) return r * TILE + (c ^ ((r & 3) << 2)) * 8;
+    else if constexpr (KB == 64) return r * KB + (c ^ ((((r >> 1) & 1) << 2) | ((r >> 2) & 3))) * 8;
+    else return r * KB + (c ^ ((r >> 2) & 3)) * 8;
 }
 
-// the epilogue of four neighbouring columns n .. n + 3 of row m
-template <typename T>
-__device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float (&x)[4]) {
-    const int cnt = a.N - n < 4 ? a.N - n : 4;
-    const long long at = (long long)m * a.N + n;
-    if (a.bias) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < cnt) x[j] += a.bias32 ? ((const float *)a.bias)[n + j] : tk_up(((const T *)a.bias)[n + j]);
+// A workgroup's share of one operand's tile: thread t moves the 8-element slots t, t + threads, ...
+template <typename T, int TILE, bool ACROSS, bool DMA>
+struct LnStage {
+    static constexpr int KB = ln_kb<T>(), NT = 64 * LnTile<TILE>::WAVES, CH = (ACROSS ? TILE : KB) / 8, N = TILE * KB / 8 / NT, PLANE = TILE * KB;
+    static constexpr int NR = DMA ? 1 : N;
+    TkFrag<T> r[NR];
+    const T *base;
+    long long ld;
+    int rows, cols, row0, col0;          // of the stored matrix, and the tile's corner (the corner along k moves)
+    __device__ __forceinline__ void init(const void *p, long long ld_, int m0, int M, int K) {
+        base = (const T *)p, ld = ld_;
+        rows = ACROSS ? K : M, cols = ACROSS ? M : K, row0 = ACROSS ? 0 : m0, col0 = ACROSS ? m0 : 0;
     }
-    T zs[4];
-    float r[4] = {0.f, 0.f, 0.f, 0.f};
-    if (a.res) {
-        if (a.vc) {
-            if constexpr (sizeof(T) == 2) {
-                const tks4 t = *reinterpret_cast<const tks4 *>((const T *)a.res + at);
+    __device__ __forceinline__ static int row(int i, int tid) { return (tid + NT * i) / CH; }
+    __device__ __forceinline__ static int chunk(int i, int tid) { return (tid + NT * i) % CH; }
+    // DMA (16-byte aligned rows, whole chunks): the chunk whose place the slot is
+    __device__ __forceinline__ static int source(int i, int tid) { return (ln_at<TILE, KB, ACROSS>(row(i, tid), chunk(i, tid)) / 8) % CH; }
+    __device__ __forceinline__ void fetch(tkh *tile, int k0, int tid) {
+        const int ra = ACROSS ? k0 : row0, ca = ACROSS ? col0 : k0;
+        const T *src = base + (long long)ra * ld + ca;
+        const bool whole = ra + (ACROSS ? KB : TILE) <= rows && ca + (ACROSS ? TILE : KB) <= cols;
+        if constexpr (DMA) {
+            typedef __attribute__((address_space(3))) tkh *ldsp;
+            const unsigned dst = (unsigned)(uintptr_t)(ldsp)tile + (tid >> 6) * 1024;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) r[j] = tk_up((tkh)t[j]);
-            } else {
-                const tkf4 t = *reinterpret_cast<const tkf4 *>((const T *)a.res + at);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) r[j] = t[j];
+            for (int i = 0; i < N; ++i) {
+                int rr = row(i, tid), cc = source(i, tid) * 8;
+                if (!whole) {            // beyond the matrix: any element of it (settle() clears what must not count)
+                    rr = min(rr, rows - 1 - ra);
+                    cc = ca + cc < cols ? cc : 0;
+                }
+                tk_dma16(src, (unsigned)(rr * (int)ld + cc) * 2, dst + i * NT * 16);
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < cnt) r[j] = tk_up(((const T *)a.res)[at + j]);
-        }
-    }
-    float y[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        zs[j] = tk_down<T>(x[j]);
-        y[j] = tk_act(x[j], a.act) + r[j];
-    }
-    if (a.z) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < cnt) ((T *)a.z)[at + j] = zs[j];
-    }
-    if (a.out32) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < cnt) ((float *)a.y)[at + j] = y[j];
-    } else if (a.vc && sizeof(T) == 2) {
-        tks4 w;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = (short)tk_down<tkh>(y[j]);
-        *reinterpret_cast<tks4 *>((tkh *)a.y + at) = w;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (j < cnt) ((T *)a.y)[at + j] = tk_down<T>(y[j]);
-    }
-}
-
-template <typename T, bool AX, bool BX>
-__global__ __launch_bounds__(256) void linear_kernel(LinArgs a) {
-    constexpr int KB = ln_kb<T>();
-    __shared__ __attribute__((aligned(16))) T As[ln_tile<T, AX>()];
-    __shared__ __attribute__((aligned(16))) T Bs[ln_tile<T, BX>()];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-    const int n0 = blockIdx.x * LN_T, m0 = blockIdx.y * LN_T;
-    const int steps = (a.K + KB - 1) / KB, per = (steps + a.nsplit - 1) / a.nsplit;
-    const int k1 = ((int)blockIdx.z + 1) * per < steps ? ((int)blockIdx.z + 1) * per : steps;
-    tk16 acc[2][2] = {};
-    for (int ks = blockIdx.z * per; ks < k1; ++ks) {
-        __syncthreads();
-        ln_stage<T, AX>(As, (const T *)a.A, a.lda, m0, a.M, ks * KB, a.K, a.va, tid);
-        ln_stage<T, BX>(Bs, (const T *)a.B, a.ldb, n0, a.N, ks * KB, a.K, a.vb, tid);
-        __syncthreads();
-#pragma unroll
-        for (int kk = 0; kk < KB / 16; ++kk) {
-            TkFrag<T> fa[2], fb[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                fa[u] = ln_frag<T, AX>(As, wm + 32 * u, kk, lane);
-                fb[u] = ln_frag<T, BX>(Bs, wn + 32 * u, kk, lane);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int v = 0; v < 2; ++v) acc[u][v] = tk_mma(fb[v], fa[u], acc[u][v]);
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int m = m0 + wm + 32 * u + (lane & 31);
-        if (m >= a.M) continue;
-#pragma unroll
-        for (int v = 0; v < 2; ++v)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int n = n0 + wn + 32 * v + 8 * q + 4 * h;
-                if (n >= a.N) continue;
-                float x[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = acc[u][v][4 * q + j];
-                if (a.nsplit > 1) {
-                    float *dst = a.part + ((long long)blockIdx.z * a.M + m) * a.N + n;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (n + j < a.N) dst[j] = x[j];
+            for (int i = 0; i < N; ++i) {
+                const int rr = row(i, tid), cc = chunk(i, tid) * 8;
+                if (whole || (ra + rr < rows && ca + cc + 8 <= cols)) {
+                    __builtin_memcpy(&r[i], src + rr * ld + cc, sizeof(T) * 8);          // any alignment
                 } else {
-                    ln_finish<T>(a, m, n, x);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) r[i].set(j, ra + rr < rows && ca + cc + j < cols ? tk_up(src[rr * ld + cc + j]) : 0.f);
                 }
             }
+        }
+    }
+    __device__ __forceinline__ void settle(tkh *tile, int k0, int K, int tid) {
+        if constexpr (DMA) {
+            if (k0 + KB > K)
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (k0 + (ACROSS ? row(i, tid) : source(i, tid) * 8) >= K) *reinterpret_cast<tku4 *>(tile + (tid + NT * i) * 8) = tku4{0, 0, 0, 0};
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                tkh *p = tile + ln_at<TILE, KB, ACROSS>(row(i, tid), chunk(i, tid));
+                if constexpr (sizeof(T) == 2) {
+                    tk_store8(p, r[i]);
+                } else {
+                    tku4 h[3];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        unsigned a = __float_as_uint(r[i].v[2 * j]), b = __float_as_uint(r[i].v[2 * j + 1]);
+#pragma unroll
+                        for (int t = 0; t < 3; ++t) {
+                            h[t][j] = __builtin_amdgcn_perm(b, a, 0x07060302);
+                            a = __float_as_uint(__uint_as_float(a) - __uint_as_float(a & 0xffff0000u));
+                            b = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xffff0000u));
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < 3; ++t) *reinterpret_cast<tku4 *>(p + t * PLANE) = h[t];
+                }
+            }
+        }
+    }
+};
+template <int TILE, int KB, bool ACROSS>
+__device__ __forceinline__ TkFrag<tkh> ln_frag(const tkh *tile, int m0, int kk, int lane) {
+    if constexpr (ACROSS) {
+        typedef __attribute__((address_space(3))) tks4 *lds4;
+        const int r = 16 * kk + 8 * (lane >> 5) + ((lane & 15) >> 2), d = m0 + (lane & 16) + 4 * (lane & 3);
+        const tks4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(tile + ln_at<TILE, KB, true>(r, d >> 3) + (d & 7)));
+        const tks4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(tile + ln_at<TILE, KB, true>(r + 4, d >> 3) + (d & 7)));
+        return {__builtin_bit_cast(tkb8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7))};
+    } else {
+        return tk_row(tile + ln_at<TILE, KB, false>(m0 + (lane & 31), 2 * kk + (lane >> 5)));
+    }
+}
+
+// 8 neighbouring values of a row, `cnt` of them inside it; any alignment
+template <typename T>
+__device__ __forceinline__ void ln_get8(const T *p, int cnt, float (&x)[8]) {
+    TkFrag<T> f;
+    if (cnt >= 8) {
+        __builtin_memcpy(&f, p, 8 * sizeof(T));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f.set(j, j < cnt ? tk_up(p[j]) : 0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = (float)f.v[j];
+}
+template <typename T>
+__device__ __forceinline__ void ln_put8(T *p, int cnt, const float (&x)[8]) {
+    if (cnt >= 8) {
+        TkFrag<T> f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f.set(j, x[j]);
+        __builtin_memcpy(p, &f, 8 * sizeof(T));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < cnt) p[j] = tk_down<T>(x[j]);
+    }
+}
+// the epilogue of columns n .. n + 7 of row m
+template <typename T>
+__device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float (&x)[8]) {
+    const int cnt = a.N - n;
+    const long long at = (long long)m * a.N + n;
+    float t[8];
+    if (a.bias) {
+        if (a.bias32) ln_get8((const float *)a.bias + n, cnt, t);
+        else ln_get8((const T *)a.bias + n, cnt, t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] += t[j];
+    }
+    if (a.z) ln_put8((T *)a.z + at, cnt, x);
+    if (a.act != HNO_ACT_NONE) tk_act8(x, a.act);
+    if (a.res) {
+        ln_get8((const T *)a.res + at, cnt, t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] += t[j];
+    }
+    if (a.out32) ln_put8((float *)a.y + at, cnt, x);
+    else ln_put8((T *)a.y + at, cnt, x);
+}
+
+// DMA: two LDS buffers, the next step's tiles on their way while this one is multiplied.  Else the next step's tiles wait in registers: one buffer.
+template <typename T, bool AX, bool BX, int TILE, bool DMA>
+__global__ __launch_bounds__(64 * LnTile<TILE>::WAVES, 2) void linear_kernel(LinArgs a) {
+    constexpr int KB = ln_kb<T>(), P = ln_planes<T>(), WM = LnTile<TILE>::WM, WN = LnTile<TILE>::WN, NB = DMA ? 2 : 1, PLANE = TILE * KB;
+    constexpr int ES = WN + 4, EP = 2 * LnTile<TILE>::WAVES * 32 * ES, TILES = 2 * NB * P * PLANE;         // (epilogue: 32 rows of floats a wave)
+    __shared__ __attribute__((aligned(16))) tkh smem[EP > TILES ? EP : TILES];
+    typedef tkh Tile[NB][P * PLANE];
+    Tile &As = *reinterpret_cast<Tile *>(smem), &Bs = *reinterpret_cast<Tile *>(smem + NB * P * PLANE);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, wm = (wave % (TILE / WM)) * WM, wn = (wave / (TILE / WM)) * WN;
+    // every XCD takes one run of the list of tiles; neighbours in a run share rows (bands of 4 tile rows, column by column)
+    const int tm = (a.M + TILE - 1) / TILE, tn = (a.N + TILE - 1) / TILE, each = gridDim.x >> 3, more = gridDim.x & 7, xcd = blockIdx.x & 7;
+    int at = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
+    const int run = at / (tm * tn);
+    at -= run * tm * tn;
+    const int band = at / (4 * tn), bm = min(4, tm - 4 * band), m0 = (4 * band + (at - band * 4 * tn) % bm) * TILE, n0 = ((at - band * 4 * tn) / bm) * TILE;
+    const int steps = (a.K + KB - 1) / KB, per = (steps + a.nsplit - 1) / a.nsplit, k1 = min((run + 1) * per, steps);
+    LnStage<T, TILE, AX, DMA> sa;
+    LnStage<T, TILE, BX, DMA> sb;
+    sa.init(a.A, a.lda, m0, a.M, a.K);
+    sb.init(a.B, a.ldb, n0, a.N, a.K);
+    tk16 acc[WM / 32][WN / 32] = {};
+    int buf = 0;
+    if (run * per < k1) {
+        sa.fetch(As[0], run * per * KB, tid);
+        sb.fetch(Bs[0], run * per * KB, tid);
+    }
+    for (int ks = run * per; ks < k1; ++ks) {
+        if constexpr (DMA) dma_wait<0>();
+        else __syncthreads();
+        sa.settle(As[buf], ks * KB, a.K, tid);
+        sb.settle(Bs[buf], ks * KB, a.K, tid);
+        __syncthreads();
+        if (ks + 1 < k1) {
+            sa.fetch(As[buf ^ (NB - 1)], (ks + 1) * KB, tid);
+            sb.fetch(Bs[buf ^ (NB - 1)], (ks + 1) * KB, tid);
+        }
+#pragma unroll
+        for (int kk = 0; kk < KB / 16; ++kk) {
+            TkFrag<tkh> fa[P][WM / 32], fb[P][WN / 32];
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+#pragma unroll
+                for (int u = 0; u < WM / 32; ++u) fa[p][u] = ln_frag<TILE, KB, AX>(As[buf] + p * PLANE, wm + 32 * u, kk, lane);
+#pragma unroll
+                for (int v = 0; v < WN / 32; ++v) fb[p][v] = ln_frag<TILE, KB, BX>(Bs[buf] + p * PLANE, wn + 32 * v, kk, lane);
+            }
+#pragma unroll
+            for (int t = P - 1; t >= 0; --t)          // smallest terms first
+#pragma unroll
+                for (int p = 0; p <= t; ++p)
+#pragma unroll
+                    for (int u = 0; u < WM / 32; ++u)
+#pragma unroll
+                        for (int v = 0; v < WN / 32; ++v) acc[u][v] = tk_mma(fb[p][v], fa[t - p][u], acc[u][v]);
+        }
+        buf ^= NB - 1;
+    }
+    // the results change places in LDS, 32 rows of a wave at a time (its own part: no barrier inside), so that memory is read and written in runs of 128 bytes
+    __syncthreads();
+    float *ep = reinterpret_cast<float *>(smem) + wave * 32 * ES;
+#pragma unroll
+    for (int u = 0; u < WM / 32; ++u) {
+#pragma unroll
+        for (int v = 0; v < WN / 32; ++v)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<tkf4 *>(ep + (lane & 31) * ES + 32 * v + 8 * q + 4 * h) =
+                    tkf4{acc[u][v][4 * q], acc[u][v][4 * q + 1], acc[u][v][4 * q + 2], acc[u][v][4 * q + 3]};
+#pragma unroll 1
+        for (int e = lane; e < 32 * WN / 8; e += 64) {
+            const int r = e / (WN / 8), c = (e - r * (WN / 8)) * 8, m = m0 + wm + 32 * u + r, n = n0 + wn + c;
+            const TkFrag<float> f = tk_row(ep + r * ES + c);
+            if (m >= a.M || n >= a.N) continue;
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = f.v[j];
+            if (a.nsplit > 1) ln_put8(a.part + ((long long)run * a.M + m) * a.N + n, a.N - n, x);
+            else ln_finish<T>(a, m, n, x);
+        }
     }
 }
 
 // sum of the runs' slabs, then the epilogue
 template <typename T>
 __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a) {
-    const int per_row = (a.N + 3) / 4;
+    const int per_row = (a.N + 7) / 8;
     const long long items = (long long)a.M * per_row, slab = (long long)a.M * a.N;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < items; i += (long long)gridDim.x * 256) {
-        const int m = (int)(i / per_row), n = 4 * (int)(i - (long long)m * per_row);
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        const int m = (int)(i / per_row), n = 8 * (int)(i - (long long)m * per_row);
+        const float *src = a.part + (long long)m * a.N + n;
+        float x[8] = {}, t[8];
+#pragma unroll 4
         for (int s = 0; s < a.nsplit; ++s) {
-            const float *src = a.part + s * slab + (long long)m * a.N + n;
+            ln_get8(src + s * slab, a.N - n, t);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n + j < a.N) x[j] += src[j];
+            for (int j = 0; j < 8; ++j) x[j] += t[j];
         }
         ln_finish<T>(a, m, n, x);
     }
@@ -224,13 +325,27 @@ __global__ __launch_bounds__(1024) void linear_db_kernel(const float *__restrict
 
 using namespace hno;
 
-// runs of the contraction: enough workgroups for the chip, no run shorter than four steps
-static int ln_splits(int M, int N, int K, int kb) {
-    const long long tiles = (long long)ceil_div(M, LN_T) * ceil_div(N, LN_T), steps = ceil_div(K, kb);
-    long long n = tiles >= 256 ? 1 : (512 + tiles - 1) / tiles;
-    if (n > steps / 4) n = steps / 4;
-    if (n > 64) n = 64;
-    return n < 1 ? 1 : (int)n;
+// tile and runs of the contraction.  256 x 256 where its tiles fill most of the chip's 256 CUs by themselves; else 128 x 128, and the contraction cut into runs (of
+// four steps at least) until there are two workgroups per CU.
+struct LnPlan {
+    int tile, nsplit;
+    long long blocks;
+};
+static LnPlan ln_plan(int M, int N, int K, int kb) {
+    LnPlan p;
+    long long tiles = (long long)ceil_div(M, 256) * ceil_div(N, 256);
+    p.tile = tiles >= 192 && kb == 64 ? 256 : 128;
+    p.nsplit = 1;
+    if (p.tile == 128) {
+        tiles = (long long)ceil_div(M, 128) * ceil_div(N, 128);
+        const long long steps = ceil_div(K, kb);
+        long long n = tiles >= 256 ? 1 : 512 / tiles;
+        if (n > steps / 4) n = steps / 4;
+        if (n > 64) n = 64;
+        p.nsplit = n < 1 ? 1 : (int)n;
+    }
+    p.blocks = tiles * p.nsplit;
+    return p;
 }
 static int ln_runs(int M) { return M <= 64 ? 1 : (ceil_div(M, 64) < 256 ? ceil_div(M, 64) : 256); }
 static size_t ln_pad(size_t b) { return (b + 255) / 256 * 256; }
@@ -239,16 +354,25 @@ static bool ln_aligned(const void *p, long long ld, int esz) { return (reinterpr
 template <typename T, bool AX, bool BX>
 static int ln_product(LinArgs a, hipStream_t s, int kid) {
     const int esz = sizeof(T);
-    // 16-byte reads: the read axis of each operand in whole chunks of 8
-    a.va = ln_aligned(a.A, a.lda, esz) && (AX ? a.M : a.K) % 8 == 0;
-    a.vb = ln_aligned(a.B, a.ldb, esz) && (BX ? a.N : a.K) % 8 == 0;
-    a.vc = a.N % 4 == 0 && ln_aligned(a.y, 0, 1) && ln_aligned(a.res, 0, 1) && !a.out32;
-    a.nsplit = ln_splits(a.M, a.N, a.K, ln_kb<T>());
+    // DMA: whole 16-byte chunks along the stored axis of each operand, and offsets within a tile in 32 bits
+    const bool dma = esz == 2 && ln_aligned(a.A, a.lda, esz) && (AX ? a.M : a.K) % 8 == 0 && ln_aligned(a.B, a.ldb, esz) && (BX ? a.N : a.K) % 8 == 0 &&
+                     a.lda < (1 << 22) && a.ldb < (1 << 22);
+    const LnPlan p = ln_plan(a.M, a.N, a.K, ln_kb<T>());
+    if (p.blocks > (1ll << 30)) return fail(HNO_ELIMIT, "hno_linear: %lld tiles exceed the grid", p.blocks);
+    a.nsplit = p.nsplit;
     ProfScope _ps(kid, s, esz * ((double)a.M * a.K + (double)a.N * a.K + (double)a.M * a.N));
-    hipLaunchKernelGGL((linear_kernel<T, AX, BX>), dim3(ceil_div(a.N, LN_T), ceil_div(a.M, LN_T), a.nsplit), dim3(256), 0, s, a);
+    const dim3 grid((unsigned)p.blocks);
+    if constexpr (sizeof(T) == 2) {
+        if (p.tile == 256 && dma) hipLaunchKernelGGL((linear_kernel<T, AX, BX, 256, true>), grid, dim3(512), 0, s, a);
+        else if (p.tile == 256) hipLaunchKernelGGL((linear_kernel<T, AX, BX, 256, false>), grid, dim3(512), 0, s, a);
+        else if (dma) hipLaunchKernelGGL((linear_kernel<T, AX, BX, 128, true>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((linear_kernel<T, AX, BX, 128, false>), grid, dim3(256), 0, s, a);
+    } else {
+        hipLaunchKernelGGL((linear_kernel<T, AX, BX, 128, false>), grid, dim3(256), 0, s, a);
+    }
     HNO_CHECK_LAUNCH();
     if (a.nsplit > 1) {
-        const long long items = (long long)a.M * ((a.N + 3) / 4), blocks = (items + 255) / 256;
+        const long long items = (long long)a.M * ((a.N + 7) / 8), blocks = (items + 255) / 256;
         hipLaunchKernelGGL((linear_join_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, a);
         HNO_CHECK_LAUNCH();
     }
@@ -260,11 +384,11 @@ static int ln_check(const char *what, int dtype, int M, int N, int K, int act) {
     HNO_REQUIRE(M > 0 && N > 0 && K > 0, "%s: bad size", what);
     HNO_REQUIRE(act == HNO_ACT_NONE || act == HNO_ACT_SELU || act == HNO_ACT_ELU || act == HNO_ACT_RELU || act == HNO_ACT_GELU || act == HNO_ACT_SILU,
                 "%s: activation %d", what, act);
-    if (M > LN_T * 65535ll || N > LN_T * 65535ll || K > LN_T * 65535ll) return fail(HNO_ELIMIT, "%s: a size exceeds the grid", what);
+    if (M > (1 << 30) || N > (1 << 30) || K > (1 << 30)) return fail(HNO_ELIMIT, "%s: a size exceeds 2^30", what);
     return HNO_OK;
 }
 static size_t ln_slab(int M, int N, int K, int kb) {
-    const int n = ln_splits(M, N, K, kb);
+    const int n = ln_plan(M, N, K, kb).nsplit;
     return n > 1 ? (size_t)n * M * N * sizeof(float) : 0;
 }
 

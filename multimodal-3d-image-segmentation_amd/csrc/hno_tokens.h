@@ -89,20 +89,59 @@ __device__ __forceinline__ TkFrag<float> tk_col(const float *tile, int stride, i
     return f;
 }
 
+// LDS-DMA: 64 lanes x 16 bytes from (wave-uniform base + per-lane byte offset) to 1024 consecutive LDS bytes at `dst` (wave-uniform).  No registers; retired by
+// dma_wait (hno_common.h).  M0 holds the destination and is put back: the compiler owns it.
+__device__ __forceinline__ void tk_dma16(const tkh *src, unsigned off, unsigned dst) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(off), "s"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory");
+}
+
 // 16 bytes of padding behind each row of a tile: the row stride in 16-byte units is odd, so 8 lanes that read 16 bytes of 8
 // consecutive rows cover all 64 banks' width once
 template <typename T> constexpr int tk_pad() { return 16 / (int)sizeof(T); }
 
 // ------------------------------------------------------------------ activations (ids: hno.h)
+// 1 - Phi(|z|) = erfc(|z| / sqrt 2) / 2 by Abramowitz and Stegun 7.1.26 (five terms, absolute error of erf 1.5e-7); e2 = exp(-z^2 / 2).  libm's erfcf
+// took longer than the product itself in the epilogue of an 8192 x 8192 x 2048 product.
+__device__ __forceinline__ float tk_phi_tail(float z, float &e2) {
+    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    e2 = __expf(-x * x);
+    return 0.5f * p * t * e2;
+}
 // act(z); the derivative is a function of z, which the backward passes recompute or keep
 __device__ __forceinline__ float tk_act(float z, int act) {
     switch (act) {
         case HNO_ACT_SELU: return z > 0.f ? HNO_SELU_SCALE * z : (HNO_SELU_SCALE * HNO_SELU_ALPHA) * neg_expm1(z);
         case HNO_ACT_ELU: return z > 0.f ? z : neg_expm1(z);
         case HNO_ACT_RELU: return z > 0.f ? z : (z == z ? 0.f : z);
-        case HNO_ACT_GELU: return z > -1e30f ? 0.5f * z * erfcf(z * -0.70710678118654752f) : (z == z ? 0.f : z);
+        case HNO_ACT_GELU: {
+            float e2;
+            const float q = tk_phi_tail(z, e2);
+            return fabsf(z) < 20.f ? z * (z > 0.f ? 1.f - q : q) : (z > 0.f ? z : (z == z ? 0.f : z));
+        }
         case HNO_ACT_SILU: return z > -80.f ? z / (1.f + __expf(-z)) : (z == z ? 0.f : z);
         default: return z;
+    }
+}
+// eight values, the choice of the function made once
+__device__ __forceinline__ void tk_act8(float (&x)[8], int act) {
+    switch (act) {
+#define TK_CASE(A)                                              \
+    case A:                                                     \
+        _Pragma("unroll") for (int j = 0; j < 8; ++j) x[j] = tk_act(x[j], A); \
+        break;
+        TK_CASE(HNO_ACT_SELU)
+        TK_CASE(HNO_ACT_ELU)
+        TK_CASE(HNO_ACT_RELU)
+        TK_CASE(HNO_ACT_GELU)
+        TK_CASE(HNO_ACT_SILU)
+#undef TK_CASE
+        default: break;
     }
 }
 __device__ __forceinline__ float tk_act_grad(float z, int act) {
@@ -112,7 +151,9 @@ __device__ __forceinline__ float tk_act_grad(float z, int act) {
         case HNO_ACT_RELU: return z > 0.f ? 1.f : (z == z ? 0.f : z);
         case HNO_ACT_GELU: {
             if (!(fabsf(z) < 20.f)) return z > 0.f ? 1.f : (z == z ? 0.f : z);
-            return 0.5f * erfcf(z * -0.70710678118654752f) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+            float e2;
+            const float q = tk_phi_tail(z, e2);
+            return (z > 0.f ? 1.f - q : q) + z * e2 * 0.39894228040143268f;
         }
         case HNO_ACT_SILU: {
             if (!(fabsf(z) < 80.f)) return z > 0.f ? 1.f : (z == z ? 0.f : z);
