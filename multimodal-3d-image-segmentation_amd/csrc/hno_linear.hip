@@ -18,17 +18,18 @@ struct LinArgs {
     int M, N, K, act, bias32, out32, nsplit;
 };
 
-// Tiles: 256 x 256 by 8 waves of 128 x 64, or 128 x 128 by 4 waves of 64 x 64 (small results); KB contraction elements a step.  With 64 x 64 per wave the
-// LDS reads of a step take as long as its matrix instructions, with 128 x 64 three quarters.
-template <int TILE> struct LnTile;
-template <> struct LnTile<256> { static constexpr int WAVES = 8, WM = 128, WN = 64; };
-template <> struct LnTile<128> { static constexpr int WAVES = 4, WM = 64, WN = 64; };
+// Tiles of the result (TM x TN), contraction elements a step (KB), LDS buffers (ST) and the part of one wave (WM x WN).  With 64 x 64 per wave the LDS reads of a step
+// take as long as its matrix instructions, with 128 x 64 three quarters.
+//   LnBig: large results; LnMid: small ones (more tiles, two workgroups a CU); LnF32: three planes per operand
+struct LnBig { static constexpr int TM = 256, TN = 256, KB = 64, ST = 2, WM = 128, WN = 64; };
+struct LnMid { static constexpr int TM = 128, TN = 128, KB = 64, ST = 2, WM = 64, WN = 64; };
+struct LnF32 { static constexpr int TM = 128, TN = 128, KB = 32, ST = 2, WM = 64, WN = 64; };
+template <typename C> constexpr int ln_waves() { return C::TM / C::WM * (C::TN / C::WN); }
 
 // fp32: a value is three bf16 terms, its leading 8 bits, the next 8 and the last 8 (cut, not rounded: their sum is the value), and a product is the six products
 // of terms down to 2^-16 on the bf16 matrix instruction -- the two dropped ones are 2^-22 at most, 2^-25 on average, of the product.
 // An fp32 matrix instruction takes 1.3 times as long for the same work (and more than twice counting that six need one set of operands).
 template <typename T> constexpr int ln_planes() { return sizeof(T) == 2 ? 1 : 3; }
-template <typename T> constexpr int ln_kb() { return sizeof(T) == 2 ? 64 : 32; }
 
 // Where 8 elements (chunk c of row r) of an operand's LDS tile stand.  Along k: TILE rows of KB; 16 consecutive rows at one chunk touch all banks.
 // Across: KB rows of TILE; 4 consecutive rows at four neighbouring chunks touch all banks (the transposed reads).
@@ -40,9 +41,9 @@ __device__ __forceinline__ int ln_at(int r, int c) {
 }
 
 // A workgroup's share of one operand's tile: thread t moves the 8-element slots t, t + threads, ...
-template <typename T, int TILE, bool ACROSS, bool DMA>
+template <typename T, int TILE, int KB, int NT, bool ACROSS, bool DMA>
 struct LnStage {
-    static constexpr int KB = ln_kb<T>(), NT = 64 * LnTile<TILE>::WAVES, CH = (ACROSS ? TILE : KB) / 8, N = TILE * KB / 8 / NT, PLANE = TILE * KB;
+    static constexpr int CH = (ACROSS ? TILE : KB) / 8, N = TILE * KB / 8 / NT, PLANE = TILE * KB;
     static constexpr int NR = DMA ? 1 : N;
     TkFrag<T> r[NR];
     const T *base;
@@ -155,75 +156,87 @@ __device__ __forceinline__ void ln_put8(T *p, int cnt, const float (&x)[8]) {
             if (j < cnt) p[j] = tk_down<T>(x[j]);
     }
 }
-// the epilogue of columns n .. n + 7 of row m
-template <typename T>
-__device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float (&x)[8]) {
+// the epilogue of columns n .. n + 7 of row m; r: the residual's values, loaded before
+template <typename T, int ACT>
+__device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float (&x)[8], const float (&r)[8]) {
     const int cnt = a.N - n;
     const long long at = (long long)m * a.N + n;
-    float t[8];
     if (a.bias) {
+        float t[8];
         if (a.bias32) ln_get8((const float *)a.bias + n, cnt, t);
         else ln_get8((const T *)a.bias + n, cnt, t);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] += t[j];
     }
-    if (a.z) ln_put8((T *)a.z + at, cnt, x);
-    if (a.act != HNO_ACT_NONE) tk_act8(x, a.act);
-    if (a.res) {
-        ln_get8((const T *)a.res + at, cnt, t);
+    if (ACT != HNO_ACT_NONE && a.z) ln_put8((T *)a.z + at, cnt, x);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] += t[j];
-    }
+    for (int j = 0; j < 8; ++j) x[j] = tk_act(x[j], ACT);
+    if (a.res)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] += r[j];
     if (a.out32) ln_put8((float *)a.y + at, cnt, x);
     else ln_put8((T *)a.y + at, cnt, x);
 }
 
-// DMA: two LDS buffers, the next step's tiles on their way while this one is multiplied.  Else the next step's tiles wait in registers: one buffer.
-template <typename T, bool AX, bool BX, int TILE, bool DMA>
-__global__ __launch_bounds__(64 * LnTile<TILE>::WAVES, 2) void linear_kernel(LinArgs a) {
-    constexpr int KB = ln_kb<T>(), P = ln_planes<T>(), WM = LnTile<TILE>::WM, WN = LnTile<TILE>::WN, NB = DMA ? 2 : 1, PLANE = TILE * KB;
-    constexpr int ES = WN + 4, EP = 2 * LnTile<TILE>::WAVES * 32 * ES, TILES = 2 * NB * P * PLANE;         // (epilogue: 32 rows of floats a wave)
-    __shared__ __attribute__((aligned(16))) tkh smem[EP > TILES ? EP : TILES];
-    typedef tkh Tile[NB][P * PLANE];
-    Tile &As = *reinterpret_cast<Tile *>(smem), &Bs = *reinterpret_cast<Tile *>(smem + NB * P * PLANE);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, wm = (wave % (TILE / WM)) * WM, wn = (wave / (TILE / WM)) * WN;
+// DMA: ST LDS buffers, the next ST - 1 steps' tiles on their way while this one is multiplied.  Else the next step's tiles wait in registers: one buffer.
+template <typename T, bool AX, bool BX, typename C, bool DMA, int ACT>
+__global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a) {
+    constexpr int TM = C::TM, TN = C::TN, KB = C::KB, P = ln_planes<T>(), WM = C::WM, WN = C::WN, NT = 64 * ln_waves<C>(), NB = DMA ? C::ST : 1;
+    constexpr int PA = TM * KB, PB = TN * KB, BUF = P * (PA + PB);
+    constexpr int ES = WN + 4, EP = 2 * ln_waves<C>() * 32 * ES;                  // (epilogue: 32 rows of floats a wave)
+    __shared__ __attribute__((aligned(16))) tkh smem[EP > NB * BUF ? EP : NB * BUF];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, wm = (wave % (TM / WM)) * WM, wn = (wave / (TM / WM)) * WN;
     // every XCD takes one run of the list of tiles; neighbours in a run share rows (bands of 4 tile rows, column by column)
-    const int tm = (a.M + TILE - 1) / TILE, tn = (a.N + TILE - 1) / TILE, each = gridDim.x >> 3, more = gridDim.x & 7, xcd = blockIdx.x & 7;
+    const int tm = (a.M + TM - 1) / TM, tn = (a.N + TN - 1) / TN, each = gridDim.x >> 3, more = gridDim.x & 7, xcd = blockIdx.x & 7;
     int at = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
     const int run = at / (tm * tn);
     at -= run * tm * tn;
-    const int band = at / (4 * tn), bm = min(4, tm - 4 * band), m0 = (4 * band + (at - band * 4 * tn) % bm) * TILE, n0 = ((at - band * 4 * tn) / bm) * TILE;
-    const int steps = (a.K + KB - 1) / KB, per = (steps + a.nsplit - 1) / a.nsplit, k1 = min((run + 1) * per, steps);
-    LnStage<T, TILE, AX, DMA> sa;
-    LnStage<T, TILE, BX, DMA> sb;
+    const int band = at / (4 * tn), bm = min(4, tm - 4 * band), m0 = (4 * band + (at - band * 4 * tn) % bm) * TM, n0 = ((at - band * 4 * tn) / bm) * TN;
+    const int steps = (a.K + KB - 1) / KB, per = (steps + a.nsplit - 1) / a.nsplit, k0 = run * per, k1 = min(k0 + per, steps);
+    LnStage<T, TM, KB, NT, AX, DMA> sa;
+    LnStage<T, TN, KB, NT, BX, DMA> sb;
     sa.init(a.A, a.lda, m0, a.M, a.K);
     sb.init(a.B, a.ldb, n0, a.N, a.K);
+    const auto fetch = [&](int ks, int buf) {
+        sa.fetch(smem + buf * BUF, ks * KB, tid);
+        sb.fetch(smem + buf * BUF + P * PA, ks * KB, tid);
+    };
     tk16 acc[WM / 32][WN / 32] = {};
-    int buf = 0;
-    if (run * per < k1) {
-        sa.fetch(As[0], run * per * KB, tid);
-        sb.fetch(Bs[0], run * per * KB, tid);
-    }
-    for (int ks = run * per; ks < k1; ++ks) {
-        if constexpr (DMA) dma_wait<0>();
-        else __syncthreads();
-        sa.settle(As[buf], ks * KB, a.K, tid);
-        sb.settle(Bs[buf], ks * KB, a.K, tid);
-        __syncthreads();
-        if (ks + 1 < k1) {
-            sa.fetch(As[buf ^ (NB - 1)], (ks + 1) * KB, tid);
-            sb.fetch(Bs[buf ^ (NB - 1)], (ks + 1) * KB, tid);
-        }
 #pragma unroll
-        for (int kk = 0; kk < KB / 16; ++kk) {
-            TkFrag<tkh> fa[P][WM / 32], fb[P][WN / 32];
+    for (int i = 0; i < (DMA ? NB - 1 : 1); ++i)
+        if (k0 + i < k1) fetch(k0 + i, i);
+    int buf = 0;
+    for (int ks = k0; ks < k1; ++ks) {
+        if constexpr (DMA) {
+            if (ks + NB - 2 < k1 - 1) dma_wait<(NB - 2) * (sa.N + sb.N)>();      // the steps behind this one stay in flight
+            else dma_wait<0>();
+        } else {
+            __syncthreads();
+        }
+        tkh *As = smem + buf * BUF, *Bs = As + P * PA;
+        sa.settle(As, ks * KB, a.K, tid);
+        sb.settle(Bs, ks * KB, a.K, tid);
+        __syncthreads();
+        const int ahead = DMA ? NB - 1 : 1;
+        if (ks + ahead < k1) fetch(ks + ahead, DMA ? (buf == 0 ? NB - 1 : buf - 1) : 0);
+        // fragments are read one chunk ahead of their products
+        constexpr int FB = P == 1 ? 2 : 1;
+        TkFrag<tkh> fa[FB][P][WM / 32], fb[FB][P][WN / 32];
+        const auto read = [&](int kk) {
 #pragma unroll
             for (int p = 0; p < P; ++p) {
 #pragma unroll
-                for (int u = 0; u < WM / 32; ++u) fa[p][u] = ln_frag<TILE, KB, AX>(As[buf] + p * PLANE, wm + 32 * u, kk, lane);
+                for (int v = 0; v < WN / 32; ++v) fb[kk % FB][p][v] = ln_frag<TN, KB, BX>(Bs + p * PB, wn + 32 * v, kk, lane);
 #pragma unroll
-                for (int v = 0; v < WN / 32; ++v) fb[p][v] = ln_frag<TILE, KB, BX>(Bs[buf] + p * PLANE, wn + 32 * v, kk, lane);
+                for (int u = 0; u < WM / 32; ++u) fa[kk % FB][p][u] = ln_frag<TM, KB, AX>(As + p * PA, wm + 32 * u, kk, lane);
             }
+        };
+        if (FB == 2) read(0);
+#pragma unroll
+        for (int kk = 0; kk < KB / 16; ++kk) {
+            if (FB == 1) read(kk);
+            else if (kk + 1 < KB / 16) read(kk + 1);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int t = P - 1; t >= 0; --t)          // smallest terms first
 #pragma unroll
@@ -231,51 +244,61 @@ __global__ __launch_bounds__(64 * LnTile<TILE>::WAVES, 2) void linear_kernel(Lin
 #pragma unroll
                     for (int u = 0; u < WM / 32; ++u)
 #pragma unroll
-                        for (int v = 0; v < WN / 32; ++v) acc[u][v] = tk_mma(fb[p][v], fa[t - p][u], acc[u][v]);
+                        for (int v = 0; v < WN / 32; ++v) acc[u][v] = tk_mma(fb[kk % FB][p][v], fa[kk % FB][t - p][u], acc[u][v]);
+            __builtin_amdgcn_s_setprio(0);
         }
-        buf ^= NB - 1;
+        if constexpr (DMA) buf = buf == NB - 1 ? 0 : buf + 1;
     }
     // the results change places in LDS, 32 rows of a wave at a time (its own part: no barrier inside), so that memory is read and written in runs of 128 bytes
     __syncthreads();
     float *ep = reinterpret_cast<float *>(smem) + wave * 32 * ES;
+    constexpr int PASS = 32 * WN / 8 / 64;
 #pragma unroll
     for (int u = 0; u < WM / 32; ++u) {
+        float r[PASS][8];
+#pragma unroll
+        for (int e = 0; e < PASS; ++e) {              // the residual's loads are on their way together
+            const int i = lane + 64 * e, m = m0 + wm + 32 * u + i / (WN / 8), n = n0 + wn + (i % (WN / 8)) * 8;
+            if (a.res && a.nsplit == 1 && m < a.M && n < a.N) ln_get8((const T *)a.res + (long long)m * a.N + n, a.N - n, r[e]);
+        }
 #pragma unroll
         for (int v = 0; v < WN / 32; ++v)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
                 *reinterpret_cast<tkf4 *>(ep + (lane & 31) * ES + 32 * v + 8 * q + 4 * h) =
                     tkf4{acc[u][v][4 * q], acc[u][v][4 * q + 1], acc[u][v][4 * q + 2], acc[u][v][4 * q + 3]};
-#pragma unroll 1
-        for (int e = lane; e < 32 * WN / 8; e += 64) {
-            const int r = e / (WN / 8), c = (e - r * (WN / 8)) * 8, m = m0 + wm + 32 * u + r, n = n0 + wn + c;
-            const TkFrag<float> f = tk_row(ep + r * ES + c);
-            if (m >= a.M || n >= a.N) continue;
+#pragma unroll
+        for (int e = 0; e < PASS; ++e) {
+            const int i = lane + 64 * e, c = (i % (WN / 8)) * 8, m = m0 + wm + 32 * u + i / (WN / 8), n = n0 + wn + c;
+            const TkFrag<float> f = tk_row(ep + (i / (WN / 8)) * ES + c);
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = f.v[j];
-            if (a.nsplit > 1) ln_put8(a.part + ((long long)run * a.M + m) * a.N + n, a.N - n, x);
-            else ln_finish<T>(a, m, n, x);
+            if (m < a.M && n < a.N) {
+                if (a.nsplit > 1) ln_put8(a.part + ((long long)run * a.M + m) * a.N + n, a.N - n, x);
+                else ln_finish<T, ACT>(a, m, n, x, r[e]);
+            }
         }
     }
 }
 
 // sum of the runs' slabs, then the epilogue
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a) {
     const int per_row = (a.N + 7) / 8;
     const long long items = (long long)a.M * per_row, slab = (long long)a.M * a.N;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < items; i += (long long)gridDim.x * 256) {
         const int m = (int)(i / per_row), n = 8 * (int)(i - (long long)m * per_row);
         const float *src = a.part + (long long)m * a.N + n;
-        float x[8] = {}, t[8];
+        float x[8] = {}, t[8], r[8] = {};
+        if (a.res) ln_get8((const T *)a.res + (long long)m * a.N + n, a.N - n, r);
 #pragma unroll 4
         for (int s = 0; s < a.nsplit; ++s) {
             ln_get8(src + s * slab, a.N - n, t);
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] += t[j];
         }
-        ln_finish<T>(a, m, n, x);
+        ln_finish<T, ACT>(a, m, n, x, r);
     }
 }
 
@@ -325,20 +348,21 @@ __global__ __launch_bounds__(1024) void linear_db_kernel(const float *__restrict
 
 using namespace hno;
 
-// tile and runs of the contraction.  256 x 256 where its tiles fill most of the chip's 256 CUs by themselves; else 128 x 128, and the contraction cut into runs (of
-// four steps at least) until there are two workgroups per CU.
+// tile and runs of the contraction.  LnBig (8192 x 8192 x 8192: 994 TFLOP/s, LnMid 898) where its tiles fill most of the 256 CUs by themselves and DMA can feed it; else 128 x 128,
+// and the contraction cut into runs (of four steps at least) until there are two workgroups per CU.
 struct LnPlan {
-    int tile, nsplit;
+    bool big;
+    int nsplit;
     long long blocks;
 };
-static LnPlan ln_plan(int M, int N, int K, int kb) {
+static LnPlan ln_plan(int M, int N, int K, bool f32, bool dma) {
     LnPlan p;
-    long long tiles = (long long)ceil_div(M, 256) * ceil_div(N, 256);
-    p.tile = tiles >= 192 && kb == 64 ? 256 : 128;
+    long long tiles = (long long)ceil_div(M, LnBig::TM) * ceil_div(N, LnBig::TN);
+    p.big = tiles >= 192 && !f32 && dma;
     p.nsplit = 1;
-    if (p.tile == 128) {
+    if (!p.big) {
         tiles = (long long)ceil_div(M, 128) * ceil_div(N, 128);
-        const long long steps = ceil_div(K, kb);
+        const long long steps = ceil_div(K, f32 ? LnF32::KB : LnMid::KB);
         long long n = tiles >= 256 ? 1 : 512 / tiles;
         if (n > steps / 4) n = steps / 4;
         if (n > 64) n = 64;
@@ -351,29 +375,25 @@ static int ln_runs(int M) { return M <= 64 ? 1 : (ceil_div(M, 64) < 256 ? ceil_d
 static size_t ln_pad(size_t b) { return (b + 255) / 256 * 256; }
 static bool ln_aligned(const void *p, long long ld, int esz) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * esz % 16 == 0; }
 
-template <typename T, bool AX, bool BX>
-static int ln_product(LinArgs a, hipStream_t s, int kid) {
+template <typename T, bool AX, bool BX, int ACT>
+static int ln_product(LinArgs a, hipStream_t s) {
     const int esz = sizeof(T);
     // DMA: whole 16-byte chunks along the stored axis of each operand, and offsets within a tile in 32 bits
     const bool dma = esz == 2 && ln_aligned(a.A, a.lda, esz) && (AX ? a.M : a.K) % 8 == 0 && ln_aligned(a.B, a.ldb, esz) && (BX ? a.N : a.K) % 8 == 0 &&
                      a.lda < (1 << 22) && a.ldb < (1 << 22);
-    const LnPlan p = ln_plan(a.M, a.N, a.K, ln_kb<T>());
+    const LnPlan p = ln_plan(a.M, a.N, a.K, sizeof(T) == 4, dma);
     if (p.blocks > (1ll << 30)) return fail(HNO_ELIMIT, "hno_linear: %lld tiles exceed the grid", p.blocks);
     a.nsplit = p.nsplit;
-    ProfScope _ps(kid, s, esz * ((double)a.M * a.K + (double)a.N * a.K + (double)a.M * a.N));
+    ProfScope _ps(KID_LINEAR, s, esz * ((double)a.M * a.K + (double)a.N * a.K + (double)a.M * a.N));
     const dim3 grid((unsigned)p.blocks);
-    if constexpr (sizeof(T) == 2) {
-        if (p.tile == 256 && dma) hipLaunchKernelGGL((linear_kernel<T, AX, BX, 256, true>), grid, dim3(512), 0, s, a);
-        else if (p.tile == 256) hipLaunchKernelGGL((linear_kernel<T, AX, BX, 256, false>), grid, dim3(512), 0, s, a);
-        else if (dma) hipLaunchKernelGGL((linear_kernel<T, AX, BX, 128, true>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((linear_kernel<T, AX, BX, 128, false>), grid, dim3(256), 0, s, a);
-    } else {
-        hipLaunchKernelGGL((linear_kernel<T, AX, BX, 128, false>), grid, dim3(256), 0, s, a);
-    }
+    if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((linear_kernel<T, AX, BX, LnF32, false, ACT>), grid, dim3(64 * ln_waves<LnF32>()), 0, s, a);
+    else if (p.big) hipLaunchKernelGGL((linear_kernel<T, AX, BX, LnBig, true, ACT>), grid, dim3(64 * ln_waves<LnBig>()), 0, s, a);
+    else if (dma) hipLaunchKernelGGL((linear_kernel<T, AX, BX, LnMid, true, ACT>), grid, dim3(64 * ln_waves<LnMid>()), 0, s, a);
+    else hipLaunchKernelGGL((linear_kernel<T, AX, BX, LnMid, false, ACT>), grid, dim3(64 * ln_waves<LnMid>()), 0, s, a);
     HNO_CHECK_LAUNCH();
     if (a.nsplit > 1) {
         const long long items = (long long)a.M * ((a.N + 7) / 8), blocks = (items + 255) / 256;
-        hipLaunchKernelGGL((linear_join_kernel<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((linear_join_kernel<T, ACT>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, a);
         HNO_CHECK_LAUNCH();
     }
     return HNO_OK;
@@ -387,17 +407,29 @@ static int ln_check(const char *what, int dtype, int M, int N, int K, int act) {
     if (M > (1 << 30) || N > (1 << 30) || K > (1 << 30)) return fail(HNO_ELIMIT, "%s: a size exceeds 2^30", what);
     return HNO_OK;
 }
-static size_t ln_slab(int M, int N, int K, int kb) {
-    const int n = ln_plan(M, N, K, kb).nsplit;
+static size_t ln_slab(int M, int N, int K, bool f32) {
+    const int n = ln_plan(M, N, K, f32, false).nsplit;          // (where LnBig is taken, one)
     return n > 1 ? (size_t)n * M * N * sizeof(float) : 0;
 }
 
 extern "C" size_t hno_linear_workspace_bytes(int dtype, int M, int N, int K, int act, int backward) {
     if (ln_check("hno_linear_workspace_bytes", dtype, M, N, K, act)) return 0;
-    const int kb = dtype == HNO_BF16 ? ln_kb<tkh>() : ln_kb<float>();
-    if (!backward) return ln_slab(M, N, K, kb);
-    const size_t dx = ln_slab(M, K, N, kb), dw = ln_slab(N, K, M, kb), dz = act == HNO_ACT_NONE ? 0 : (size_t)M * N * (dtype == HNO_BF16 ? 2 : 4);
+    const bool f32 = dtype == HNO_F32;
+    if (!backward) return ln_slab(M, N, K, f32);
+    const size_t dx = ln_slab(M, K, N, f32), dw = ln_slab(N, K, M, f32), dz = act == HNO_ACT_NONE ? 0 : (size_t)M * N * (dtype == HNO_BF16 ? 2 : 4);
     return ln_pad(dz) + ln_pad((size_t)ln_runs(M) * N * sizeof(float)) + (dx > dw ? dx : dw);
+}
+
+template <typename T>
+static int ln_forward(const LinArgs &a, hipStream_t s) {
+    switch (a.act) {
+        case HNO_ACT_SELU: return ln_product<T, false, false, HNO_ACT_SELU>(a, s);
+        case HNO_ACT_ELU: return ln_product<T, false, false, HNO_ACT_ELU>(a, s);
+        case HNO_ACT_RELU: return ln_product<T, false, false, HNO_ACT_RELU>(a, s);
+        case HNO_ACT_GELU: return ln_product<T, false, false, HNO_ACT_GELU>(a, s);
+        case HNO_ACT_SILU: return ln_product<T, false, false, HNO_ACT_SILU>(a, s);
+        default: return ln_product<T, false, false, HNO_ACT_NONE>(a, s);
+    }
 }
 
 extern "C" int hno_linear_fwd(int dtype, const void *x, long long ldx, const void *w, const void *bias, int bias_dtype, const void *residual, void *z, void *y,
@@ -409,8 +441,7 @@ extern "C" int hno_linear_fwd(int dtype, const void *x, long long ldx, const voi
     LinArgs a = {};
     a.A = x; a.lda = ldx; a.B = w; a.ldb = K; a.bias = bias; a.bias32 = bias_dtype == HNO_F32; a.res = residual; a.z = z; a.y = y;
     a.M = M; a.N = N; a.K = K; a.act = act; a.part = (float *)workspace;
-    if (dtype == HNO_BF16) return ln_product<tkh, false, false>(a, (hipStream_t)stream, KID_LINEAR);
-    return ln_product<float, false, false>(a, (hipStream_t)stream, KID_LINEAR);
+    return dtype == HNO_BF16 ? ln_forward<tkh>(a, (hipStream_t)stream) : ln_forward<float>(a, (hipStream_t)stream);
 }
 
 template <typename T>
@@ -434,11 +465,11 @@ static int ln_backward(const void *dy, const void *z, const void *x, long long l
     a.part = part;
     if (dx) {
         a.A = d; a.lda = N; a.B = w; a.ldb = K; a.y = dx; a.M = M; a.N = K; a.K = N;
-        if (int rc = ln_product<T, false, true>(a, s, KID_LINEAR)) return rc;
+        if (int rc = ln_product<T, false, true, HNO_ACT_NONE>(a, s)) return rc;
     }
     if (dw) {
         a.A = d; a.lda = N; a.B = x; a.ldb = ldx; a.y = dw; a.out32 = sizeof(T) == 2 && dw_dtype == HNO_F32; a.M = N; a.N = K; a.K = M;
-        if (int rc = ln_product<T, true, true>(a, s, KID_LINEAR)) return rc;
+        if (int rc = ln_product<T, true, true, HNO_ACT_NONE>(a, s)) return rc;
     }
     return HNO_OK;
 }

@@ -128,22 +128,6 @@ __device__ __forceinline__ float tk_act(float z, int act) {
         default: return z;
     }
 }
-// eight values, the choice of the function made once
-__device__ __forceinline__ void tk_act8(float (&x)[8], int act) {
-    switch (act) {
-#define TK_CASE(A)                                              \
-    case A:                                                     \
-        _Pragma("unroll") for (int j = 0; j < 8; ++j) x[j] = tk_act(x[j], A); \
-        break;
-        TK_CASE(HNO_ACT_SELU)
-        TK_CASE(HNO_ACT_ELU)
-        TK_CASE(HNO_ACT_RELU)
-        TK_CASE(HNO_ACT_GELU)
-        TK_CASE(HNO_ACT_SILU)
-#undef TK_CASE
-        default: break;
-    }
-}
 __device__ __forceinline__ float tk_act_grad(float z, int act) {
     switch (act) {
         case HNO_ACT_SELU: return z > 0.f ? HNO_SELU_SCALE : (HNO_SELU_SCALE * HNO_SELU_ALPHA) * __expf(z);
