@@ -47,23 +47,40 @@ __device__ __forceinline__ void gn_store(T *p, const GnVec<T, W> &r) {
     }
 }
 
-// sums of the workgroup's rows: lanes that own the same channels are added through LDS; slab[b][run][2][C]
+// the same, kept as it lies in memory
+template <typename T, int W> struct GnRaw { TkFrag<T> f; };
+template <typename T> struct GnRaw<T, 1> { T f; };
+template <typename T, int W>
+__device__ __forceinline__ GnRaw<T, W> gn_raw(const T *p) {
+    if constexpr (W == 8) return {tk_row(p)};
+    else return {p[0]};
+}
+template <typename T, int W>
+__device__ __forceinline__ float gn_at(const GnRaw<T, W> &r, int j) {
+    if constexpr (W == 8) return (float)r.f.v[j];
+    else return tk_up(r.f);
+}
+
+// sums of the workgroup's rows -> slab[b][run][2][C].  The lanes that own the same channels meet in LDS; each of the 2 W cw sums is taken by `per` neighbouring
+// threads (with one thread a sum, 24 channels left 3 of 256 threads 1360 additions each: 26 us for 65^3 x 24 instead of 8).
 template <int W>
-__device__ __forceinline__ void gn_block_sums(const GnArgs &a, float (&s1)[W], float (&s2)[W], int chunk, int rl, int nrl, int tid, float *lds) {
+__device__ __forceinline__ void gn_block_sums(const GnArgs &a, float (&s1)[W], float (&s2)[W], int nrl, int tid, float *lds) {
+    constexpr int S = 2 * W + 1;
 #pragma unroll
-    for (int j = 0; j < W; ++j) lds[tid * (2 * W + 1) + j] = s1[j], lds[tid * (2 * W + 1) + W + j] = s2[j];
+    for (int j = 0; j < W; ++j) lds[tid * S + j] = s1[j], lds[tid * S + W + j] = s2[j];
     __syncthreads();
-    if (rl != 0 || chunk >= a.chunks) return;
-    float *dst = a.slab + ((long long)blockIdx.z * a.runs + blockIdx.x) * 2 * a.C + chunk * W;
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-        float t1 = 0.f, t2 = 0.f;
-        for (int r = 0; r < nrl; ++r) {
-            t1 += lds[(tid + r * a.cw) * (2 * W + 1) + j];
-            t2 += lds[(tid + r * a.cw) * (2 * W + 1) + W + j];
-        }
-        dst[j] = t1;
-        dst[a.C + j] = t2;
+    const int nout = 2 * W * a.cw;
+    int per = 1;
+    while (per < 64 && 2 * per * nout <= 256) per *= 2;
+    float *dst = a.slab + ((long long)blockIdx.z * a.runs + blockIdx.x) * 2 * a.C;
+    for (int o0 = 0; o0 < nout; o0 += 256 / per) {
+        const int o = o0 + tid / per, sl = tid & (per - 1), ch = o / (2 * W), j = o - ch * 2 * W, c = (blockIdx.y * a.cw + ch) * W;
+        const bool on = o < nout && c < a.C;
+        float t = 0.f;
+        if (on)
+            for (int r = sl; r < nrl; r += per) t += lds[(ch + r * a.cw) * S + j];
+        for (int k = per >> 1; k; k >>= 1) t += __shfl_xor(t, k);
+        if (on && sl == 0) dst[j < W ? c + j : a.C + c + j - W] = t;
     }
 }
 
@@ -78,6 +95,7 @@ __global__ __launch_bounds__(256) void gncl_stats_kernel(GnArgs a) {
         const T *x = (const T *)a.x + (long long)blockIdx.z * a.V * a.C + chunk * W;
         const long long r1 = ((long long)blockIdx.x + 1) * a.rows_per < a.V ? ((long long)blockIdx.x + 1) * a.rows_per : a.V;
         const GnVec<T, W> p = gn_load<T, W>(x);
+#pragma unroll 2
         for (long long r = blockIdx.x * a.rows_per + rl; r < r1; r += nrl) {
             const GnVec<T, W> v = gn_load<T, W>(x + r * a.C);
 #pragma unroll
@@ -88,42 +106,36 @@ __global__ __launch_bounds__(256) void gncl_stats_kernel(GnArgs a) {
             }
         }
     }
-    gn_block_sums<W>(a, s1, s2, chunk, rl, nrl, tid, lds);
+    gn_block_sums<W>(a, s1, s2, nrl, tid, lds);
 }
 
-// (count, mean, M2) of two disjoint sets
-__device__ __forceinline__ void gn_join(double &n, double &mean, double &m2, double n2, double mean2, double m22) {
-    if (n2 == 0.0) return;
-    const double t = n + n2, d = mean2 - mean;
-    mean += d * n2 / t;
-    m2 += m22 + d * d * n * n2 / t;
-    n = t;
-}
+// joins the runs of a group in 64 bits: with mean_i, M2_i of channel run i of n_i values and any reference r,
+//   N (mean - r) = sum n_i (mean_i - r),  M2 = sum M2_i + sum n_i (mean_i - r)^2 - N (mean - r)^2      (r: the group's first value)
 template <typename T>
-__global__ __launch_bounds__(256) void gncl_finish_kernel(GnArgs a) {
-    __shared__ double sh[3][256];
+__global__ __launch_bounds__(1024) void gncl_finish_kernel(GnArgs a) {
+    __shared__ double sh[2][1024];
     const int tid = threadIdx.x, g = blockIdx.x, b = blockIdx.y, cpg = a.C / a.G;
-    const T *x = (const T *)a.x + (long long)b * a.V * a.C;
-    double n = 0.0, mean = 0.0, m2 = 0.0;
-    for (long long i = tid; i < (long long)cpg * a.runs; i += 256) {
-        const int run = (int)(i / cpg), c = g * cpg + (int)(i - (long long)run * cpg);
-        const long long left = a.V - run * a.rows_per;
-        const double cnt = (double)(left < a.rows_per ? left : a.rows_per);
-        const float *src = a.slab + ((long long)b * a.runs + run) * 2 * a.C + c;
-        const double s1 = src[0], s2 = src[a.C];
-        gn_join(n, mean, m2, cnt, (double)tk_up(x[c]) + s1 / cnt, s2 - s1 * s1 / cnt);
+    const T *x = (const T *)a.x + (long long)b * a.V * a.C + g * cpg;
+    const float *slab = a.slab + (long long)b * a.runs * 2 * a.C + g * cpg;
+    const double ref = tk_up(x[0]), inv = 1.0 / (double)a.rows_per, left = (double)(a.V - (a.runs - 1) * a.rows_per), inv_last = 1.0 / left;
+    double d1 = 0.0, m2 = 0.0;
+#pragma unroll 4
+    for (long long i = tid; i < (long long)cpg * a.runs; i += 1024) {
+        const int run = (int)(i / cpg), c = (int)(i - (long long)run * cpg);
+        const bool last = run == a.runs - 1;
+        const double n = last ? left : (double)a.rows_per, s1 = slab[run * 2ll * a.C + c], s2 = slab[(run * 2ll + 1) * a.C + c];
+        const double mi = s1 * (last ? inv_last : inv), d = (double)tk_up(x[c]) - ref + mi;
+        d1 += n * d;
+        m2 += s2 - s1 * mi + n * d * d;
     }
-    sh[0][tid] = n, sh[1][tid] = mean, sh[2][tid] = m2;
-    for (int o = 128; o; o >>= 1) {
+    sh[0][tid] = d1, sh[1][tid] = m2;
+    for (int o = 512; o; o >>= 1) {
         __syncthreads();
-        if (tid < o) {
-            gn_join(n, mean, m2, sh[0][tid + o], sh[1][tid + o], sh[2][tid + o]);
-            sh[0][tid] = n, sh[1][tid] = mean, sh[2][tid] = m2;
-        }
+        if (tid < o) sh[0][tid] += sh[0][tid + o], sh[1][tid] += sh[1][tid + o];
     }
     if (tid == 0) {
-        const double var = m2 / n;
-        a.mr[2 * (b * a.G + g)] = (float)mean;
+        const double N = (double)a.V * cpg, d = sh[0][0] / N, var = (sh[1][0] - N * d * d) / N;
+        a.mr[2 * (b * a.G + g)] = (float)(ref + d);
         a.mr[2 * (b * a.G + g) + 1] = (float)(1.0 / sqrt((var > 0.0 ? var : (var == var ? 0.0 : var)) + (double)a.eps));
     }
 }
@@ -142,6 +154,7 @@ __global__ __launch_bounds__(256) void gncl_apply_kernel(GnArgs a) {
     }
     const long long base = (long long)b * a.V * a.C + chunk * W;
     const long long r1 = ((long long)blockIdx.x + 1) * a.rows_per < a.V ? ((long long)blockIdx.x + 1) * a.rows_per : a.V;
+#pragma unroll 2
     for (long long r = blockIdx.x * a.rows_per + rl; r < r1; r += nrl) {
         GnVec<T, W> v = gn_load<T, W>((const T *)a.x + base + r * a.C);
 #pragma unroll
@@ -180,51 +193,55 @@ __global__ __launch_bounds__(256) void gncl_bwd_sums_kernel(GnArgs a) {
             }
         }
     }
-    gn_block_sums<W>(a, s1, s2, chunk, rl, nrl, tid, lds);
+    gn_block_sums<W>(a, s1, s2, nrl, tid, lds);
 }
 
 // one workgroup per group: dgamma, dbeta of its channels and, per sample, mean(du gamma) and mean(du gamma xh).  `cw` threads across the
 // channels, the others across the runs.
-__global__ __launch_bounds__(256) void gncl_bwd_finish_kernel(GnArgs a, int cw) {
-    __shared__ float sh[2][256];
-    __shared__ float tot[2][256];
-    const int tid = threadIdx.x, cpg = a.C / a.G, g = blockIdx.x, cl = tid % cw, rl = tid / cw, nrl = 256 / cw;
+__global__ __launch_bounds__(1024) void gncl_bwd_finish_kernel(GnArgs a, int cw) {
+    __shared__ float sh[2][1024];
+    const int tid = threadIdx.x, cpg = a.C / a.G, g = blockIdx.x, cl = tid & (cw - 1), rl = tid / cw, nrl = 1024 / cw;
     for (int c0 = 0; c0 < cpg; c0 += cw) {
         const int c = g * cpg + c0 + cl;
         const bool on = c0 + cl < cpg;
         float db = 0.f, dg = 0.f;
         for (int b = 0; b < a.B; ++b) {
             float s1 = 0.f, s2 = 0.f;
-            if (on && rl < nrl)
+            const float *src = a.slab + (long long)b * a.runs * 2 * a.C + c;
+            if (on)
+#pragma unroll 8
                 for (int r = rl; r < a.runs; r += nrl) {
-                    const float *src = a.slab + ((long long)b * a.runs + r) * 2 * a.C + c;
-                    s1 += src[0];
-                    s2 += src[a.C];
+                    s1 += src[r * 2ll * a.C];
+                    s2 += src[(r * 2ll + 1) * a.C];
                 }
             __syncthreads();
             sh[0][tid] = s1, sh[1][tid] = s2;
+            for (int o = 512; o >= cw; o >>= 1) {          // across the runs
+                __syncthreads();
+                if (tid < o) sh[0][tid] += sh[0][tid + o], sh[1][tid] += sh[1][tid + o];
+            }
             __syncthreads();
             if (tid < cw) {
-                s1 = s2 = 0.f;
-                for (int r = 0; r < nrl; ++r) s1 += sh[0][r * cw + tid], s2 += sh[1][r * cw + tid];
-                db += s1, dg += s2;
-                const float w = on ? (a.gamma ? a.gamma[c] : 1.f) : 0.f;
-                tot[0][tid] = w * s1, tot[1][tid] = w * s2;
+                db += sh[0][tid], dg += sh[1][tid];
+                const float w = on && a.gamma ? a.gamma[c] : 1.f;
+                sh[0][tid] *= w, sh[1][tid] *= w;
             }
-            __syncthreads();
-            if (tid < 2) {
-                float t = 0.f;
-                for (int k = 0; k < cw; ++k) t += tot[tid][k];
-                float *dst = &a.coef[2 * (b * a.G + g) + tid];
-                t = c0 ? *dst + t : t;
-                *dst = c0 + cw >= cpg ? t / ((float)a.V * (float)cpg) : t;
+            for (int o = cw >> 1; o; o >>= 1) {            // across the channels
+                __syncthreads();
+                if (tid < o) sh[0][tid] += sh[0][tid + o], sh[1][tid] += sh[1][tid + o];
             }
+            if (tid == 0)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float *dst = &a.coef[2 * (b * a.G + g) + k];
+                    const float t = c0 ? *dst + sh[k][0] : sh[k][0];
+                    *dst = c0 + cw >= cpg ? t / ((float)a.V * (float)cpg) : t;
+                }
         }
         if (tid < cw && on) {
             if (a.dbeta) a.dbeta[c] = db;
             if (a.dgamma) a.dgamma[c] = dg;
         }
-        __syncthreads();
     }
 }
 
@@ -245,6 +262,7 @@ __global__ __launch_bounds__(256) void gncl_bwd_apply_kernel(GnArgs a) {
     }
     const long long base = (long long)b * a.V * a.C + chunk * W;
     const long long r1 = ((long long)blockIdx.x + 1) * a.rows_per < a.V ? ((long long)blockIdx.x + 1) * a.rows_per : a.V;
+#pragma unroll 2
     for (long long r = blockIdx.x * a.rows_per + rl; r < r1; r += nrl) {
         GnVec<T, W> v = gn_load<T, W>((const T *)a.x + base + r * a.C);
         const GnVec<T, W> d = gn_load<T, W>((const T *)a.dy + base + r * a.C);
@@ -255,6 +273,162 @@ __global__ __launch_bounds__(256) void gncl_bwd_apply_kernel(GnArgs a) {
         }
         gn_store<T, W>((T *)a.dx + base + r * a.C, v);
     }
+}
+
+// ------------------------------------------------------------------ small groups: one launch
+// A workgroup owns one group of one sample and keeps it in registers: x is read once, the statistics are those of the kept values (mean first, then squared
+// distances), and the backward pass needs no second launch but the sum over samples of dgamma, dbeta.  Threads: chunk (of W channels) x row; a thread keeps gn_keep
+// rows.  2 x 960 x 256 in 32 groups: forward 20 -> 10 us, backward 31 -> 15 us of kernels.
+constexpr int GN_THREADS = 1024;
+template <typename T, int W, bool BWD> constexpr int gn_keep() { return BWD && sizeof(T) == 4 && W == 8 ? 4 : 8; }       // (128 registers a thread)
+template <typename T, int W, bool BWD> inline bool gn_small(long long V, int cpg) {
+    return cpg % W == 0 && cpg / W <= 64 && V <= (long long)(GN_THREADS / (cpg / W)) * gn_keep<T, W, BWD>();
+}
+__device__ __forceinline__ float gn_block_sum(float v, float *sh, int tid) {
+#pragma unroll
+    for (int k = 32; k; k >>= 1) v += __shfl_xor(v, k);
+    __syncthreads();
+    if ((tid & 63) == 0) sh[tid >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < GN_THREADS / 64; ++k) s += sh[k];
+    return s;
+}
+template <typename T, int W>
+__global__ __launch_bounds__(GN_THREADS) void gncl_small_fwd_kernel(GnArgs a) {
+    __shared__ float sh[GN_THREADS / 64];
+    const int tid = threadIdx.x, g = blockIdx.x, b = blockIdx.y, cpg = a.C / a.G, nch = cpg / W, nr = GN_THREADS / nch, rl = tid / nch, c = g * cpg + (tid - rl * nch) * W;
+    constexpr int KEEP = gn_keep<T, W, false>();
+    const T *x = (const T *)a.x + (long long)b * a.V * a.C + c;
+    const float first = tk_up(((const T *)a.x)[(long long)b * a.V * a.C + g * cpg]), n = (float)a.V * (float)cpg;
+    GnRaw<T, W> v[KEEP];
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k) {
+        const int r = rl + k * nr;
+        const bool in = rl < nr && r < a.V;
+        if (in) v[k] = gn_raw<T, W>(x + (long long)r * a.C);
+#pragma unroll
+        for (int j = 0; j < W; ++j) s += in ? gn_at(v[k], j) - first : 0.f;
+    }
+    const float mean = first + gn_block_sum(s, sh, tid) / n;
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k) {
+        const bool in = rl < nr && rl + k * nr < a.V;
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const float d = in ? gn_at(v[k], j) - mean : 0.f;
+            s = fmaf(d, d, s);
+        }
+    }
+    const float rstd = 1.f / sqrtf(gn_block_sum(s, sh, tid) / n + a.eps);
+    if (tid == 0) a.mr[2 * (b * a.G + g)] = mean, a.mr[2 * (b * a.G + g) + 1] = rstd;
+    float ga[W], be[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        ga[j] = rstd * (a.gamma ? a.gamma[c + j] : 1.f);
+        be[j] = a.beta ? a.beta[c + j] : 0.f;
+    }
+    T *y = (T *)a.y + (long long)b * a.V * a.C + c;
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k) {
+        const int r = rl + k * nr;
+        if (!(rl < nr && r < a.V)) continue;
+        GnVec<T, W> u;
+#pragma unroll
+        for (int j = 0; j < W; ++j) u.v[j] = tk_act(fmaf(gn_at(v[k], j) - mean, ga[j], be[j]), a.act);
+        gn_store<T, W>(y + (long long)r * a.C, u);
+    }
+}
+// slab: (B, 2, C), the sums of each sample
+template <typename T, int W>
+__global__ __launch_bounds__(GN_THREADS) void gncl_small_bwd_kernel(GnArgs a) {
+    __shared__ float part[GN_THREADS * (2 * W + 1)];
+    __shared__ float tot[2 * 64 * W];
+    const int tid = threadIdx.x, g = blockIdx.x, b = blockIdx.y, cpg = a.C / a.G, nch = cpg / W, nr = GN_THREADS / nch, rl = tid / nch, ch = tid - rl * nch, c = g * cpg + ch * W;
+    const T *x = (const T *)a.x + (long long)b * a.V * a.C + c, *dy = (const T *)a.dy + (long long)b * a.V * a.C + c;
+    const float mean = a.mr[2 * (b * a.G + g)], rstd = a.mr[2 * (b * a.G + g) + 1];
+    float ga[W], be[W], s1[W], s2[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        ga[j] = a.gamma ? a.gamma[c + j] : 1.f;
+        be[j] = a.beta ? a.beta[c + j] : 0.f;
+        s1[j] = s2[j] = 0.f;
+    }
+    constexpr int KEEP = gn_keep<T, W, true>();
+    GnRaw<T, W> v[KEEP], d[KEEP];
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k) {
+        const int r = rl + k * nr;
+        if (rl < nr && r < a.V) {
+            v[k] = gn_raw<T, W>(x + (long long)r * a.C);
+            d[k] = gn_raw<T, W>(dy + (long long)r * a.C);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k)
+        if (rl < nr && rl + k * nr < a.V)
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const float xh = (gn_at(v[k], j) - mean) * rstd, du = gn_at(d[k], j) * tk_act_grad(fmaf(xh, ga[j], be[j]), a.act);
+                s1[j] += du;
+                s2[j] = fmaf(du, xh, s2[j]);
+            }
+    // per channel: 2 cpg sums over the nr row lanes, each by several threads, then by one
+#pragma unroll
+    for (int j = 0; j < W; ++j) part[tid * (2 * W + 1) + j] = s1[j], part[tid * (2 * W + 1) + W + j] = s2[j];
+    __syncthreads();
+    const int nout = 2 * cpg, per = GN_THREADS / nout, o = tid / (per > 0 ? per : 1), sl = tid - o * per;      // (cpg <= 64 W <= 512: per >= 1)
+    const int wh = o >= cpg, oc = o - wh * cpg, at = (oc / W) * (2 * W + 1) + wh * W + oc % W;
+    float t = 0.f;
+    if (o < nout)
+        for (int r = sl; r < nr; r += per) t += part[r * nch * (2 * W + 1) + at];
+    __syncthreads();
+    part[tid] = t;
+    __syncthreads();
+    if (tid < nout) {
+        t = 0.f;
+        for (int k = 0; k < per; ++k) t += part[tid * per + k];
+        const int cc = g * cpg + (tid < cpg ? tid : tid - cpg);
+        if (a.B == 1) {
+            if (tid < cpg ? a.dbeta != nullptr : a.dgamma != nullptr) (tid < cpg ? a.dbeta : a.dgamma)[cc] = t;
+        } else {
+            a.slab[((long long)b * 2 + (tid >= cpg)) * a.C + cc] = t;
+        }
+        tot[tid] = t * (a.gamma ? a.gamma[cc] : 1.f);
+    }
+    __syncthreads();
+    if (!a.dx) return;
+    float t1 = 0.f, t2 = 0.f;
+    for (int k = 0; k < cpg; ++k) t1 += tot[k], t2 += tot[cpg + k];
+    const float inv = 1.f / ((float)a.V * (float)cpg);
+    t1 *= inv, t2 *= inv;
+    T *dx = (T *)a.dx + (long long)b * a.V * a.C + c;
+#pragma unroll
+    for (int k = 0; k < KEEP; ++k) {
+        const int r = rl + k * nr;
+        if (!(rl < nr && r < a.V)) continue;
+        GnVec<T, W> u;
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const float xh = (gn_at(v[k], j) - mean) * rstd, du = gn_at(d[k], j) * tk_act_grad(fmaf(xh, ga[j], be[j]), a.act);
+            u.v[j] = rstd * (fmaf(du, ga[j], -t1) - xh * t2);
+        }
+        gn_store<T, W>(dx + (long long)r * a.C, u);
+    }
+}
+__global__ __launch_bounds__(256) void gncl_params_kernel(GnArgs a) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= a.C) return;
+    float db = 0.f, dg = 0.f;
+    for (int b = 0; b < a.B; ++b) {
+        db += a.slab[(b * 2ll) * a.C + c];
+        dg += a.slab[(b * 2ll + 1) * a.C + c];
+    }
+    if (a.dbeta) a.dbeta[c] = db;
+    if (a.dgamma) a.dgamma[c] = dg;
 }
 
 }  // namespace hno
@@ -313,8 +487,18 @@ static int gn_forward(const void *x, const float *gamma, const float *beta, void
     GnArgs a = gn_args(p, B, V, C, G, act);
     a.x = x; a.gamma = gamma; a.beta = beta; a.y = y; a.mr = mr; a.eps = eps; a.slab = (float *)ws;
     ProfScope _ps(KID_GNCL, s, 2.0 * sizeof(T) * B * V * C);
+    if (p.W == 8 && gn_small<T, 8, false>(V, C / G)) {
+        hipLaunchKernelGGL((gncl_small_fwd_kernel<T, 8>), dim3(G, B), dim3(GN_THREADS), 0, s, a);
+        HNO_CHECK_LAUNCH();
+        return HNO_OK;
+    }
+    if (gn_small<T, 1, false>(V, C / G)) {
+        hipLaunchKernelGGL((gncl_small_fwd_kernel<T, 1>), dim3(G, B), dim3(GN_THREADS), 0, s, a);
+        HNO_CHECK_LAUNCH();
+        return HNO_OK;
+    }
     GN_LAUNCH(gncl_stats_kernel);
-    hipLaunchKernelGGL((gncl_finish_kernel<T>), dim3(G, B), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((gncl_finish_kernel<T>), dim3(G, B), dim3(1024), 0, s, a);
     HNO_CHECK_LAUNCH();
     GN_LAUNCH(gncl_apply_kernel);
     return HNO_OK;
@@ -328,10 +512,21 @@ static int gn_backward(const void *dy, const void *x, const float *gamma, const 
     a.coef = (float *)ws;
     a.slab = (float *)((char *)ws + gn_pad((size_t)B * G * 2 * sizeof(float)));
     ProfScope _ps(KID_GNCL, s, 3.0 * sizeof(T) * B * V * C);
+    const bool s8 = p.W == 8 && gn_small<T, 8, true>(V, C / G);
+    if (s8 || gn_small<T, 1, true>(V, C / G)) {
+        if (s8) hipLaunchKernelGGL((gncl_small_bwd_kernel<T, 8>), dim3(G, B), dim3(GN_THREADS), 0, s, a);
+        else hipLaunchKernelGGL((gncl_small_bwd_kernel<T, 1>), dim3(G, B), dim3(GN_THREADS), 0, s, a);
+        HNO_CHECK_LAUNCH();
+        if (B > 1 && (dgamma || dbeta)) {
+            hipLaunchKernelGGL(gncl_params_kernel, dim3(ceil_div(C, 256)), dim3(256), 0, s, a);
+            HNO_CHECK_LAUNCH();
+        }
+        return HNO_OK;
+    }
     GN_LAUNCH(gncl_bwd_sums_kernel);
     int cw = 1;
-    while (cw < C / G && cw < 256) cw *= 2;
-    hipLaunchKernelGGL(gncl_bwd_finish_kernel, dim3(G), dim3(256), 0, s, a, cw);
+    while (cw < C / G && cw < 1024) cw *= 2;
+    hipLaunchKernelGGL(gncl_bwd_finish_kernel, dim3(G), dim3(1024), 0, s, a, cw);
     HNO_CHECK_LAUNCH();
     if (dx) GN_LAUNCH(gncl_bwd_apply_kernel);
     return HNO_OK;
@@ -341,7 +536,7 @@ static int gn_backward(const void *dy, const void *x, const float *gamma, const 
 extern "C" size_t hno_gncl_workspace_bytes(int B, long long V, int C, int G) {
     if (gn_check("hno_gncl_workspace_bytes", HNO_F32, B, V, C, G, 0)) return 0;
     const int r0 = gn_plan(0, B, V, C, false).runs, r1 = C % 8 == 0 ? gn_plan(0, B, V, C, true).runs : 0;
-    return gn_pad((size_t)B * G * 2 * sizeof(float)) + (size_t)B * (r0 > r1 ? r0 : r1) * 2 * C * sizeof(float);
+    return gn_pad((size_t)B * G * 2 * sizeof(float)) + (size_t)B * (r0 > r1 ? r0 : r1) * 2 * C * sizeof(float);       // (small groups: B x 2 x C)
 }
 extern "C" int hno_gncl_fwd(int dtype, const void *x, const float *gamma, const float *beta, void *y, float *mean_rstd, void *workspace, size_t workspace_bytes,
                             int B, long long V, int C, int G, float eps, int act, void *stream) {
