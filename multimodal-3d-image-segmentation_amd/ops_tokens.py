@@ -4,17 +4,15 @@ their backward passes.
 
 Tensors are torch containers; nothing computes through ATen and there is no CPU path (meta tensors get shape inference only).  Parameters may
 stay fp32 next to bf16 activations: the matrix product then rounds its weight to bf16, as the bf16 convolutions do, and returns an fp32 gradient.
-Gradients of gradients are refused (``once_differentiable``).
+Gradients of gradients are refused.
 """
-import contextlib
 import ctypes
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
-from ._lib import check, stream_ptr
+from ._lib import check
 from .ops import _HnoFunction, _m
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}                     # HNO_F32, HNO_BF16
@@ -45,11 +43,23 @@ def _same_device(what, first, *others):
             raise ValueError(f'{what}: tensors on {first.device} and {t.device}')
 
 
-def _on(t):
-    """the tensor's device as the current one (launches and workspaces go by the current device and its current stream)"""
+def _apply(fn, t, *args):
+    """fn.apply(*args) with the device of `t` as the current one (launches and workspaces go by the current device and its current stream)"""
     if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+        return fn.apply(*args)
+    with torch.cuda.device(t.device):
+        return fn.apply(*args)
+
+
+def _stream(t):
+    """the current stream of the tensor's device, as the library takes it (torch.cuda.current_stream() builds a Stream object: 4 us of a 20 us call)"""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def _once():
+    """called by every backward pass: a graph of the gradients (create_graph) would hold nothing of these kernels"""
+    if torch.is_grad_enabled():
+        raise RuntimeError('the token operators cannot be differentiated twice')
 
 
 def _p(t):
@@ -105,17 +115,18 @@ class AttentionFn(_HnoFunction):
         if out.numel():
             L = _lib.lib()
             a = _attn_args(q, k, v, mask, kv_lens, causal, scale)
-            n = L.hno_attn_workspace_bytes(ctypes.byref(a), 0)
+            ref = ctypes.byref(a)
+            n = L.hno_attn_workspace_bytes(ref, 0)
             ws = _ws(n, q.device)
-            check(L.hno_attn_fwd(ctypes.byref(a), _p(out), _p(res), _p(lse), _p(ws), n, stream_ptr()), 'hno_attn_fwd')
+            check(L.hno_attn_fwd(ref, _p(out), _p(res), _p(lse), _p(ws), n, _stream(q)), 'hno_attn_fwd')
         if train:
             ctx.save_for_backward(q, k, v, mask, kv_lens, out, res, lse)
             ctx.cfg = (causal, scale, Dk, Dv)
         return out if out.shape[3] == Dv else out[..., :Dv].contiguous()
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        _once()
         q, k, v, mask, kv_lens, out, res, lse = ctx.saved_tensors
         causal, scale, Dk, Dv = ctx.cfg
         need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
@@ -123,14 +134,13 @@ class AttentionFn(_HnoFunction):
         dq = new(q.shape, device=q.device, dtype=q.dtype) if need_q else None
         dk, dv = (new(t.shape, device=q.device, dtype=q.dtype) if need_kv else None for t in (k, v))
         if out.numel():
-            with _on(q):
-                L = _lib.lib()
-                g = _heads(g, g.element_size()).contiguous()
-                a = _attn_args(q, k, v, mask, kv_lens, causal, scale)
-                n = L.hno_attn_workspace_bytes(ctypes.byref(a), 1)
-                ws = _ws(n, q.device)
-                check(L.hno_attn_bwd(ctypes.byref(a), _p(out), _p(res), _p(lse), _p(g), _p(dq), _p(dk), _p(dv), _p(ws), n, stream_ptr()),
-                      'hno_attn_bwd')
+            L = _lib.lib()
+            g = _heads(g, g.element_size()).contiguous()
+            a = _attn_args(q, k, v, mask, kv_lens, causal, scale)
+            ref = ctypes.byref(a)
+            n = L.hno_attn_workspace_bytes(ref, 1)
+            ws = _ws(n, q.device)
+            check(L.hno_attn_bwd(ref, _p(out), _p(res), _p(lse), _p(g), _p(dq), _p(dk), _p(dv), _p(ws), n, _stream(q)), 'hno_attn_bwd')
         dq, dk, dv = (t if t is None or t.shape[3] == D else t[..., :D] for t, D in ((dq, Dk), (dk, Dk), (dv, Dv)))
         return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None, None
 
@@ -174,10 +184,9 @@ def attention(q, k, v, *, causal=False, mask=None, kv_lens=None, scale=None):
     if q.is_meta:
         return AttentionFn.apply(q, k, v, mask, kv_lens, bool(causal), scale)
     _same_device('attention', q, k, v, mask, kv_lens)
-    with _on(q):
-        if kv_lens is not None and (kv_lens.dtype != torch.int32 or not kv_lens.is_contiguous()):
-            kv_lens = kv_lens.clamp(0, Tk).to(torch.int32).contiguous()
-        return AttentionFn.apply(q, k, v, mask, kv_lens, bool(causal), scale)
+    if kv_lens is not None and (kv_lens.dtype != torch.int32 or not kv_lens.is_contiguous()):
+        kv_lens = kv_lens.clamp(0, Tk).to(torch.int32).contiguous()
+    return _apply(AttentionFn, q, q, k, v, mask, kv_lens, bool(causal), scale)
 
 
 # ----------------------------------------------------------------------------------------------- linear
@@ -195,7 +204,7 @@ def _rows(x):
 
 def _bf16_weight(w):
     out = torch.empty(w.shape, device=w.device, dtype=torch.bfloat16)
-    check(_lib.lib().hno_cast_f32_bf16(_p(w), _p(out), w.numel(), stream_ptr()), 'hno_cast_f32_bf16')
+    check(_lib.lib().hno_cast_f32_bf16(_p(w), _p(out), w.numel(), _stream(w)), 'hno_cast_f32_bf16')
     return out
 
 
@@ -225,15 +234,15 @@ class LinearFn(_HnoFunction):
             n = L.hno_linear_workspace_bytes(dt, M, N, K, act, 0)
             ws = _ws(n, x.device)
             check(L.hno_linear_fwd(dt, _p(x2), ldx, _p(w), _p(b), 0 if b is None else _DTYPES[b.dtype], _p(r), _p(z), _p(y), M, N, K, act, _p(ws), n,
-                                   stream_ptr()), 'hno_linear_fwd')
+                                   _stream(x)), 'hno_linear_fwd')
         if train:
             ctx.save_for_backward(x2, w, z, weight)
             ctx.cfg = (act, tuple(x.shape), None if bias is None else bias.dtype)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        _once()
         x, w, z, weight = ctx.saved_tensors
         act, xshape, bias_dtype = ctx.cfg
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
@@ -244,23 +253,22 @@ class LinearFn(_HnoFunction):
                     zeros((N,), bias_dtype) if need_b else None, g if need_r else None, None)
         dx = dw = db = None
         if need_x or need_w or need_b:
-            with _on(g):
-                L = _lib.lib()
-                gc = g.contiguous()
-                x2, ldx = _rows(x)
-                M = x2.shape[0]
-                if need_x:
-                    dx = torch.empty(xshape, device=g.device, dtype=g.dtype)
-                if need_w:
-                    own = weight.is_leaf and weight.dtype == torch.float32 and weight.is_contiguous()
-                    dw = ops._grad_buffer(weight) if own else torch.empty((N, K), device=g.device, dtype=weight.dtype)
-                if need_b:
-                    db = torch.empty(N, device=g.device, dtype=bias_dtype)
-                dt = _DTYPES[g.dtype]
-                n = L.hno_linear_workspace_bytes(dt, M, N, K, act, 1)
-                ws = _ws(n, g.device)
-                check(L.hno_linear_bwd(dt, _p(gc), _p(z), _p(x2), ldx, _p(w), _p(dx), _p(dw), 0 if dw is None else _DTYPES[dw.dtype], _p(db),
-                                       0 if db is None else _DTYPES[db.dtype], M, N, K, act, _p(ws), n, stream_ptr()), 'hno_linear_bwd')
+            L = _lib.lib()
+            gc = g.contiguous()
+            x2, ldx = _rows(x)
+            M = x2.shape[0]
+            if need_x:
+                dx = torch.empty(xshape, device=g.device, dtype=g.dtype)
+            if need_w:
+                own = weight.is_leaf and weight.dtype == torch.float32 and weight.is_contiguous()
+                dw = ops._grad_buffer(weight) if own else torch.empty((N, K), device=g.device, dtype=weight.dtype)
+            if need_b:
+                db = torch.empty(N, device=g.device, dtype=bias_dtype)
+            dt = _DTYPES[g.dtype]
+            n = L.hno_linear_workspace_bytes(dt, M, N, K, act, 1)
+            ws = _ws(n, g.device)
+            check(L.hno_linear_bwd(dt, _p(gc), _p(z), _p(x2), ldx, _p(w), _p(dx), _p(dw), 0 if dw is None else _DTYPES[dw.dtype], _p(db),
+                                   0 if db is None else _DTYPES[db.dtype], M, N, K, act, _p(ws), n, _stream(g)), 'hno_linear_bwd')
         return dx, dw, db, g if need_r else None, None
 
 
@@ -287,8 +295,7 @@ def linear(x, weight, bias=None, *, act=None, residual=None):
     if x.is_meta:
         return LinearFn.apply(x, weight, bias, residual, a)
     _same_device('linear', x, weight, bias, residual)
-    with _on(x):
-        return LinearFn.apply(x, weight, bias, residual, a)
+    return _apply(LinearFn, x, x, weight, bias, residual, a)
 
 
 # ----------------------------------------------------------------------------------------------- group norm
@@ -311,15 +318,15 @@ class GroupNormClFn(_HnoFunction):
             V = x.numel() // (B * C)
             n = L.hno_gncl_workspace_bytes(B, V, C, groups)
             ws = _ws(n, x.device)
-            check(L.hno_gncl_fwd(_DTYPES[x.dtype], _p(x), _p(w), _p(b), _p(y), _p(mr), _p(ws), n, B, V, C, groups, eps, act, stream_ptr()), 'hno_gncl_fwd')
+            check(L.hno_gncl_fwd(_DTYPES[x.dtype], _p(x), _p(w), _p(b), _p(y), _p(mr), _p(ws), n, B, V, C, groups, eps, act, _stream(x)), 'hno_gncl_fwd')
         if ops.backward_wanted(ctx):
             ctx.save_for_backward(x, w, b, mr)
             ctx.cfg = (groups, act, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
+        _once()
         x, w, b, mr = ctx.saved_tensors
         groups, act, wt, bt = ctx.cfg
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
@@ -328,14 +335,13 @@ class GroupNormClFn(_HnoFunction):
         dx = torch.empty_like(x) if need_x else None
         dw, db = (new(C, device=x.device, dtype=torch.float32) if n else None for n in (need_w, need_b))
         if x.numel():
-            with _on(x):
-                L = _lib.lib()
-                g = g.contiguous()
-                V = x.numel() // (B * C)
-                n = L.hno_gncl_workspace_bytes(B, V, C, groups)
-                ws = _ws(n, x.device)
-                check(L.hno_gncl_bwd(_DTYPES[x.dtype], _p(g), _p(x), _p(w), _p(b), _p(mr), _p(dx), _p(dw), _p(db), _p(ws), n, B, V, C, groups, act,
-                                     stream_ptr()), 'hno_gncl_bwd')
+            L = _lib.lib()
+            g = g.contiguous()
+            V = x.numel() // (B * C)
+            n = L.hno_gncl_workspace_bytes(B, V, C, groups)
+            ws = _ws(n, x.device)
+            check(L.hno_gncl_bwd(_DTYPES[x.dtype], _p(g), _p(x), _p(w), _p(b), _p(mr), _p(dx), _p(dw), _p(db), _p(ws), n, B, V, C, groups, act, _stream(x)),
+                  'hno_gncl_bwd')
         return dx, dw if wt in (None, torch.float32) or dw is None else dw.to(wt), db if bt in (None, torch.float32) or db is None else db.to(bt), None, None, None
 
 
@@ -359,5 +365,4 @@ def group_norm(x, num_groups, weight=None, bias=None, *, eps=1e-5, act=None):
     if x.is_meta:
         return GroupNormClFn.apply(x, weight, bias, num_groups, eps, a)
     _same_device('group_norm', x, weight, bias)
-    with _on(x):
-        return GroupNormClFn.apply(x, weight, bias, num_groups, eps, a)
+    return _apply(GroupNormClFn, x, x, weight, bias, num_groups, eps, a)

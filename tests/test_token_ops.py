@@ -634,3 +634,12 @@ def test_meta_tensors_give_shapes(ot):
     m = lambda *s: torch.empty(s, device='meta', dtype=torch.bfloat16)  # noqa: E731
     assert ot.attention(m(2, 5, 4, 32), m(2, 7, 2, 32), m(2, 7, 2, 16)).shape == (2, 5, 4, 16)
     assert ot.linear(m(2, 5, 8), m(3, 8)).shape == (2, 5, 3) and ot.group_norm(m(2, 5, 8), 4).dtype == torch.bfloat16
+
+
+@pytest.mark.gpu
+def test_no_second_derivative(ot):
+    x = rand((2, 9, 8), torch.float32, 1).requires_grad_(True)
+    for y in (ot.group_norm(x, 2, act='silu'), ot.linear(x, rand((4, 8), torch.float32, 2), act='gelu'),
+              ot.attention(x.unflatten(2, (1, 8)), x.unflatten(2, (1, 8)), x.unflatten(2, (1, 8)))):
+        with pytest.raises(RuntimeError, match='twice'):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
