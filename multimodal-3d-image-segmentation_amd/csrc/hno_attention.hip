@@ -10,7 +10,7 @@
 //
 // A wave owns 32 rows of its side as the COLUMNS of its products (lane & 31): the softmax statistics are then one value per lane, and the
 // registers of a product are the operand of the next (hno_tokens.h).  The other side comes through LDS, row by row as in memory; its
-// transposed reads are ds_read_b64_tr_b16 (bf16) or single words (fp32).
+// transposed reads are ds_read_b64_tr_b16.  fp32 tiles lie in LDS as three bf16 ones (hno_tokens.h).
 #include "hno_tokens.h"
 
 namespace hno {
@@ -37,12 +37,12 @@ __device__ __forceinline__ int at_length(const AttnArgs &a, int b) {
 __device__ __forceinline__ float at_other_half(float x) { return __shfl_xor(x, 32); }
 __device__ __forceinline__ int at_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }   // result register -> row of the tile
 
-// Where element d (a multiple of 4) of row `row` stands in an LDS tile of DP channels.  bf16: rows without padding whose 16-byte chunks change places, so
+// Where element d (a multiple of 4) of row `row` stands in an LDS tile of DP channels: rows without padding whose 16-byte chunks change places, so
 // that 16 consecutive rows read at one chunk (row reads) and 4 consecutive rows read at four neighbouring chunks (transposed reads)
 // touch 64 different banks each; with padded rows the transposed reads met 4-way conflicts (dk / dv of 2x16x4096x128: XX us).
 // DP = 96: a row is 3/4 of the banks, rows shift by themselves and the chunks rotate by row / 4; else an exclusive or.
 template <int DP>
-__device__ __forceinline__ int at_at(const tkh *, int row, int d) {
+__device__ __forceinline__ int at_at(int row, int d) {
     const int c = d >> 3;
     int slot;
     if constexpr (DP == 128) slot = c ^ (((row & 3) << 2) | ((row >> 2) & 3));
@@ -51,21 +51,19 @@ __device__ __forceinline__ int at_at(const tkh *, int row, int d) {
     else slot = c + ((row >> 2) & 3) - (c + ((row >> 2) & 3) >= 12 ? 12 : 0);
     return row * DP + slot * 8 + (d & 7);
 }
-template <int DP>
-__device__ __forceinline__ int at_at(const float *, int row, int d) { return row * (DP + 4) + d; }
-template <typename T, int DP> constexpr int at_stride() { return sizeof(T) == 2 ? DP : DP + 4; }
-// the fragment of the transposed tile: channel 32 dt + (lane & 31), rows r0 .. r0 + 3 and r0 + 8 .. r0 + 11
-template <int DP>
-__device__ __forceinline__ TkFrag<tkh> at_col(const tkh *tile, int dt, int r0, int lane) {
+// the fragment of the transposed tile: channel 32 dt + (lane & 31), rows r0 .. r0 + 3 and r0 + 8 .. r0 + 11 (PLANE: elements of one term's tile)
+template <typename T, int DP, int PLANE>
+__device__ __forceinline__ TkOp<T> at_col(const tkh *tile, int dt, int r0, int lane) {
     typedef __attribute__((address_space(3))) tks4 *lds4;
     const int row = r0 + ((lane & 15) >> 2), d = 32 * dt + (lane & 16) + 4 * (lane & 3);
-    const tks4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(tile + at_at<DP>(tile, row, d)));
-    const tks4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(tile + at_at<DP>(tile, row + 8, d)));
-    return {__builtin_bit_cast(tkb8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7))};
-}
-template <int DP>
-__device__ __forceinline__ TkFrag<float> at_col(const float *tile, int dt, int r0, int lane) {
-    return tk_col(tile, DP + 4, 32 * dt, r0, r0 + 8, lane);
+    TkOp<T> o;
+#pragma unroll
+    for (int p = 0; p < tk_planes<T>(); ++p) {
+        const tks4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(tile + p * PLANE + at_at<DP>(row, d)));
+        const tks4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(tile + p * PLANE + at_at<DP>(row + 8, d)));
+        o.p[p].v = __builtin_bit_cast(tkb8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    return o;
 }
 
 // 8 channels of a row (D % 8 == 0, 16-byte aligned: checked by the entry points); channels from D on are zeros
@@ -141,7 +139,7 @@ struct AtTile<float, DP, ROWS> {
     int D;
     __device__ __forceinline__ static int row(int i, int tid) { return (tid + 64 * AT_WAVES * i) / CH; }
     __device__ __forceinline__ void init(long long st_, int D_, int) { st = st_, D = D_; }
-    __device__ __forceinline__ void fetch(float *, const float *base, int t0, int end, int tid) {
+    __device__ __forceinline__ void fetch(tkh *, const float *base, int t0, int end, int tid) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int k = row(i, tid), d = (tid + 64 * AT_WAVES * i - k * CH) * 8, t = t0 + k;
@@ -149,14 +147,17 @@ struct AtTile<float, DP, ROWS> {
         }
     }
     template <typename P>
-    __device__ __forceinline__ void settle(float *tile, int tid, P dead) {
+    __device__ __forceinline__ void settle(tkh *tile, int tid, P dead) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int k = row(i, tid), d = (tid + 64 * AT_WAVES * i - k * CH) * 8;
             if (dead(i))
 #pragma unroll
                 for (int j = 0; j < 8; ++j) r[i].set(j, 0.f);
-            if (k < ROWS) tk_store8(tile + at_at<DP>(tile, k, d), r[i]);
+            if (k >= ROWS) continue;
+            const TkOp<float> o = tk_op(r[i]);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) tk_store8(tile + p * ROWS * DP + at_at<DP>(k, d), o.p[p]);
         }
     }
 };
@@ -195,25 +196,33 @@ __device__ __forceinline__ AtMask at_mask_row(const AttnArgs &a, const unsigned 
 __device__ __forceinline__ bool at_mask_on(const AtMask &m, int e) { return (m.w[e >> 2] >> (8 * (e & 3))) & 0xffu; }
 
 // acc(32 rows of the tile x 32 own columns) = tile rows . own fragments
-template <typename T, int DP>
-__device__ __forceinline__ tk16 at_product(const T *tile, int row0, const TkFrag<T> (&own)[DP / 16], int lane) {
+template <typename T, int DP, int PLANE>
+__device__ __forceinline__ tk16 at_product(const tkh *tile, int row0, const TkOp<T> (&own)[DP / 16], int lane) {
     tk16 acc = {};
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) acc = tk_mma(tk_row(tile + at_at<DP>(tile, row0 + (lane & 31), 16 * kk + 8 * (lane >> 5))), own[kk], acc);
+    for (int kk = 0; kk < DP / 16; ++kk) {
+        TkOp<T> o;
+#pragma unroll
+        for (int p = 0; p < tk_planes<T>(); ++p) o.p[p] = tk_row(tile + p * PLANE + at_at<DP>(row0 + (lane & 31), 16 * kk + 8 * (lane >> 5)));
+        acc = tk_mma(o, own[kk], acc);
+    }
     return acc;
 }
 // acc[dt] += (tile rows row0 .. row0 + 31)^T . w, w being a result over the same rows
-template <typename T, int DP>
-__device__ __forceinline__ void at_accumulate(tk16 (&acc)[DP / 32], const T *tile, int row0, const tk16 &w, int lane) {
+template <typename T, int DP, int PLANE>
+__device__ __forceinline__ void at_accumulate(tk16 (&acc)[DP / 32], const tkh *tile, int row0, const tk16 &w, int lane) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         TkFrag<T> f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) f.set(j, w[8 * t + j]);
+        const TkOp<T> o = tk_op(f);
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = tk_mma(at_col<DP>(tile, dt, row0 + 16 * t + 4 * (lane >> 5), lane), f, acc[dt]);
+        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = tk_mma(at_col<T, DP, PLANE>(tile, dt, row0 + 16 * t + 4 * (lane >> 5), lane), o, acc[dt]);
     }
 }
+// LDS buffers of the streamed side: two (one barrier a step), one where two would leave room for a single workgroup per CU
+template <typename T, int DP> constexpr int at_buffers() { return sizeof(T) == 4 && DP == 128 ? 1 : 2; }
 
 // store a transposed accumulator (register = channel, lane = row) as row `dst` of a contiguous tensor
 template <typename T, int DP, typename F>
@@ -319,10 +328,10 @@ __device__ __forceinline__ void at_weights(TkFrag<float> &f, const tk16 &s, int 
 }
 
 template <typename T, int DP, bool MASK>
-__global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) void attn_fwd_kernel(AttnArgs a) {
-    constexpr int KT = at_tile<T>(), S = at_stride<T, DP>();
-    __shared__ __attribute__((aligned(16))) T Ks[2][KT * S];
-    __shared__ __attribute__((aligned(16))) T Vs[2][KT * S];
+__global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 4 ? (DP <= 96 ? 2 : 1) : (DP <= 64 ? 3 : 2)) void attn_fwd_kernel(AttnArgs a) {
+    constexpr int KT = at_tile<T>(), PLANE = KT * DP, NB = at_buffers<T, DP>();
+    __shared__ __attribute__((aligned(16))) tkh Ks[NB][tk_planes<T>() * PLANE];
+    __shared__ __attribute__((aligned(16))) tkh Vs[NB][tk_planes<T>() * PLANE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const AtBlock w0 = at_block(a, a.pack ? 1 : a.H / a.Hk);
     const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk, hb = hk * grp + w0.gi, nrows = a.pack ? grp * a.Tq : a.Tq;
@@ -337,10 +346,10 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) 
     at_key_range(a, L, (r0 + AT_ROWS < nrows ? r0 + AT_ROWS : nrows) - 1, nrows, sp, KT, j0, j1);
     const int lim_all = MASK ? 0 : at_wave_min(w.lim), lim_any = -at_wave_min(-w.lim);
 
-    TkFrag<T> qf[DP / 16];
+    TkOp<T> qf[DP / 16];
     const T *qrow = (const T *)a.q + b * a.qs[0] + (long long)w.i * a.qs[1] + w.head * a.qs[2];
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) qf[kk] = at_load8(qrow, 16 * kk + 8 * h, a.Dk);
+    for (int kk = 0; kk < DP / 16; ++kk) qf[kk] = tk_op(at_load8(qrow, 16 * kk + 8 * h, a.Dk));
     const T *kb = (const T *)a.k + b * a.ks[0] + hk * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + hk * a.vs[2];
     const unsigned char *mrow = MASK ? a.mask + b * a.ms[0] + w.head * a.ms[1] + (long long)w.i * a.ms[2] : nullptr;
     // a mask that hides a key from every query of this workgroup takes the value row out too: 0 x NaN would be NaN
@@ -364,10 +373,11 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) 
     const float slack = 8.f / a.scale2;           // the maximum is raised, and the sums rescaled, only where weights would exceed 2^8
     int buf = 0;
     if (j0 < j1) fetch(0, j0);
-    for (int j = j0; j < j1; j += KT, buf ^= 1) {
+    for (int j = j0; j < j1; j += KT, buf ^= NB - 1) {
+        if (NB == 1) __syncthreads();
         settle(buf);
         __syncthreads();
-        if (j + KT < j1) fetch(buf ^ 1, j + KT);
+        if (j + KT < j1) fetch(buf ^ (NB - 1), j + KT);
         if (j >= lim_any) continue;             // none of this wave's rows sees the tile
         tk16 s[KT / 32];
         AtMask mk[KT / 32];
@@ -375,7 +385,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) 
 #pragma unroll
             for (int n = 0; n < KT / 32; ++n) mk[n] = at_mask_row(a, mrow, j + 32 * n, h);
 #pragma unroll
-        for (int n = 0; n < KT / 32; ++n) s[n] = at_product<T, DP>(Ks[buf], 32 * n, qf, lane);
+        for (int n = 0; n < KT / 32; ++n) s[n] = at_product<T, DP, PLANE>(Ks[buf], 32 * n, qf, lane);
         if (j + KT > lim_all) {
 #pragma unroll
             for (int n = 0; n < KT / 32; ++n)
@@ -409,9 +419,10 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) 
             for (int t = 0; t < 2; ++t) {
                 TkFrag<T> f;
                 at_weights(f, s[n], t, l);
+                const TkOp<T> o = tk_op(f);
                 const int row = 32 * n + 16 * t + 4 * h;
 #pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = tk_mma(at_col<DP>(Vs[buf], dt, row, lane), f, acc[dt]);
+                for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = tk_mma(at_col<T, DP, PLANE>(Vs[buf], dt, row, lane), o, acc[dt]);
             }
     }
     l += at_other_half(l);
@@ -520,9 +531,9 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const T *__restrict__ g
 
 template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(AttnArgs a) {
-    constexpr int KT = at_tile<T>(), S = at_stride<T, DP>();
-    __shared__ __attribute__((aligned(16))) T Ks[2][KT * S];
-    __shared__ __attribute__((aligned(16))) T Vs[2][KT * S];
+    constexpr int KT = at_tile<T>(), PLANE = KT * DP, NB = at_buffers<T, DP>();
+    __shared__ __attribute__((aligned(16))) tkh Ks[NB][tk_planes<T>() * PLANE];
+    __shared__ __attribute__((aligned(16))) tkh Vs[NB][tk_planes<T>() * PLANE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const AtBlock w0 = at_block(a, a.pack ? 1 : a.H / a.Hk);
     const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk, hb = hk * grp + w0.gi, nrows = a.pack ? grp * a.Tq : a.Tq;
@@ -536,12 +547,12 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
     int j0, j1;
     at_key_range(a, L, (r0 + AT_ROWS < nrows ? r0 + AT_ROWS : nrows) - 1, nrows, sp, KT, j0, j1);
     const long long row = ((long long)b * a.Tq + w.i) * a.H + w.head;
-    TkFrag<T> qf[DP / 16], gf[DP / 16];
+    TkOp<T> qf[DP / 16], gf[DP / 16];
     const T *qrow = (const T *)a.q + b * a.qs[0] + (long long)w.i * a.qs[1] + w.head * a.qs[2], *grow = (const T *)a.g + row * a.Dv;
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
-        qf[kk] = at_load8(qrow, 16 * kk + 8 * h, a.Dk);
-        gf[kk] = at_load8(grow, 16 * kk + 8 * h, a.Dv);
+        qf[kk] = tk_op(at_load8(qrow, 16 * kk + 8 * h, a.Dk));
+        gf[kk] = tk_op(at_load8(grow, 16 * kk + 8 * h, a.Dv));
     }
     const float lse = a.lse[row], delta = a.delta[row];
     const T *kb = (const T *)a.k + b * a.ks[0] + hk * a.ks[2], *vb = (const T *)a.v + b * a.vs[0] + hk * a.vs[2];
@@ -564,18 +575,19 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
     tk16 acc[DP / 32] = {};
     int buf = 0;
     if (j0 < j1) fetch(0, j0);
-    for (int j = j0; j < j1; j += KT, buf ^= 1) {
+    for (int j = j0; j < j1; j += KT, buf ^= NB - 1) {
+        if (NB == 1) __syncthreads();
         settle(buf);
         __syncthreads();
-        if (j + KT < j1) fetch(buf ^ 1, j + KT);
+        if (j + KT < j1) fetch(buf ^ (NB - 1), j + KT);
         if (j >= lim_any) continue;             // none of this wave's rows sees the tile
         const bool whole = j + KT <= lim_all;
 #pragma unroll
         for (int n = 0; n < KT / 32; ++n) {
             AtMask mk;
             if (MASK) mk = at_mask_row(a, mrow, j + 32 * n, h);
-            tk16 s = at_product<T, DP>(Ks[buf], 32 * n, qf, lane);
-            const tk16 dp = at_product<T, DP>(Vs[buf], 32 * n, gf, lane);
+            tk16 s = at_product<T, DP, PLANE>(Ks[buf], 32 * n, qf, lane);
+            const tk16 dp = at_product<T, DP, PLANE>(Vs[buf], 32 * n, gf, lane);
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse)) * (dp[e] - delta);
             if (!whole)
@@ -584,7 +596,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
                     const bool on = j + 32 * n + at_row(e, h) < w.lim && (!MASK || at_mask_on(mk, e));
                     s[e] = on ? s[e] : 0.f;
                 }
-            at_accumulate<T, DP>(acc, Ks[buf], 32 * n, s, lane);
+            at_accumulate<T, DP, PLANE>(acc, Ks[buf], 32 * n, s, lane);
         }
     }
     if (!w.valid) continue;
@@ -599,10 +611,10 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
 
 template <typename T, int DP, bool MASK, int WHAT>
 __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
-    constexpr int QT = at_tile<T>(), S = at_stride<T, DP>();
-    __shared__ __attribute__((aligned(16))) T Qs[2][QT * S];
-    __shared__ __attribute__((aligned(16))) T Gs[2][QT * S];
-    __shared__ __attribute__((aligned(16))) float lses[2][QT], deltas[2][QT];
+    constexpr int QT = at_tile<T>(), PLANE = QT * DP, NB = at_buffers<T, DP>();
+    __shared__ __attribute__((aligned(16))) tkh Qs[NB][tk_planes<T>() * PLANE];
+    __shared__ __attribute__((aligned(16))) tkh Gs[NB][tk_planes<T>() * PLANE];
+    __shared__ __attribute__((aligned(16))) float lses[NB][QT], deltas[NB][QT];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const AtBlock w0 = at_block(a, 1);
     const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk;
@@ -617,13 +629,13 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
     // queries that see this key: [first, Tq)
     const int first = key >= L ? 0x7fffffff : (a.causal ? key - off : 0);
     constexpr bool DK = WHAT & 1, DV = WHAT & 2;
-    TkFrag<T> kf[DP / 16], vf[DP / 16];
+    TkOp<T> kf[DP / 16], vf[DP / 16];
     const T *krow = (const T *)a.k + b * a.ks[0] + (long long)kc * a.ks[1] + hk * a.ks[2];
     const T *vrow = (const T *)a.v + b * a.vs[0] + (long long)kc * a.vs[1] + hk * a.vs[2];
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) {
-        kf[kk] = at_load8(krow, 16 * kk + 8 * h, a.Dk);
-        if (DK) vf[kk] = at_load8(vrow, 16 * kk + 8 * h, a.Dv);
+        kf[kk] = tk_op(at_load8(krow, 16 * kk + 8 * h, a.Dk));
+        if (DK) vf[kk] = tk_op(at_load8(vrow, 16 * kk + 8 * h, a.Dv));
     }
     tk16 acck[DK ? DP / 32 : 1] = {}, accv[DV ? DP / 32 : 1] = {};
     // the list of (head of the group, query tile) that sees any key of this tile, cut into nsplit runs
@@ -663,10 +675,11 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
     };
     int buf = 0;
     if (sp * per < it1) fetch(0, sp * per);
-    for (int it = sp * per; it < it1; ++it, buf ^= 1) {
+    for (int it = sp * per; it < it1; ++it, buf ^= NB - 1) {
+        if (NB == 1) __syncthreads();
         settle(buf);
         __syncthreads();
-        if (it + 1 < it1) fetch(buf ^ 1, it + 1);
+        if (it + 1 < it1) fetch(buf ^ (NB - 1), it + 1);
         const int gi = it / each, i0 = (qt0 + it - gi * each) * QT, head = hk * grp + gi;
         const bool whole = i0 >= first_all && i0 + QT <= a.Tq;
         const unsigned char *mcol = MASK ? a.mask + b * a.ms[0] + head * a.ms[1] + kc * a.ms[3] : nullptr;
@@ -676,9 +689,9 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
             if (MASK)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) mk[e] = mcol[min(i0 + 32 * n + at_row(e, h), a.Tq - 1) * a.ms[2]];
-            tk16 s = at_product<T, DP>(Qs[buf], 32 * n, kf, lane);
+            tk16 s = at_product<T, DP, PLANE>(Qs[buf], 32 * n, kf, lane);
             tk16 dp = {};
-            if (DK) dp = at_product<T, DP>(Gs[buf], 32 * n, vf, lane);
+            if (DK) dp = at_product<T, DP, PLANE>(Gs[buf], 32 * n, vf, lane);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const tkf4 le = *reinterpret_cast<const tkf4 *>(&lses[buf][32 * n + 8 * u + 4 * h]), de = *reinterpret_cast<const tkf4 *>(&deltas[buf][32 * n + 8 * u + 4 * h]);
@@ -697,8 +710,8 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
                     s[e] = on ? s[e] : 0.f;
                     dp[e] = on ? dp[e] : 0.f;
                 }
-            if constexpr (DV) at_accumulate<T, DP>(accv, Gs[buf], 32 * n, s, lane);
-            if constexpr (DK) at_accumulate<T, DP>(acck, Qs[buf], 32 * n, dp, lane);
+            if constexpr (DV) at_accumulate<T, DP, PLANE>(accv, Gs[buf], 32 * n, s, lane);
+            if constexpr (DK) at_accumulate<T, DP, PLANE>(acck, Qs[buf], 32 * n, dp, lane);
         }
     }
     if (!valid) continue;

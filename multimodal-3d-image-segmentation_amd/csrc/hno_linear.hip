@@ -26,11 +26,6 @@ struct LnMid { static constexpr int TM = 128, TN = 128, KB = 64, ST = 2, WM = 64
 struct LnF32 { static constexpr int TM = 128, TN = 128, KB = 32, ST = 2, WM = 64, WN = 64; };
 template <typename C> constexpr int ln_waves() { return C::TM / C::WM * (C::TN / C::WN); }
 
-// fp32: a value is three bf16 terms, its leading 8 bits, the next 8 and the last 8 (cut, not rounded: their sum is the value), and a product is the six products
-// of terms down to 2^-16 on the bf16 matrix instruction -- the two dropped ones are 2^-22 at most, 2^-25 on average, of the product.
-// An fp32 matrix instruction takes 1.3 times as long for the same work (and more than twice counting that six need one set of operands).
-template <typename T> constexpr int ln_planes() { return sizeof(T) == 2 ? 1 : 3; }
-
 // Where 8 elements (chunk c of row r) of an operand's LDS tile stand.  Along k: TILE rows of KB; 16 consecutive rows at one chunk touch all banks.
 // Across: KB rows of TILE; 4 consecutive rows at four neighbouring chunks touch all banks (the transposed reads).
 template <int TILE, int KB, bool ACROSS>
@@ -96,23 +91,9 @@ struct LnStage {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 tkh *p = tile + ln_at<TILE, KB, ACROSS>(row(i, tid), chunk(i, tid));
-                if constexpr (sizeof(T) == 2) {
-                    tk_store8(p, r[i]);
-                } else {
-                    tku4 h[3];
+                const TkOp<T> o = tk_op(r[i]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        unsigned a = __float_as_uint(r[i].v[2 * j]), b = __float_as_uint(r[i].v[2 * j + 1]);
-#pragma unroll
-                        for (int t = 0; t < 3; ++t) {
-                            h[t][j] = __builtin_amdgcn_perm(b, a, 0x07060302);
-                            a = __float_as_uint(__uint_as_float(a) - __uint_as_float(a & 0xffff0000u));
-                            b = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xffff0000u));
-                        }
-                    }
-#pragma unroll
-                    for (int t = 0; t < 3; ++t) *reinterpret_cast<tku4 *>(p + t * PLANE) = h[t];
-                }
+                for (int t = 0; t < tk_planes<T>(); ++t) tk_store8(p + t * PLANE, o.p[t]);
             }
         }
     }
@@ -181,7 +162,7 @@ __device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float 
 // DMA: ST LDS buffers, the next ST - 1 steps' tiles on their way while this one is multiplied.  Else the next step's tiles wait in registers: one buffer.
 template <typename T, bool AX, bool BX, typename C, bool DMA, int ACT>
 __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a) {
-    constexpr int TM = C::TM, TN = C::TN, KB = C::KB, P = ln_planes<T>(), WM = C::WM, WN = C::WN, NT = 64 * ln_waves<C>(), NB = DMA ? C::ST : 1;
+    constexpr int TM = C::TM, TN = C::TN, KB = C::KB, P = tk_planes<T>(), WM = C::WM, WN = C::WN, NT = 64 * ln_waves<C>(), NB = DMA ? C::ST : 1;
     constexpr int PA = TM * KB, PB = TN * KB, BUF = P * (PA + PB);
     constexpr int ES = WN + 4, EP = 2 * ln_waves<C>() * 32 * ES;                  // (epilogue: 32 rows of floats a wave)
     __shared__ __attribute__((aligned(16))) tkh smem[EP > NB * BUF ? EP : NB * BUF];
@@ -221,14 +202,14 @@ __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a
         if (ks + ahead < k1) fetch(ks + ahead, DMA ? (buf == 0 ? NB - 1 : buf - 1) : 0);
         // fragments are read one chunk ahead of their products
         constexpr int FB = P == 1 ? 2 : 1;
-        TkFrag<tkh> fa[FB][P][WM / 32], fb[FB][P][WN / 32];
+        TkOp<T> fa[FB][WM / 32], fb[FB][WN / 32];
         const auto read = [&](int kk) {
 #pragma unroll
             for (int p = 0; p < P; ++p) {
 #pragma unroll
-                for (int v = 0; v < WN / 32; ++v) fb[kk % FB][p][v] = ln_frag<TN, KB, BX>(Bs + p * PB, wn + 32 * v, kk, lane);
+                for (int v = 0; v < WN / 32; ++v) fb[kk % FB][v].p[p] = ln_frag<TN, KB, BX>(Bs + p * PB, wn + 32 * v, kk, lane);
 #pragma unroll
-                for (int u = 0; u < WM / 32; ++u) fa[kk % FB][p][u] = ln_frag<TM, KB, AX>(As + p * PA, wm + 32 * u, kk, lane);
+                for (int u = 0; u < WM / 32; ++u) fa[kk % FB][u].p[p] = ln_frag<TM, KB, AX>(As + p * PA, wm + 32 * u, kk, lane);
             }
         };
         if (FB == 2) read(0);
@@ -238,13 +219,9 @@ __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a
             else if (kk + 1 < KB / 16) read(kk + 1);
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int t = P - 1; t >= 0; --t)          // smallest terms first
+            for (int u = 0; u < WM / 32; ++u)
 #pragma unroll
-                for (int p = 0; p <= t; ++p)
-#pragma unroll
-                    for (int u = 0; u < WM / 32; ++u)
-#pragma unroll
-                        for (int v = 0; v < WN / 32; ++v) acc[u][v] = tk_mma(fb[kk % FB][p][v], fa[kk % FB][t - p][u], acc[u][v]);
+                for (int v = 0; v < WN / 32; ++v) acc[u][v] = tk_mma(fb[kk % FB][v], fa[kk % FB][u], acc[u][v]);
             __builtin_amdgcn_s_setprio(0);
         }
         if constexpr (DMA) buf = buf == NB - 1 ? 0 : buf + 1;

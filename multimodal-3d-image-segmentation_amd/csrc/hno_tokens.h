@@ -3,8 +3,10 @@
 // Matrix products run on the 32 x 32 tile of one wave.  A fragment is 8 contraction elements of one operand row per lane:
 //   lane l holds row (or column) l & 31; its elements are the contraction indices the instruction assigns to half h = l >> 5
 //   result    lane l, register r holds row 8 (r / 4) + 4 h + r % 4 of column l & 31
-// bf16: ONE v_mfma_f32_32x32x16_bf16 per fragment pair.  fp32: eight v_mfma_f32_32x32x2_f32 (element j of both halves per instruction).
-// The sum does not depend on which index sits in which slot as long as both operands agree; the attention kernels use this to feed
+// on v_mfma_f32_32x32x16_bf16.  fp32 values are three bf16 terms: the leading 8 bits, the next 8 and the last 8 (cut, not rounded: their sum is the value); a product
+// is the six products of terms down to 2^-16, smallest first -- the two dropped ones are at most 2^-22, on average 2^-25, of it.  The fp32 matrix instruction takes
+// 2.7 times as long for the same work.  (An infinity becomes inf + NaN + NaN: products with it are NaN.)
+// A sum does not depend on which index sits in which slot as long as both operands agree; the attention kernels use this to feed
 // a result back as an operand without moving it between lanes: registers 8 t .. 8 t + 7 of a result are the fragment whose
 // slots stand for rows 16 t + 4 h + {0..3} and 16 t + 8 + 4 h + {0..3}.
 #pragma once
@@ -25,7 +27,7 @@ template <typename T> __device__ __forceinline__ T tk_down(float v);
 template <> __device__ __forceinline__ float tk_down<float>(float v) { return v; }
 template <> __device__ __forceinline__ tkh tk_down<tkh>(float v) { return __builtin_bit_cast(tkh, (__bf16)v); }   // to nearest even
 
-struct TkF8 { float v[8]; };
+// 8 values of a type as they lie in memory
 template <typename T> struct TkFrag;
 template <> struct TkFrag<tkh> {
     tkb8 v;
@@ -35,13 +37,34 @@ template <> struct TkFrag<float> {
     float v[8];
     __device__ __forceinline__ void set(int j, float x) { v[j] = x; }
 };
-
-__device__ __forceinline__ tk16 tk_mma(const TkFrag<tkh> &a, const TkFrag<tkh> &b, tk16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
-}
-__device__ __forceinline__ tk16 tk_mma(const TkFrag<float> &a, const TkFrag<float> &b, tk16 c) {
+// the same as an operand: its bf16 terms
+template <typename T> constexpr int tk_planes() { return sizeof(T) == 2 ? 1 : 3; }
+template <typename T> struct TkOp { TkFrag<tkh> p[tk_planes<T>()]; };
+__device__ __forceinline__ TkOp<tkh> tk_op(const TkFrag<tkh> &f) { return {{f}}; }
+__device__ __forceinline__ TkOp<float> tk_op(const TkFrag<float> &f) {
+    TkOp<float> o;
+    tku4 h[3];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[j], b.v[j], c, 0, 0, 0);
+    for (int j = 0; j < 4; ++j) {
+        unsigned a = __float_as_uint(f.v[2 * j]), b = __float_as_uint(f.v[2 * j + 1]);
+#pragma unroll
+        for (int t = 0; t < 3; ++t) {
+            h[t][j] = __builtin_amdgcn_perm(b, a, 0x07060302);
+            a = __float_as_uint(__uint_as_float(a) - __uint_as_float(a & 0xffff0000u));
+            b = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xffff0000u));
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 3; ++t) o.p[t].v = __builtin_bit_cast(tkb8, h[t]);
+    return o;
+}
+template <typename T>
+__device__ __forceinline__ tk16 tk_mma(const TkOp<T> &a, const TkOp<T> &b, tk16 c) {
+    constexpr int P = tk_planes<T>();
+#pragma unroll
+    for (int t = P - 1; t >= 0; --t)
+#pragma unroll
+        for (int p = 0; p <= t; ++p) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[p].v, b.p[t - p].v, c, 0, 0, 0);
     return c;
 }
 
@@ -59,36 +82,6 @@ __device__ __forceinline__ void tk_store8(float *p, const TkFrag<float> &f) {
     *reinterpret_cast<tkf4 *>(p) = tkf4{f.v[0], f.v[1], f.v[2], f.v[3]};
     *reinterpret_cast<tkf4 *>(p + 4) = tkf4{f.v[4], f.v[5], f.v[6], f.v[7]};
 }
-// 8 elements of one tensor row starting at element d of D; `vec`: every row is 16-byte aligned and D % 8 == 0
-template <typename T>
-__device__ __forceinline__ TkFrag<T> tk_load8(const T *row, int d, int D, bool vec) {
-    if (vec && d < D) return tk_row(row + d);
-    TkFrag<T> f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f.set(j, 0.f);
-    if (!vec)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (d + j < D) f.set(j, tk_up(row[d + j]));
-    return f;
-}
-// the fragment of the TRANSPOSE of a row-major LDS tile: column `col0 + (lane & 31)`, rows r0 .. r0 + 3 and r1 .. r1 + 3.
-// bf16: ds_read_b64_tr_b16, which hands lane i of a group of 16 the column i of the 4 x 16 block whose rows the group's lanes address
-__device__ __forceinline__ TkFrag<tkh> tk_col(const tkh *tile, int stride, int col0, int r0, int r1, int lane) {
-    typedef __attribute__((address_space(3))) tks4 *lds4;
-    const tkh *p = tile + ((lane & 15) >> 2) * stride + col0 + (lane & 16) + 4 * (lane & 3);
-    const tks4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + r0 * stride));
-    const tks4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + r1 * stride));
-    return {__builtin_bit_cast(tkb8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7))};
-}
-__device__ __forceinline__ TkFrag<float> tk_col(const float *tile, int stride, int col0, int r0, int r1, int lane) {
-    TkFrag<float> f;
-    const float *p = tile + col0 + (lane & 31);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) f.v[j] = p[(r0 + j) * stride], f.v[4 + j] = p[(r1 + j) * stride];
-    return f;
-}
-
 // LDS-DMA: 64 lanes x 16 bytes from (wave-uniform base + per-lane byte offset) to 1024 consecutive LDS bytes at `dst` (wave-uniform).  No registers; retired by
 // dma_wait (hno_common.h).  M0 holds the destination and is put back: the compiler owns it.
 __device__ __forceinline__ void tk_dma16(const tkh *src, unsigned off, unsigned dst) {
@@ -96,10 +89,6 @@ __device__ __forceinline__ void tk_dma16(const tkh *src, unsigned off, unsigned 
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep) : "v"(off), "s"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory");
 }
-
-// 16 bytes of padding behind each row of a tile: the row stride in 16-byte units is odd, so 8 lanes that read 16 bytes of 8
-// consecutive rows cover all 64 banks' width once
-template <typename T> constexpr int tk_pad() { return 16 / (int)sizeof(T); }
 
 // ------------------------------------------------------------------ activations (ids: hno.h)
 // 1 - Phi(|z|) = erfc(|z| / sqrt 2) / 2 by Abramowitz and Stegun 7.1.26 (five terms, absolute error of erf 1.5e-7); e2 = exp(-z^2 / 2).  libm's erfcf
