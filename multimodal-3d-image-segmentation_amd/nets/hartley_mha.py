@@ -4,8 +4,10 @@ Frequency-domain self-attention: Hartley transform + mode truncation (hno_dht3_c
 query/key/value projections (pointwise MFMA convs over the mode axis), patch grouping (pure index
 permutation), att = act(Q^T K / sqrt(C)) and out = V att^T on the batched fp32 MFMA GEMM (hno_bmm),
 output projection, zero pad + unscaled inverse transform (hno_pad_idht3).  SELU, not softmax, is the
-default attention activation, so no online normalisation is needed.
+default attention activation, so no online normalisation is needed there; a softmax over the keys
+(``functools.partial(F.softmax, dim=-1)``) goes through ops_tokens.attention.
 """
+import functools
 import math
 import os
 from typing import Union
@@ -14,7 +16,7 @@ import numpy as np
 import torch
 from torch.nn import Module, Parameter, init
 
-from .. import ops
+from .. import ops, ops_tokens
 
 
 def grouping3d(x, patch_size):
@@ -48,6 +50,15 @@ def ungrouping2d(x, num_channels, patch_size):
     """Inverse of grouping2d (reference :448-470)."""
     assert len(patch_size) == 2
     return ungrouping3d(x.unsqueeze(3), num_channels, (1,) + tuple(patch_size)).squeeze(3)
+
+
+def softmax_over_keys(act):
+    """whether an attention activation normalises the scores (B, Z, Tq, Tk) over the keys: ``functools.partial(F.softmax, dim=-1)`` (or 3, or
+    torch.softmax) and ``nn.Softmax(-1)``.  The name 'softmax' alone is refused: without ``dim`` torch would normalise over the heads."""
+    if isinstance(act, torch.nn.Softmax):
+        return act.dim in (-1, 3)
+    return (isinstance(act, functools.partial) and act.func in (torch.nn.functional.softmax, torch.softmax) and not act.args
+            and set(act.keywords) == {'dim'} and act.keywords['dim'] in (-1, 3))
 
 
 class HartleyMultiHeadAttention(Module):
@@ -127,7 +138,8 @@ class HartleyMultiHeadAttention(Module):
         else:
             specs = srcs
         q_src, k_src, v_src = specs[0], specs[min(1, len(specs) - 1)], specs[-1]
-        act_att = ops.act_id(self.attention_activation)
+        softmax = softmax_over_keys(self.attention_activation)
+        act_att = ops.ACT_NONE if softmax else ops.act_id(self.attention_activation)
         Z = self.num_heads
         # freq_conv3d 'zoi,bidhw->bzodhw' for all heads at once: the head axis folds into the output channels, and with a
         # single source (self-attention) the three projections are ONE pointwise conv with the stacked weights
@@ -149,7 +161,7 @@ class HartleyMultiHeadAttention(Module):
         one_pass = (patch is not None and q_src is k_src and k_src is v_src and (y.is_cuda or y.is_meta)
                     and os.environ.get('HNO_MHA_GROUP', '1') != '0')
         Kq, Kv = wq.shape[0] // Z, wv.shape[0] // Z
-        if (one_pass and wk.shape[0] == wq.shape[0] and os.environ.get('HNO_MHA_GROUP', '1') != '2'
+        if (one_pass and not softmax and wk.shape[0] == wq.shape[0] and os.environ.get('HNO_MHA_GROUP', '1') != '2'
                 and (y.is_meta or ops.GroupedAttentionFn.supported(Z, Kq, Kv, tuple(patch), act_att))):
             # grouping, attention and ungrouping as one node: the attention's partial sums are added by the ungrouping permutation
             out = ops.GroupedAttentionFn.apply(y, Z, Kq, Kv, tuple(patch), 1.0 / math.sqrt(Kq * int(np.prod(patch))), act_att)
@@ -170,7 +182,10 @@ class HartleyMultiHeadAttention(Module):
             freq_shape = tuple(q.shape[3:])
             q, k, v = (t.reshape(t.shape[0], Z, t.shape[2], -1).contiguous() for t in (q, k, v))   # (B, Z, C', T)
         alpha = 1.0 / math.sqrt(k.shape[2])
-        if q.is_meta or (q.shape[3] == k.shape[3] and ops.hmha_supported(q.shape[2], v.shape[2])):
+        if softmax:      # tokens x channels instead of channels x tokens; the scores are never written
+            out = ops_tokens.attention(*(t.permute(0, 3, 1, 2) for t in (q, k, v)), scale=alpha).permute(0, 2, 3, 1)
+            out = out.contiguous()
+        elif q.is_meta or (q.shape[3] == k.shape[3] and ops.hmha_supported(q.shape[2], v.shape[2])):
             # fused: QK^T -> scale -> activation -> .V in one kernel each way, the (T, T) matrix is never written
             out = ops.HartleyAttentionFn.apply(q, k, v, alpha, act_att)                           # (B, Z, C', Tq)
         else:   # > 128 grouped channels per head: batched GEMMs with the attention matrix in memory

@@ -80,7 +80,7 @@ def _heads(t, esize):
         return t
     if D % 8 == 0:
         return t.clone(memory_format=torch.contiguous_format)
-    return torch.nn.functional.pad(t, (0, -D % 8))
+    return torch.nn.functional.pad(t.contiguous(), (0, -D % 8))          # (pad keeps the order of the strides)
 
 
 def _attn_args(q, k, v, mask, kv_lens, causal, scale):
