@@ -208,6 +208,24 @@ __device__ __forceinline__ tk16 at_product(const tkh *tile, int row0, const TkOp
     }
     return acc;
 }
+// two independent products, step by step: neither waits for its own last step
+template <typename T, int DP, int PLANE>
+__device__ __forceinline__ void at_product2(tk16 &x, tk16 &y, const tkh *tx, int rx, const TkOp<T> (&ox)[DP / 16], const tkh *ty, int ry, const TkOp<T> (&oy)[DP / 16],
+                                            int lane) {
+    x = tk16{};
+    y = tk16{};
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+        TkOp<T> a, b;
+#pragma unroll
+        for (int p = 0; p < tk_planes<T>(); ++p) {
+            a.p[p] = tk_row(tx + p * PLANE + at_at<DP>(rx + (lane & 31), 16 * kk + 8 * (lane >> 5)));
+            b.p[p] = tk_row(ty + p * PLANE + at_at<DP>(ry + (lane & 31), 16 * kk + 8 * (lane >> 5)));
+        }
+        x = tk_mma(a, ox[kk], x);
+        y = tk_mma(b, oy[kk], y);
+    }
+}
 // acc[dt] += (tile rows row0 .. row0 + 31)^T . w, w being a result over the same rows
 template <typename T, int DP, int PLANE>
 __device__ __forceinline__ void at_accumulate(tk16 (&acc)[DP / 32], const tkh *tile, int row0, const tk16 &w, int lane) {
@@ -387,6 +405,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 4 ? (DP <= 96 ? 2 : 1) 
 #pragma unroll
         for (int n = 0; n < KT / 32; ++n) s[n] = at_product<T, DP, PLANE>(Ks[buf], 32 * n, qf, lane);
         if (j + KT > lim_all) {
+            asm volatile("");               // (a branch: the comparisons are not to be made for whole tiles)
 #pragma unroll
             for (int n = 0; n < KT / 32; ++n)
 #pragma unroll
@@ -586,16 +605,18 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
         for (int n = 0; n < KT / 32; ++n) {
             AtMask mk;
             if (MASK) mk = at_mask_row(a, mrow, j + 32 * n, h);
-            tk16 s = at_product<T, DP, PLANE>(Ks[buf], 32 * n, qf, lane);
-            const tk16 dp = at_product<T, DP, PLANE>(Vs[buf], 32 * n, gf, lane);
+            tk16 s, dp;
+            at_product2<T, DP, PLANE>(s, dp, Ks[buf], 32 * n, qf, Vs[buf], 32 * n, gf, lane);
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse)) * (dp[e] - delta);
-            if (!whole)
+            if (!whole) {
+                asm volatile("");           // (a branch: the comparisons are not to be made for whole tiles)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const bool on = j + 32 * n + at_row(e, h) < w.lim && (!MASK || at_mask_on(mk, e));
                     s[e] = on ? s[e] : 0.f;
                 }
+            }
             at_accumulate<T, DP, PLANE>(acc, Ks[buf], 32 * n, s, lane);
         }
     }
@@ -653,8 +674,8 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
     float nlse = 0.f, ndelta = 0.f;               // row tid of the tile
     const int empty = a.causal ? -off : 0;        // queries before it see nothing
     int i_next = 0;
-    const auto fetch = [&](int to, int it) {
-        const int gi = it / each, i0 = (qt0 + it - gi * each) * QT, head = hk * grp + gi;
+    const auto fetch = [&](int to, int gi, int qt) {
+        const int i0 = qt * QT, head = hk * grp + gi;
         const long long row0 = ((long long)b * a.Tq) * a.H + head;
         i_next = i0;
         qs.fetch(Qs[to], (const T *)a.q + b * a.qs[0] + head * a.qs[2], i0, a.Tq, tid);
@@ -674,13 +695,15 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
         if (tid < QT) lses[to][tid] = nlse, deltas[to][tid] = ndelta;
     };
     int buf = 0;
-    if (sp * per < it1) fetch(0, sp * per);
+    int gi = each > 0 ? sp * per / each : 0, qt = qt0 + sp * per - gi * each;
+    if (sp * per < it1) fetch(0, gi, qt);
     for (int it = sp * per; it < it1; ++it, buf ^= NB - 1) {
         if (NB == 1) __syncthreads();
         settle(buf);
         __syncthreads();
-        if (it + 1 < it1) fetch(buf ^ (NB - 1), it + 1);
-        const int gi = it / each, i0 = (qt0 + it - gi * each) * QT, head = hk * grp + gi;
+        const int i0 = qt * QT, head = hk * grp + gi;
+        if (++qt == nqt) qt = qt0, ++gi;
+        if (it + 1 < it1) fetch(buf ^ (NB - 1), gi, qt);
         const bool whole = i0 >= first_all && i0 + QT <= a.Tq;
         const unsigned char *mcol = MASK ? a.mask + b * a.ms[0] + head * a.ms[1] + kc * a.ms[3] : nullptr;
 #pragma unroll
@@ -689,9 +712,9 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
             if (MASK)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) mk[e] = mcol[min(i0 + 32 * n + at_row(e, h), a.Tq - 1) * a.ms[2]];
-            tk16 s = at_product<T, DP, PLANE>(Qs[buf], 32 * n, kf, lane);
-            tk16 dp = {};
-            if (DK) dp = at_product<T, DP, PLANE>(Gs[buf], 32 * n, vf, lane);
+            tk16 s, dp = {};
+            if constexpr (DK) at_product2<T, DP, PLANE>(s, dp, Qs[buf], 32 * n, kf, Gs[buf], 32 * n, vf, lane);
+            else s = at_product<T, DP, PLANE>(Qs[buf], 32 * n, kf, lane);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const tkf4 le = *reinterpret_cast<const tkf4 *>(&lses[buf][32 * n + 8 * u + 4 * h]), de = *reinterpret_cast<const tkf4 *>(&deltas[buf][32 * n + 8 * u + 4 * h]);
@@ -702,7 +725,8 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
                     dp[e] = s[e] * (dp[e] - de[j]);
                 }
             }
-            if (!whole)
+            if (!whole) {
+                asm volatile("");           // (a branch: the comparisons are not to be made for whole tiles)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int i = i0 + 32 * n + at_row(e, h);
@@ -710,6 +734,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
                     s[e] = on ? s[e] : 0.f;
                     dp[e] = on ? dp[e] : 0.f;
                 }
+            }
             if constexpr (DV) at_accumulate<T, DP, PLANE>(accv, Gs[buf], 32 * n, s, lane);
             if constexpr (DK) at_accumulate<T, DP, PLANE>(acck, Qs[buf], 32 * n, dp, lane);
         }

@@ -18,12 +18,12 @@ struct LinArgs {
     int M, N, K, act, bias32, out32, nsplit;
 };
 
-// Tiles of the result (TM x TN), contraction elements a step (KB), LDS buffers (ST) and the part of one wave (WM x WN).  With 64 x 64 per wave the LDS reads of a step
+// Tiles of the result (TM x TN), contraction elements a step (KB) and the part of one wave (WM x WN).  With 64 x 64 per wave the LDS reads of a step
 // take as long as its matrix instructions, with 128 x 64 three quarters.
 //   LnBig: large results; LnMid: small ones (more tiles, two workgroups a CU); LnF32: three planes per operand
-struct LnBig { static constexpr int TM = 256, TN = 256, KB = 64, ST = 2, WM = 128, WN = 64; };
-struct LnMid { static constexpr int TM = 128, TN = 128, KB = 64, ST = 2, WM = 64, WN = 64; };
-struct LnF32 { static constexpr int TM = 128, TN = 128, KB = 32, ST = 2, WM = 64, WN = 64; };
+struct LnBig { static constexpr int TM = 256, TN = 256, KB = 64, WM = 128, WN = 64; };
+struct LnMid { static constexpr int TM = 128, TN = 128, KB = 64, WM = 64, WN = 64; };
+struct LnF32 { static constexpr int TM = 128, TN = 128, KB = 32, WM = 64, WN = 64; };
 template <typename C> constexpr int ln_waves() { return C::TM / C::WM * (C::TN / C::WN); }
 
 // Where 8 elements (chunk c of row r) of an operand's LDS tile stand.  Along k: TILE rows of KB; 16 consecutive rows at one chunk touch all banks.
@@ -41,32 +41,36 @@ struct LnStage {
     static constexpr int CH = (ACROSS ? TILE : KB) / 8, N = TILE * KB / 8 / NT, PLANE = TILE * KB;
     static constexpr int NR = DMA ? 1 : N;
     TkFrag<T> r[NR];
+    unsigned off[DMA ? N : 1];           // DMA: byte offset of each slot's source from the tile's corner
     const T *base;
     long long ld;
     int rows, cols, row0, col0;          // of the stored matrix, and the tile's corner (the corner along k moves)
-    __device__ __forceinline__ void init(const void *p, long long ld_, int m0, int M, int K) {
+    __device__ __forceinline__ void init(const void *p, long long ld_, int m0, int M, int K, int tid) {
         base = (const T *)p, ld = ld_;
         rows = ACROSS ? K : M, cols = ACROSS ? M : K, row0 = ACROSS ? 0 : m0, col0 = ACROSS ? m0 : 0;
+        if constexpr (DMA)
+#pragma unroll
+            for (int i = 0; i < N; ++i) off[i] = offset(row(i, tid), source(i, tid) * 8, ACROSS ? KB : rows - row0, ACROSS ? cols - col0 : KB);
     }
     __device__ __forceinline__ static int row(int i, int tid) { return (tid + NT * i) / CH; }
     __device__ __forceinline__ static int chunk(int i, int tid) { return (tid + NT * i) % CH; }
     // DMA (16-byte aligned rows, whole chunks): the chunk whose place the slot is
     __device__ __forceinline__ static int source(int i, int tid) { return (ln_at<TILE, KB, ACROSS>(row(i, tid), chunk(i, tid)) / 8) % CH; }
+    // beyond the `nr` rows or `nc` columns left of the matrix: any element of it (settle() clears what must not count)
+    __device__ __forceinline__ unsigned offset(int rr, int cc, int nr, int nc) const { return (unsigned)(min(rr, nr - 1) * (int)ld + (cc < nc ? cc : 0)) * 2; }
     __device__ __forceinline__ void fetch(tkh *tile, int k0, int tid) {
         const int ra = ACROSS ? k0 : row0, ca = ACROSS ? col0 : k0;
         const T *src = base + (long long)ra * ld + ca;
         const bool whole = ra + (ACROSS ? KB : TILE) <= rows && ca + (ACROSS ? TILE : KB) <= cols;
         if constexpr (DMA) {
             typedef __attribute__((address_space(3))) tkh *ldsp;
-            const unsigned dst = (unsigned)(uintptr_t)(ldsp)tile + (tid >> 6) * 1024;
+            const unsigned dst = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(ldsp)tile + (tid >> 6) * 1024);
+            if (k0 + KB <= (ACROSS ? rows : cols)) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                int rr = row(i, tid), cc = source(i, tid) * 8;
-                if (!whole) {            // beyond the matrix: any element of it (settle() clears what must not count)
-                    rr = min(rr, rows - 1 - ra);
-                    cc = ca + cc < cols ? cc : 0;
-                }
-                tk_dma16(src, (unsigned)(rr * (int)ld + cc) * 2, dst + i * NT * 16);
+                for (int i = 0; i < N; ++i) tk_dma16(src, off[i], dst + i * NT * 16);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) tk_dma16(src, offset(row(i, tid), source(i, tid) * 8, rows - ra, cols - ca), dst + i * NT * 16);
             }
         } else {
 #pragma unroll
@@ -159,11 +163,11 @@ __device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float 
     else ln_put8((T *)a.y + at, cnt, x);
 }
 
-// DMA: ST LDS buffers, the next ST - 1 steps' tiles on their way while this one is multiplied.  Else the next step's tiles wait in registers: one buffer.
+// DMA: two LDS buffers, the next step's tiles on their way while this one is multiplied.  Else the next step's tiles wait in registers: one buffer.
 template <typename T, bool AX, bool BX, typename C, bool DMA, int ACT>
 __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a) {
-    constexpr int TM = C::TM, TN = C::TN, KB = C::KB, P = tk_planes<T>(), WM = C::WM, WN = C::WN, NT = 64 * ln_waves<C>(), NB = DMA ? C::ST : 1;
-    constexpr int PA = TM * KB, PB = TN * KB, BUF = P * (PA + PB);
+    constexpr int TM = C::TM, TN = C::TN, KB = C::KB, P = tk_planes<T>(), WM = C::WM, WN = C::WN, NT = 64 * ln_waves<C>(), NB = DMA ? 2 : 1;
+    constexpr int PA = TM * KB, PB = TN * KB, BUF = P * (PA + PB);      // LDS: A's buffers, then B's
     constexpr int ES = WN + 4, EP = 2 * ln_waves<C>() * 32 * ES;                  // (epilogue: 32 rows of floats a wave)
     __shared__ __attribute__((aligned(16))) tkh smem[EP > NB * BUF ? EP : NB * BUF];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, wm = (wave % (TM / WM)) * WM, wn = (wave / (TM / WM)) * WN;
@@ -176,55 +180,79 @@ __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a
     const int steps = (a.K + KB - 1) / KB, per = (steps + a.nsplit - 1) / a.nsplit, k0 = run * per, k1 = min(k0 + per, steps);
     LnStage<T, TM, KB, NT, AX, DMA> sa;
     LnStage<T, TN, KB, NT, BX, DMA> sb;
-    sa.init(a.A, a.lda, m0, a.M, a.K);
-    sb.init(a.B, a.ldb, n0, a.N, a.K);
+    sa.init(a.A, a.lda, m0, a.M, a.K, tid);
+    sb.init(a.B, a.ldb, n0, a.N, a.K, tid);
     const auto fetch = [&](int ks, int buf) {
-        sa.fetch(smem + buf * BUF, ks * KB, tid);
-        sb.fetch(smem + buf * BUF + P * PA, ks * KB, tid);
+        sa.fetch(smem + buf * P * PA, ks * KB, tid);
+        sb.fetch(smem + (NB * PA + buf * PB) * P, ks * KB, tid);
+    };
+    const auto settle = [&](int ks, int buf) {
+        sa.settle(smem + buf * P * PA, ks * KB, a.K, tid);
+        sb.settle(smem + (NB * PA + buf * PB) * P, ks * KB, a.K, tid);
+    };
+    // fragments of chunk kk; two sets where registers allow, so that they are read one chunk ahead of their products
+    constexpr int FB = P == 1 ? 2 : 1, KC = KB / 16;
+    TkOp<T> fa[FB][WM / 32], fb[FB][WN / 32];
+    const auto read = [&](int buf, int kk) {
+        const tkh *As = smem + buf * P * PA, *Bs = smem + (NB * PA + buf * PB) * P;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+#pragma unroll
+            for (int v = 0; v < WN / 32; ++v) fb[kk % FB][v].p[p] = ln_frag<TN, KB, BX>(Bs + p * PB, wn + 32 * v, kk, lane);
+#pragma unroll
+            for (int u = 0; u < WM / 32; ++u) fa[kk % FB][u].p[p] = ln_frag<TM, KB, AX>(As + p * PA, wm + 32 * u, kk, lane);
+        }
     };
     tk16 acc[WM / 32][WN / 32] = {};
+    const auto multiply = [&](int kk) {
 #pragma unroll
-    for (int i = 0; i < (DMA ? NB - 1 : 1); ++i)
-        if (k0 + i < k1) fetch(k0 + i, i);
-    int buf = 0;
-    for (int ks = k0; ks < k1; ++ks) {
-        if constexpr (DMA) {
-            if (ks + NB - 2 < k1 - 1) dma_wait<(NB - 2) * (sa.N + sb.N)>();      // the steps behind this one stay in flight
-            else dma_wait<0>();
-        } else {
+        for (int u = 0; u < WM / 32; ++u)
+#pragma unroll
+            for (int v = 0; v < WN / 32; ++v) acc[u][v] = tk_mma(fb[kk % FB][v], fa[kk % FB][u], acc[u][v]);
+    };
+    if constexpr (DMA) {
+        // one barrier a step, before its last chunk, whose fragments every wave has by then: behind it the next step's tiles are whole, this step's buffer
+        // is free for the step after, and the next step's first fragments are read beside the last chunk's products
+        static_assert(NB == 2 && FB == 2 && KC % 2 == 0, "two buffers, an even number of chunks");
+        const auto turn = [&](int ks, int buf) {          // step ks is complete in `buf`; ks + 1 goes to the other buffer
+            dma_wait<0>();
+            settle(ks, buf);
             __syncthreads();
-        }
-        tkh *As = smem + buf * BUF, *Bs = As + P * PA;
-        sa.settle(As, ks * KB, a.K, tid);
-        sb.settle(Bs, ks * KB, a.K, tid);
-        __syncthreads();
-        const int ahead = DMA ? NB - 1 : 1;
-        if (ks + ahead < k1) fetch(ks + ahead, DMA ? (buf == 0 ? NB - 1 : buf - 1) : 0);
-        // fragments are read one chunk ahead of their products
-        constexpr int FB = P == 1 ? 2 : 1;
-        TkOp<T> fa[FB][WM / 32], fb[FB][WN / 32];
-        const auto read = [&](int kk) {
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-#pragma unroll
-                for (int v = 0; v < WN / 32; ++v) fb[kk % FB][v].p[p] = ln_frag<TN, KB, BX>(Bs + p * PB, wn + 32 * v, kk, lane);
-#pragma unroll
-                for (int u = 0; u < WM / 32; ++u) fa[kk % FB][u].p[p] = ln_frag<TM, KB, AX>(As + p * PA, wm + 32 * u, kk, lane);
-            }
+            if (ks + 1 < k1) fetch(ks + 1, buf ^ 1);
+            read(buf, 0);
         };
-        if (FB == 2) read(0);
+        const auto step = [&](int ks, int buf) {
 #pragma unroll
-        for (int kk = 0; kk < KB / 16; ++kk) {
-            if (FB == 1) read(kk);
-            else if (kk + 1 < KB / 16) read(kk + 1);
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int u = 0; u < WM / 32; ++u)
-#pragma unroll
-                for (int v = 0; v < WN / 32; ++v) acc[u][v] = tk_mma(fb[kk % FB][v], fa[kk % FB][u], acc[u][v]);
-            __builtin_amdgcn_s_setprio(0);
+            for (int kk = 0; kk + 1 < KC; ++kk) {
+                read(buf, kk + 1);
+                multiply(kk);
+            }
+            if (ks + 1 < k1) turn(ks + 1, buf ^ 1);
+            multiply(KC - 1);
+        };
+        if (k0 < k1) {
+            fetch(k0, 0);
+            turn(k0, 0);
         }
-        if constexpr (DMA) buf = buf == NB - 1 ? 0 : buf + 1;
+        for (int ks = k0; ks < k1; ks += 2) {          // (the buffers by name: their addresses are then constants)
+            step(ks, 0);
+            if (ks + 1 < k1) step(ks + 1, 1);
+        }
+    } else {
+        if (k0 < k1) fetch(k0, 0);
+        for (int ks = k0; ks < k1; ++ks) {
+            __syncthreads();
+            settle(ks, 0);
+            __syncthreads();
+            if (ks + 1 < k1) fetch(ks + 1, 0);
+            if (FB == 2) read(0, 0);
+#pragma unroll
+            for (int kk = 0; kk < KC; ++kk) {
+                if (FB == 1) read(0, kk);
+                else if (kk + 1 < KC) read(0, kk + 1);
+                multiply(kk);
+            }
+        }
     }
     // the results change places in LDS, 32 rows of a wave at a time (its own part: no barrier inside), so that memory is read and written in runs of 128 bytes
     __syncthreads();
