@@ -58,7 +58,8 @@ struct LnStage {
     __device__ __forceinline__ static int source(int i, int tid) { return (ln_at<TILE, KB, ACROSS>(row(i, tid), chunk(i, tid)) / 8) % CH; }
     // beyond the `nr` rows or `nc` columns left of the matrix: any element of it (settle() clears what must not count)
     __device__ __forceinline__ unsigned offset(int rr, int cc, int nr, int nc) const { return (unsigned)(min(rr, nr - 1) * (int)ld + (cc < nc ? cc : 0)) * 2; }
-    __device__ __forceinline__ void fetch(tkh *tile, int k0, int tid) {
+    // slots i0 ... i1 - 1 (DMA; the last, partial step goes whole with the first of them)
+    __device__ __forceinline__ void fetch(tkh *tile, int k0, int tid, int i0 = 0, int i1 = N) {
         const int ra = ACROSS ? k0 : row0, ca = ACROSS ? col0 : k0;
         const T *src = base + (long long)ra * ld + ca;
         const bool whole = ra + (ACROSS ? KB : TILE) <= rows && ca + (ACROSS ? TILE : KB) <= cols;
@@ -67,8 +68,9 @@ struct LnStage {
             const unsigned dst = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(ldsp)tile + (tid >> 6) * 1024);
             if (k0 + KB <= (ACROSS ? rows : cols)) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) tk_dma16(src, off[i], dst + i * NT * 16);
-            } else {
+                for (int i = 0; i < N; ++i)
+                    if (i >= i0 && i < i1) tk_dma16(src, off[i], dst + i * NT * 16);
+            } else if (i0 == 0) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) tk_dma16(src, offset(row(i, tid), source(i, tid) * 8, rows - ra, cols - ca), dst + i * NT * 16);
             }
@@ -204,35 +206,50 @@ __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a
         }
     };
     tk16 acc[WM / 32][WN / 32] = {};
-    const auto multiply = [&](int kk) {
+    const auto multiply = [&](int kk, auto between) {          // between(u): what is issued behind row u of the products
 #pragma unroll
-        for (int u = 0; u < WM / 32; ++u)
+        for (int u = 0; u < WM / 32; ++u) {
 #pragma unroll
             for (int v = 0; v < WN / 32; ++v) acc[u][v] = tk_mma(fb[kk % FB][v], fa[kk % FB][u], acc[u][v]);
+            between(u);
+        }
     };
+    const auto nothing = [](int) {};
     if constexpr (DMA) {
         // one barrier a step, before its last chunk, whose fragments every wave has by then: behind it the next step's tiles are whole, this step's buffer
         // is free for the step after, and the next step's first fragments are read beside the last chunk's products
         static_assert(NB == 2 && FB == 2 && KC % 2 == 0, "two buffers, an even number of chunks");
-        const auto turn = [&](int ks, int buf) {          // step ks is complete in `buf`; ks + 1 goes to the other buffer
-            dma_wait<0>();
-            settle(ks, buf);
-            __syncthreads();
-            if (ks + 1 < k1) fetch(ks + 1, buf ^ 1);
-            read(buf, 0);
-        };
+        // the DMA of a step's tiles is issued in pieces between products: those of A beside the last chunk, those of B beside the first of the next step
+        constexpr int U = WM / 32;
+        static_assert(sa.N % U == 0 && sb.N % U == 0, "whole pieces");
+        const auto fetch_a = [&](int ks, int buf, int u) { sa.fetch(smem + buf * P * PA, ks * KB, tid, u * (sa.N / U), (u + 1) * (sa.N / U)); };
+        const auto fetch_b = [&](int ks, int buf, int u) { sb.fetch(smem + (NB * PA + buf * PB) * P, ks * KB, tid, u * (sb.N / U), (u + 1) * (sb.N / U)); };
         const auto step = [&](int ks, int buf) {
+            const bool next = ks + 1 < k1, after = ks + 2 < k1;
+            read(buf, 1);
+            multiply(0, [&](int u) { if (next) fetch_b(ks + 1, buf ^ 1, u); });
 #pragma unroll
-            for (int kk = 0; kk + 1 < KC; ++kk) {
+            for (int kk = 1; kk + 1 < KC; ++kk) {
                 read(buf, kk + 1);
-                multiply(kk);
+                multiply(kk, nothing);
             }
-            if (ks + 1 < k1) turn(ks + 1, buf ^ 1);
-            multiply(KC - 1);
+            if (next) {
+                dma_wait<0>();
+                settle(ks + 1, buf ^ 1);
+                __syncthreads();
+                read(buf ^ 1, 0);
+            }
+            multiply(KC - 1, [&](int u) { if (after) fetch_a(ks + 2, buf, u); });
         };
         if (k0 < k1) {
             fetch(k0, 0);
-            turn(k0, 0);
+            if (k0 + 1 < k1)
+#pragma unroll
+                for (int u = 0; u < U; ++u) fetch_a(k0 + 1, 1, u);
+            dma_wait<0>();
+            settle(k0, 0);
+            __syncthreads();
+            read(0, 0);
         }
         for (int ks = k0; ks < k1; ks += 2) {          // (the buffers by name: their addresses are then constants)
             step(ks, 0);
@@ -250,7 +267,7 @@ __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a
             for (int kk = 0; kk < KC; ++kk) {
                 if (FB == 1) read(0, kk);
                 else if (kk + 1 < KC) read(0, kk + 1);
-                multiply(kk);
+                multiply(kk, nothing);
             }
         }
     }

@@ -83,11 +83,9 @@ __device__ __forceinline__ void tk_store8(float *p, const TkFrag<float> &f) {
     *reinterpret_cast<tkf4 *>(p + 4) = tkf4{f.v[4], f.v[5], f.v[6], f.v[7]};
 }
 // LDS-DMA: 64 lanes x 16 bytes from (wave-uniform base + per-lane byte offset) to 1024 consecutive LDS bytes at `dst` (wave-uniform).  No registers; retired by
-// dma_wait (hno_common.h).  M0 holds the destination and is put back: the compiler owns it.
+// dma_wait (hno_common.h).  M0 holds the destination.
 __device__ __forceinline__ void tk_dma16(const tkh *src, unsigned off, unsigned dst) {
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(off), "s"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
 }
 
 // ------------------------------------------------------------------ activations (ids: hno.h)
