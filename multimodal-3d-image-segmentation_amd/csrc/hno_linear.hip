@@ -324,29 +324,41 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a) {
     }
 }
 
-// dz = dy act'(z) and the column sums of dz: a workgroup owns 64 columns of a run of rows and leaves one slab row per run.
-// dz == nullptr: act is none, dz is dy itself and only the sums are wanted.
-template <typename T>
+// dz = dy act'(z) and the column sums of dz: a workgroup owns 256 columns (32 lanes of 8) of a run of rows and leaves one slab row per run; single columns a lane
+// took 16 us for 3920 x 1536 bf16 instead of 11.  dz == nullptr: act is none, dz is dy itself and only the sums are wanted.
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void linear_dz_kernel(const T *__restrict__ dy, const T *__restrict__ z, T *__restrict__ dz, float *__restrict__ slab,
-                                                        int M, int N, int act, int rows_per) {
-    __shared__ float red[4][64];
-    const int n = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-    const int m0 = blockIdx.y * rows_per, m1 = m0 + rows_per < M ? m0 + rows_per : M;
-    float s = 0.f;
-    if (n < N)
-        for (int m = m0 + w; m < m1; m += 4) {
+                                                        int M, int N, int rows_per) {
+    __shared__ float red[8][32 * 9];
+    const int c = threadIdx.x & 31, w = threadIdx.x >> 5, n = blockIdx.x * 256 + 8 * c, cnt = N - n;
+    const int m0 = blockIdx.y * rows_per, m1 = min(m0 + rows_per, M);
+    float s[8] = {};
+    if (cnt > 0)
+#pragma unroll 2
+        for (int m = m0 + w; m < m1; m += 8) {
             const long long at = (long long)m * N + n;
-            float g = tk_up(dy[at]);
-            if (dz) {
-                g *= tk_act_grad(tk_up(z[at]), act);
-                dz[at] = tk_down<T>(g);
+            float g[8];
+            ln_get8(dy + at, cnt, g);
+            if constexpr (ACT != HNO_ACT_NONE) {
+                float t[8];
+                ln_get8(z + at, cnt, t);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g[j] *= tk_act_grad(t[j], ACT);
+                ln_put8(dz + at, cnt, g);
             }
-            s += g;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[j] += g[j];
         }
     if (!slab) return;
-    red[w][threadIdx.x & 63] = s;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) red[w][9 * c + j] = s[j];
     __syncthreads();
-    if (w == 0 && n < N) slab[(long long)blockIdx.y * N + n] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+    const int col = blockIdx.x * 256 + threadIdx.x, at = 9 * (threadIdx.x >> 3) + (threadIdx.x & 7);
+    if (col >= N) return;
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += red[k][at];
+    slab[(long long)blockIdx.y * N + col] = t;
 }
 template <typename T>
 __global__ __launch_bounds__(1024) void linear_db_kernel(const float *__restrict__ slab, int runs, int N, void *db, int db32) {
@@ -393,7 +405,7 @@ static LnPlan ln_plan(int M, int N, int K, bool f32, bool dma) {
     p.blocks = tiles * p.nsplit;
     return p;
 }
-static int ln_runs(int M) { return M <= 64 ? 1 : (ceil_div(M, 64) < 256 ? ceil_div(M, 64) : 256); }
+static int ln_runs(int M) { return ceil_div(M, 32) < 256 ? ceil_div(M, 32) : 256; }          // runs of rows of dz: 4 rows a thread at least
 static size_t ln_pad(size_t b) { return (b + 255) / 256 * 256; }
 static bool ln_aligned(const void *p, long long ld, int esz) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * esz % 16 == 0; }
 
@@ -474,8 +486,18 @@ static int ln_backward(const void *dy, const void *z, const void *x, long long l
     float *slab = (float *)(ws + ln_pad(dz ? (size_t)M * N * sizeof(T) : 0)), *part = (float *)((char *)slab + ln_pad((size_t)runs * N * sizeof(float)));
     if (dz || db) {
         ProfScope _ps(KID_LINEAR, s, (double)M * N * sizeof(T) * (dz ? 3 : 1));
-        hipLaunchKernelGGL((linear_dz_kernel<T>), dim3(ceil_div(N, 64), runs), dim3(256), 0, s, (const T *)dy, (const T *)z, dz, db ? slab : nullptr, M, N, act,
-                           ceil_div(M, runs));
+        const dim3 grid(ceil_div(N, 256), runs);
+        const int per = ceil_div(M, runs);
+#define LN_DZ(ACT) hipLaunchKernelGGL((linear_dz_kernel<T, ACT>), grid, dim3(256), 0, s, (const T *)dy, (const T *)z, dz, db ? slab : nullptr, M, N, per)
+        switch (act) {
+            case HNO_ACT_SELU: LN_DZ(HNO_ACT_SELU); break;
+            case HNO_ACT_ELU: LN_DZ(HNO_ACT_ELU); break;
+            case HNO_ACT_RELU: LN_DZ(HNO_ACT_RELU); break;
+            case HNO_ACT_GELU: LN_DZ(HNO_ACT_GELU); break;
+            case HNO_ACT_SILU: LN_DZ(HNO_ACT_SILU); break;
+            default: LN_DZ(HNO_ACT_NONE);
+        }
+#undef LN_DZ
         HNO_CHECK_LAUNCH();
         if (db) {
             hipLaunchKernelGGL((linear_db_kernel<T>), dim3(ceil_div(N, 64)), dim3(1024), 0, s, (const float *)slab, runs, N, db, db_dtype == HNO_F32);
