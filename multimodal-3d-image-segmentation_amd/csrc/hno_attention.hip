@@ -272,9 +272,9 @@ __device__ __forceinline__ void at_store(T *dst, const tk16 (&acc)[DP / 32], int
 struct AtBlock {
     int b, hk, tile, gi, sp;
 };
-__device__ __forceinline__ AtBlock at_block(const AttnArgs &a, int grp) {
-    const int n = gridDim.x, xcd = blockIdx.x & 7, each = n >> 3, more = n & 7;
-    int at = xcd * each + min(xcd, more) + (blockIdx.x >> 3);
+__device__ __forceinline__ AtBlock at_block(const AttnArgs &a, int grp, int id, int n) {
+    const int xcd = id & 7, each = n >> 3, more = n & 7;
+    int at = xcd * each + min(xcd, more) + (id >> 3);
     AtBlock w;
     w.sp = at % a.nsplit, at /= a.nsplit;
     w.gi = at % grp, at /= grp;
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 4 ? (DP <= 96 ? 2 : 1) 
     __shared__ __attribute__((aligned(16))) tkh Ks[NB][tk_planes<T>() * PLANE];
     __shared__ __attribute__((aligned(16))) tkh Vs[NB][tk_planes<T>() * PLANE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const AtBlock w0 = at_block(a, a.pack ? 1 : a.H / a.Hk);
+    const AtBlock w0 = at_block(a, a.pack ? 1 : a.H / a.Hk, blockIdx.x, gridDim.x);
     const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk, hb = hk * grp + w0.gi, nrows = a.pack ? grp * a.Tq : a.Tq;
     const int L = at_length(a, b);
     for (int half = 0; half < 2; ++half) {
@@ -548,13 +548,16 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(const T *__restrict__ g
     if (row < rows && c == 0) delta[row] = s;
 }
 
+// LDS of a backward workgroup: the streamed side's two tensors, then lse and D of their rows
+template <typename T, int DP> constexpr int at_half() { return at_buffers<T, DP>() * tk_planes<T>() * at_tile<T>() * DP; }
+
+// dq of a tile of queries
 template <typename T, int DP, bool MASK>
-__global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(AttnArgs a) {
+__device__ __forceinline__ void at_dq(const AttnArgs &a, const AtBlock &w0, tkh *smem) {
     constexpr int KT = at_tile<T>(), PLANE = KT * DP, NB = at_buffers<T, DP>();
-    __shared__ __attribute__((aligned(16))) tkh Ks[NB][tk_planes<T>() * PLANE];
-    __shared__ __attribute__((aligned(16))) tkh Vs[NB][tk_planes<T>() * PLANE];
+    typedef tkh Tile[NB][tk_planes<T>() * PLANE];
+    Tile &Ks = *reinterpret_cast<Tile *>(smem), &Vs = *reinterpret_cast<Tile *>(smem + at_half<T, DP>());
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const AtBlock w0 = at_block(a, a.pack ? 1 : a.H / a.Hk);
     const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk, hb = hk * grp + w0.gi, nrows = a.pack ? grp * a.Tq : a.Tq;
     const int L = at_length(a, b);
     for (int half = 0; half < 2; ++half) {
@@ -630,14 +633,15 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dq
     }
 }
 
+// dk (WHAT & 1) and dv (WHAT & 2) of a tile of keys
 template <typename T, int DP, bool MASK, int WHAT>
-__global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dkv_kernel(AttnArgs a) {
+__device__ __forceinline__ void at_dkv(const AttnArgs &a, const AtBlock &w0, tkh *smem) {
     constexpr int QT = at_tile<T>(), PLANE = QT * DP, NB = at_buffers<T, DP>();
-    __shared__ __attribute__((aligned(16))) tkh Qs[NB][tk_planes<T>() * PLANE];
-    __shared__ __attribute__((aligned(16))) tkh Gs[NB][tk_planes<T>() * PLANE];
-    __shared__ __attribute__((aligned(16))) float lses[NB][QT], deltas[NB][QT];
+    typedef tkh Tile[NB][tk_planes<T>() * PLANE];
+    typedef float Rows[NB][QT];
+    Tile &Qs = *reinterpret_cast<Tile *>(smem), &Gs = *reinterpret_cast<Tile *>(smem + at_half<T, DP>());
+    Rows &lses = *reinterpret_cast<Rows *>(smem + 2 * at_half<T, DP>()), &deltas = *reinterpret_cast<Rows *>(smem + 2 * at_half<T, DP>() + 2 * NB * QT);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const AtBlock w0 = at_block(a, 1);
     const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk;
     const int L = at_length(a, b), off = L - a.Tq;
     for (int half = 0; half < 2; ++half) {
@@ -752,23 +756,46 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_dk
     }
 }
 
-// out = sum over splits, in split order, of one or two tensors (4 elements a thread; n is a multiple of 8)
+// The three gradients in one launch: the runs of workgroups stand one behind the other in the grid, each padded to whole rounds of the XCDs, dk and dq
+// (three products) before dv (two).  dk and dv are one workgroup's work where the registers of both leave two waves per SIMD, else two's.
+template <typename T, int DP> constexpr bool at_joint() { return sizeof(T) == 4 || DP <= 64; }
+template <typename T, int DP, bool MASK>
+__global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_bwd_kernel(AttnArgs aq, AttnArgs ak, int nq, int nk) {
+    __shared__ __attribute__((aligned(16))) tkh smem[2 * at_half<T, DP>() + 4 * at_buffers<T, DP>() * at_tile<T>()];
+    const int nq8 = (nq + 7) & ~7, nk8 = (nk + 7) & ~7;
+    int id = blockIdx.x;
+    if (id < nk8) {
+        if (id < nk) at_dkv<T, DP, MASK, at_joint<T, DP>() ? 3 : 1>(ak, at_block(ak, 1, id, nk), smem);
+        return;
+    }
+    id -= nk8;
+    if (id < nq8) {
+        if (id < nq) at_dq<T, DP, MASK>(aq, at_block(aq, aq.pack ? 1 : aq.H / aq.Hk, id, nq), smem);
+        return;
+    }
+    id -= nq8;
+    if constexpr (!at_joint<T, DP>())
+        if (id < nk) at_dkv<T, DP, MASK, 2>(ak, at_block(ak, 1, id, nk), smem);
+}
+
+// out = sum over splits, in split order, of up to three tensors (4 elements a thread; n is a multiple of 8)
 struct AtSum {
-    const float *part[2];
-    void *out[2];
-    long long n[2];
+    const float *part[3];
+    void *out[3];
+    long long n[3];
+    int nsplit[3];
 };
 template <typename T>
-__global__ __launch_bounds__(256) void attn_sum_kernel(AtSum a, int nsplit) {
+__global__ __launch_bounds__(256) void attn_sum_kernel(AtSum a) {
     long long i = 4 * ((long long)blockIdx.x * 256 + threadIdx.x);
-    const int k = i >= a.n[0];
-    if (k) i -= a.n[0];
+    int k = 0;
+    while (k < 2 && i >= a.n[k]) i -= a.n[k++];
     const long long n = a.n[k];
     if (i >= n) return;
     const float *p = a.part[k] + i;
     tkf4 x = *reinterpret_cast<const tkf4 *>(p);
 #pragma unroll 4
-    for (int s = 1; s < nsplit; ++s) x += *reinterpret_cast<const tkf4 *>(p + s * n);
+    for (int s = 1; s < a.nsplit[k]; ++s) x += *reinterpret_cast<const tkf4 *>(p + s * n);
     if constexpr (sizeof(T) == 2) {
         tks4 t;
 #pragma unroll
@@ -783,10 +810,13 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(AtSum a, int nsplit) {
 
 using namespace hno;
 
-// how many runs the streamed side is cut into: enough workgroups for the chip (two per CU), no run shorter than two tiles
-static int at_splits(long long groups, long long steps) {
+// how many runs the streamed side is cut into: two workgroups per CU, no run shorter than `least` tiles; where that is not to be had, one per CU and runs of two tiles.
+// The backward kernel holds three gradients' workgroups: with 16 tiles at least, causal 2x16x4096x128 takes 725 us in runs of four and 815 in runs of two, while 3x6x777x1033x80 takes
+// 79 us with one workgroup per CU and gradient (135 with two, in launches of their own).
+static int at_splits(long long groups, long long steps, int least) {
     if (groups < 1) return 1;                                  // no keys at all
     long long n = groups >= 512 ? 1 : (512 + groups - 1) / groups;
+    if (least > 2 && steps < least * n) n = groups >= 256 ? 1 : (256 + groups - 1) / groups;
     if (n > steps / 2) n = steps / 2;
     if (n > 64) n = 64;
     return n < 1 ? 1 : (int)n;
@@ -795,7 +825,7 @@ struct AtPlan {
     int pack, q_tiles, q_heads, q_split, q_pair, k_tiles, k_split, k_pair;
     long long q_blocks, k_blocks;
 };
-static AtPlan at_plan(const hno_attn_t *p) {
+static AtPlan at_plan(const hno_attn_t *p, bool backward) {
     AtPlan n;
     const int grp = p->H / p->Hk, KT = p->dtype == HNO_BF16 ? 64 : 32;
     n.pack = grp > 1 && p->Tq < AT_ROWS;
@@ -807,8 +837,9 @@ static AtPlan at_plan(const hno_attn_t *p) {
     n.k_pair = p->causal && k * n.k_tiles <= 1024;
     q *= n.q_pair ? (n.q_tiles + 1) / 2 : n.q_tiles;
     k *= n.k_pair ? (n.k_tiles + 1) / 2 : n.k_tiles;
-    n.q_split = at_splits(q, ceil_div(p->Tk, KT));
-    n.k_split = at_splits(k, (long long)ceil_div(p->Tq, KT) * grp);
+    const int least = backward ? 16 : 2;
+    n.q_split = at_splits(q, ceil_div(p->Tk, KT), least);
+    n.k_split = at_splits(k, (long long)ceil_div(p->Tq, KT) * grp, least);
     n.q_blocks = q * n.q_split;
     n.k_blocks = k * n.k_split;
     return n;
@@ -821,7 +852,7 @@ static int at_check(const hno_attn_t *p, const char *what) {
     HNO_REQUIRE(p->dtype == HNO_F32 || p->dtype == HNO_BF16, "%s: dtype %d is neither HNO_F32 nor HNO_BF16", what, p->dtype);
     HNO_REQUIRE(p->B > 0 && p->Tq > 0 && p->Tk >= 0 && p->H > 0 && p->Hk > 0 && p->Dk > 0 && p->Dv > 0, "%s: bad size", what);
     HNO_REQUIRE(p->H % p->Hk == 0, "%s: %d query heads do not share %d key heads evenly", what, p->H, p->Hk);
-    HNO_REQUIRE(p->scale > 0.f && p->scale < 3e38f, "%s: scale must be positive and finite", what);
+    HNO_REQUIRE(p->scale >= 1e-30f && p->scale <= 1e30f, "%s: scale must be positive, from 1e-30 to 1e30", what);
     if (p->Dk > 128 || p->Dv > 128) return fail(HNO_ELIMIT, "%s: head sizes %d, %d exceed 128", what, p->Dk, p->Dv);
     if ((double)p->B * p->H * (ceil_div(p->Tq, AT_ROWS) + ceil_div(p->Tk, AT_ROWS)) > 1e8) return fail(HNO_ELIMIT, "%s: the grid is too large", what);
     if (p->Tq > (1 << 28) || p->Tk > (1 << 28) || (long long)(p->H / p->Hk) * p->Tq > (1ll << 30)) return fail(HNO_ELIMIT, "%s: too many tokens", what);
@@ -850,31 +881,31 @@ static double at_bytes(const hno_attn_t *p, int q_tensors, int k_tensors) {
 }
 
 // the kernel of one type for the padded head size, with or without a mask
-#define AT_LAUNCH(KERNEL, DP, ...)                                                                                      \
+#define AT_LAUNCH(KERNEL, DP, ...)                                                                                 \
     do {                                                                                                           \
-        if (a.mask) hipLaunchKernelGGL((KERNEL<T, DP, true __VA_ARGS__>), dim3(n_), dim3(64 * AT_WAVES), 0, s, a);             \
-        else hipLaunchKernelGGL((KERNEL<T, DP, false __VA_ARGS__>), dim3(n_), dim3(64 * AT_WAVES), 0, s, a);                   \
+        if (p->mask) hipLaunchKernelGGL((KERNEL<T, DP, true>), dim3(n_), dim3(64 * AT_WAVES), 0, s, __VA_ARGS__);  \
+        else hipLaunchKernelGGL((KERNEL<T, DP, false>), dim3(n_), dim3(64 * AT_WAVES), 0, s, __VA_ARGS__);         \
     } while (0)
-#define AT_DISPATCH(KERNEL, blocks, s, a)                                                                          \
+#define AT_DISPATCH(KERNEL, blocks, ...)                                                                           \
     do {                                                                                                           \
-        const int dp_ = round_up(a.Dk > a.Dv ? a.Dk : a.Dv, 32);                                                   \
+        const int dp_ = round_up(p->Dk > p->Dv ? p->Dk : p->Dv, 32);                                               \
         const unsigned n_ = (unsigned)(blocks);                                                                    \
-        if (dp_ == 32) AT_LAUNCH(KERNEL, 32, );                                                                      \
-        else if (dp_ == 64) AT_LAUNCH(KERNEL, 64, );                                                                 \
-        else if (dp_ == 96) AT_LAUNCH(KERNEL, 96, );                                                                 \
-        else AT_LAUNCH(KERNEL, 128, );                                                                               \
+        if (dp_ == 32) AT_LAUNCH(KERNEL, 32, __VA_ARGS__);                                                         \
+        else if (dp_ == 64) AT_LAUNCH(KERNEL, 64, __VA_ARGS__);                                                    \
+        else if (dp_ == 96) AT_LAUNCH(KERNEL, 96, __VA_ARGS__);                                                    \
+        else AT_LAUNCH(KERNEL, 128, __VA_ARGS__);                                                                  \
     } while (0)
 
 template <typename T>
 static int at_forward(const hno_attn_t *p, void *out, void *out_res, float *lse, void *workspace, hipStream_t s) {
-    const AtPlan n = at_plan(p);
+    const AtPlan n = at_plan(p, false);
     AttnArgs a = at_args(p);
     const long long rows = (long long)p->B * p->Tq * p->H;
     a.out = out; a.outres = out_res; a.lse = lse; a.pack = n.pack; a.nsplit = n.q_split; a.tiles = n.q_tiles, a.pair = n.q_pair;
     a.part = (float *)workspace;
     a.part2 = (float *)((char *)workspace + at_pad((size_t)n.q_split * rows * p->Dv * sizeof(float)));
     ProfScope _ps(KID_ATTN, s, at_bytes(p, 2, 2));
-    AT_DISPATCH(attn_fwd_kernel, n.q_blocks, s, a);
+    AT_DISPATCH(attn_fwd_kernel, n.q_blocks, a);
     HNO_CHECK_LAUNCH();
     if (n.q_split > 1) {
         hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)(n.q_split >= 8 ? rows : (rows + 7) / 8)), dim3(256), 0, s, (const float *)a.part, (const float *)a.part2,
@@ -884,78 +915,60 @@ static int at_forward(const hno_attn_t *p, void *out, void *out_res, float *lse,
     return HNO_OK;
 }
 
-// dk and dv in one kernel, or each in its own (where one kernel would not leave registers for two waves per SIMD)
-template <typename T>
-static int at_launch_dkv(const AttnArgs &a, unsigned n_, hipStream_t s) {
-    const int dp = round_up(a.Dk > a.Dv ? a.Dk : a.Dv, 32);
-    if (dp == 32) AT_LAUNCH(attn_dkv_kernel, 32, , 3);
-    else if (dp == 64) AT_LAUNCH(attn_dkv_kernel, 64, , 3);
-    else if constexpr (sizeof(T) == 4) {
-        if (dp == 96) AT_LAUNCH(attn_dkv_kernel, 96, , 3);
-        else AT_LAUNCH(attn_dkv_kernel, 128, , 3);
-    } else if (dp == 96) {
-        AT_LAUNCH(attn_dkv_kernel, 96, , 1);
-        AT_LAUNCH(attn_dkv_kernel, 96, , 2);
-    } else {
-        AT_LAUNCH(attn_dkv_kernel, 128, , 1);
-        AT_LAUNCH(attn_dkv_kernel, 128, , 2);
-    }
-    HNO_CHECK_LAUNCH();
-    return HNO_OK;
-}
-
-template <typename T>
-static int at_sum(const AtSum &a, int nsplit, hipStream_t s) {
-    hipLaunchKernelGGL((attn_sum_kernel<T>), dim3((unsigned)((a.n[0] + a.n[1] + 1023) / 1024)), dim3(256), 0, s, a, nsplit);
-    HNO_CHECK_LAUNCH();
-    return HNO_OK;
+// floats of the backward pass's slabs: dq, dk, dv
+struct AtSlabs {
+    size_t q, k, v;
+};
+static AtSlabs at_slabs(const hno_attn_t *p, const AtPlan &n) {
+    const size_t rows = (size_t)p->B * p->Tq * p->H, krows = (size_t)p->B * p->Tk * p->Hk, f = sizeof(float);
+    return {n.q_split > 1 ? at_pad(n.q_split * rows * p->Dk * f) : 0, n.k_split > 1 ? at_pad(n.k_split * krows * p->Dk * f) : 0,
+            n.k_split > 1 ? at_pad(n.k_split * krows * p->Dv * f) : 0};
 }
 
 template <typename T>
 static int at_backward(const hno_attn_t *p, const void *out, const void *out_res, const float *lse, const void *dout, void *dq, void *dk, void *dv,
                        void *workspace, hipStream_t s) {
-    const AtPlan n = at_plan(p);
-    AttnArgs a = at_args(p);
+    const AtPlan n = at_plan(p, true);
+    const AtSlabs slabs = at_slabs(p, n);
     const long long rows = (long long)p->B * p->Tq * p->H, krows = (long long)p->B * p->Tk * p->Hk;
-    a.g = dout; a.lse = const_cast<float *>(lse); a.delta = (float *)workspace;
-    a.dq = dq; a.dk = dk; a.dv = dv;
-    a.part = (float *)((char *)workspace + at_pad(rows * sizeof(float)));
-    {
-        ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 2, 0));
-        hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, (const T *)dout, (const T *)out,
-                           (const T *)out_res, lse, a.delta, rows, p->Dv);
-        HNO_CHECK_LAUNCH();
+    char *ws = (char *)workspace + at_pad(rows * sizeof(float));
+    AttnArgs aq = at_args(p);
+    aq.g = dout; aq.lse = const_cast<float *>(lse); aq.delta = (float *)workspace;
+    aq.dq = dq; aq.dk = dk; aq.dv = dv;
+    AttnArgs ak = aq;
+    aq.pack = n.pack; aq.nsplit = n.q_split; aq.tiles = n.q_tiles; aq.pair = n.q_pair;
+    aq.part = (float *)ws;
+    ak.nsplit = n.k_split; ak.tiles = n.k_tiles; ak.pair = n.k_pair;
+    ak.part = (float *)(ws + slabs.q);
+    ak.part2 = (float *)(ws + slabs.q + slabs.k);
+    ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 4, 4));
+    hipLaunchKernelGGL((attn_delta_kernel<T>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, (const T *)dout, (const T *)out, (const T *)out_res, lse,
+                       aq.delta, rows, p->Dv);
+    HNO_CHECK_LAUNCH();
+    const int nq = dq ? (int)n.q_blocks : 0, nk = dk && p->Tk > 0 ? (int)n.k_blocks : 0, nv = sizeof(T) == 4 || (p->Dk <= 64 && p->Dv <= 64) ? 0 : nk;
+    if (nq + nk == 0) return HNO_OK;
+    AT_DISPATCH(attn_bwd_kernel, round_up(nk, 8) + round_up(nq, 8) + nv, aq, ak, nq, nk);
+    HNO_CHECK_LAUNCH();
+    AtSum sum = {};
+    if (nq && n.q_split > 1) sum.part[0] = aq.part, sum.out[0] = dq, sum.n[0] = rows * p->Dk, sum.nsplit[0] = n.q_split;
+    if (nk && n.k_split > 1) {
+        sum.part[1] = ak.part, sum.out[1] = dk, sum.n[1] = krows * p->Dk, sum.nsplit[1] = n.k_split;
+        sum.part[2] = ak.part2, sum.out[2] = dv, sum.n[2] = krows * p->Dv, sum.nsplit[2] = n.k_split;
     }
-    if (dq) {
-        ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 3, 2));
-        a.pack = n.pack;
-        a.nsplit = n.q_split;
-        a.tiles = n.q_tiles, a.pair = n.q_pair;
-        AT_DISPATCH(attn_dq_kernel, n.q_blocks, s, a);
+    if (const long long total = sum.n[0] + sum.n[1] + sum.n[2]) {
+        hipLaunchKernelGGL((attn_sum_kernel<T>), dim3((unsigned)((total + 1023) / 1024)), dim3(256), 0, s, sum);
         HNO_CHECK_LAUNCH();
-        if (n.q_split > 1)
-            if (int rc = at_sum<T>({{a.part, nullptr}, {dq, nullptr}, {rows * p->Dk, 0}}, n.q_split, s)) return rc;
-    }
-    if (dk && p->Tk > 0) {
-        ProfScope _ps(KID_ATTN_BWD, s, at_bytes(p, 2, 4));
-        a.nsplit = n.k_split;
-        a.tiles = n.k_tiles, a.pair = n.k_pair;
-        a.part2 = (float *)((char *)a.part + at_pad((size_t)n.k_split * krows * p->Dk * sizeof(float)));
-        if (int rc = at_launch_dkv<T>(a, (unsigned)n.k_blocks, s)) return rc;
-        HNO_CHECK_LAUNCH();
-        if (n.k_split > 1)
-            if (int rc = at_sum<T>({{a.part, a.part2}, {dk, dv}, {krows * p->Dk, krows * p->Dv}}, n.k_split, s)) return rc;
     }
     return HNO_OK;
 }
 
 extern "C" size_t hno_attn_workspace_bytes(const hno_attn_t *p, int backward) {
     if (at_check(p, "hno_attn_workspace_bytes") != HNO_OK) return 0;
-    const AtPlan n = at_plan(p);
-    const size_t rows = (size_t)p->B * p->Tq * p->H, krows = (size_t)p->B * p->Tk * p->Hk, f = sizeof(float);
+    const AtPlan n = at_plan(p, backward != 0);
+    const size_t rows = (size_t)p->B * p->Tq * p->H, f = sizeof(float);
     if (!backward) return n.q_split > 1 ? at_pad(n.q_split * rows * p->Dv * f) + n.q_split * rows * 2 * f : 0;
-    const size_t q = n.q_split > 1 ? n.q_split * rows * p->Dk * f : 0, k = n.k_split > 1 ? at_pad(n.k_split * krows * p->Dk * f) + n.k_split * krows * p->Dv * f : 0;
-    return at_pad(rows * f) + (q > k ? q : k);
+    const AtSlabs slabs = at_slabs(p, n);
+    return at_pad(rows * f) + slabs.q + slabs.k + slabs.v;
 }
 
 extern "C" int hno_attn_fwd(const hno_attn_t *p, void *out, void *out_res, float *lse, void *workspace, size_t workspace_bytes, void *stream) {

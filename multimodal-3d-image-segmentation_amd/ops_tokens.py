@@ -170,8 +170,8 @@ def attention(q, k, v, *, causal=False, mask=None, kv_lens=None, scale=None):
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f'attention: q, k, v are {q.dtype}, {k.dtype}, {v.dtype}: one type is needed')
     scale = 1.0 / math.sqrt(Dk) if scale is None else float(scale)
-    if not 0.0 < scale < 3e38:
-        raise ValueError('attention: scale must be positive and finite')
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError('attention: scale must be positive, from 1e-30 to 1e30')
     if mask is not None:
         if mask.dtype != torch.bool:
             raise ValueError('attention: mask must be bool (True: visible); additive masks are not provided')

@@ -568,7 +568,7 @@ def test_attention_refusals(ot):
     q, k = t(1, 4, 4, 32), t(1, 6, 2, 32)
     bad = [((q[0], k, k), {}), ((q, k, t(1, 5, 2, 32)), {}), ((q, t(2, 6, 2, 32), k), {}), ((q, t(1, 6, 2, 16), k), {}), ((q, t(1, 6, 3, 32), t(1, 6, 3, 32)), {}),
            ((t(1, 4, 4, 129), t(1, 6, 2, 129), k), {}), ((q, k, t(1, 6, 2, 129)), {}), ((q.half(), k.half(), k.half()), {}), ((q, k.bfloat16(), k), {}),
-           ((q.double(), k.double(), k.double()), {}), ((q, k, k), {'scale': 0.0}), ((q, k, k), {'scale': -1.0}), ((q, k, k), {'scale': math.inf}),
+           ((q.double(), k.double(), k.double()), {}), ((q, k, k), {'scale': 0.0}), ((q, k, k), {'scale': -1.0}), ((q, k, k), {'scale': 1e-31}), ((q, k, k), {'scale': 1e31}), ((q, k, k), {'scale': math.inf}),
            ((q, k, k), {'scale': math.nan}), ((q, k, k), {'mask': t(4, 6)}), ((q, k, k), {'mask': t(4, 5).bool()}), ((q, k, k), {'mask': t(1, 1, 1, 4, 6).bool()}),
            ((q, k, k), {'kv_lens': t(2).int()}), ((q, k, k), {'kv_lens': t(1)}), ((t(1, 4, 4, 0), t(1, 6, 2, 0), k), {}), ((t(1, 4, 0, 32), k, k), {})]
     for args, kw in bad:
