@@ -837,9 +837,10 @@ static AtPlan at_plan(const hno_attn_t *p, bool backward) {
     n.k_pair = p->causal && k * n.k_tiles <= 1024;
     q *= n.q_pair ? (n.q_tiles + 1) / 2 : n.q_tiles;
     k *= n.k_pair ? (n.k_tiles + 1) / 2 : n.k_tiles;
-    const int least = backward ? 16 : 2;
-    n.q_split = at_splits(q, ceil_div(p->Tk, KT), least);
-    n.k_split = at_splits(k, (long long)ceil_div(p->Tq, KT) * grp, least);
+    // (a few new tokens: all the chip's loads at once, 4x1x16x128 against 6000 keys 17.9 us in 32 runs, 21 in 16)
+    const int q_least = backward || n.q_tiles > 1 ? 16 : 2;
+    n.q_split = at_splits(q, ceil_div(p->Tk, KT), q_least);
+    n.k_split = at_splits(k, (long long)ceil_div(p->Tq, KT) * grp, 16);
     n.q_blocks = q * n.q_split;
     n.k_blocks = k * n.k_split;
     return n;

@@ -314,7 +314,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a) {
         const float *src = a.part + (long long)m * a.N + n;
         float x[8] = {}, t[8], r[8] = {};
         if (a.res) ln_get8((const T *)a.res + (long long)m * a.N + n, a.N - n, r);
-#pragma unroll 4
+#pragma unroll 8
         for (int s = 0; s < a.nsplit; ++s) {
             ln_get8(src + s * slab, a.N - n, t);
 #pragma unroll
@@ -384,7 +384,7 @@ using namespace hno;
 
 // Tile, and runs of the contraction.  LnBig (8192 x 8192 x 8192: 994 TFLOP/s, LnMid 898) where its tiles fill most of the 256 CUs by themselves and DMA can feed it.
 // Else 128 x 128 tiles, whose contraction is cut into n runs where that is expected to be quicker: a step takes a workgroup 0.65 us (fp32: 2.5) while there are places for all
-// (two a CU), the slabs cost 2.5 us for the second launch and 0.65 us per megabyte.  Measured with these: 3920 x 384 x 1536 bf16 n = 1: 17.6 us (2: 22.9, 5: 24.5),
+// (two a CU), the slabs cost 2.5 us for the second launch, 0.12 us each and 0.65 us per megabyte.  Measured with these: 3920 x 384 x 1536 bf16 n = 1: 17.6 us (2: 22.9, 5: 24.5),
 // 1536 x 384 x 3920 n = 5: 22.9 (1: 55, 12: 25), 300 x 300 x 4000 n = 8: 13.8 (1: 36, 24: 17.9), 771 x 387 x 3001 fp32 n = 16: 33.5 (1: 239, 32: 40).
 struct LnPlan {
     bool big;
@@ -402,7 +402,7 @@ static LnPlan ln_plan(int M, int N, int K, bool f32, bool dma) {
         const double step_us = f32 ? 2.5 : 0.65, slab_us = 0.65e-6 * 4.0 * M * N;
         double best = 0.0;
         for (int n = 1; n <= 64 && n <= steps && (n == 1 || tiles * n <= 512); ++n) {
-            const double cost = ceil_div(steps, n) * step_us + (n > 1 ? 2.5 + n * slab_us : 0.0);
+            const double cost = ceil_div(steps, n) * step_us + (n > 1 ? 2.5 + n * (0.12 + slab_us) : 0.0);
             if (n == 1 || cost < best) best = cost, p.nsplit = n;
         }
     }
