@@ -13,7 +13,7 @@ import torch
 
 from . import _lib, ops
 from ._lib import check
-from .ops import _HnoFunction, _m
+from .ops import _m
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}                     # HNO_F32, HNO_BF16
 _ACTS = {None: 0, 'none': 0, 'selu': 1, 'elu': 2, 'relu': 4, 'gelu': 5, 'silu': 6}
@@ -43,12 +43,29 @@ def _same_device(what, first, *others):
             raise ValueError(f'{what}: tensors on {first.device} and {t.device}')
 
 
-def _apply(fn, t, *args):
-    """fn.apply(*args) with the device of `t` as the current one (launches and workspaces go by the current device and its current stream)"""
-    if t.device.index == torch.cuda.current_device():
-        return fn.apply(*args)
-    with torch.cuda.device(t.device):
-        return fn.apply(*args)
+def _call(fn, *args):
+    """fn.run(...) -> result, kept; as a node of the autograd graph where a gradient can be asked for (4 us of host time: a call for one token took 24
+    with a node that nobody asks, 20 without).  The device of the first argument is the current one meanwhile: launches and workspaces go by it and its
+    current stream."""
+    if args[0].device.index != torch.cuda.current_device():
+        with torch.cuda.device(args[0].device):
+            return _call(fn, *args)
+    if torch.is_grad_enabled():
+        for t in args:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                return _leaves(fn.apply(*args))
+    return fn.run(False, *args)[0]
+
+
+def _leaves(y):
+    """Refuses a capture that the backward pass could not survive.  A leaf's accumulation node belongs to the stream on which it was made and lives as long as
+    any graph that holds it: one left over from another stream would join that stream to the capture in the backward pass, which ends the process."""
+    stream = _stream(y)
+    for node, _ in y.grad_fn.next_functions:
+        if node is not None and hasattr(node, 'variable'):
+            if node.metadata.setdefault('hno_stream', stream) != stream and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError('a graph of the same leaf, made on another stream before the capture, is still alive: delete its outputs first')
+    return y
 
 
 def _stream(t):
@@ -95,17 +112,12 @@ def _attn_args(q, k, v, mask, kv_lens, causal, scale):
     return a
 
 
-class AttentionFn(_HnoFunction):
+class AttentionFn(torch.autograd.Function):
     """out = softmax(scale q k^T) v over the visible keys; the backward pass recomputes the probabilities from lse (``attention`` has the
     contract)."""
 
     @staticmethod
-    def meta(q, k, v, mask, kv_lens, causal, scale):
-        return _m(tuple(q.shape[:3]) + (v.shape[3],), q.dtype)
-
-    @staticmethod
-    def forward(ctx, q, k, v, mask, kv_lens, causal, scale):
-        train = ops.backward_wanted(ctx)
+    def run(train, q, k, v, mask, kv_lens, causal, scale):
         Dk, Dv = q.shape[3], v.shape[3]
         q, k, v = (_heads(t, t.element_size()) for t in (q, k, v))
         B, Tq, H, _ = q.shape
@@ -119,10 +131,13 @@ class AttentionFn(_HnoFunction):
             n = L.hno_attn_workspace_bytes(ref, 0)
             ws = _ws(n, q.device)
             check(L.hno_attn_fwd(ref, _p(out), _p(res), _p(lse), _p(ws), n, _stream(q)), 'hno_attn_fwd')
-        if train:
-            ctx.save_for_backward(q, k, v, mask, kv_lens, out, res, lse)
-            ctx.cfg = (causal, scale, Dk, Dv)
-        return out if out.shape[3] == Dv else out[..., :Dv].contiguous()
+        return out if out.shape[3] == Dv else out[..., :Dv].contiguous(), (q, k, v, mask, kv_lens, out, res, lse), (causal, scale, Dk, Dv)
+
+    @staticmethod
+    def forward(ctx, *args):
+        y, kept, ctx.cfg = AttentionFn.run(True, *args)
+        ctx.save_for_backward(*kept)
+        return y
 
     @staticmethod
     def backward(ctx, g):
@@ -182,11 +197,11 @@ def attention(q, k, v, *, causal=False, mask=None, kv_lens=None, scale=None):
         if tuple(kv_lens.shape) != (B,) or kv_lens.dtype not in (torch.int32, torch.int64):
             raise ValueError(f'attention: kv_lens must be {B} integers')
     if q.is_meta:
-        return AttentionFn.apply(q, k, v, mask, kv_lens, bool(causal), scale)
+        return _m((B, Tq, H, Dv), q.dtype)
     _same_device('attention', q, k, v, mask, kv_lens)
     if kv_lens is not None and (kv_lens.dtype != torch.int32 or not kv_lens.is_contiguous()):
         kv_lens = kv_lens.clamp(0, Tk).to(torch.int32).contiguous()
-    return _apply(AttentionFn, q, q, k, v, mask, kv_lens, bool(causal), scale)
+    return _call(AttentionFn, q, k, v, mask, kv_lens, bool(causal), scale)
 
 
 # ----------------------------------------------------------------------------------------------- linear
@@ -208,16 +223,11 @@ def _bf16_weight(w):
     return out
 
 
-class LinearFn(_HnoFunction):
+class LinearFn(torch.autograd.Function):
     """y = act(x W^T + b) + r with the whole epilogue in the product's kernel (``linear`` has the contract)."""
 
     @staticmethod
-    def meta(x, weight, bias, residual, act):
-        return _m(tuple(x.shape[:-1]) + (weight.shape[0],), x.dtype)
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, act):
-        train = ops.backward_wanted(ctx)
+    def run(train, x, weight, bias, residual, act):
         N, K = weight.shape
         y = torch.empty(tuple(x.shape[:-1]) + (N,), device=x.device, dtype=x.dtype)
         z, w, x2 = None, weight.contiguous(), x
@@ -235,9 +245,12 @@ class LinearFn(_HnoFunction):
             ws = _ws(n, x.device)
             check(L.hno_linear_fwd(dt, _p(x2), ldx, _p(w), _p(b), 0 if b is None else _DTYPES[b.dtype], _p(r), _p(z), _p(y), M, N, K, act, _p(ws), n,
                                    _stream(x)), 'hno_linear_fwd')
-        if train:
-            ctx.save_for_backward(x2, w, z, weight)
-            ctx.cfg = (act, tuple(x.shape), None if bias is None else bias.dtype)
+        return y, (x2, w, z, weight), (act, x.shape, None if bias is None else bias.dtype)
+
+    @staticmethod
+    def forward(ctx, *args):
+        y, kept, ctx.cfg = LinearFn.run(True, *args)
+        ctx.save_for_backward(*kept)
         return y
 
     @staticmethod
@@ -293,21 +306,17 @@ def linear(x, weight, bias=None, *, act=None, residual=None):
     if residual is not None and (tuple(residual.shape) != tuple(x.shape[:-1]) + (N,) or residual.dtype != x.dtype):
         raise ValueError(f'linear: residual must have the shape and type of the result, {tuple(x.shape[:-1]) + (N,)} {x.dtype}')
     if x.is_meta:
-        return LinearFn.apply(x, weight, bias, residual, a)
+        return _m(tuple(x.shape[:-1]) + (N,), x.dtype)
     _same_device('linear', x, weight, bias, residual)
-    return _apply(LinearFn, x, x, weight, bias, residual, a)
+    return _call(LinearFn, x, weight, bias, residual, a)
 
 
 # ----------------------------------------------------------------------------------------------- group norm
-class GroupNormClFn(_HnoFunction):
+class GroupNormClFn(torch.autograd.Function):
     """act(GroupNorm(G, C)(x)) on channels-last tokens (``group_norm`` has the contract)."""
 
     @staticmethod
-    def meta(x, weight, bias, groups, eps, act):
-        return _m(x.shape, x.dtype)
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act):
+    def run(train, x, weight, bias, groups, eps, act):
         x = x.contiguous()
         y = torch.empty_like(x)
         B, C = x.shape[0], x.shape[-1]
@@ -319,9 +328,12 @@ class GroupNormClFn(_HnoFunction):
             n = L.hno_gncl_workspace_bytes(B, V, C, groups)
             ws = _ws(n, x.device)
             check(L.hno_gncl_fwd(_DTYPES[x.dtype], _p(x), _p(w), _p(b), _p(y), _p(mr), _p(ws), n, B, V, C, groups, eps, act, _stream(x)), 'hno_gncl_fwd')
-        if ops.backward_wanted(ctx):
-            ctx.save_for_backward(x, w, b, mr)
-            ctx.cfg = (groups, act, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        return y, (x, w, b, mr), (groups, act, None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+
+    @staticmethod
+    def forward(ctx, *args):
+        y, kept, ctx.cfg = GroupNormClFn.run(True, *args)
+        ctx.save_for_backward(*kept)
         return y
 
     @staticmethod
@@ -363,6 +375,6 @@ def group_norm(x, num_groups, weight=None, bias=None, *, eps=1e-5, act=None):
         if t is not None and (tuple(t.shape) != (C,) or t.dtype not in (x.dtype, torch.float32)):
             raise ValueError(f'group_norm: weight and bias must be ({C},) of {x.dtype} or fp32')
     if x.is_meta:
-        return GroupNormClFn.apply(x, weight, bias, num_groups, eps, a)
+        return _m(x.shape, x.dtype)
     _same_device('group_norm', x, weight, bias)
-    return _apply(GroupNormClFn, x, x, weight, bias, num_groups, eps, a)
+    return _call(GroupNormClFn, x, weight, bias, num_groups, eps, a)

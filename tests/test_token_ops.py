@@ -3,6 +3,7 @@
 Tolerances are bounds by arithmetic, element by element, computed next to the float64 result: E = 2^-24 for each fp32 operation (n E for a sum of n
 terms), U = half a step of the operand type (bf16 2^-8, fp32 E) for each value that is rounded to it: the probabilities and score gradients that are
 operands of a second product, the kept argument of an activation, the result."""
+import gc
 import math
 
 import pytest
@@ -560,6 +561,35 @@ def test_captured_step_replays(ot, dtype):
         for i, (graph, x, out, _) in enumerate(graphs):
             for a, b in zip(out, want[(n + i) % 4]):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_capture_with_a_live_eager_graph_is_refused(ot):
+    """the accumulation node of a leaf that an eager graph holds belongs to another stream than the capture's"""
+    x = torch.randn(8, 32, device='cuda', dtype=torch.bfloat16)
+    w = torch.randn(16, 32, device='cuda', requires_grad=True)
+    alive = ot.linear(x, w)
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match='still alive'):
+        with torch.cuda.graph(g, stream=side):
+            ot.linear(x, w)
+    alive.float().sum().backward()
+    want = w.grad.clone()
+    del alive
+    gc.collect()
+    w.grad = None
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=side):
+        y = ot.linear(x, w)
+        y.backward(torch.ones_like(y))
+    for _ in range(3):
+        w.grad.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(w.grad, want)
 
 
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
