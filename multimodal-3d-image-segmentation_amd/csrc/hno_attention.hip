@@ -855,8 +855,10 @@ static int at_check(const hno_attn_t *p, const char *what) {
     HNO_REQUIRE(p->H % p->Hk == 0, "%s: %d query heads do not share %d key heads evenly", what, p->H, p->Hk);
     HNO_REQUIRE(p->scale >= 1e-30f && p->scale <= 1e30f, "%s: scale must be positive, from 1e-30 to 1e30", what);
     if (p->Dk > 128 || p->Dv > 128) return fail(HNO_ELIMIT, "%s: head sizes %d, %d exceed 128", what, p->Dk, p->Dv);
-    if ((double)p->B * p->H * (ceil_div(p->Tq, AT_ROWS) + ceil_div(p->Tk, AT_ROWS)) > 1e8) return fail(HNO_ELIMIT, "%s: the grid is too large", what);
     if (p->Tq > (1 << 28) || p->Tk > (1 << 28) || (long long)(p->H / p->Hk) * p->Tq > (1ll << 30)) return fail(HNO_ELIMIT, "%s: too many tokens", what);
+    // a grid holds fewer than 2^32 threads: tiles of 128 rows (dk and dv apart) of 256 threads, and 16 threads a row
+    if ((double)p->B * p->H * ((double)ceil_div(p->Tq, AT_ROWS) + 2.0 * ceil_div(p->Tk, AT_ROWS)) > 1.6e7 || (double)p->B * p->H * p->Tq > 2.6e8)
+        return fail(HNO_ELIMIT, "%s: the grid is too large", what);
     HNO_REQUIRE(p->q && (p->Tk == 0 || (p->k && p->v)), "%s: null pointer", what);
     const int esz = p->dtype == HNO_BF16 ? 2 : 4;
     bool ok = p->Dk % 8 == 0 && p->Dv % 8 == 0 && at_aligned(p->q) && at_aligned(p->k) && at_aligned(p->v);

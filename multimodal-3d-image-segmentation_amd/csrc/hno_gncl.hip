@@ -459,7 +459,7 @@ static int gn_check(const char *what, int dtype, int B, long long V, int C, int 
     HNO_REQUIRE(C % G == 0, "%s: %d channels do not fall into %d groups", what, C, G);
     HNO_REQUIRE(act == HNO_ACT_NONE || act == HNO_ACT_SELU || act == HNO_ACT_ELU || act == HNO_ACT_RELU || act == HNO_ACT_GELU || act == HNO_ACT_SILU,
                 "%s: activation %d", what, act);
-    if (B > 65535 || C > (1 << 20) || V > (1ll << 40)) return fail(HNO_ELIMIT, "%s: a size exceeds the grid", what);
+    if (B > 65535 || C > (1 << 20) || V > (1ll << 40) || (long long)B * G >= 1ll << 30) return fail(HNO_ELIMIT, "%s: a size exceeds the grid", what);
     return HNO_OK;
 }
 static size_t gn_pad(size_t b) { return (b + 255) / 256 * 256; }

@@ -420,7 +420,7 @@ static int ln_product(LinArgs a, hipStream_t s) {
     const bool dma = esz == 2 && ln_aligned(a.A, a.lda, esz) && (AX ? a.M : a.K) % 8 == 0 && ln_aligned(a.B, a.ldb, esz) && (BX ? a.N : a.K) % 8 == 0 &&
                      a.lda < (1 << 22) && a.ldb < (1 << 22);
     const LnPlan p = ln_plan(a.M, a.N, a.K, sizeof(T) == 4, dma);
-    if (p.blocks > (1ll << 30)) return fail(HNO_ELIMIT, "hno_linear: %lld tiles exceed the grid", p.blocks);
+    if (p.blocks >= 1ll << 23) return fail(HNO_ELIMIT, "hno_linear: %lld tiles exceed the grid", p.blocks);          // (of 2^32 threads)
     a.nsplit = p.nsplit;
     ProfScope _ps(KID_LINEAR, s, esz * ((double)a.M * a.K + (double)a.N * a.K + (double)a.M * a.N));
     const dim3 grid((unsigned)p.blocks);

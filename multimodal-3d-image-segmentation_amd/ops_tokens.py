@@ -35,6 +35,12 @@ def _dtype(t, what):
     return _DTYPES[t.dtype]
 
 
+def _sizes(what, *sizes):
+    """the library takes sizes as 32-bit integers"""
+    if max(sizes) > 0x7fffffff:
+        raise ValueError(f'{what}: a size of {max(sizes)} is not provided')
+
+
 def _same_device(what, first, *others):
     if not first.is_cuda:
         raise _lib.HnoError('the HIP path needs CUDA/HIP tensors; there is no CPU fallback (use oracle/ for CPU checks)')
@@ -181,6 +187,7 @@ def attention(q, k, v, *, causal=False, mask=None, kv_lens=None, scale=None):
         raise ValueError(f'attention: {H} query heads do not share {Hk} key heads evenly')
     if not 1 <= Dk <= MAX_HEAD or not 1 <= Dv <= MAX_HEAD:
         raise ValueError(f'attention: head sizes {Dk}, {Dv} are outside 1 ... {MAX_HEAD}')
+    _sizes('attention', B, Tq, Tk, H)
     _dtype(q, 'attention')
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f'attention: q, k, v are {q.dtype}, {k.dtype}, {v.dtype}: one type is needed')
@@ -298,6 +305,7 @@ def linear(x, weight, bias=None, *, act=None, residual=None):
     N, K = weight.shape
     if N == 0 or K == 0:
         raise ValueError('linear: empty weight')
+    _sizes('linear', math.prod(x.shape[:-1]), N, K)
     _dtype(x, 'linear')
     if weight.dtype not in (x.dtype, torch.float32):
         raise ValueError(f'linear: weight is {weight.dtype}, x is {x.dtype}')
@@ -370,6 +378,7 @@ def group_norm(x, num_groups, weight=None, bias=None, *, eps=1e-5, act=None):
         raise ValueError(f'group_norm: {C} channels do not fall into {num_groups} groups')
     if not eps >= 0.0:
         raise ValueError('group_norm: eps must not be negative')
+    _sizes('group_norm', x.shape[0], C)
     _dtype(x, 'group_norm')
     for t in (weight, bias):
         if t is not None and (tuple(t.shape) != (C,) or t.dtype not in (x.dtype, torch.float32)):

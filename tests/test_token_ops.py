@@ -661,6 +661,29 @@ def test_entry_points_check_before_any_launch():
     assert L.hno_gncl_bwd(0, 4096, 4096, None, None, 4096, None, None, None, 4096, 1 << 40, 1, 8, 8, 2, 0, None) == -1
 
 
+def test_sizes_beyond_32_bits_are_refused(ot):
+    """a row count of 2^32 + 1 would reach the library as 1"""
+    m = lambda *s: torch.empty(s, device='meta', dtype=torch.bfloat16)  # noqa: E731
+    n = 2 ** 32 + 1
+    for call in (lambda: ot.linear(m(n, 8), m(4, 8)), lambda: ot.linear(m(2 ** 16, 2 ** 16, 8), m(4, 8)), lambda: ot.linear(m(2, 8), m(n, 8)),
+                 lambda: ot.attention(m(n, 2, 1, 8), m(n, 2, 1, 8), m(n, 2, 1, 8)), lambda: ot.attention(m(1, 2, 1, 8), m(1, n, 1, 8), m(1, n, 1, 8)),
+                 lambda: ot.group_norm(m(n, 2, 8), 2), lambda: ot.group_norm(m(2, 2, n - 1), 2)):
+        with pytest.raises(ValueError, match='size'):
+            call()
+    import ctypes
+
+    import multimodal_3d_image_segmentation_amd as pkg
+    L = pkg._lib.lib()
+    # more threads than a grid holds, and statistics whose index passes 32 bits
+    a = pkg._lib.AttnArgs()
+    for kw in (dict(B=1, Tq=1 << 28, H=2), dict(B=1 << 20, Tq=1, H=16), dict(B=1 << 20, Tq=400, H=1)):
+        for k, v in {**dict(dtype=1, Tk=4, Hk=1, Dk=32, Dv=32, scale=1.0, q=4096, k=4096, v=4096), **kw}.items():
+            setattr(a, k, v)
+        assert L.hno_attn_fwd(ctypes.byref(a), 4096, None, None, None, 0, None) == -2
+    assert L.hno_linear_fwd(0, 4096, 8, 4096, None, 0, None, None, 4096, 1 << 30, 512, 8, 0, None, 0, None) == -2
+    assert L.hno_gncl_fwd(0, 4096, None, None, 4096, 4096, 4096, 1 << 62, 65535, 1, 32768, 32768, 1e-5, 0, None) == -2
+
+
 def test_meta_tensors_give_shapes(ot):
     m = lambda *s: torch.empty(s, device='meta', dtype=torch.bfloat16)  # noqa: E731
     assert ot.attention(m(2, 5, 4, 32), m(2, 7, 2, 32), m(2, 7, 2, 16)).shape == (2, 5, 4, 16)
