@@ -119,7 +119,7 @@ __device__ __forceinline__ TkFrag<tkh> ln_frag(const tkh *tile, int m0, int kk, 
 
 // 8 neighbouring values of a row, `cnt` of them inside it; any alignment
 template <typename T>
-__device__ __forceinline__ void ln_get8(const T *p, int cnt, float (&x)[8]) {
+__device__ __forceinline__ TkFrag<T> ln_raw8(const T *p, int cnt) {
     TkFrag<T> f;
     if (cnt >= 8) {
         __builtin_memcpy(&f, p, 8 * sizeof(T));
@@ -127,6 +127,11 @@ __device__ __forceinline__ void ln_get8(const T *p, int cnt, float (&x)[8]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) f.set(j, j < cnt ? tk_up(p[j]) : 0.f);
     }
+    return f;
+}
+template <typename T>
+__device__ __forceinline__ void ln_get8(const T *p, int cnt, float (&x)[8]) {
+    const TkFrag<T> f = ln_raw8(p, cnt);
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = (float)f.v[j];
 }
@@ -145,7 +150,7 @@ __device__ __forceinline__ void ln_put8(T *p, int cnt, const float (&x)[8]) {
 }
 // the epilogue of columns n .. n + 7 of row m; r: the residual's values, loaded before
 template <typename T, int ACT>
-__device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float (&x)[8], const float (&r)[8]) {
+__device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float (&x)[8], const TkFrag<T> &r) {
     const int cnt = a.N - n;
     const long long at = (long long)m * a.N + n;
     if (a.bias) {
@@ -160,7 +165,7 @@ __device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float 
     for (int j = 0; j < 8; ++j) x[j] = tk_act(x[j], ACT);
     if (a.res)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] += r[j];
+        for (int j = 0; j < 8; ++j) x[j] += (float)r.v[j];
     if (a.out32) ln_put8((float *)a.y + at, cnt, x);
     else ln_put8((T *)a.y + at, cnt, x);
 }
@@ -272,17 +277,20 @@ __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a
         }
     }
     // the results change places in LDS, 32 rows of a wave at a time (its own part: no barrier inside), so that memory is read and written in runs of 128 bytes
+    constexpr int PASS = 32 * WN / 8 / 64;
+    TkFrag<T> r[WM / 32][PASS];                           // (the residual's loads are all on their way by then)
+    if (a.res && a.nsplit == 1)
+#pragma unroll
+        for (int u = 0; u < WM / 32; ++u)
+#pragma unroll
+            for (int e = 0; e < PASS; ++e) {
+                const int i = lane + 64 * e, m = m0 + wm + 32 * u + i / (WN / 8), n = n0 + wn + (i % (WN / 8)) * 8;
+                if (m < a.M && n < a.N) r[u][e] = ln_raw8((const T *)a.res + (long long)m * a.N + n, a.N - n);
+            }
     __syncthreads();
     float *ep = reinterpret_cast<float *>(smem) + wave * 32 * ES;
-    constexpr int PASS = 32 * WN / 8 / 64;
 #pragma unroll
     for (int u = 0; u < WM / 32; ++u) {
-        float r[PASS][8];
-#pragma unroll
-        for (int e = 0; e < PASS; ++e) {              // the residual's loads are on their way together
-            const int i = lane + 64 * e, m = m0 + wm + 32 * u + i / (WN / 8), n = n0 + wn + (i % (WN / 8)) * 8;
-            if (a.res && a.nsplit == 1 && m < a.M && n < a.N) ln_get8((const T *)a.res + (long long)m * a.N + n, a.N - n, r[e]);
-        }
 #pragma unroll
         for (int v = 0; v < WN / 32; ++v)
 #pragma unroll
@@ -298,7 +306,7 @@ __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a
             for (int j = 0; j < 8; ++j) x[j] = f.v[j];
             if (m < a.M && n < a.N) {
                 if (a.nsplit > 1) ln_put8(a.part + ((long long)run * a.M + m) * a.N + n, a.N - n, x);
-                else ln_finish<T, ACT>(a, m, n, x, r[e]);
+                else ln_finish<T, ACT>(a, m, n, x, r[u][e]);
             }
         }
     }
@@ -312,8 +320,9 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a) {
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < items; i += (long long)gridDim.x * 256) {
         const int m = (int)(i / per_row), n = 8 * (int)(i - (long long)m * per_row);
         const float *src = a.part + (long long)m * a.N + n;
-        float x[8] = {}, t[8], r[8] = {};
-        if (a.res) ln_get8((const T *)a.res + (long long)m * a.N + n, a.N - n, r);
+        float x[8] = {}, t[8];
+        TkFrag<T> r = {};
+        if (a.res) r = ln_raw8((const T *)a.res + (long long)m * a.N + n, a.N - n);
 #pragma unroll 8
         for (int s = 0; s < a.nsplit; ++s) {
             ln_get8(src + s * slab, a.N - n, t);

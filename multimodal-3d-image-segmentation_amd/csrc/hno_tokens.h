@@ -92,15 +92,16 @@ __device__ __forceinline__ void tk_dma16(const tkh *src, unsigned off, unsigned 
 // 1 - Phi(|z|) = erfc(|z| / sqrt 2) / 2 by Abramowitz and Stegun 7.1.26 (five terms, absolute error of erf 1.5e-7); e2 = exp(-z^2 / 2).  libm's erfcf
 // took longer than the product itself in the epilogue of an 8192 x 8192 x 2048 product.
 __device__ __forceinline__ float tk_phi_tail(float z, float &e2) {
-    const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
-    float p = fmaf(1.061405429f, t, -1.453152027f);
-    p = fmaf(p, t, 1.421413741f);
-    p = fmaf(p, t, -0.284496736f);
-    p = fmaf(p, t, 0.254829592f);
-    e2 = __expf(-x * x);
-    return 0.5f * p * t * e2;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
+    float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+    p = fmaf(p, t, 0.5f * 1.421413741f);
+    p = fmaf(p, t, 0.5f * -0.284496736f);
+    p = fmaf(p, t, 0.5f * 0.254829592f);
+    e2 = __builtin_amdgcn_exp2f(z * z * (-0.5f * 1.4426950408889634f));
+    return p * t * e2;
 }
-// act(z); the derivative is a function of z, which the backward passes recompute or keep
+// act(z); the derivative is a function of z, which the backward passes recompute or keep.  Infinite arguments give the limits and NaN stays NaN without
+// comparisons: where a factor is 0 the other one is bounded, and at a NaN the factor beside the bounded one is NaN.
 __device__ __forceinline__ float tk_act(float z, int act) {
     switch (act) {
         case HNO_ACT_SELU: return z > 0.f ? HNO_SELU_SCALE * z : (HNO_SELU_SCALE * HNO_SELU_ALPHA) * neg_expm1(z);
@@ -109,9 +110,9 @@ __device__ __forceinline__ float tk_act(float z, int act) {
         case HNO_ACT_GELU: {
             float e2;
             const float q = tk_phi_tail(z, e2);
-            return fabsf(z) < 20.f ? z * (z > 0.f ? 1.f - q : q) : (z > 0.f ? z : (z == z ? 0.f : z));
+            return fmaf(-fminf(fabsf(z), 20.f), q, fmaxf(z, 0.f));          // z > 0: z (1 - q), else z q
         }
-        case HNO_ACT_SILU: return z > -80.f ? z / (1.f + __expf(-z)) : (z == z ? 0.f : z);
+        case HNO_ACT_SILU: return fmaxf(z, -200.f) * __builtin_amdgcn_rcpf(1.f + __expf(-z));
         default: return z;
     }
 }
@@ -121,15 +122,13 @@ __device__ __forceinline__ float tk_act_grad(float z, int act) {
         case HNO_ACT_ELU: return z > 0.f ? 1.f : __expf(z);
         case HNO_ACT_RELU: return z > 0.f ? 1.f : (z == z ? 0.f : z);
         case HNO_ACT_GELU: {
-            if (!(fabsf(z) < 20.f)) return z > 0.f ? 1.f : (z == z ? 0.f : z);
             float e2;
             const float q = tk_phi_tail(z, e2);
-            return (z > 0.f ? 1.f - q : q) + z * e2 * 0.39894228040143268f;
+            return fmaf(fminf(fmaxf(z, -20.f), 20.f) * 0.39894228040143268f, e2, z > 0.f ? 1.f - q : q);
         }
         case HNO_ACT_SILU: {
-            if (!(fabsf(z) < 80.f)) return z > 0.f ? 1.f : (z == z ? 0.f : z);
-            const float s = 1.f / (1.f + __expf(-z));
-            return s * (1.f + z * (1.f - s));
+            const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
+            return s * fmaf(fminf(fmaxf(z, -200.f), 200.f), 1.f - s, 1.f);
         }
         default: return 1.f;
     }

@@ -326,6 +326,21 @@ def test_linear_large_activation_arguments(ot):
         assert torch.allclose(dx[ok].double(), slope[ok], rtol=1e-6, atol=1e-6), act
 
 
+@pytest.mark.gpu
+def test_linear_infinite_activation_arguments(ot):
+    """an infinite bias gives the activations' limits"""
+    x, w = torch.zeros(3, 4, device='cuda'), torch.ones(2, 4, device='cuda')
+    b = torch.tensor([math.inf, -math.inf], device='cuda')
+    for act, low in ((None, -math.inf), ('selu', -1.7580993408473766), ('elu', -1.0), ('relu', 0.0), ('gelu', 0.0), ('silu', 0.0)):
+        xx = x.clone().requires_grad_(True)
+        y = ot.linear(xx, w, b, act=act)
+        (dx,) = torch.autograd.grad(y, xx, torch.ones_like(y))
+        assert torch.isinf(y[:, 0]).all() and (y[:, 0] > 0).all(), act
+        assert (y[:, 1] == low).all() or torch.allclose(y[:, 1], torch.tensor(low, device='cuda'), rtol=2e-7, atol=0), act
+        slope = {None: 2.0, 'selu': 1.0507009873554805}.get(act, 1.0)      # of column 0, and 0 of column 1
+        assert torch.allclose(dx, torch.full_like(dx, slope), rtol=2e-7, atol=0), act
+
+
 # ------------------------------------------------------------------------------------------------ group norm
 def check_group_norm(ot, x, G, w, b, act, eps=1e-5):
     leaves = [t.detach().requires_grad_(True) for t in (x, w, b) if t is not None]
