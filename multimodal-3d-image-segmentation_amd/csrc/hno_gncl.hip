@@ -9,6 +9,8 @@
 // (count, mean, M2) are joined pairwise in 64 bits.
 #include "hno_tokens.h"
 
+#include <type_traits>
+
 namespace hno {
 
 struct GnArgs {
@@ -44,6 +46,19 @@ __device__ __forceinline__ void gn_store(T *p, const GnVec<T, W> &r) {
         tk_store8(p, f);
     } else {
         p[0] = tk_down<T>(r.v[0]);
+    }
+}
+
+// f(activation as a constant): one loop for each activation instead of a branch for each value
+template <typename F>
+__device__ __forceinline__ void gn_with_act(int act, F f) {
+    switch (act) {
+        case HNO_ACT_SELU: f(std::integral_constant<int, HNO_ACT_SELU>()); break;
+        case HNO_ACT_ELU: f(std::integral_constant<int, HNO_ACT_ELU>()); break;
+        case HNO_ACT_RELU: f(std::integral_constant<int, HNO_ACT_RELU>()); break;
+        case HNO_ACT_GELU: f(std::integral_constant<int, HNO_ACT_GELU>()); break;
+        case HNO_ACT_SILU: f(std::integral_constant<int, HNO_ACT_SILU>()); break;
+        default: f(std::integral_constant<int, HNO_ACT_NONE>());
     }
 }
 
@@ -154,13 +169,15 @@ __global__ __launch_bounds__(256) void gncl_apply_kernel(GnArgs a) {
     }
     const long long base = (long long)b * a.V * a.C + chunk * W;
     const long long r1 = ((long long)blockIdx.x + 1) * a.rows_per < a.V ? ((long long)blockIdx.x + 1) * a.rows_per : a.V;
+    gn_with_act(a.act, [&](auto act) {
 #pragma unroll 2
-    for (long long r = blockIdx.x * a.rows_per + rl; r < r1; r += nrl) {
-        GnVec<T, W> v = gn_load<T, W>((const T *)a.x + base + r * a.C);
+        for (long long r = blockIdx.x * a.rows_per + rl; r < r1; r += nrl) {
+            GnVec<T, W> v = gn_load<T, W>((const T *)a.x + base + r * a.C);
 #pragma unroll
-        for (int j = 0; j < W; ++j) v.v[j] = tk_act(fmaf(v.v[j] - mean[j], ga[j], be[j]), a.act);
-        gn_store<T, W>((T *)a.y + base + r * a.C, v);
-    }
+            for (int j = 0; j < W; ++j) v.v[j] = tk_act(fmaf(v.v[j] - mean[j], ga[j], be[j]), act);
+            gn_store<T, W>((T *)a.y + base + r * a.C, v);
+        }
+    });
 }
 
 // per channel: sum du and sum du xh over a run of rows
@@ -183,15 +200,18 @@ __global__ __launch_bounds__(256) void gncl_bwd_sums_kernel(GnArgs a) {
         }
         const long long base = (long long)b * a.V * a.C + chunk * W;
         const long long r1 = ((long long)blockIdx.x + 1) * a.rows_per < a.V ? ((long long)blockIdx.x + 1) * a.rows_per : a.V;
-        for (long long r = blockIdx.x * a.rows_per + rl; r < r1; r += nrl) {
-            const GnVec<T, W> v = gn_load<T, W>((const T *)a.x + base + r * a.C), d = gn_load<T, W>((const T *)a.dy + base + r * a.C);
+        gn_with_act(a.act, [&](auto act) {
+#pragma unroll 2
+            for (long long r = blockIdx.x * a.rows_per + rl; r < r1; r += nrl) {
+                const GnVec<T, W> v = gn_load<T, W>((const T *)a.x + base + r * a.C), d = gn_load<T, W>((const T *)a.dy + base + r * a.C);
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                const float xh = (v.v[j] - mean[j]) * rstd[j], du = d.v[j] * tk_act_grad(fmaf(xh, ga[j], be[j]), a.act);
-                s1[j] += du;
-                s2[j] = fmaf(du, xh, s2[j]);
+                for (int j = 0; j < W; ++j) {
+                    const float xh = (v.v[j] - mean[j]) * rstd[j], du = d.v[j] * tk_act_grad(fmaf(xh, ga[j], be[j]), act);
+                    s1[j] += du;
+                    s2[j] = fmaf(du, xh, s2[j]);
+                }
             }
-        }
+        });
     }
     gn_block_sums<W>(a, s1, s2, nrl, tid, lds);
 }
@@ -262,17 +282,19 @@ __global__ __launch_bounds__(256) void gncl_bwd_apply_kernel(GnArgs a) {
     }
     const long long base = (long long)b * a.V * a.C + chunk * W;
     const long long r1 = ((long long)blockIdx.x + 1) * a.rows_per < a.V ? ((long long)blockIdx.x + 1) * a.rows_per : a.V;
+    gn_with_act(a.act, [&](auto act) {
 #pragma unroll 2
-    for (long long r = blockIdx.x * a.rows_per + rl; r < r1; r += nrl) {
-        GnVec<T, W> v = gn_load<T, W>((const T *)a.x + base + r * a.C);
-        const GnVec<T, W> d = gn_load<T, W>((const T *)a.dy + base + r * a.C);
+        for (long long r = blockIdx.x * a.rows_per + rl; r < r1; r += nrl) {
+            GnVec<T, W> v = gn_load<T, W>((const T *)a.x + base + r * a.C);
+            const GnVec<T, W> d = gn_load<T, W>((const T *)a.dy + base + r * a.C);
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-            const float xh = (v.v[j] - mean[j]) * rstd[j], du = d.v[j] * tk_act_grad(fmaf(xh, ga[j], be[j]), a.act);
-            v.v[j] = rstd[j] * (fmaf(du, ga[j], -t1[j]) - xh * t2[j]);
+            for (int j = 0; j < W; ++j) {
+                const float xh = (v.v[j] - mean[j]) * rstd[j], du = d.v[j] * tk_act_grad(fmaf(xh, ga[j], be[j]), act);
+                v.v[j] = rstd[j] * (fmaf(du, ga[j], -t1[j]) - xh * t2[j]);
+            }
+            gn_store<T, W>((T *)a.dx + base + r * a.C, v);
         }
-        gn_store<T, W>((T *)a.dx + base + r * a.C, v);
-    }
+    });
 }
 
 // ------------------------------------------------------------------ small groups: one launch
