@@ -467,7 +467,8 @@ static GnPlan gn_plan(int dtype, int B, long long V, int C, bool vec) {
     p.chunks = C / p.W;
     p.cw = p.chunks < 256 ? p.chunks : 256;
     p.yblocks = ceil_div(p.chunks, p.cw);
-    const long long nrl = 256 / p.cw, most = 2048 / ((long long)B * p.yblocks) > 1 ? 2048 / ((long long)B * p.yblocks) : 1;
+    // (four workgroups a CU: 2 x 491520 x 64 bf16 forward and backward 195 us of kernels, with eight 205, with two 229: the loads of two rows a thread no longer hide)
+    const long long nrl = 256 / p.cw, most = 1024 / ((long long)B * p.yblocks) > 1 ? 1024 / ((long long)B * p.yblocks) : 1;
     long long runs = (V + 4 * nrl - 1) / (4 * nrl);            // four rows per thread at least
     if (runs > most) runs = most;
     if (runs < 1) runs = 1;
