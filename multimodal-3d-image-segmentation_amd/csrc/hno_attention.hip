@@ -51,16 +51,42 @@ __device__ __forceinline__ int at_at(int row, int d) {
     else slot = c + ((row >> 2) & 3) - (c + ((row >> 2) & 3) >= 12 ? 12 : 0);
     return row * DP + slot * 8 + (d & 7);
 }
-// the fragment of the transposed tile: channel 32 dt + (lane & 31), rows r0 .. r0 + 3 and r0 + 8 .. r0 + 11 (PLANE: elements of one term's tile)
+// LDS byte addresses of a lane's fragments in the tile at `base`: r of row lane & 31, channels 16 kk + 8 (lane >> 5) + {0..7}; c of the transposed tile, channel
+// 32 dt + (lane & 31), rows 4 (lane >> 5) + {0..3} and 8 rows on.  Other tiles, planes and rows a multiple of 16 away are immediate offsets of the reads, the
+// other buffer is a step of all addresses: worked out for each read they were a third of the vector instructions.
+template <int DP>
+struct AtAddr {
+    unsigned r[DP / 16], c[DP / 16];
+    __device__ __forceinline__ void init(const tkh *base, int lane) {
+        typedef const __attribute__((address_space(3))) tkh *ldsp;
+        const unsigned b = (unsigned)(uintptr_t)(ldsp)base;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            r[i] = b + 2 * at_at<DP>(lane & 31, 16 * i + 8 * (lane >> 5));
+            c[i] = b + 2 * at_at<DP>(4 * (lane >> 5) + ((lane & 15) >> 2) + 8 * (i & 1), 32 * (i >> 1) + (lane & 16) + 4 * (lane & 3));
+        }
+    }
+    __device__ __forceinline__ void move(int bytes) {
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) r[i] += bytes, c[i] += bytes;
+    }
+};
 template <typename T, int DP, int PLANE>
-__device__ __forceinline__ TkOp<T> at_col(const tkh *tile, int dt, int r0, int lane) {
+__device__ __forceinline__ TkOp<T> at_rows(const AtAddr<DP> &at, int off, int kk) {
+    typedef const __attribute__((address_space(3))) tkb8 *lds8;
+    TkOp<T> o;
+#pragma unroll
+    for (int p = 0; p < tk_planes<T>(); ++p) o.p[p].v = *(lds8)(uintptr_t)(at.r[kk] + 2 * (off + p * PLANE));
+    return o;
+}
+template <typename T, int DP, int PLANE>
+__device__ __forceinline__ TkOp<T> at_col(const AtAddr<DP> &at, int off, int dt) {
     typedef __attribute__((address_space(3))) tks4 *lds4;
-    const int row = r0 + ((lane & 15) >> 2), d = 32 * dt + (lane & 16) + 4 * (lane & 3);
     TkOp<T> o;
 #pragma unroll
     for (int p = 0; p < tk_planes<T>(); ++p) {
-        const tks4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(tile + p * PLANE + at_at<DP>(row, d)));
-        const tks4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(tile + p * PLANE + at_at<DP>(row + 8, d)));
+        const tks4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(at.c[2 * dt] + 2 * (off + p * PLANE)));
+        const tks4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(at.c[2 * dt + 1] + 2 * (off + p * PLANE)));
         o.p[p].v = __builtin_bit_cast(tkb8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     }
     return o;
@@ -195,49 +221,54 @@ __device__ __forceinline__ AtMask at_mask_row(const AttnArgs &a, const unsigned 
 }
 __device__ __forceinline__ bool at_mask_on(const AtMask &m, int e) { return (m.w[e >> 2] >> (8 * (e & 3))) & 0xffu; }
 
-// acc(32 rows of the tile x 32 own columns) = tile rows . own fragments
-template <typename T, int DP, int PLANE>
-__device__ __forceinline__ tk16 at_product(const tkh *tile, int row0, const TkOp<T> (&own)[DP / 16], int lane) {
-    tk16 acc = {};
+// use(i, load(i)) for i = 0 ... N - 1, the LDS reads DEPTH ahead of the products that take them.  (Left to itself the compiler reads one product ahead, and
+// each product waits for most of an LDS access.)  Vector instructions may move across the steps, reads and products may not.
+template <typename T> constexpr int at_ahead() { return sizeof(T) == 2 ? 4 : 2; }
+template <int N, int DEPTH, typename L, typename U>
+__device__ __forceinline__ void at_pipe(L load, U use) {
+    decltype(load(0)) ring[DEPTH];
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-        TkOp<T> o;
+    for (int i = 0; i < DEPTH && i < N; ++i) ring[i] = load(i);
+    __builtin_amdgcn_sched_barrier(0x406);
 #pragma unroll
-        for (int p = 0; p < tk_planes<T>(); ++p) o.p[p] = tk_row(tile + p * PLANE + at_at<DP>(row0 + (lane & 31), 16 * kk + 8 * (lane >> 5)));
-        acc = tk_mma(o, own[kk], acc);
+    for (int i = 0; i < N; ++i) {
+        use(i, ring[i % DEPTH]);
+        if (i + DEPTH < N) ring[i % DEPTH] = load(i + DEPTH);
+        __builtin_amdgcn_sched_barrier(0x406);
     }
+}
+// acc(32 rows of the tile x 32 own columns) = tile rows . own fragments; `off`: element offset of the tile's first of these rows
+template <typename T, int DP, int PLANE>
+__device__ __forceinline__ tk16 at_product(const AtAddr<DP> &at, int off, const TkOp<T> (&own)[DP / 16]) {
+    tk16 acc = {};
+    at_pipe<DP / 16, at_ahead<T>()>([&](int kk) { return at_rows<T, DP, PLANE>(at, off, kk); }, [&](int kk, const TkOp<T> &o) { acc = tk_mma(o, own[kk], acc); });
     return acc;
 }
 // two independent products, step by step: neither waits for its own last step
 template <typename T, int DP, int PLANE>
-__device__ __forceinline__ void at_product2(tk16 &x, tk16 &y, const tkh *tx, int rx, const TkOp<T> (&ox)[DP / 16], const tkh *ty, int ry, const TkOp<T> (&oy)[DP / 16],
-                                            int lane) {
+__device__ __forceinline__ void at_product2(tk16 &x, tk16 &y, const AtAddr<DP> &at, int offx, const TkOp<T> (&ox)[DP / 16], int offy, const TkOp<T> (&oy)[DP / 16]) {
     x = tk16{};
     y = tk16{};
-#pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-        TkOp<T> a, b;
-#pragma unroll
-        for (int p = 0; p < tk_planes<T>(); ++p) {
-            a.p[p] = tk_row(tx + p * PLANE + at_at<DP>(rx + (lane & 31), 16 * kk + 8 * (lane >> 5)));
-            b.p[p] = tk_row(ty + p * PLANE + at_at<DP>(ry + (lane & 31), 16 * kk + 8 * (lane >> 5)));
-        }
-        x = tk_mma(a, ox[kk], x);
-        y = tk_mma(b, oy[kk], y);
-    }
+    at_pipe<DP / 8, at_ahead<T>()>([&](int i) { return at_rows<T, DP, PLANE>(at, i & 1 ? offy : offx, i >> 1); },
+                                   [&](int i, const TkOp<T> &o) {
+                                       if (i & 1) y = tk_mma(o, oy[i >> 1], y);
+                                       else x = tk_mma(o, ox[i >> 1], x);
+                                   });
 }
-// acc[dt] += (tile rows row0 .. row0 + 31)^T . w, w being a result over the same rows
+// acc[dt] += (32 tile rows)^T . w, w being a result over the same rows
 template <typename T, int DP, int PLANE>
-__device__ __forceinline__ void at_accumulate(tk16 (&acc)[DP / 32], const tkh *tile, int row0, const tk16 &w, int lane) {
+__device__ __forceinline__ void at_accumulate(tk16 (&acc)[DP / 32], const AtAddr<DP> &at, int off, const tk16 &w) {
+    constexpr int ND = DP / 32;
+    TkOp<T> o[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         TkFrag<T> f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) f.set(j, w[8 * t + j]);
-        const TkOp<T> o = tk_op(f);
-#pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = tk_mma(at_col<T, DP, PLANE>(tile, dt, row0 + 16 * t + 4 * (lane >> 5), lane), o, acc[dt]);
+        o[t] = tk_op(f);
     }
+    at_pipe<2 * ND, at_ahead<T>()>([&](int i) { return at_col<T, DP, PLANE>(at, off + 16 * (i / ND) * DP, i % ND); },
+                                   [&](int i, const TkOp<T> &x) { acc[i % ND] = tk_mma(x, o[i / ND], acc[i % ND]); });
 }
 // LDS buffers of the streamed side: two (one barrier a step), one where two would leave room for a single workgroup per CU
 template <typename T, int DP> constexpr int at_buffers() { return sizeof(T) == 4 && DP == 128 ? 1 : 2; }
@@ -348,8 +379,8 @@ __device__ __forceinline__ void at_weights(TkFrag<float> &f, const tk16 &s, int 
 template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 4 ? (DP <= 96 ? 2 : 1) : (DP <= 64 ? 3 : 2)) void attn_fwd_kernel(AttnArgs a) {
     constexpr int KT = at_tile<T>(), PLANE = KT * DP, NB = at_buffers<T, DP>();
-    __shared__ __attribute__((aligned(16))) tkh Ks[NB][tk_planes<T>() * PLANE];
-    __shared__ __attribute__((aligned(16))) tkh Vs[NB][tk_planes<T>() * PLANE];
+    constexpr int TILE = tk_planes<T>() * PLANE, V = NB * TILE;             // LDS: the buffers of the keys, then those of the values
+    __shared__ __attribute__((aligned(16))) tkh smem[2 * NB * TILE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const AtBlock w0 = at_block(a, a.pack ? 1 : a.H / a.Hk, blockIdx.x, gridDim.x);
     const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk, hb = hk * grp + w0.gi, nrows = a.pack ? grp * a.Tq : a.Tq;
@@ -377,21 +408,23 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 4 ? (DP <= 96 ? 2 : 1) 
     ks.init(a.ks[1], a.Dk, tid);
     vs.init(a.vs[1], a.Dv, tid);
     const auto fetch = [&](int to, int j) {
-        ks.fetch(Ks[to], kb, j, j1, tid);
-        vs.fetch(Vs[to], vb, j, j1, tid);
+        ks.fetch(smem + to * TILE, kb, j, j1, tid);
+        vs.fetch(smem + V + to * TILE, vb, j, j1, tid);
         if (MASK && mkey) flag.load(j, j1, tid, [&](int t) { return mkey[t * a.ms[3]]; });
     };
     const auto settle = [&](int to) {
-        ks.settle(Ks[to], tid, [](int) { return false; });
-        vs.settle(Vs[to], tid, [&](int i) { return MASK && mkey && !flag.f[i]; });
+        ks.settle(smem + to * TILE, tid, [](int) { return false; });
+        vs.settle(smem + V + to * TILE, tid, [&](int i) { return MASK && mkey && !flag.f[i]; });
     };
 
     tk16 acc[DP / 32] = {};
     float m = -INFINITY, l = 0.f, shift = 0.f;
     const float slack = 8.f / a.scale2;           // the maximum is raised, and the sums rescaled, only where weights would exceed 2^8
+    AtAddr<DP> at;
+    at.init(smem, lane);
     int buf = 0;
     if (j0 < j1) fetch(0, j0);
-    for (int j = j0; j < j1; j += KT, buf ^= NB - 1) {
+    for (int j = j0; j < j1; j += KT, buf ^= NB - 1, at.move(NB == 1 ? 0 : (buf ? 2 * TILE : -2 * TILE))) {
         if (NB == 1) __syncthreads();
         settle(buf);
         __syncthreads();
@@ -402,8 +435,8 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 4 ? (DP <= 96 ? 2 : 1) 
         if (MASK)
 #pragma unroll
             for (int n = 0; n < KT / 32; ++n) mk[n] = at_mask_row(a, mrow, j + 32 * n, h);
-#pragma unroll
-        for (int n = 0; n < KT / 32; ++n) s[n] = at_product<T, DP, PLANE>(Ks[buf], 32 * n, qf, lane);
+        if constexpr (KT == 64) at_product2<T, DP, PLANE>(s[0], s[1], at, 0, qf, 32 * DP, qf);
+        else s[0] = at_product<T, DP, PLANE>(at, 0, qf);
         if (j + KT > lim_all) {
             asm volatile("");               // (a branch: the comparisons are not to be made for whole tiles)
 #pragma unroll
@@ -432,17 +465,17 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 4 ? (DP <= 96 ? 2 : 1) 
         for (int n = 0; n < KT / 32; ++n)
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[n][e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], a.scale2, -shift));
-#pragma unroll
-        for (int n = 0; n < KT / 32; ++n)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                TkFrag<T> f;
-                at_weights(f, s[n], t, l);
-                const TkOp<T> o = tk_op(f);
-                const int row = 32 * n + 16 * t + 4 * h;
-#pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt) acc[dt] = tk_mma(at_col<T, DP, PLANE>(Vs[buf], dt, row, lane), o, acc[dt]);
-            }
+        constexpr int ND = DP / 32;
+        TkOp<T> o;
+        at_pipe<KT / 16 * ND, at_ahead<T>()>([&](int i) { return at_col<T, DP, PLANE>(at, V + 16 * (i / ND) * DP, i % ND); },
+                                             [&](int i, const TkOp<T> &x) {
+                                                 if (i % ND == 0) {
+                                                     TkFrag<T> f;
+                                                     at_weights(f, s[i / ND / 2], i / ND % 2, l);
+                                                     o = tk_op(f);
+                                                 }
+                                                 acc[i % ND] = tk_mma(x, o, acc[i % ND]);
+                                             });
     }
     l += at_other_half(l);
     if (!w.valid) continue;
@@ -555,8 +588,7 @@ template <typename T, int DP> constexpr int at_half() { return at_buffers<T, DP>
 template <typename T, int DP, bool MASK>
 __device__ __forceinline__ void at_dq(const AttnArgs &a, const AtBlock &w0, tkh *smem) {
     constexpr int KT = at_tile<T>(), PLANE = KT * DP, NB = at_buffers<T, DP>();
-    typedef tkh Tile[NB][tk_planes<T>() * PLANE];
-    Tile &Ks = *reinterpret_cast<Tile *>(smem), &Vs = *reinterpret_cast<Tile *>(smem + at_half<T, DP>());
+    constexpr int TILE = tk_planes<T>() * PLANE, V = at_half<T, DP>();
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk, hb = hk * grp + w0.gi, nrows = a.pack ? grp * a.Tq : a.Tq;
     const int L = at_length(a, b);
@@ -586,18 +618,20 @@ __device__ __forceinline__ void at_dq(const AttnArgs &a, const AtBlock &w0, tkh 
     ks.init(a.ks[1], a.Dk, tid);
     vs.init(a.vs[1], a.Dv, tid);
     const auto fetch = [&](int to, int j) {
-        ks.fetch(Ks[to], kb, j, j1, tid);
-        vs.fetch(Vs[to], vb, j, j1, tid);
+        ks.fetch(smem + to * TILE, kb, j, j1, tid);
+        vs.fetch(smem + V + to * TILE, vb, j, j1, tid);
         if (MASK && mkey) flag.load(j, j1, tid, [&](int t) { return mkey[t * a.ms[3]]; });
     };
     const auto settle = [&](int to) {
-        ks.settle(Ks[to], tid, [&](int i) { return MASK && mkey && !flag.f[i]; });
-        vs.settle(Vs[to], tid, [](int) { return false; });
+        ks.settle(smem + to * TILE, tid, [&](int i) { return MASK && mkey && !flag.f[i]; });
+        vs.settle(smem + V + to * TILE, tid, [](int) { return false; });
     };
     tk16 acc[DP / 32] = {};
+    AtAddr<DP> at;
+    at.init(smem, lane);
     int buf = 0;
     if (j0 < j1) fetch(0, j0);
-    for (int j = j0; j < j1; j += KT, buf ^= NB - 1) {
+    for (int j = j0; j < j1; j += KT, buf ^= NB - 1, at.move(NB == 1 ? 0 : (buf ? 2 * TILE : -2 * TILE))) {
         if (NB == 1) __syncthreads();
         settle(buf);
         __syncthreads();
@@ -609,7 +643,7 @@ __device__ __forceinline__ void at_dq(const AttnArgs &a, const AtBlock &w0, tkh 
             AtMask mk;
             if (MASK) mk = at_mask_row(a, mrow, j + 32 * n, h);
             tk16 s, dp;
-            at_product2<T, DP, PLANE>(s, dp, Ks[buf], 32 * n, qf, Vs[buf], 32 * n, gf, lane);
+            at_product2<T, DP, PLANE>(s, dp, at, 32 * n * DP, qf, V + 32 * n * DP, gf);
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse)) * (dp[e] - delta);
             if (!whole) {
@@ -620,7 +654,7 @@ __device__ __forceinline__ void at_dq(const AttnArgs &a, const AtBlock &w0, tkh 
                     s[e] = on ? s[e] : 0.f;
                 }
             }
-            at_accumulate<T, DP, PLANE>(acc, Ks[buf], 32 * n, s, lane);
+            at_accumulate<T, DP, PLANE>(acc, at, 32 * n * DP, s);
         }
     }
     if (!w.valid) continue;
@@ -637,9 +671,8 @@ __device__ __forceinline__ void at_dq(const AttnArgs &a, const AtBlock &w0, tkh 
 template <typename T, int DP, bool MASK, int WHAT>
 __device__ __forceinline__ void at_dkv(const AttnArgs &a, const AtBlock &w0, tkh *smem) {
     constexpr int QT = at_tile<T>(), PLANE = QT * DP, NB = at_buffers<T, DP>();
-    typedef tkh Tile[NB][tk_planes<T>() * PLANE];
+    constexpr int TILE = tk_planes<T>() * PLANE, G = at_half<T, DP>();
     typedef float Rows[NB][QT];
-    Tile &Qs = *reinterpret_cast<Tile *>(smem), &Gs = *reinterpret_cast<Tile *>(smem + at_half<T, DP>());
     Rows &lses = *reinterpret_cast<Rows *>(smem + 2 * at_half<T, DP>()), &deltas = *reinterpret_cast<Rows *>(smem + 2 * at_half<T, DP>() + 2 * NB * QT);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int b = w0.b, sp = w0.sp, grp = a.H / a.Hk, hk = w0.hk;
@@ -682,8 +715,8 @@ __device__ __forceinline__ void at_dkv(const AttnArgs &a, const AtBlock &w0, tkh
         const int i0 = qt * QT, head = hk * grp + gi;
         const long long row0 = ((long long)b * a.Tq) * a.H + head;
         i_next = i0;
-        qs.fetch(Qs[to], (const T *)a.q + b * a.qs[0] + head * a.qs[2], i0, a.Tq, tid);
-        gs.fetch(Gs[to], (const T *)a.g + row0 * a.Dv, i0, a.Tq, tid);
+        qs.fetch(smem + to * TILE, (const T *)a.q + b * a.qs[0] + head * a.qs[2], i0, a.Tq, tid);
+        gs.fetch(smem + G + to * TILE, (const T *)a.g + row0 * a.Dv, i0, a.Tq, tid);
         if (MASK) flag.load(i0, a.Tq, tid, [&](int t) { return a.lse[row0 + (long long)t * a.H]; });
         if (tid < QT) {
             const int i = i0 + tid < a.Tq ? i0 + tid : a.Tq - 1;
@@ -694,14 +727,16 @@ __device__ __forceinline__ void at_dkv(const AttnArgs &a, const AtBlock &w0, tkh
     const auto settle = [&](int to) {
         // queries that see nothing, by their position or by the mask
         const auto dead = [&](int i) { return i_next + AtTile<T, DP, QT>::row(i, tid) < empty || (MASK && flag.f[i] == INFINITY); };
-        qs.settle(Qs[to], tid, dead);
-        gs.settle(Gs[to], tid, dead);
+        qs.settle(smem + to * TILE, tid, dead);
+        gs.settle(smem + G + to * TILE, tid, dead);
         if (tid < QT) lses[to][tid] = nlse, deltas[to][tid] = ndelta;
     };
+    AtAddr<DP> at;
+    at.init(smem, lane);
     int buf = 0;
     int gi = each > 0 ? sp * per / each : 0, qt = qt0 + sp * per - gi * each;
     if (sp * per < it1) fetch(0, gi, qt);
-    for (int it = sp * per; it < it1; ++it, buf ^= NB - 1) {
+    for (int it = sp * per; it < it1; ++it, buf ^= NB - 1, at.move(NB == 1 ? 0 : (buf ? 2 * TILE : -2 * TILE))) {
         if (NB == 1) __syncthreads();
         settle(buf);
         __syncthreads();
@@ -717,8 +752,8 @@ __device__ __forceinline__ void at_dkv(const AttnArgs &a, const AtBlock &w0, tkh
 #pragma unroll
                 for (int e = 0; e < 16; ++e) mk[e] = mcol[min(i0 + 32 * n + at_row(e, h), a.Tq - 1) * a.ms[2]];
             tk16 s, dp = {};
-            if constexpr (DK) at_product2<T, DP, PLANE>(s, dp, Qs[buf], 32 * n, kf, Gs[buf], 32 * n, vf, lane);
-            else s = at_product<T, DP, PLANE>(Qs[buf], 32 * n, kf, lane);
+            if constexpr (DK) at_product2<T, DP, PLANE>(s, dp, at, 32 * n * DP, kf, G + 32 * n * DP, vf);
+            else s = at_product<T, DP, PLANE>(at, 32 * n * DP, kf);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const tkf4 le = *reinterpret_cast<const tkf4 *>(&lses[buf][32 * n + 8 * u + 4 * h]), de = *reinterpret_cast<const tkf4 *>(&deltas[buf][32 * n + 8 * u + 4 * h]);
@@ -739,8 +774,8 @@ __device__ __forceinline__ void at_dkv(const AttnArgs &a, const AtBlock &w0, tkh
                     dp[e] = on ? dp[e] : 0.f;
                 }
             }
-            if constexpr (DV) at_accumulate<T, DP, PLANE>(accv, Gs[buf], 32 * n, s, lane);
-            if constexpr (DK) at_accumulate<T, DP, PLANE>(acck, Qs[buf], 32 * n, dp, lane);
+            if constexpr (DV) at_accumulate<T, DP, PLANE>(accv, at, G + 32 * n * DP, s);
+            if constexpr (DK) at_accumulate<T, DP, PLANE>(acck, at, 32 * n * DP, dp);
         }
     }
     if (!valid) continue;
