@@ -222,19 +222,19 @@ __device__ __forceinline__ AtMask at_mask_row(const AttnArgs &a, const unsigned 
 __device__ __forceinline__ bool at_mask_on(const AtMask &m, int e) { return (m.w[e >> 2] >> (8 * (e & 3))) & 0xffu; }
 
 // use(i, load(i)) for i = 0 ... N - 1, the LDS reads DEPTH ahead of the products that take them.  (Left to itself the compiler reads one product ahead, and
-// each product waits for most of an LDS access.)  Vector instructions may move across the steps, reads and products may not.
+// each product waits for most of an LDS access.)  Vector instructions may move across the steps, reads and products may not; with FREE = 4 they may not either.
 template <typename T> constexpr int at_ahead() { return sizeof(T) == 2 ? 4 : 2; }
-template <int N, int DEPTH, typename L, typename U>
+template <int N, int DEPTH, int FREE = 0x406, typename L, typename U>
 __device__ __forceinline__ void at_pipe(L load, U use) {
     decltype(load(0)) ring[DEPTH];
 #pragma unroll
     for (int i = 0; i < DEPTH && i < N; ++i) ring[i] = load(i);
-    __builtin_amdgcn_sched_barrier(0x406);
+    __builtin_amdgcn_sched_barrier(FREE);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         use(i, ring[i % DEPTH]);
         if (i + DEPTH < N) ring[i % DEPTH] = load(i + DEPTH);
-        __builtin_amdgcn_sched_barrier(0x406);
+        __builtin_amdgcn_sched_barrier(FREE);
     }
 }
 // acc(32 rows of the tile x 32 own columns) = tile rows . own fragments; `off`: element offset of the tile's first of these rows
@@ -461,21 +461,29 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 4 ? (DP <= 96 ? 2 : 1) 
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt) acc[dt] *= old;
         }
+        // the weights of 8 keys at a time, those of the next 8 between the products of these (2x8x8192x64: 258 us, with all of them in front 273)
+        constexpr int ND = DP / 32, G = KT / 16;
+        const auto weigh = [&](int g, int e0, int e1) {
 #pragma unroll
-        for (int n = 0; n < KT / 32; ++n)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[n][e] = __builtin_amdgcn_exp2f(fmaf(s[n][e], a.scale2, -shift));
-        constexpr int ND = DP / 32;
-        TkOp<T> o;
-        at_pipe<KT / 16 * ND, at_ahead<T>()>([&](int i) { return at_col<T, DP, PLANE>(at, V + 16 * (i / ND) * DP, i % ND); },
-                                             [&](int i, const TkOp<T> &x) {
-                                                 if (i % ND == 0) {
-                                                     TkFrag<T> f;
-                                                     at_weights(f, s[i / ND / 2], i / ND % 2, l);
-                                                     o = tk_op(f);
-                                                 }
-                                                 acc[i % ND] = tk_mma(x, o, acc[i % ND]);
-                                             });
+            for (int e = 0; e < 8; ++e)
+                if (e >= e0 && e < e1) s[g >> 1][8 * (g & 1) + e] = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][8 * (g & 1) + e], a.scale2, -shift));
+        };
+        const auto pack = [&](int g) {
+            TkFrag<T> f;
+            at_weights(f, s[g >> 1], g & 1, l);
+            return tk_op(f);
+        };
+        weigh(0, 0, 8);
+        TkOp<T> o = pack(0);
+        at_pipe<G * ND, at_ahead<T>(), 4>([&](int i) { return at_col<T, DP, PLANE>(at, V + 16 * (i / ND) * DP, i % ND); },
+                                          [&](int i, const TkOp<T> &x) {
+                                              const int g = i / ND, d = i % ND;
+                                              acc[d] = tk_mma(x, o, acc[d]);
+                                              if (g + 1 < G) {
+                                                  weigh(g + 1, 8 * d / ND, 8 * (d + 1) / ND);
+                                                  if (d == ND - 1) o = pack(g + 1);
+                                              }
+                                          });
     }
     l += at_other_half(l);
     if (!w.valid) continue;
