@@ -237,38 +237,45 @@ __device__ __forceinline__ void at_pipe(L load, U use) {
         __builtin_amdgcn_sched_barrier(FREE);
     }
 }
-// acc(32 rows of the tile x 32 own columns) = tile rows . own fragments; `off`: element offset of the tile's first of these rows
+// acc(32 rows of the tile x 32 own columns) += tile rows . own fragments; `off`: element offset of the tile's first of these rows
 template <typename T, int DP, int PLANE>
-__device__ __forceinline__ tk16 at_product(const AtAddr<DP> &at, int off, const TkOp<T> (&own)[DP / 16]) {
-    tk16 acc = {};
+__device__ __forceinline__ void at_product(tk16 &acc, const AtAddr<DP> &at, int off, const TkOp<T> (&own)[DP / 16]) {
     at_pipe<DP / 16, at_ahead<T>()>([&](int kk) { return at_rows<T, DP, PLANE>(at, off, kk); }, [&](int kk, const TkOp<T> &o) { acc = tk_mma(o, own[kk], acc); });
-    return acc;
 }
 // two independent products, step by step: neither waits for its own last step
 template <typename T, int DP, int PLANE>
 __device__ __forceinline__ void at_product2(tk16 &x, tk16 &y, const AtAddr<DP> &at, int offx, const TkOp<T> (&ox)[DP / 16], int offy, const TkOp<T> (&oy)[DP / 16]) {
-    x = tk16{};
-    y = tk16{};
     at_pipe<DP / 8, at_ahead<T>()>([&](int i) { return at_rows<T, DP, PLANE>(at, i & 1 ? offy : offx, i >> 1); },
                                    [&](int i, const TkOp<T> &o) {
                                        if (i & 1) y = tk_mma(o, oy[i >> 1], y);
                                        else x = tk_mma(o, ox[i >> 1], x);
                                    });
 }
-// acc[dt] += (32 tile rows)^T . w, w being a result over the same rows
-template <typename T, int DP, int PLANE>
-__device__ __forceinline__ void at_accumulate(tk16 (&acc)[DP / 32], const AtAddr<DP> &at, int off, const tk16 &w) {
+// acc[dt] += (32 tile rows)^T . w, w being a result over the same rows.  make(e) brings element e of w about: the second half's between the products of the
+// first.
+template <typename T, int DP, int PLANE, typename M>
+__device__ __forceinline__ void at_accumulate(tk16 (&acc)[DP / 32], const AtAddr<DP> &at, int off, tk16 &w, M make) {
     constexpr int ND = DP / 32;
-    TkOp<T> o[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    const auto pack = [&](int t) {
         TkFrag<T> f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) f.set(j, w[8 * t + j]);
-        o[t] = tk_op(f);
-    }
-    at_pipe<2 * ND, at_ahead<T>()>([&](int i) { return at_col<T, DP, PLANE>(at, off + 16 * (i / ND) * DP, i % ND); },
-                                   [&](int i, const TkOp<T> &x) { acc[i % ND] = tk_mma(x, o[i / ND], acc[i % ND]); });
+        return tk_op(f);
+    };
+#pragma unroll
+    for (int e = 0; e < 8; ++e) make(e);
+    TkOp<T> o = pack(0);
+    at_pipe<2 * ND, at_ahead<T>(), 4>([&](int i) { return at_col<T, DP, PLANE>(at, off + 16 * (i / ND) * DP, i % ND); },
+                                      [&](int i, const TkOp<T> &x) {
+                                          const int d = i % ND;
+                                          acc[d] = tk_mma(x, o, acc[d]);
+                                          if (i < ND) {
+#pragma unroll
+                                              for (int e = 0; e < 8; ++e)
+                                                  if (e >= 8 * d / ND && e < 8 * (d + 1) / ND) make(8 + e);
+                                              if (d == ND - 1) o = pack(1);
+                                          }
+                                      });
 }
 // LDS buffers of the streamed side: two (one barrier a step), one where two would leave room for a single workgroup per CU
 template <typename T, int DP> constexpr int at_buffers() { return sizeof(T) == 4 && DP == 128 ? 1 : 2; }
@@ -430,13 +437,13 @@ __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 4 ? (DP <= 96 ? 2 : 1) 
         __syncthreads();
         if (j + KT < j1) fetch(buf ^ (NB - 1), j + KT);
         if (j >= lim_any) continue;             // none of this wave's rows sees the tile
-        tk16 s[KT / 32];
+        tk16 s[KT / 32] = {};
         AtMask mk[KT / 32];
         if (MASK)
 #pragma unroll
             for (int n = 0; n < KT / 32; ++n) mk[n] = at_mask_row(a, mrow, j + 32 * n, h);
         if constexpr (KT == 64) at_product2<T, DP, PLANE>(s[0], s[1], at, 0, qf, 32 * DP, qf);
-        else s[0] = at_product<T, DP, PLANE>(at, 0, qf);
+        else at_product<T, DP, PLANE>(s[0], at, 0, qf);
         if (j + KT > lim_all) {
             asm volatile("");               // (a branch: the comparisons are not to be made for whole tiles)
 #pragma unroll
@@ -650,19 +657,19 @@ __device__ __forceinline__ void at_dq(const AttnArgs &a, const AtBlock &w0, tkh 
         for (int n = 0; n < KT / 32; ++n) {
             AtMask mk;
             if (MASK) mk = at_mask_row(a, mrow, j + 32 * n, h);
-            tk16 s, dp;
+            tk16 s = {}, dp = {};
             at_product2<T, DP, PLANE>(s, dp, at, 32 * n * DP, qf, V + 32 * n * DP, gf);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse)) * (dp[e] - delta);
             if (!whole) {
                 asm volatile("");           // (a branch: the comparisons are not to be made for whole tiles)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const bool on = j + 32 * n + at_row(e, h) < w.lim && (!MASK || at_mask_on(mk, e));
-                    s[e] = on ? s[e] : 0.f;
+                    s[e] = on ? s[e] : -INFINITY;
+                    dp[e] = on ? dp[e] : 0.f;           // (whatever a hidden value holds)
                 }
             }
-            at_accumulate<T, DP, PLANE>(acc, at, 32 * n * DP, s);
+            at_accumulate<T, DP, PLANE>(acc, at, 32 * n * DP, s,
+                                        [&](int e) { s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse)) * (dp[e] - delta); });
         }
     }
     if (!w.valid) continue;
@@ -717,6 +724,7 @@ __device__ __forceinline__ void at_dkv(const AttnArgs &a, const AtBlock &w0, tkh
     qs.init(a.qs[1], a.Dk, tid);
     gs.init((long long)a.H * a.Dv, a.Dv, tid);
     float nlse = 0.f, ndelta = 0.f;               // row tid of the tile
+    const float unscale = -1.f / a.scale2;
     const int empty = a.causal ? -off : 0;        // queries before it see nothing
     int i_next = 0;
     const auto fetch = [&](int to, int gi, int qt) {
@@ -737,7 +745,7 @@ __device__ __forceinline__ void at_dkv(const AttnArgs &a, const AtBlock &w0, tkh
         const auto dead = [&](int i) { return i_next + AtTile<T, DP, QT>::row(i, tid) < empty || (MASK && flag.f[i] == INFINITY); };
         qs.settle(smem + to * TILE, tid, dead);
         gs.settle(smem + G + to * TILE, tid, dead);
-        if (tid < QT) lses[to][tid] = nlse, deltas[to][tid] = ndelta;
+        if (tid < QT) lses[to][tid] = sizeof(T) == 2 ? nlse * unscale : -nlse, deltas[to][tid] = -ndelta;
     };
     AtAddr<DP> at;
     at.init(smem, lane);
@@ -759,31 +767,42 @@ __device__ __forceinline__ void at_dkv(const AttnArgs &a, const AtBlock &w0, tkh
             if (MASK)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) mk[e] = mcol[min(i0 + 32 * n + at_row(e, h), a.Tq - 1) * a.ms[2]];
-            tk16 s, dp = {};
-            if constexpr (DK) at_product2<T, DP, PLANE>(s, dp, at, 32 * n * DP, kf, G + 32 * n * DP, vf);
-            else s = at_product<T, DP, PLANE>(at, 32 * n * DP, kf);
+            // bf16: the products start at -lse / (scale log2 e) and -D (fp32 would lose bits of s to them)
+            constexpr bool START = sizeof(T) == 2;
+            tk16 s = {}, dp = {};
+            const auto rows4 = [&](const float *x, int e) { return *reinterpret_cast<const tkf4 *>(x + 32 * n + 2 * e + 4 * h); };       // e: a multiple of 4
+            if constexpr (START)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const tkf4 le = *reinterpret_cast<const tkf4 *>(&lses[buf][32 * n + 8 * u + 4 * h]), de = *reinterpret_cast<const tkf4 *>(&deltas[buf][32 * n + 8 * u + 4 * h]);
+                for (int e = 0; e < 16; e += 4) {
+                    const tkf4 le = rows4(lses[buf], e), de = DK ? rows4(deltas[buf], e) : tkf4{};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int e = 4 * u + j;
-                    s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -le[j]));
-                    dp[e] = s[e] * (dp[e] - de[j]);
+                    for (int j = 0; j < 4; ++j) s[e + j] = le[j], dp[e + j] = de[j];
                 }
-            }
+            if constexpr (DK) at_product2<T, DP, PLANE>(s, dp, at, 32 * n * DP, kf, G + 32 * n * DP, vf);
+            else at_product<T, DP, PLANE>(s, at, 32 * n * DP, kf);
+            if constexpr (!START)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const tkf4 le = rows4(lses[buf], e), de = rows4(deltas[buf], e);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[e + j] = fmaf(s[e + j], a.scale2, le[j]), dp[e + j] += de[j];
+                }
             if (!whole) {
                 asm volatile("");           // (a branch: the comparisons are not to be made for whole tiles)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const int i = i0 + 32 * n + at_row(e, h);
                     const bool on = i >= first && i < a.Tq && (!MASK || mk[e]);
-                    s[e] = on ? s[e] : 0.f;
-                    dp[e] = on ? dp[e] : 0.f;
+                    s[e] = on ? s[e] : -INFINITY;
+                    if (DK) dp[e] = on ? dp[e] : 0.f;
                 }
             }
-            if constexpr (DV) at_accumulate<T, DP, PLANE>(accv, at, G + 32 * n * DP, s);
-            if constexpr (DK) at_accumulate<T, DP, PLANE>(acck, at, 32 * n * DP, dp);
+            const auto make = [&](int e) {
+                s[e] = __builtin_amdgcn_exp2f(START ? s[e] * a.scale2 : s[e]);
+                if (DK) dp[e] *= s[e];
+            };
+            if constexpr (DV) at_accumulate<T, DP, PLANE>(accv, at, G + 32 * n * DP, s, make);
+            if constexpr (DK) at_accumulate<T, DP, PLANE>(acck, at, 32 * n * DP, dp, [&](int e) { if (!DV) make(e); });
         }
     }
     if (!valid) continue;
