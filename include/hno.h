@@ -609,10 +609,11 @@ int hno_affine_nearest(const float *x, float *out, const double *matrix12, float
  *
  * hno_attn_fwd: out (B, Tq, H, Dv) = softmax(scale q k^T) v per head over the visible keys; a row without any is zero.
  *   q (B, Tq, H, Dk), k (B, Tk, Hk, Dk), v (B, Tk, Hk, Dv) with element strides of (batch, token, head) and unit stride of the last axis; query head h
- *   reads key head h / (H / Hk).  Head sizes: multiples of 8 up to 128; every row starts on 16 bytes.  With L = kv_lens[b] (clamped to 0 ... Tk; NULL: Tk), key j is visible to query i when
- *   j < L, and j <= i + L - Tq if causal (the last query is aligned with the last key), and mask[b, h, i, j] != 0 (NULL: all; strides of 0 broadcast).
- *   Rows of k and v from L on, and those that a mask without query and head axis hides, are not looked at: they may hold anything.  Value rows that
- *   only some queries may see have to be finite.
+ *   reads key head h / (H / Hk).  Head sizes: multiples of 8 up to 128; every row starts on 16 bytes; token strides below 2^24 elements; scale from
+ *   1e-30 to 1e30.  With L = kv_lens[b] (clamped to 0 ... Tk; NULL: Tk), key j is visible to query i when j < L, and j <= i + L - Tq if causal (the last
+ *   query is aligned with the last key), and mask[b, h, i, j] != 0 (NULL: all; strides of 0 broadcast).
+ *   Rows of k and v from L on, and those that a mask without query and head axis hides, are not looked at: they may hold anything.  Other rows have to
+ *   be finite, also where a mask hides them.  fp32 products are formed from three bf16 terms per value (errors as in fp32; an infinity becomes NaN).
  *   For the backward pass: lse (B, Tq, H) fp32, +inf for an empty row, and out_res (bf16 only), the rounding error of out; both NULL otherwise.
  * hno_attn_bwd: dq, dk, dv (contiguous; dq or both of dk, dv may be NULL) from out, out_res, lse and dout (contiguous). */
 typedef struct hno_attn {
@@ -629,6 +630,7 @@ int hno_attn_bwd(const hno_attn_t *p, const void *out, const void *out_res, cons
                  void *workspace, size_t workspace_bytes, void *stream);
 /* hno_linear_fwd: y (M, N) = act(x w^T + bias) + residual, x (M, K) with row stride ldx, w (N, K); bias (N) of bias_dtype and residual (M, N) may be
  *   NULL.  z (M, N), if not NULL, receives the argument of the activation, which hno_linear_bwd reads (act != NONE).
+ *   fp32 products are formed from three bf16 terms per value (errors as in fp32; an infinity becomes NaN).
  * hno_linear_bwd: dx (M, K), dw (N, K) of dw_dtype, db (N) of db_dtype from dy (M, N); any of them may be NULL.  (The residual's gradient is dy.) */
 size_t hno_linear_workspace_bytes(int dtype, int M, int N, int K, int act, int backward);
 int hno_linear_fwd(int dtype, const void *x, long long ldx, const void *w, const void *bias, int bias_dtype, const void *residual, void *z, void *y, int M,

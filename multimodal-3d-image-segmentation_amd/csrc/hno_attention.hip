@@ -4,9 +4,9 @@
 //   D_i = sum_c do_ic o_ic,  ds_ij = p_ij (do_i . v_j - D_i),  dq = scale ds k,  dk = scale ds^T q,  dv = p^T do
 //
 // Neither p nor ds is written to memory.  The forward pass keeps the running maximum and sum of each row and leaves
-// lse_i = log2 sum_j exp(s_ij); the backward kernels recompute p_ij = 2^(s_ij log2(e) - lse_i).  They are two: one walks the keys for a
-// tile of queries (dq), one walks the queries (of all heads that share the keys) for a tile of keys (dk, dv) -- 7 products where one
-// kernel with atomic sums would need 5, but every sum has one owner and a fixed order, so results do not change from run to run.
+// lse_i = log2 sum_j exp(s_ij); the backward kernel recomputes p_ij = 2^(s_ij log2(e) - lse_i).  Some of its workgroups walk the keys for a
+// tile of queries (dq), others the queries (of all heads that share the keys) for a tile of keys (dk, dv) -- 7 or 8 products where
+// atomic sums would need 5, but every sum has one owner and a fixed order, so results do not change from run to run.
 //
 // A wave owns 32 rows of its side as the COLUMNS of its products (lane & 31): the softmax statistics are then one value per lane, and the
 // registers of a product are the operand of the next (hno_tokens.h).  The other side comes through LDS, row by row as in memory; its
@@ -39,7 +39,7 @@ __device__ __forceinline__ int at_row(int r, int h) { return 8 * (r >> 2) + 4 * 
 
 // Where element d (a multiple of 4) of row `row` stands in an LDS tile of DP channels: rows without padding whose 16-byte chunks change places, so
 // that 16 consecutive rows read at one chunk (row reads) and 4 consecutive rows read at four neighbouring chunks (transposed reads)
-// touch 64 different banks each; with padded rows the transposed reads met 4-way conflicts (dk / dv of 2x16x4096x128: XX us).
+// touch 64 different banks each (measured conflicts: none); with padded rows the transposed reads met 4-way conflicts.
 // DP = 96: a row is 3/4 of the banks, rows shift by themselves and the chunks rotate by row / 4; else an exclusive or.
 template <int DP>
 __device__ __forceinline__ int at_at(int row, int d) {
@@ -107,14 +107,14 @@ __device__ __forceinline__ TkFrag<T> at_load8(const T *row, int d, int D) {
 // Rows from `end` on may hold any row of the tensor: their scores are hidden.  Rows whose flag is set in settle() are zeroed: nobody looks at
 // them, so they may hold NaN, and 0 x NaN must not reach a sum.
 //
-// bf16: LDS-DMA (global_load_lds_dwordx4), which needs no registers: with tiles staged through registers dk / dv of 128 channels took 357 of them and
-// spilled 25 when held to two waves per SIMD.  The DMA writes its slots in lane order, so the slot permutation of at_at is applied to the source.
+// bf16: LDS-DMA (global_load_lds_dwordx4), which needs no registers: with tiles staged through registers dk and dv of 128 channels took 357 of them, and
+// spilled when held to two waves per SIMD.  The DMA writes its slots in lane order, so the slot permutation of at_at is applied to the source.
 template <typename T, int DP, int ROWS>
 struct AtTile;
 template <int DP, int ROWS>
 struct AtTile<tkh, DP, ROWS> {
     static constexpr int CH = DP / 8, N = ROWS * CH / (64 * AT_WAVES);
-    static_assert(ROWS * CH % (64 * AT_WAVES) == 0, "whole slots per thread");    
+    static_assert(ROWS * CH % (64 * AT_WAVES) == 0, "whole slots per thread");
     unsigned off[N];          // byte offset of the slot's source from the tile's first row
     long long st;
     int D;
@@ -383,6 +383,10 @@ __device__ __forceinline__ void at_weights(TkFrag<float> &f, const tk16 &s, int 
     }
 }
 
+// Per tile of 32 rows x 32 keys: D / 8 matrix instructions (fp32: six times as many) and about 100 vector ones, the exponentials among them at a quarter of the
+// rate; both are bounds.  bf16 2x8x8192x64: 258 us = 1065 TFLOP/s (matrix pipes 34 % busy, vector pipes 50 %), causal 2x16x4096x128: 172 us = 800 TFLOP/s
+// of what is visible (39 % and 38 %, two waves a SIMD); fp32 4x1960x96: 53 us = 111 TFLOP/s.  New tokens against a long cache: bound by reading it
+// (4 tokens, 16 heads over 6000 keys of 128 channels: 16 us).
 template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 4 ? (DP <= 96 ? 2 : 1) : (DP <= 64 ? 3 : 2)) void attn_fwd_kernel(AttnArgs a) {
     constexpr int KT = at_tile<T>(), PLANE = KT * DP, NB = at_buffers<T, DP>();
@@ -819,7 +823,10 @@ __device__ __forceinline__ void at_dkv(const AttnArgs &a, const AtBlock &w0, tkh
 }
 
 // The three gradients in one launch: the runs of workgroups stand one behind the other in the grid, each padded to whole rounds of the XCDs, dk and dq
-// (three products) before dv (two).  dk and dv are one workgroup's work where the registers of both leave two waves per SIMD, else two's.
+// (three products) before dv (two).  dk and dv are one workgroup's work where the registers of both leave two waves per SIMD (bf16 up to 64 channels) or one wave
+// is all there is anyway (fp32), else two's.  Two waves with a few spilled registers are better than one with none: masked, 128 channels, 320 us against 379.
+// bf16 causal 2x16x4096x128 (4 key heads): 653 us, 840 TFLOP/s of the 8 products it forms, 525 of the 5 that the gradients need; matrix pipes 46 % busy, vector
+// pipes 33 %.  fp32 4x1960x96: 145 us.
 template <typename T, int DP> constexpr bool at_joint() { return sizeof(T) == 4 || DP <= 64; }
 template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_bwd_kernel(AttnArgs aq, AttnArgs ak, int nq, int nk) {
@@ -872,9 +879,9 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(AtSum a) {
 
 using namespace hno;
 
-// how many runs the streamed side is cut into: two workgroups per CU, no run shorter than `least` tiles; where that is not to be had, one per CU and runs of two tiles.
-// The backward kernel holds three gradients' workgroups: with 16 tiles at least, causal 2x16x4096x128 takes 725 us in runs of four and 815 in runs of two, while 3x6x777x1033x80 takes
-// 79 us with one workgroup per CU and gradient (135 with two, in launches of their own).
+// how many runs the streamed side is cut into: two workgroups per CU, no run shorter than `least` tiles; where that is not to be had, one per CU and runs of
+// two tiles.  The backward kernel holds three gradients' workgroups: causal 2x16x4096x128 takes 12 % longer in runs of two than in the four that this rule gives,
+// while 3x6x777x1033x80 takes 69 us with one workgroup per CU and gradient (135 with two, in launches of their own).
 static int at_splits(long long groups, long long steps, int least) {
     if (groups < 1) return 1;                                  // no keys at all
     long long n = groups >= 512 ? 1 : (512 + groups - 1) / groups;
@@ -899,7 +906,7 @@ static AtPlan at_plan(const hno_attn_t *p, bool backward) {
     n.k_pair = p->causal && k * n.k_tiles <= 1024;
     q *= n.q_pair ? (n.q_tiles + 1) / 2 : n.q_tiles;
     k *= n.k_pair ? (n.k_tiles + 1) / 2 : n.k_tiles;
-    // (a few new tokens: all the chip's loads at once, 4x1x16x128 against 6000 keys 17.9 us in 32 runs, 21 in 16)
+    // (a few new tokens: all the chip's loads at once, 4x1x16x128 against 6000 keys 16 us in 32 runs, a sixth more in 16)
     const int q_least = backward || n.q_tiles > 1 ? 16 : 2;
     n.q_split = at_splits(q, ceil_div(p->Tk, KT), q_least);
     n.k_split = at_splits(k, (long long)ceil_div(p->Tq, KT) * grp, 16);

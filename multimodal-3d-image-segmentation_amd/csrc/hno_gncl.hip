@@ -7,6 +7,8 @@
 // sums of a run of rows go to a slab, and one workgroup per group joins the slabs in a fixed order.
 // Statistics: each thread sums x - p and (x - p)^2 with p the first row's value of its channel, so a channel far from zero loses nothing; the runs'
 // (count, mean, M2) are joined pairwise in 64 bits.
+// Bound by memory: 2 x 491520 x 64 bf16 (126 MB a tensor), elu: statistics 24 us, result 43, backward sums 51, gradient 62 (5.2, 5.8, 4.9 and 6.1 TB/s, some of it from the
+// last-level cache; walking the rows backwards in the second passes, to find more there, changed nothing), joins 6 and 8.  65^3 x 24 fp32 forward 7 + 5 + 13 us.
 #include "hno_tokens.h"
 
 #include <type_traits>
@@ -300,7 +302,8 @@ __global__ __launch_bounds__(256) void gncl_bwd_apply_kernel(GnArgs a) {
 // ------------------------------------------------------------------ small groups: one launch
 // A workgroup owns one group of one sample and keeps it in registers: x is read once, the statistics are those of the kept values (mean first, then squared
 // distances), and the backward pass needs no second launch but the sum over samples of dgamma, dbeta.  Threads: chunk (of W channels) x row; a thread keeps gn_keep
-// rows.  2 x 960 x 256 in 32 groups: forward 20 -> 10 us, backward 31 -> 15 us of kernels.
+// rows.  2 x 960 x 256 bf16 in 32 groups: forward 10.6 us of kernels (in three launches 20), backward 13.3 (31); what is left are the latencies of a launch, a
+// load, two or three sums over the workgroup and a store.
 constexpr int GN_THREADS = 1024;
 template <typename T, int W, bool BWD> constexpr int gn_keep() { return BWD && sizeof(T) == 4 && W == 8 ? 4 : 8; }       // (128 registers a thread)
 template <typename T, int W, bool BWD> inline bool gn_small(long long V, int cpg) {
@@ -467,7 +470,8 @@ static GnPlan gn_plan(int dtype, int B, long long V, int C, bool vec) {
     p.chunks = C / p.W;
     p.cw = p.chunks < 256 ? p.chunks : 256;
     p.yblocks = ceil_div(p.chunks, p.cw);
-    // (four workgroups a CU: 2 x 491520 x 64 bf16 forward and backward 195 us of kernels, with eight 205, with two 229: the loads of two rows a thread no longer hide)
+    // (four workgroups a CU: 2 x 491520 x 64 bf16 forward and backward 195 us of kernels; with eight 205, the joins have more runs to read; with two 229, too few
+    // loads are on their way)
     const long long nrl = 256 / p.cw, most = 1024 / ((long long)B * p.yblocks) > 1 ? 1024 / ((long long)B * p.yblocks) : 1;
     long long runs = (V + 4 * nrl - 1) / (4 * nrl);            // four rows per thread at least
     if (runs > most) runs = most;

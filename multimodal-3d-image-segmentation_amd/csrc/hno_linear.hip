@@ -171,6 +171,9 @@ __device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float 
 }
 
 // DMA: two LDS buffers, the next step's tiles on their way while this one is multiplied.  Else the next step's tiles wait in registers: one buffer.
+// Bound by the matrix pipes: 8192 x 8192 x 2048 bf16 238 us = 1155 TFLOP/s (the library's product 222), with residual 257, with gelu 257, with bias, gelu and residual
+// 285 (LnMid: 330) -- the epilogue of a tile waits for its products, one workgroup a CU.  fp32 (six bf16 products each): 2000 x 512 x 512 27 us.  4 x 2048 x 2048:
+// 6 us and 4 for the join, both near an empty launch.
 template <typename T, bool AX, bool BX, typename C, bool DMA, int ACT>
 __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a) {
     constexpr int TM = C::TM, TN = C::TN, KB = C::KB, P = tk_planes<T>(), WM = C::WM, WN = C::WN, NT = 64 * ln_waves<C>(), NB = DMA ? 2 : 1;
@@ -391,10 +394,11 @@ __global__ __launch_bounds__(1024) void linear_db_kernel(const float *__restrict
 
 using namespace hno;
 
-// Tile, and runs of the contraction.  LnBig (8192 x 8192 x 8192: 994 TFLOP/s, LnMid 898) where its tiles fill most of the 256 CUs by themselves and DMA can feed it.
-// Else 128 x 128 tiles, whose contraction is cut into n runs where that is expected to be quicker: a step takes a workgroup 0.65 us (fp32: 2.5) while there are places for all
-// (two a CU), the slabs cost 2.5 us for the second launch, 0.12 us each and 0.65 us per megabyte.  Measured with these: 3920 x 384 x 1536 bf16 n = 1: 17.6 us (2: 22.9, 5: 24.5),
-// 1536 x 384 x 3920 n = 5: 22.9 (1: 55, 12: 25), 300 x 300 x 4000 n = 8: 13.8 (1: 36, 24: 17.9), 771 x 387 x 3001 fp32 n = 16: 33.5 (1: 239, 32: 40).
+// Tile, and runs of the contraction.  LnBig (8192 x 8192 x 8192 bf16: 1238 TFLOP/s, LnMid 1034) where its tiles fill most of the 256 CUs by themselves and DMA can
+// feed it.  Else 128 x 128 tiles, whose contraction is cut into n runs where that is expected to be quicker: a step takes a workgroup 0.65 us (fp32: 2.5) while
+// there are places for all (two a CU), the slabs cost 2.5 us for the second launch, 0.12 us each and 0.65 us per megabyte.  Measured with these:
+// 3920 x 384 x 1536 bf16 n = 1: 17.2 us (2: 22.5, 4: 24.1), 1536 x 384 x 3920 n = 5: 22.9 (1: 55, 12: 25), 300 x 300 x 4000 n = 8: 13.8 (1: 36, 24: 17.9),
+// fp32 771 x 387 x 3001 n = 16: 32.5 (1: 240, 8: 41), 3001 x 387 x 771 n = 5: 32.1 (1: 66, 12: 48), 4096 x 1024 x 256 n = 1: 21.1 (2: 32.8).
 struct LnPlan {
     bool big;
     int nsplit;

@@ -95,9 +95,8 @@ def _ws(nbytes, device):
 
 # ----------------------------------------------------------------------------------------------- attention
 def _heads(t, esize):
-    """a (B, T, H, D) operand as the kernels take it: unit stride along D, D a multiple of 8, rows 16-byte aligned and
-    less than 2^24 elements apart -- the tensor itself where it is so,
-    else a copy padded with zeros (which change no score; padded channels of the result are cut off)"""
+    """a (B, T, H, D) operand as the kernels take it: unit stride along D, D a multiple of 8, rows 16-byte aligned and less than 2^24 elements apart --
+    the tensor itself where it is so, else a copy padded with zeros (which change no score; padded channels of the result are cut off)"""
     D, step = t.shape[3], 16 // esize
     if D % 8 == 0 and (t.stride(3) == 1) and t.data_ptr() % 16 == 0 and all(s % step == 0 for s in t.stride()[:3]) and t.stride(1) < 1 << 24:
         return t
@@ -174,8 +173,9 @@ def attention(q, k, v, *, causal=False, mask=None, kv_lens=None, scale=None):
     Visible to query i are the keys j < L with L = ``kv_lens[b]`` (integers (B,) on the device, clamped to 0 ... Tk; default Tk);
     with ``causal`` those with j <= i + L - Tq (the last query is aligned with the last key);
     with ``mask`` (bool, broadcastable to (B, H, Tq, Tk)) those that it marks True.  A query that sees no key gives zeros and has no gradient.
-    Keys and values from L on, and those that a mask of shape (B, 1, 1, Tk) hides, may hold anything (inf, NaN); a value that some
-    queries see and others do not has to be finite.  Additive (floating) masks are refused.
+    Keys and values from L on, and those that a mask of shape (B, 1, 1, Tk) hides, may hold anything (inf, NaN); all others have to be finite, also
+    where a mask hides them.  Additive (floating) masks are refused.  fp32 products are formed from three bf16 terms per value, so an
+    infinity comes out as NaN.
     Differentiable in q, k, v; the probabilities are recomputed in the backward pass, memory grows with Tq + Tk only."""
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError('attention: q, k, v must be (batch, tokens, heads, channels)')
@@ -368,7 +368,8 @@ class GroupNormClFn(torch.autograd.Function):
 def group_norm(x, num_groups, weight=None, bias=None, *, eps=1e-5, act=None):
     """act(gamma (x - mean) / sqrt(var + eps) + beta) on channels-last x (B, ..., C), fp32 or bf16, statistics per sample and group of
     C / num_groups neighbouring channels over all positions; weight, bias (C,) fp32 or x's type.  ``act``: see ``act_id``.
-    Statistics are joined in 64 bits.  Differentiable in x, weight, bias; the backward pass keeps x and the statistics."""
+    Statistics are sums of differences from a value of the group, in fp32 and, over more than a few thousand values, joined in 64 bits.  Differentiable in x,
+    weight, bias; the backward pass keeps x and the statistics."""
     a = act_id(act)
     num_groups, eps = int(num_groups), float(eps)
     if x.ndim < 2:
