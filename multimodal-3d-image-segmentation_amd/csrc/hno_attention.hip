@@ -384,8 +384,8 @@ __device__ __forceinline__ void at_weights(TkFrag<float> &f, const tk16 &s, int 
 }
 
 // Per tile of 32 rows x 32 keys: D / 8 matrix instructions (fp32: six times as many) and about 100 vector ones, the exponentials among them at a quarter of the
-// rate; both are bounds.  bf16 2x8x8192x64: 258 us = 1065 TFLOP/s (matrix pipes 34 % busy, vector pipes 50 %), causal 2x16x4096x128: 172 us = 800 TFLOP/s
-// of what is visible (39 % and 38 %, two waves a SIMD); fp32 4x1960x96: 53 us = 111 TFLOP/s.  New tokens against a long cache: bound by reading it
+// rate; both are bounds.  bf16 2x8x8192x64: 258 us = 1065 TFLOP/s (matrix pipes 38 % busy, vector pipes 54 %), causal 2x16x4096x128: 172 us = 800 TFLOP/s
+// of what is visible (41 % and 38 %, two waves a SIMD); fp32 4x1960x96: 46 us = 128 TFLOP/s.  New tokens against a long cache: bound by reading it
 // (4 tokens, 16 heads over 6000 keys of 128 channels: 16 us).
 template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 4 ? (DP <= 96 ? 2 : 1) : (DP <= 64 ? 3 : 2)) void attn_fwd_kernel(AttnArgs a) {
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const float *__restrict_
                                                         T *__restrict__ outres, float *__restrict__ lse, long long rows, int Dv, int nsplit) {
     __shared__ tkf4 sum[8][32];
     __shared__ float wsum[8][32], top[8][32];
-    const int c = threadIdx.x & 31, y = threadIdx.x >> 5, ys = nsplit >= 8 ? 8 : 1, s0 = ys > 1 ? y : 0;
+    const int c = threadIdx.x & 31, y = threadIdx.x >> 5, ys = nsplit > 8 ? 8 : 1, s0 = ys > 1 ? y : 0;
     const long long row = ys > 1 ? blockIdx.x : (long long)blockIdx.x * 8 + y;
     const bool on = row < rows, in = on && 4 * c < Dv;
     float ms[8], ls[8], m = -INFINITY, l = 0.f;
@@ -825,8 +825,8 @@ __device__ __forceinline__ void at_dkv(const AttnArgs &a, const AtBlock &w0, tkh
 // The three gradients in one launch: the runs of workgroups stand one behind the other in the grid, each padded to whole rounds of the XCDs, dk and dq
 // (three products) before dv (two).  dk and dv are one workgroup's work where the registers of both leave two waves per SIMD (bf16 up to 64 channels) or one wave
 // is all there is anyway (fp32), else two's.  Two waves with a few spilled registers are better than one with none: masked, 128 channels, 320 us against 379.
-// bf16 causal 2x16x4096x128 (4 key heads): 653 us, 840 TFLOP/s of the 8 products it forms, 525 of the 5 that the gradients need; matrix pipes 46 % busy, vector
-// pipes 33 %.  fp32 4x1960x96: 145 us.
+// bf16 causal 2x16x4096x128 (4 key heads): 653 us, 840 TFLOP/s of the 8 products it forms, 525 of the 5 that the gradients need; matrix pipes 47 % busy, vector
+// pipes 34 %.  fp32 4x1960x96: 145 us.
 template <typename T, int DP> constexpr bool at_joint() { return sizeof(T) == 4 || DP <= 64; }
 template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 2 ? 2 : 1) void attn_bwd_kernel(AttnArgs aq, AttnArgs ak, int nq, int nk) {
@@ -906,8 +906,10 @@ static AtPlan at_plan(const hno_attn_t *p, bool backward) {
     n.k_pair = p->causal && k * n.k_tiles <= 1024;
     q *= n.q_pair ? (n.q_tiles + 1) / 2 : n.q_tiles;
     k *= n.k_pair ? (n.k_tiles + 1) / 2 : n.k_tiles;
-    // (a few new tokens: all the chip's loads at once, 4x1x16x128 against 6000 keys 16 us in 32 runs, a sixth more in 16)
-    const int q_least = backward || n.q_tiles > 1 ? 16 : 2;
+    // Forward: a few new tokens want all the chip's loads at once (4x1x16x128 against 6000 keys 16 us in 32 runs, a sixth more in 16); a tile of fp32 is so much work
+    // that a second workgroup per CU is worth more slabs (4x1960x96: 8 runs 46 + 5.6 us with the join, 4 runs 54 + 4.4), one of bf16 is not
+    // (causal 4x4096x128, 1 key head: 8 runs 38.5 + 12.8, 4 runs 43 + 7.8)
+    const int q_least = backward ? 16 : (n.q_tiles == 1 ? 2 : (p->dtype == HNO_F32 ? 6 : 16));
     n.q_split = at_splits(q, ceil_div(p->Tk, KT), q_least);
     n.k_split = at_splits(k, (long long)ceil_div(p->Tq, KT) * grp, 16);
     n.q_blocks = q * n.q_split;
@@ -980,7 +982,7 @@ static int at_forward(const hno_attn_t *p, void *out, void *out_res, float *lse,
     AT_DISPATCH(attn_fwd_kernel, n.q_blocks, a);
     HNO_CHECK_LAUNCH();
     if (n.q_split > 1) {
-        hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)(n.q_split >= 8 ? rows : (rows + 7) / 8)), dim3(256), 0, s, (const float *)a.part, (const float *)a.part2,
+        hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)(n.q_split > 8 ? rows : (rows + 7) / 8)), dim3(256), 0, s, (const float *)a.part, (const float *)a.part2,
                            (T *)out, (T *)out_res, lse, rows, p->Dv, n.q_split);
         HNO_CHECK_LAUNCH();
     }
