@@ -386,7 +386,7 @@ __device__ __forceinline__ void at_weights(TkFrag<float> &f, const tk16 &s, int 
 // Per tile of 32 rows x 32 keys: D / 8 matrix instructions (fp32: six times as many) and about 100 vector ones, the exponentials among them at a quarter of the
 // rate; both are bounds.  bf16 2x8x8192x64: 258 us = 1065 TFLOP/s (matrix pipes 38 % busy, vector pipes 54 %), causal 2x16x4096x128: 172 us = 800 TFLOP/s
 // of what is visible (41 % and 38 %, two waves a SIMD); fp32 4x1960x96: 46 us = 128 TFLOP/s.  New tokens against a long cache: bound by reading it
-// (4 tokens, 16 heads over 6000 keys of 128 channels: 16 us).
+// (4 sequences of about 6000 keys, 4 key heads of 128 channels: 16 us, and 4 for the join).
 template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(64 * AT_WAVES, sizeof(T) == 4 ? (DP <= 96 ? 2 : 1) : (DP <= 64 ? 3 : 2)) void attn_fwd_kernel(AttnArgs a) {
     constexpr int KT = at_tile<T>(), PLANE = KT * DP, NB = at_buffers<T, DP>();
