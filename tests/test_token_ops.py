@@ -607,6 +607,32 @@ def test_capture_with_a_live_eager_graph_is_refused(ot):
         assert torch.equal(w.grad, want)
 
 
+@pytest.mark.gpu
+def test_weight_gradients_reach_registered_destinations(ot):
+    """an fp32 weight's gradient is written where the data-parallel replica wants it; a weight that is used twice gets the sum"""
+    import multimodal_3d_image_segmentation_amd as pkg
+    x = rand((2, 30, 16), torch.bfloat16, 1)
+    w, u = (rand((16, 16), torch.float32, n).requires_grad_(True) for n in (2, 3))
+
+    def grads():
+        w.grad = u.grad = None
+        y = ot.linear(ot.linear(ot.linear(x, w, act='gelu'), u), w)
+        y.backward(rand(y.shape, y.dtype, 4))
+        return w.grad, u.grad
+    want = [g.clone() for g in grads()]
+    flat = torch.full((512,), 7.0, device='cuda')
+    old = pkg.ops.set_grad_destinations({w: flat[:256].view(16, 16), u: flat[256:].view(16, 16)})
+    try:
+        for _ in range(2):
+            pkg.ops.new_grad_pass()
+            got = grads()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            assert got[1].data_ptr() == flat[256:].data_ptr()
+    finally:
+        pkg.ops.set_grad_destinations(None)
+        pkg.ops._grad_dest = old
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
 def test_attention_refusals(ot):
     t = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype)  # noqa: E731
