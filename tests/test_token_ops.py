@@ -113,6 +113,34 @@ def test_attention_sizes(ot, B, Tq, Tk, H, Hk, Dk, Dv, causal, dtype):
     check_attention(ot, q, k, v, causal=causal)
 
 
+# packed heads over several tiles; runs of a long axis on either side, few and many; a long causal triangle; one query of many heads
+ATTENTION_RUNS = [(1, 100, 260, 8, 2, 64, 64, True), (2, 127, 130, 3, 1, 128, 128, False), (1, 2100, 70, 2, 2, 64, 64, False), (1, 300, 5000, 2, 1, 96, 96, False),
+                  (1, 1100, 1300, 2, 1, 32, 32, True), (1, 1500, 900, 2, 2, 128, 128, True), (2, 1, 3000, 16, 2, 80, 80, False), (1, 4, 9000, 4, 4, 32, 32, True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('B,Tq,Tk,H,Hk,Dk,Dv,causal', ATTENTION_RUNS)
+def test_attention_runs(ot, B, Tq, Tk, H, Hk, Dk, Dv, causal, dtype):
+    q, k, v = rand((B, Tq, H, Dk), dtype, 31), rand((B, Tk, Hk, Dk), dtype, 32), rand((B, Tk, Hk, Dv), dtype, 33)
+    check_attention(ot, q, k, v, causal=causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('causal', [False, True])
+@pytest.mark.parametrize('D', [32, 96, 128])
+def test_attention_mask_lengths_and_causal_together(ot, D, causal, dtype):
+    B, Tq, Tk, H, Hk = 3, 140, 230, 4, 2
+    q, k, v = rand((B, Tq, H, D), dtype, 34), rand((B, Tk, Hk, D), dtype, 35), rand((B, Tk, Hk, D), dtype, 36)
+    gen = torch.Generator().manual_seed(37)
+    mask = (torch.rand((B, H, Tq, Tk), generator=gen) < 0.6).cuda()
+    mask[1, :, 20:90] = False                                           # rows that see nothing
+    lens = torch.tensor([230, 97, 0], device='cuda', dtype=torch.int32)
+    check_attention(ot, q, k, v, causal=causal, mask=mask, kv_lens=lens)
+    check_attention(ot, q, k, v, causal=causal, mask=mask[:, :1, :1], kv_lens=lens)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 @pytest.mark.parametrize('causal', [False, True])
@@ -274,6 +302,14 @@ def test_linear_sizes(ot, M, N, K, dtype):
     x, w = rand((M, K), dtype, 1), rand((N, K), dtype, 2, 1.0 / math.sqrt(K))
     check_linear(ot, x, w, rand((N,), dtype, 3), rand((M, N), dtype, 4), 'gelu')
     check_linear(ot, x, w, None, None, None)
+
+
+# results of hundreds of large tiles in the forward product, in dx and in dw; rows and columns that end inside a tile, contractions that end inside a step
+@pytest.mark.gpu
+@pytest.mark.parametrize('M,N,K', [(3500, 3592, 72), (3600, 40, 3592), (40, 3592, 3608), (3500, 3590, 200), (3500, 3592, 65)])
+def test_linear_large_tiles(ot, M, N, K):
+    x, w = rand((M, K), torch.bfloat16, 21), rand((N, K), torch.bfloat16, 22, 1.0 / math.sqrt(K))
+    check_linear(ot, x, w, rand((N,), torch.bfloat16, 23), rand((M, N), torch.bfloat16, 24), 'silu')
 
 
 @pytest.mark.gpu
