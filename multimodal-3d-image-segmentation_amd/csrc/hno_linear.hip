@@ -172,8 +172,7 @@ __device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float 
 
 // DMA: two LDS buffers, the next step's tiles on their way while this one is multiplied.  Else the next step's tiles wait in registers: one buffer.
 // Bound by the matrix pipes: 8192 x 8192 x 2048 bf16 238 us = 1155 TFLOP/s (the library's product 222), with residual 257, with gelu 257, with bias, gelu and residual
-// 285 (LnMid: 330) -- the epilogue of a tile waits for its products, one workgroup a CU.  fp32 (six bf16 products each): 2000 x 512 x 512 27 us.  4 x 2048 x 2048:
-// 6 us and 4 for the join, both near an empty launch.
+// 285 (LnMid: 330) -- the epilogue of a tile waits for its products, one workgroup a CU.  fp32 (six bf16 products each): 2000 x 512 x 512 27 us. 
 template <typename T, bool AX, bool BX, typename C, bool DMA, int ACT>
 __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a) {
     constexpr int TM = C::TM, TN = C::TN, KB = C::KB, P = tk_planes<T>(), WM = C::WM, WN = C::WN, NT = 64 * ln_waves<C>(), NB = DMA ? 2 : 1;
@@ -336,6 +335,64 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a) {
     }
 }
 
+// Up to four rows: bound by reading the weight once, so no tiles.  A workgroup owns two columns, its lanes walk the contraction 8 elements at a time, every
+// product and sum in fp32; the lanes' sums meet in shuffles, the waves' in LDS; one launch.  bf16 4 x 2048 x 2048: 5.0 us (tiles in 32 runs 10.3), 4 x 16384 x 8192: 60 us =
+// 4.5 TB/s (72), one row 43 us = 6.2 TB/s (72, the weight partly from the last-level cache).  Eight rows are quicker in tiles (8 x 8192 x 2048: 12.0 us, 30.8 here: every
+// workgroup reads all of x).
+constexpr int LN_ROWS = 4, LN_COLS = 2;
+__device__ __forceinline__ float ln_dot8(const TkFrag<tkh> &x, const TkFrag<tkh> &w, float s) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) s = __builtin_amdgcn_fdot2_f32_bf16(b2{x.v[j], x.v[j + 1]}, b2{w.v[j], w.v[j + 1]}, s, false);
+    return s;
+}
+__device__ __forceinline__ float ln_dot8(const TkFrag<float> &x, const TkFrag<float> &w, float s) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(x.v[j], w.v[j], s);
+    return s;
+}
+template <typename T, int MR>
+__global__ __launch_bounds__(256) void linear_rows_kernel(LinArgs a) {
+    __shared__ float part[4][MR * LN_COLS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n0 = blockIdx.x * LN_COLS;
+    const T *x = (const T *)a.A, *w = (const T *)a.B;
+    constexpr int V = MR * LN_COLS;
+    float acc[V] = {};
+#pragma unroll 2
+    for (int k = 8 * tid; k < a.K; k += 8 * 256) {
+        const int cnt = a.K - k;
+        TkFrag<T> fw[LN_COLS], fx[MR];
+#pragma unroll
+        for (int c = 0; c < LN_COLS; ++c) fw[c] = ln_raw8(w + (long long)min(n0 + c, a.N - 1) * a.ldb + k, cnt);
+#pragma unroll
+        for (int m = 0; m < MR; ++m) fx[m] = ln_raw8(x + min(m, a.M - 1) * a.lda + k, cnt);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = ln_dot8(fx[i / LN_COLS], fw[i % LN_COLS], acc[i]);
+    }
+    // in each exchange a lane hands over the half of its sums that its partner keeps
+    int step = 32;
+#pragma unroll
+    for (int h = V / 2; h; h >>= 1, step >>= 1)
+#pragma unroll
+        for (int i = 0; i < h; ++i) {
+            const bool up = lane & step;
+            acc[i] = (up ? acc[i + h] : acc[i]) + __shfl_xor(up ? acc[i] : acc[i + h], step);
+        }
+    const int left = 2 * step;                          // lanes that hold the same sum
+    for (; step; step >>= 1) acc[0] += __shfl_xor(acc[0], step);
+    if ((lane & (left - 1)) == 0) part[wave][lane / left] = acc[0];
+    __syncthreads();
+    const int m = tid / LN_COLS, n = n0 + tid % LN_COLS;
+    if (m >= a.M || n >= a.N) return;
+    const long long at = (long long)m * a.N + n;
+    float z = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+    if (a.bias) z += a.bias32 ? ((const float *)a.bias)[n] : tk_up(((const T *)a.bias)[n]);
+    if (a.z && a.act != HNO_ACT_NONE) ((T *)a.z)[at] = tk_down<T>(z);
+    float y = tk_act(z, a.act);
+    if (a.res) y += tk_up(((const T *)a.res)[at]);
+    ((T *)a.y)[at] = tk_down<T>(y);
+}
+
 // dz = dy act'(z) and the column sums of dz: a workgroup owns 256 columns (32 lanes of 8) of a run of rows and leaves one slab row per run; single columns a lane
 // took 16 us for 3920 x 1536 bf16 instead of 11.  dz == nullptr: act is none, dz is dy itself and only the sums are wanted.
 template <typename T, int ACT>
@@ -466,13 +523,25 @@ static size_t ln_slab(int M, int N, int K, bool f32) {
 extern "C" size_t hno_linear_workspace_bytes(int dtype, int M, int N, int K, int act, int backward) {
     if (ln_check("hno_linear_workspace_bytes", dtype, M, N, K, act)) return 0;
     const bool f32 = dtype == HNO_F32;
-    if (!backward) return ln_slab(M, N, K, f32);
+    if (!backward) return M <= LN_ROWS ? 0 : ln_slab(M, N, K, f32);
     const size_t dx = ln_slab(M, K, N, f32), dw = ln_slab(N, K, M, f32), dz = act == HNO_ACT_NONE ? 0 : (size_t)M * N * (dtype == HNO_BF16 ? 2 : 4);
     return ln_pad(dz) + ln_pad((size_t)ln_runs(M) * N * sizeof(float)) + (dx > dw ? dx : dw);
 }
 
 template <typename T>
+static int ln_rows(const LinArgs &a, hipStream_t s) {
+    ProfScope _ps(KID_LINEAR, s, sizeof(T) * ((double)a.M * a.K + (double)a.N * a.K + (double)a.M * a.N));
+    const dim3 grid(ceil_div(a.N, LN_COLS));
+    if (grid.x >= 1u << 24) return fail(HNO_ELIMIT, "hno_linear: %d columns exceed the grid", a.N);
+    if (a.M == 1) hipLaunchKernelGGL((linear_rows_kernel<T, 1>), grid, dim3(256), 0, s, a);
+    else if (a.M == 2) hipLaunchKernelGGL((linear_rows_kernel<T, 2>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((linear_rows_kernel<T, 4>), grid, dim3(256), 0, s, a);
+    HNO_CHECK_LAUNCH();
+    return HNO_OK;
+}
+template <typename T>
 static int ln_forward(const LinArgs &a, hipStream_t s) {
+    if (a.M <= LN_ROWS) return ln_rows<T>(a, s);
     switch (a.act) {
         case HNO_ACT_SELU: return ln_product<T, false, false, HNO_ACT_SELU>(a, s);
         case HNO_ACT_ELU: return ln_product<T, false, false, HNO_ACT_ELU>(a, s);
