@@ -172,7 +172,7 @@ __device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float 
 
 // DMA: two LDS buffers, the next step's tiles on their way while this one is multiplied.  Else the next step's tiles wait in registers: one buffer.
 // Bound by the matrix pipes: 8192 x 8192 x 2048 bf16 238 us = 1155 TFLOP/s (the library's product 222), with residual 257, with gelu 257, with bias, gelu and residual
-// 285 (LnMid: 330) -- the epilogue of a tile waits for its products, one workgroup a CU.  fp32 (six bf16 products each): 2000 x 512 x 512 27 us. 
+// 285 (LnMid: 330) -- the epilogue of a tile waits for its products, one workgroup a CU.  fp32 (six bf16 products each): 2000 x 512 x 512 27 us.
 template <typename T, bool AX, bool BX, typename C, bool DMA, int ACT>
 __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a) {
     constexpr int TM = C::TM, TN = C::TN, KB = C::KB, P = tk_planes<T>(), WM = C::WM, WN = C::WN, NT = 64 * ln_waves<C>(), NB = DMA ? 2 : 1;

@@ -98,7 +98,8 @@ def _heads(t, esize):
     """a (B, T, H, D) operand as the kernels take it: unit stride along D, D a multiple of 8, rows 16-byte aligned and less than 2^24 elements apart --
     the tensor itself where it is so, else a copy padded with zeros (which change no score; padded channels of the result are cut off)"""
     D, step = t.shape[3], 16 // esize
-    if D % 8 == 0 and (t.stride(3) == 1) and t.data_ptr() % 16 == 0 and all(s % step == 0 for s in t.stride()[:3]) and t.stride(1) < 1 << 24:
+    sb, st, sh, sd = t.stride()
+    if not (D % 8 or sd != 1 or t.data_ptr() % 16 or sb % step or st % step or sh % step or st >= 1 << 24):
         return t
     if D % 8 == 0:
         return t.clone(memory_format=torch.contiguous_format)
@@ -367,7 +368,7 @@ class GroupNormClFn(torch.autograd.Function):
 
 def group_norm(x, num_groups, weight=None, bias=None, *, eps=1e-5, act=None):
     """act(gamma (x - mean) / sqrt(var + eps) + beta) on channels-last x (B, ..., C), fp32 or bf16, statistics per sample and group of
-    C / num_groups neighbouring channels over all positions; weight, bias (C,) fp32 or x's type.  ``act``: see ``act_id``.
+    C / num_groups neighbouring channels over all positions; weight, bias (C,) fp32 or x's type; at most 65535 samples.  ``act``: see ``act_id``.
     Statistics are sums of differences from a value of the group, in fp32 and, over more than a few thousand values, joined in 64 bits.  Differentiable in x,
     weight, bias; the backward pass keeps x and the statistics."""
     a = act_id(act)
