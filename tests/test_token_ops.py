@@ -669,6 +669,29 @@ def test_weight_gradients_reach_registered_destinations(ot):
         pkg.ops._grad_dest = old
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_empty_batches(ot, dtype):
+    """no sample, no token: empty results, and parameters whose gradients are zero"""
+    p = lambda *s: torch.randn(s, device='cuda', dtype=dtype).requires_grad_(True)  # noqa: E731
+    for B, Tq in ((0, 5), (2, 0)):
+        q, k, v = p(B, Tq, 4, 16), p(B, 7, 2, 16), p(B, 7, 2, 24)
+        y = ot.attention(q, k, v, causal=True)
+        assert y.shape == (B, Tq, 4, 24)
+        for t, g in zip((q, k, v), torch.autograd.grad(y, (q, k, v), torch.ones_like(y))):
+            assert g.shape == t.shape and (g == 0).all()
+        x, w, b = p(B, Tq, 16), p(8, 16), p(8)
+        y = ot.linear(x, w, b, act='silu', residual=p(B, Tq, 8))
+        assert y.shape == (B, Tq, 8)
+        for t, g in zip((x, w, b), torch.autograd.grad(y, (x, w, b), torch.ones_like(y))):
+            assert g.shape == t.shape and (g == 0).all()
+        gamma, beta = p(16), p(16)
+        y = ot.group_norm(x, 4, gamma, beta, act='elu')
+        assert y.shape == x.shape
+        for t, g in zip((x, gamma, beta), torch.autograd.grad(y, (x, gamma, beta), torch.ones_like(y))):
+            assert g.shape == t.shape and g.dtype == t.dtype and (g == 0).all()
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
 def test_attention_refusals(ot):
     t = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype)  # noqa: E731
