@@ -5,10 +5,11 @@
 //
 // Passes over x are what these kernels cost.  A thread owns a few neighbouring channels and walks rows, so a row is read in one piece; the
 // sums of a run of rows go to a slab, and one workgroup per group joins the slabs in a fixed order.
-// Statistics: each thread sums x - p and (x - p)^2 with p the first row's value of its channel, so a channel far from zero loses nothing; the runs'
-// (count, mean, M2) are joined pairwise in 64 bits.
-// Bound by memory: 2 x 491520 x 64 bf16 (126 MB a tensor), elu: statistics 24 us, result 43, backward sums 51, gradient 62 (5.2, 5.8, 4.9 and 6.1 TB/s, some of it from the
-// last-level cache; walking the rows backwards in the second passes, to find more there, changed nothing), joins 6 and 8.  65^3 x 24 fp32 forward 7 + 5 + 13 us.
+// Statistics: no row is special.  Each thread keeps a running mean and sum of squared distances of its rows, re-centred every four rows; the lanes of a run are
+// joined around a mean of several of them, the runs in 64 bits.  Neither a channel far from zero nor an outlier in any row (a padded volume's first voxel, a
+// spectrum's constant mode) makes large numbers cancel.
+// Bound by memory: 2 x 491520 x 64 bf16 (126 MB a tensor), elu: statistics 25 us, result 44, backward sums 51, gradient 62 (5.0, 5.7, 4.9 and 6.1 TB/s, some of it from the
+// last-level cache; walking the rows backwards in the second passes, to find more there, changed nothing), joins 6 and 8.  65^3 x 24 fp32 forward 8 + 6 + 13 us.
 #include "hno_tokens.h"
 
 #include <type_traits>
@@ -78,9 +79,9 @@ __device__ __forceinline__ float gn_at(const GnRaw<T, W> &r, int j) {
     else return tk_up(r.f);
 }
 
-// sums of the workgroup's rows -> slab[b][run][2][C].  The lanes that own the same channels meet in LDS; each of the 2 W cw sums is taken by `per` neighbouring
+// sums of the workgroup's rows -> the first two of slab[b][run][ROWS][C].  The lanes that own the same channels meet in LDS; each of the 2 W cw sums is taken by `per` neighbouring
 // threads (with one thread a sum, 24 channels left 3 of 256 threads 1360 additions each: 26 us for 65^3 x 24 instead of 8).
-template <int W>
+template <int W, int ROWS>
 __device__ __forceinline__ void gn_block_sums(const GnArgs &a, float (&s1)[W], float (&s2)[W], int nrl, int tid, float *lds) {
     constexpr int S = 2 * W + 1;
 #pragma unroll
@@ -89,7 +90,7 @@ __device__ __forceinline__ void gn_block_sums(const GnArgs &a, float (&s1)[W], f
     const int nout = 2 * W * a.cw;
     int per = 1;
     while (per < 64 && 2 * per * nout <= 256) per *= 2;
-    float *dst = a.slab + ((long long)blockIdx.z * a.runs + blockIdx.x) * 2 * a.C;
+    float *dst = a.slab + ((long long)blockIdx.z * a.runs + blockIdx.x) * ROWS * a.C;
     for (int o0 = 0; o0 < nout; o0 += 256 / per) {
         const int o = o0 + tid / per, sl = tid & (per - 1), ch = o / (2 * W), j = o - ch * 2 * W, c = (blockIdx.y * a.cw + ch) * W;
         const bool on = o < nout && c < a.C;
@@ -101,47 +102,92 @@ __device__ __forceinline__ void gn_block_sums(const GnArgs &a, float (&s1)[W], f
     }
 }
 
+// per channel and run of rows: a reference value and the sums of x - reference and (x - reference)^2 (three slab rows)
 template <typename T, int W>
 __global__ __launch_bounds__(256) void gncl_stats_kernel(GnArgs a) {
     __shared__ float lds[256 * (2 * W + 1)];
+    __shared__ float refs[256 * W];
     const int tid = threadIdx.x, nrl = 256 / a.cw, rl = tid / a.cw, chunk = blockIdx.y * a.cw + tid - rl * a.cw;
-    float s1[W], s2[W];
+    const long long r0 = (long long)blockIdx.x * a.rows_per, r1 = r0 + a.rows_per < a.V ? r0 + a.rows_per : a.V;
+    const bool own = chunk < a.chunks && rl < nrl && r0 + rl < r1;
+    float p[W], m[W], q[W], n = 0.f;          // p: the thread's first row; n rows of mean p + m, q: their squared distances from it
 #pragma unroll
-    for (int j = 0; j < W; ++j) s1[j] = s2[j] = 0.f;
-    if (chunk < a.chunks && rl < nrl) {
+    for (int j = 0; j < W; ++j) p[j] = m[j] = q[j] = 0.f;
+    if (own) {
         const T *x = (const T *)a.x + (long long)blockIdx.z * a.V * a.C + chunk * W;
-        const long long r1 = ((long long)blockIdx.x + 1) * a.rows_per < a.V ? ((long long)blockIdx.x + 1) * a.rows_per : a.V;
-        const GnVec<T, W> p = gn_load<T, W>(x);
-#pragma unroll 2
-        for (long long r = blockIdx.x * a.rows_per + rl; r < r1; r += nrl) {
-            const GnVec<T, W> v = gn_load<T, W>(x + r * a.C);
+        const GnVec<T, W> first = gn_load<T, W>(x + (r0 + rl) * a.C);
+#pragma unroll
+        for (int j = 0; j < W; ++j) p[j] = first.v[j];
+        // k more rows with deviations d from the mean: mean += sum d / n, q += sum d^2 - (sum d)^2 / n with the new n.  The difference takes at most half of
+        // sum d^2; of the first four rows, one of whose d is zero, three quarters.
+        const auto rows4 = [&](long long r, auto whole) {
+            GnRaw<T, W> v[4];
+            bool in[4];
+            int k = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                in[i] = whole || r + i * nrl < r1;
+                k += in[i];
+                v[i] = gn_raw<T, W>(x + (in[i] ? r + i * nrl : r) * a.C);
+            }
+            n += (float)k;
+            const float inv = __builtin_amdgcn_rcpf(n);
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                const float d = v.v[j] - p.v[j];
-                s1[j] += d;
-                s2[j] = fmaf(d, d, s2[j]);
+                float s = 0.f, t = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float d = in[i] ? (gn_at(v[i], j) - p[j]) - m[j] : 0.f;
+                    s += d;
+                    t = fmaf(d, d, t);
+                }
+                m[j] = fmaf(s, inv, m[j]);
+                q[j] += fmaf(-s * inv, s, t);
             }
-        }
+        };
+        long long r = r0 + rl;
+        for (; r + 3 * nrl < r1; r += 4 * nrl) rows4(r, std::true_type());
+        if (r < r1) rows4(r, std::false_type());
     }
-    gn_block_sums<W>(a, s1, s2, nrl, tid, lds);
+    // the run's reference: the mean of the means of its first (at most eight) lanes, an outlier's share of it being small
+#pragma unroll
+    for (int j = 0; j < W; ++j) lds[tid * (W + 1) + j] = p[j] + m[j];
+    __syncthreads();
+    const int few = (int)min((long long)min(nrl, 8), r1 - r0);
+    for (int o = tid; o < W * a.cw; o += 256) {
+        const int ch = o / W, j = o - ch * W, c = (blockIdx.y * a.cw + ch) * W + j;
+        float t = 0.f;
+        for (int l = 0; l < few; ++l) t += lds[(ch + l * a.cw) * (W + 1) + j];
+        t /= (float)few;
+        refs[o] = t;
+        if (c < a.C) a.slab[(((long long)blockIdx.z * a.runs + blockIdx.x) * 3 + 2) * a.C + c] = t;
+    }
+    __syncthreads();
+    float s1[W], s2[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        const float d = own ? (p[j] - refs[(tid - rl * a.cw) * W + j]) + m[j] : 0.f;
+        s1[j] = n * d;
+        s2[j] = fmaf(n * d, d, q[j]);
+    }
+    gn_block_sums<W, 3>(a, s1, s2, nrl, tid, lds);
 }
 
 // joins the runs of a group in 64 bits: with mean_i, M2_i of channel run i of n_i values and any reference r,
-//   N (mean - r) = sum n_i (mean_i - r),  M2 = sum M2_i + sum n_i (mean_i - r)^2 - N (mean - r)^2      (r: the group's first value)
-template <typename T>
+//   N (mean - r) = sum n_i (mean_i - r),  M2 = sum M2_i + sum n_i (mean_i - r)^2 - N (mean - r)^2      (r: the first run's reference)
 __global__ __launch_bounds__(1024) void gncl_finish_kernel(GnArgs a) {
     __shared__ double sh[2][1024];
     const int tid = threadIdx.x, g = blockIdx.x, b = blockIdx.y, cpg = a.C / a.G;
-    const T *x = (const T *)a.x + (long long)b * a.V * a.C + g * cpg;
-    const float *slab = a.slab + (long long)b * a.runs * 2 * a.C + g * cpg;
-    const double ref = tk_up(x[0]), inv = 1.0 / (double)a.rows_per, left = (double)(a.V - (a.runs - 1) * a.rows_per), inv_last = 1.0 / left;
+    const float *slab = a.slab + (long long)b * a.runs * 3 * a.C + g * cpg;
+    const double ref = slab[2ll * a.C], inv = 1.0 / (double)a.rows_per, left = (double)(a.V - (a.runs - 1) * a.rows_per), inv_last = 1.0 / left;
     double d1 = 0.0, m2 = 0.0;
 #pragma unroll 4
     for (long long i = tid; i < (long long)cpg * a.runs; i += 1024) {
         const int run = (int)(i / cpg), c = (int)(i - (long long)run * cpg);
         const bool last = run == a.runs - 1;
-        const double n = last ? left : (double)a.rows_per, s1 = slab[run * 2ll * a.C + c], s2 = slab[(run * 2ll + 1) * a.C + c];
-        const double mi = s1 * (last ? inv_last : inv), d = (double)tk_up(x[c]) - ref + mi;
+        const float *src = slab + run * 3ll * a.C + c;
+        const double n = last ? left : (double)a.rows_per, s1 = src[0], s2 = src[a.C];
+        const double mi = s1 * (last ? inv_last : inv), d = (double)src[2ll * a.C] - ref + mi;
         d1 += n * d;
         m2 += s2 - s1 * mi + n * d * d;
     }
@@ -215,7 +261,7 @@ __global__ __launch_bounds__(256) void gncl_bwd_sums_kernel(GnArgs a) {
             }
         });
     }
-    gn_block_sums<W>(a, s1, s2, nrl, tid, lds);
+    gn_block_sums<W, 2>(a, s1, s2, nrl, tid, lds);
 }
 
 // one workgroup per group: dgamma, dbeta of its channels and, per sample, mean(du gamma) and mean(du gamma xh).  `cw` threads across the
@@ -525,7 +571,7 @@ static int gn_forward(const void *x, const float *gamma, const float *beta, void
         return HNO_OK;
     }
     GN_LAUNCH(gncl_stats_kernel);
-    hipLaunchKernelGGL((gncl_finish_kernel<T>), dim3(G, B), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL(gncl_finish_kernel, dim3(G, B), dim3(1024), 0, s, a);
     HNO_CHECK_LAUNCH();
     GN_LAUNCH(gncl_apply_kernel);
     return HNO_OK;
@@ -563,7 +609,7 @@ static int gn_backward(const void *dy, const void *x, const float *gamma, const 
 extern "C" size_t hno_gncl_workspace_bytes(int B, long long V, int C, int G) {
     if (gn_check("hno_gncl_workspace_bytes", HNO_F32, B, V, C, G, 0)) return 0;
     const int r0 = gn_plan(0, B, V, C, false).runs, r1 = C % 8 == 0 ? gn_plan(0, B, V, C, true).runs : 0;
-    return gn_pad((size_t)B * G * 2 * sizeof(float)) + (size_t)B * (r0 > r1 ? r0 : r1) * 2 * C * sizeof(float);       // (small groups: B x 2 x C)
+    return gn_pad((size_t)B * G * 2 * sizeof(float)) + (size_t)B * (r0 > r1 ? r0 : r1) * 3 * C * sizeof(float);       // (small groups: B x 2 x C)
 }
 extern "C" int hno_gncl_fwd(int dtype, const void *x, const float *gamma, const float *beta, void *y, float *mean_rstd, void *workspace, size_t workspace_bytes,
                             int B, long long V, int C, int G, float eps, int act, void *stream) {

@@ -1,0 +1,74 @@
+"""The token operators where their own way of summing could show: bounds here come from the definitions alone, not from a choice inside the kernels."""
+import math
+
+import pytest
+import torch
+
+from test_token_ops import ACT64, DTYPES, E, HALF, close, ot, rand, slope64  # noqa: F401
+
+
+# ------------------------------------------------------------------------------------------------ group norm
+def check_group_norm_definition(ot, x, G, w, b, act, eps=1e-5):
+    """Errors of a summation that is at most 128 rounding steps deep and takes no difference of large numbers: 128 E of the standard deviation for the mean (and its own
+    rounding), 128 E of the variance, 512 E of the mean of absolute values for the backward sums; each value then takes a handful of operations."""
+    x = x.detach().requires_grad_(True)
+    leaves = [x] + [t.requires_grad_(True) for t in (w, b) if t is not None]
+    y = ot.group_norm(x, G, w, b, eps=eps, act=act)
+    g = rand(x.shape, x.dtype, 66)
+    grads = torch.autograd.grad(y, leaves, g)
+    B, C, u = x.shape[0], x.shape[-1], HALF[x.dtype]
+    X, Gr = x.detach().double().reshape(B, -1, G, C // G), g.double().reshape(B, -1, G, C // G)
+    one, zero = torch.ones(C, device=x.device), torch.zeros(C, device=x.device)
+    W, Bt = ((t.detach() if t is not None else d).double().view(G, C // G) for t, d in ((w, one), (b, zero)))
+    mean, var = X.mean((1, 3), keepdim=True), X.var((1, 3), unbiased=False, keepdim=True)
+    rstd = 1.0 / torch.sqrt(var + eps)
+    xh = (X - mean) * rstd
+    z = xh * W + Bt
+    a, slope = ACT64[act](z), slope64(z, act)
+    er = 64 * E + 4 * E                                                   # (of rstd: half of the variance's)
+    em = 128 * E / rstd + 4 * E * mean.abs()
+    eh = xh.abs() * (er + 4 * E) + rstd * (em + 2 * E * (X.abs() + mean.abs()))
+    ez = eh * W.abs() + 4 * E * (z.abs() + (xh * W).abs() + Bt.abs())
+    close('y', y.detach(), a.reshape(x.shape), (1.8 * ez + 24 * E * (a.abs() + z.abs()) + (u + 2 * E) * a.abs()).reshape(x.shape))
+    du = Gr * slope
+    edu = Gr.abs() * (1.8 * ez + 24 * E) if act else torch.zeros_like(du)
+    t, et = du * W, edu * W.abs() + 2 * E * (du * W).abs()
+    s = 512 * E
+    m1, m2 = t.mean((1, 3), keepdim=True), (t * xh).mean((1, 3), keepdim=True)
+    e1 = (et + s * t.abs()).mean((1, 3), keepdim=True)
+    e2 = (et * xh.abs() + t.abs() * eh + s * (t * xh).abs()).mean((1, 3), keepdim=True)
+    dx = rstd * (t - m1 - xh * m2)
+    edx = dx.abs() * (er + 4 * E) + rstd * (et + e1 + eh * m2.abs() + xh.abs() * e2 + 4 * E * (t.abs() + m1.abs() + (xh * m2).abs()))
+    close('dx', grads[0], dx.reshape(x.shape), (edx + u * dx.abs()).reshape(x.shape))
+    if w is not None:
+        dw = (du * xh).sum((0, 1))
+        close('dw', grads[1], dw.reshape(C), ((edu * xh.abs() + du.abs() * eh + s * (du * xh).abs()).sum((0, 1)) + HALF[w.dtype] * dw.abs()).reshape(C))
+    if b is not None:
+        db = du.sum((0, 1))
+        close('db', grads[-1], db.reshape(C), ((edu + s * du.abs()).sum((0, 1)) + HALF[b.dtype] * db.abs()).reshape(C))
+
+
+# many row lanes and runs with a short last one; single channels; one run a sample; groups of one channel; more channels than a workgroup's threads
+LARGE = [((1, 65 ** 3, 24), 6), ((2, 24577, 64), 8), ((3, 5001, 17), 1), ((600, 700, 24), 2), ((1, 60001, 8), 8), ((2, 1201, 2056), 1), ((1, 4099, 264), 3)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('shape,G', LARGE)
+def test_group_norm_large_form(ot, shape, G, dtype):
+    x, C = rand(shape, dtype, 1, 1.5, 0.3), shape[-1]
+    check_group_norm_definition(ot, x, G, rand((C,), torch.float32, 2, 0.2, 1.0), rand((C,), torch.float32, 3, 0.2), 'silu')
+    check_group_norm_definition(ot, x, G, None, None, None)
+
+
+# the first row is where a padded volume has its background and a spectrum its constant mode; `rest`: (mean, deviation) of the others
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('at', [0, -1, 777])
+@pytest.mark.parametrize('row,rest', [(100.0, (0.0, 1.0)), (1e4, (0.3, 0.01)), (0.0, (1000.0, 1.0)), (-3e5, (7.0, 0.0))])
+@pytest.mark.parametrize('shape,G', [((1, 65 ** 3, 24), 6), ((2, 24577, 64), 8), ((600, 700, 24), 2), ((3, 5001, 17), 1)])
+def test_group_norm_outlying_row(ot, shape, G, row, rest, at, dtype):
+    mean, dev = rest
+    x = rand(shape, dtype, 4, dev, mean)
+    x[:, at % shape[1] if at < 0 else at % min(shape[1], 1000)] = row
+    check_group_norm_definition(ot, x, G, None, None, None)
