@@ -346,10 +346,11 @@ __global__ __launch_bounds__(256) void gncl_bwd_apply_kernel(GnArgs a) {
 }
 
 // ------------------------------------------------------------------ small groups: one launch
-// A workgroup owns one group of one sample and keeps it in registers: x is read once, the statistics are those of the kept values (mean first, then squared
-// distances), and the backward pass needs no second launch but the sum over samples of dgamma, dbeta.  Threads: chunk (of W channels) x row; a thread keeps gn_keep
-// rows.  2 x 960 x 256 bf16 in 32 groups: forward 10.6 us of kernels (in three launches 20), backward 13.3 (31); what is left are the latencies of a launch, a
-// load, two or three sums over the workgroup and a store.
+// A workgroup owns one group of one sample and keeps it in registers: x is read once, the statistics are those of the kept values (mean first, then the
+// distances from it and their squares: what the distances add up to corrects the mean, which lost bits if the group's first value is far from it), and the backward
+// pass needs no second launch but the sum over samples of dgamma, dbeta.  Threads: chunk (of W channels) x row; a thread keeps gn_keep rows.
+// 2 x 960 x 256 bf16 in 32 groups: forward 9.5 us of kernels (in three launches 20), backward 13.8 (31); what is left are the latencies of a launch, a load, two or
+// three sums over the workgroup and a store.
 constexpr int GN_THREADS = 1024;
 template <typename T, int W, bool BWD> constexpr int gn_keep() { return BWD && sizeof(T) == 4 && W == 8 ? 4 : 8; }       // (128 registers a thread)
 template <typename T, int W, bool BWD> inline bool gn_small(long long V, int cpg) {
@@ -366,9 +367,20 @@ __device__ __forceinline__ float gn_block_sum(float v, float *sh, int tid) {
     for (int k = 0; k < GN_THREADS / 64; ++k) s += sh[k];
     return s;
 }
+// two sums for the latency of one
+__device__ __forceinline__ void gn_block_sum2(float &v, float &w, float (&sh)[2][GN_THREADS / 64], int tid) {
+#pragma unroll
+    for (int k = 32; k; k >>= 1) v += __shfl_xor(v, k), w += __shfl_xor(w, k);
+    __syncthreads();
+    if ((tid & 63) == 0) sh[0][tid >> 6] = v, sh[1][tid >> 6] = w;
+    __syncthreads();
+    v = w = 0.f;
+#pragma unroll
+    for (int k = 0; k < GN_THREADS / 64; ++k) v += sh[0][k], w += sh[1][k];
+}
 template <typename T, int W>
 __global__ __launch_bounds__(GN_THREADS) void gncl_small_fwd_kernel(GnArgs a) {
-    __shared__ float sh[GN_THREADS / 64];
+    __shared__ float sh[2][GN_THREADS / 64];
     const int tid = threadIdx.x, g = blockIdx.x, b = blockIdx.y, cpg = a.C / a.G, nch = cpg / W, nr = GN_THREADS / nch, rl = tid / nch, c = g * cpg + (tid - rl * nch) * W;
     constexpr int KEEP = gn_keep<T, W, false>();
     const T *x = (const T *)a.x + (long long)b * a.V * a.C + c;
@@ -383,7 +395,7 @@ __global__ __launch_bounds__(GN_THREADS) void gncl_small_fwd_kernel(GnArgs a) {
 #pragma unroll
         for (int j = 0; j < W; ++j) s += in ? gn_at(v[k], j) - first : 0.f;
     }
-    const float mean = first + gn_block_sum(s, sh, tid) / n;
+    float mean = first + gn_block_sum(s, sh[0], tid) / n, e = 0.f;
     s = 0.f;
 #pragma unroll
     for (int k = 0; k < KEEP; ++k) {
@@ -391,10 +403,13 @@ __global__ __launch_bounds__(GN_THREADS) void gncl_small_fwd_kernel(GnArgs a) {
 #pragma unroll
         for (int j = 0; j < W; ++j) {
             const float d = in ? gn_at(v[k], j) - mean : 0.f;
+            e += d;
             s = fmaf(d, d, s);
         }
     }
-    const float rstd = 1.f / sqrtf(gn_block_sum(s, sh, tid) / n + a.eps);
+    gn_block_sum2(s, e, sh, tid);
+    const float var = fmaf(-e / n, e, s) / n, rstd = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);
+    mean += e / n;
     if (tid == 0) a.mr[2 * (b * a.G + g)] = mean, a.mr[2 * (b * a.G + g) + 1] = rstd;
     float ga[W], be[W];
 #pragma unroll

@@ -66,7 +66,8 @@ def test_group_norm_large_form(ot, shape, G, dtype):
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 @pytest.mark.parametrize('at', [0, -1, 777])
 @pytest.mark.parametrize('row,rest', [(100.0, (0.0, 1.0)), (1e4, (0.3, 0.01)), (0.0, (1000.0, 1.0)), (-3e5, (7.0, 0.0))])
-@pytest.mark.parametrize('shape,G', [((1, 65 ** 3, 24), 6), ((2, 24577, 64), 8), ((600, 700, 24), 2), ((3, 5001, 17), 1)])
+@pytest.mark.parametrize('shape,G', [((1, 65 ** 3, 24), 6), ((2, 24577, 64), 8), ((600, 700, 24), 2), ((3, 5001, 17), 1), ((2, 8192, 8), 1), ((1, 128, 512), 1),
+                                     ((2, 960, 256), 32)])
 def test_group_norm_outlying_row(ot, shape, G, row, rest, at, dtype):
     mean, dev = rest
     x = rand(shape, dtype, 4, dev, mean)
