@@ -536,6 +536,8 @@ static int ln_check(const char *what, int dtype, int M, int N, int K, int act) {
     if (M > (1 << 30) || N > (1 << 30) || K > (1 << 30)) return fail(HNO_ELIMIT, "%s: a size exceeds 2^30", what);
     return HNO_OK;
 }
+// a tensor beside the operator's own: its type or fp32 (a kernel that took another one for its own would write past its end)
+static bool ln_type(const void *t, int dtype, int own) { return !t || dtype == HNO_F32 || dtype == own; }
 static size_t ln_slab(int M, int N, int K, bool f32) {
     const int n = ln_plan(M, N, K, f32, false).nsplit;          // (where LnBig is taken, one)
     return n > 1 ? (size_t)n * M * N * sizeof(float) : 0;
@@ -577,6 +579,7 @@ extern "C" int hno_linear_fwd(int dtype, const void *x, long long ldx, const voi
                               int M, int N, int K, int act, void *workspace, size_t workspace_bytes, void *stream) {
     if (int rc = ln_check("hno_linear_fwd", dtype, M, N, K, act)) return rc;
     HNO_REQUIRE(x && w && y && ldx >= K, "hno_linear_fwd: bad argument");
+    HNO_REQUIRE(ln_type(bias, bias_dtype, dtype), "hno_linear_fwd: bias type %d beside type %d", bias_dtype, dtype);
     const size_t need = hno_linear_workspace_bytes(dtype, M, N, K, act, 0);
     HNO_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "hno_linear_fwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     LinArgs a = {};
@@ -626,6 +629,7 @@ extern "C" int hno_linear_bwd(int dtype, const void *dy, const void *z, const vo
                               int db_dtype, int M, int N, int K, int act, void *workspace, size_t workspace_bytes, void *stream) {
     if (int rc = ln_check("hno_linear_bwd", dtype, M, N, K, act)) return rc;
     HNO_REQUIRE(dy && (act == HNO_ACT_NONE || z) && (!dx || w) && (!dw || (x && ldx >= K)) && (dx || dw || db), "hno_linear_bwd: bad argument");
+    HNO_REQUIRE(ln_type(dw, dw_dtype, dtype) && ln_type(db, db_dtype, dtype), "hno_linear_bwd: gradients of types %d, %d beside type %d", dw_dtype, db_dtype, dtype);
     const size_t need = hno_linear_workspace_bytes(dtype, M, N, K, act, 1);
     HNO_REQUIRE(workspace && workspace_bytes >= need, "hno_linear_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (dtype == HNO_BF16) return ln_backward<tkh>(dy, z, x, ldx, w, dx, dw, dw_dtype, db, db_dtype, M, N, K, act, (char *)workspace, (hipStream_t)stream);
