@@ -4,12 +4,13 @@ their backward passes.
 
 Tensors are torch containers; nothing computes through ATen and there is no CPU path (meta tensors get shape inference only).  Parameters may
 stay fp32 next to bf16 activations: the matrix product then rounds its weight to bf16, as the bf16 convolutions do, and returns an fp32 gradient.
-Gradients of gradients are refused.
+Gradients of gradients and forward-mode derivatives are refused.
 """
 import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 from ._lib import check
@@ -51,8 +52,8 @@ def _same_device(what, first, *others):
 
 def _call(fn, *args):
     """fn.run(...) -> result, kept; as a node of the autograd graph where a gradient can be asked for (4 us of host time: a call for one token took 24
-    with a node that nobody asks, 20 without).  The device of the first argument is the current one meanwhile: launches and workspaces go by it and its
-    current stream."""
+    with a node that nobody asks, 20 without), and where a tensor may be dual: the node refuses it (forward-mode derivatives are not provided).
+    The device of the first argument is the current one meanwhile: launches and workspaces go by it and its current stream."""
     if args[0].device.index != torch.cuda.current_device():
         with torch.cuda.device(args[0].device):
             return _call(fn, *args)
@@ -60,7 +61,7 @@ def _call(fn, *args):
         for t in args:
             if isinstance(t, torch.Tensor) and t.requires_grad:
                 return _leaves(fn.apply(*args))
-    return fn.run(False, *args)[0]
+    return fn.apply(*args) if forward_ad._current_level >= 0 else fn.run(False, *args)[0]
 
 
 def _leaves(y):

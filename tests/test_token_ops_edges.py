@@ -75,6 +75,30 @@ def test_group_norm_outlying_row(ot, shape, G, row, rest, at, dtype):
     check_group_norm_definition(ot, x, G, None, None, None)
 
 
+# ------------------------------------------------------------------------------------------------ forward-mode derivatives
+@pytest.mark.gpu
+@pytest.mark.parametrize('grad', [False, True])
+def test_forward_mode_is_refused(ot, grad):
+    """as by the framework's other operators: a result without its tangent would be a wrong derivative"""
+    from torch.autograd import forward_ad
+    r = lambda *s: rand(s, torch.float32, 1)  # noqa: E731
+    calls = [(ot.attention, (r(1, 5, 2, 8), r(1, 7, 2, 8), r(1, 7, 2, 8)), {}), (ot.linear, (r(6, 8), r(4, 8), r(4)), {'residual': r(6, 4)}),
+             (ot.group_norm, (r(2, 5, 8), 2, r(8), r(8)), {})]
+    with torch.set_grad_enabled(grad):
+        for f, args, kw in calls:
+            with forward_ad.dual_level():
+                want = f(*args, **kw)                                      # nothing dual: nothing changes
+                for i, t in enumerate(args):
+                    if isinstance(t, torch.Tensor):
+                        dual = args[:i] + (forward_ad.make_dual(t, torch.ones_like(t)),) + args[i + 1:]
+                        with pytest.raises(NotImplementedError):
+                            f(*dual, **kw)
+                for k, t in kw.items():
+                    with pytest.raises(NotImplementedError):
+                        f(*args, **{k: forward_ad.make_dual(t, torch.ones_like(t))})
+            assert torch.equal(want, f(*args, **kw))
+
+
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
 def test_linear_entry_points_refuse_types_that_they_do_not_write():
     """types beside the operator's own: fp32 only, where there is a tensor of them"""
