@@ -155,7 +155,7 @@ class AttentionFn(torch.autograd.Function):
         new = torch.empty if out.numel() else torch.zeros
         dq = new(q.shape, device=q.device, dtype=q.dtype) if need_q else None
         dk, dv = (new(t.shape, device=q.device, dtype=q.dtype) if need_kv else None for t in (k, v))
-        if out.numel():
+        if out.numel() and (need_q or k.shape[1]):                         # (without keys dk and dv are empty: there may be nothing to write)
             L = _lib.lib()
             g = _heads(g, g.element_size()).contiguous()
             a = _attn_args(q, k, v, mask, kv_lens, causal, scale)

@@ -75,6 +75,20 @@ def test_group_norm_outlying_row(ot, shape, G, row, rest, at, dtype):
     check_group_norm_definition(ot, x, G, None, None, None)
 
 
+# ------------------------------------------------------------------------------------------------ attention
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('need', ['q', 'k', 'v', 'kv', 'qkv'])
+def test_attention_gradients_without_keys(ot, need, dtype):
+    """no keys at all: zeros, and gradients of zeros or of no elements, whichever of them are asked for"""
+    t = {'q': rand((2, 5, 4, 16), dtype, 1), 'k': rand((2, 0, 2, 16), dtype, 2), 'v': rand((2, 0, 2, 24), dtype, 3)}
+    leaves = [t[n].requires_grad_(True) for n in need]
+    y = ot.attention(t['q'], t['k'], t['v'], mask=torch.ones((2, 1, 5, 0), dtype=torch.bool, device='cuda'))
+    assert y.shape == (2, 5, 4, 24) and (y == 0).all()
+    for x, g in zip(leaves, torch.autograd.grad(y, leaves, torch.ones_like(y))):
+        assert g.shape == x.shape and (g == 0).all()
+
+
 # ------------------------------------------------------------------------------------------------ forward-mode derivatives
 @pytest.mark.gpu
 @pytest.mark.parametrize('grad', [False, True])
