@@ -630,7 +630,7 @@ int hno_attn_bwd(const hno_attn_t *p, const void *out, const void *out_res, cons
                  void *workspace, size_t workspace_bytes, void *stream);
 /* hno_linear_fwd: y (M, N) = act(x w^T + bias) + residual, x (M, K) with row stride ldx, w (N, K); bias (N) of bias_dtype and residual (M, N) may be
  *   NULL.  z (M, N), if not NULL, receives the argument of the activation, which hno_linear_bwd reads (act != NONE).
- *   fp32 products of more than four rows are formed from three bf16 terms per value (errors as in fp32; an infinity becomes NaN).
+ *   fp32 products of more than four rows are formed from three bf16 terms per value (errors as in fp32; infinities and NaN as in fp32).
  * hno_linear_bwd: dx (M, K), dw (N, K) of dw_dtype, db (N) of db_dtype from dy (M, N); any of them may be NULL.  (The residual's gradient is dy.)
  *   bias_dtype, dw_dtype and db_dtype are dtype or HNO_F32. */
 size_t hno_linear_workspace_bytes(int dtype, int M, int N, int K, int act, int backward);

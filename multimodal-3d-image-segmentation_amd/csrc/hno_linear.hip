@@ -15,7 +15,7 @@ struct LinArgs {
     void *z, *y;
     float *part;
     long long lda, ldb;
-    int M, N, K, act, bias32, out32, nsplit;
+    int M, N, K, act, bias32, out32, nsplit, across;          // across: 1: A is stored across k, 2: B is
     // beside dW: db (db_n) from the slab of column sums, one row a run
     const float *db_slab;
     void *db;
@@ -152,11 +152,34 @@ __device__ __forceinline__ void ln_put8(T *p, int cnt, const float (&x)[8]) {
             if (j < cnt) p[j] = tk_down<T>(x[j]);
     }
 }
+// fp32: a NaN of columns n .. n + 7 of row m may come from an infinity, whose lower bf16 terms are none: that product once more, in fp32 from the operands.
+// It ends at a true NaN; finite results pay a comparison.
+__device__ __forceinline__ void ln_infinite(const LinArgs &a, int m, int n, float (&x)[8]) {
+    const float none = (x[0] + x[1]) + (x[2] + x[3]) + ((x[4] + x[5]) + (x[6] + x[7]));
+    if (none == none) return;
+    const float *pa = (const float *)a.A + m * (a.across & 1 ? 1 : a.lda), *pb = (const float *)a.B;
+    const long long sa = a.across & 1 ? a.lda : 1, sb = a.across & 2 ? a.ldb : 1, sn = a.across & 2 ? 1 : a.ldb;
+    float s[8] = {};
+    bool open = true;
+#pragma unroll 1
+    for (int k = 0; k < a.K && open; ++k) {
+        const float v = pa[k * sa];
+        open = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            s[j] = fmaf(v, pb[k * sb + min(n + j, a.N - 1) * sn], s[j]);
+            open |= x[j] != x[j] && s[j] == s[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = x[j] == x[j] ? x[j] : s[j];
+}
 // the epilogue of columns n .. n + 7 of row m; r: the residual's values, loaded before
 template <typename T, int ACT>
 __device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float (&x)[8], const TkFrag<T> &r) {
     const int cnt = a.N - n;
     const long long at = (long long)m * a.N + n;
+    if constexpr (sizeof(T) == 4) ln_infinite(a, m, n, x);
     if (a.bias) {
         float t[8];
         if (a.bias32) ln_get8((const float *)a.bias + n, cnt, t);
@@ -511,6 +534,7 @@ static int ln_product(LinArgs a, hipStream_t s) {
     const LnPlan p = ln_plan(a.M, a.N, a.K, sizeof(T) == 4, dma);
     if (p.blocks >= 1ll << 23) return fail(HNO_ELIMIT, "hno_linear: %lld tiles exceed the grid", p.blocks);          // (of 2^32 threads)
     a.nsplit = p.nsplit;
+    a.across = AX + 2 * BX;
     ProfScope _ps(KID_LINEAR, s, esz * ((double)a.M * a.K + (double)a.N * a.K + (double)a.M * a.N));
     const dim3 grid((unsigned)p.blocks);
     if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((linear_kernel<T, AX, BX, LnF32, false, ACT>), grid, dim3(64 * ln_waves<LnF32>()), 0, s, a);

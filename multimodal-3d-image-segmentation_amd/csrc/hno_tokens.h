@@ -5,7 +5,7 @@
 //   result    lane l, register r holds row 8 (r / 4) + 4 h + r % 4 of column l & 31
 // on v_mfma_f32_32x32x16_bf16.  fp32 values are three bf16 terms: the leading 8 bits, the next 8 and the last 8 (cut, not rounded: their sum is the value); a product
 // is the six products of terms down to 2^-16, smallest first -- the two dropped ones are at most 2^-22, on average 2^-25, of it.  The fp32 matrix instruction takes
-// 2.7 times as long for the same work.  (An infinity becomes inf + NaN + NaN: products with it are NaN.)
+// 2.7 times as long for the same work.  (An infinity becomes inf + NaN + NaN: products with it are NaN, which linear forms again in fp32 and attention leaves.)
 // A sum does not depend on which index sits in which slot as long as both operands agree; the attention kernels use this to feed
 // a result back as an operand without moving it between lanes: registers 8 t .. 8 t + 7 of a result are the fragment whose
 // slots stand for rows 16 t + 4 h + {0..3} and 16 t + 8 + 4 h + {0..3}.

@@ -299,7 +299,7 @@ def linear(x, weight, bias=None, *, act=None, residual=None):
 
     ``act``: see ``act_id``.  weight is of x's type, or fp32 next to a bf16 x (rounded to bf16 for the product; its gradient is fp32); bias is of either
     type.  residual has the result's shape and type.  x may be any view; rows of equal stride are read where they lie.
-    fp32 products of more than four rows are formed from three bf16 terms per value, so an infinity in x or weight comes out as NaN there.
+    fp32 products of more than four rows are formed from three bf16 terms per value (errors as in fp32; infinities and NaN as in fp32).
     Differentiable in all four; with an activation the backward pass keeps the product's result, in x's type."""
     a = act_id(act)
     if x.ndim < 1 or weight.ndim != 2 or x.shape[-1] != weight.shape[1]:

@@ -75,6 +75,41 @@ def test_group_norm_outlying_row(ot, shape, G, row, rest, at, dtype):
     check_group_norm_definition(ot, x, G, None, None, None)
 
 
+# ------------------------------------------------------------------------------------------------ linear
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('act', [None, 'relu', 'elu'])
+@pytest.mark.parametrize('M,N,K', [(1, 40, 48), (4, 33, 200), (5, 40, 48), (131, 257, 70), (40, 33, 3000), (300, 130, 515)])
+def test_linear_infinities(ot, M, N, K, act, dtype):
+    """an infinity gives infinities, and NaN only where it meets a zero or its opposite, whatever the number of rows; what does not meet one keeps its value"""
+    x, w = rand((M, K), dtype, 1), rand((N, K), dtype, 2, K ** -0.5)
+    x[M // 2, 3], w[5, K - 2], w[N - 1, 7] = math.inf, -math.inf, math.nan
+    w[7, 3] = 0.0                                                         # (infinity times zero)
+    w[8, 3] = 1.0                                                         # (a value without lower bits)
+    x[M - 1, K - 1] = -math.inf if M > 1 else 1.0
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    y = ot.linear(x, w, act=act)
+    X, W = x.detach().double(), w.detach().double()
+    z = X @ W.t()
+    want = ACT64[act](z)
+
+    def same(name, got, want, bound):
+        got = got.double()
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), name
+        assert torch.equal(torch.isinf(got), torch.isinf(want)) and torch.equal(got[torch.isinf(want)], want[torch.isinf(want)]), name
+        ok = torch.isfinite(want)                                         # (a single row holds an infinity: nothing of it may be finite)
+        close(name, got[ok], want[ok], bound[ok])
+    u = HALF[dtype]
+    same('y', y.detach(), want, 1.8 * (K + 8) * E * (X.abs() @ W.abs().t()) + 24 * E * (want.abs() + z.abs()) + (u + 4 * E) * want.abs())
+    if act is None:
+        g = rand(y.shape, dtype, 3)
+        g[0, N // 2] = math.inf
+        dx, dw = torch.autograd.grad(y, (x, w), g)
+        G = g.double()
+        same('dx', dx, G @ W, (N + 8) * E * (G.abs() @ W.abs()) + (u + 4 * E) * (G @ W).abs())
+        same('dw', dw, G.t() @ X, (M + 8) * E * (G.abs().t() @ X.abs()) + (u + 4 * E) * (G.t() @ X).abs())
+
+
 # ------------------------------------------------------------------------------------------------ attention
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
