@@ -5,7 +5,7 @@ query/key/value projections (pointwise MFMA convs over the mode axis), patch gro
 permutation), att = act(Q^T K / sqrt(C)) and out = V att^T on the batched fp32 MFMA GEMM (hno_bmm),
 output projection, zero pad + unscaled inverse transform (hno_pad_idht3).  SELU, not softmax, is the
 default attention activation, so no online normalisation is needed there; a softmax over the keys
-(``functools.partial(F.softmax, dim=-1)``) goes through ops_tokens.attention.
+(``functools.partial(F.softmax, dim=-1)``) goes through ops_tokens.attention, up to 128 grouped channels a head.
 """
 import functools
 import math
@@ -86,6 +86,10 @@ class HartleyMultiHeadAttention(Module):
             self.patch_size = (self.patch_size,) * (ndim - 2)
         if isinstance(self.attention_activation, str):
             self.attention_activation = getattr(torch.nn.functional, self.attention_activation)
+        grouped = max(key_dim, self.value_dim) * int(np.prod(self.patch_size or 1))
+        if softmax_over_keys(self.attention_activation) and grouped > ops_tokens.MAX_HEAD:
+            raise ValueError(f'a softmax over the keys is provided for up to {ops_tokens.MAX_HEAD} grouped channels a head (channels x patch size), '
+                             f'not for {grouped} grouped channels')
         self.weight_query = Parameter(torch.empty((num_heads, key_dim, self.in_channels), **fk))
         self.weight_key = Parameter(torch.empty((num_heads, key_dim, self.key_in_channels), **fk))
         self.weight_value = Parameter(torch.empty((num_heads, self.value_dim, self.value_in_channels), **fk))
