@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_token_ops import ACT64, DTYPES, E, HALF, close, ot, rand, slope64  # noqa: F401
+from test_token_ops import ACT64, DTYPES, E, HALF, block, block64, block_parameters, close, ot, rand, slope64  # noqa: F401
 
 
 # ------------------------------------------------------------------------------------------------ group norm
@@ -124,6 +124,107 @@ def test_attention_gradients_without_keys(ot, need, dtype):
         assert g.shape == x.shape and (g == 0).all()
 
 
+# B, Tq, Tk, H, Hk, D, causal: long axes, cut into runs; remainders of a tile on either side
+LONG = [(1, 1, 4099, 2, 1, 64, True), (1, 4, 9000, 4, 4, 32, True), (2, 1, 3000, 16, 2, 80, False), (1, 300, 5000, 2, 1, 96, False), (1, 700, 1201, 1, 1, 64, False),
+        (1, 2100, 70, 2, 2, 64, False), (1, 5001, 300, 2, 1, 128, False), (1, 900, 1500, 2, 2, 128, True), (1, 100, 2011, 8, 2, 96, True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('B,Tq,Tk,H,Hk,D,causal', LONG)
+def test_attention_every_tile_edge_counts(ot, B, Tq, Tk, H, Hk, D, causal, dtype):
+    """Each query meets one key (the others' weights are below e^-20), first and last keys of tiles in turn: its result is that key's value, and the key's dv the sum of its
+    queries' gradients.  Errors: a rounding of the weight and one of the result, and 2^-24 of the exponent for each operation on it."""
+    u, n, c = HALF[dtype], H // Hk, {32: 8.0, 64: 4.0, 80: 4.0, 96: 4.0, 128: 2.0}[D]
+    k = torch.where(rand((B, Tk, Hk, D), torch.float32, 1) < 0, -1.0, 1.0).to(dtype)
+    v, g = rand((B, Tk, Hk, D), dtype, 2), rand((B, Tq, H, D), dtype, 3)
+    edges = sorted({t for m in range(0, Tk, 32) for t in (m, min(m + 31, Tk - 1))} | set(range(max(0, Tk - 66), Tk)))
+    edges = torch.tensor(edges, device='cuda')
+    slot = torch.arange(Tq, device='cuda')[:, None] * n + torch.arange(H, device='cuda')[None] % n                # (Tq, H): running number in its key head
+    sees = torch.arange(Tq, device='cuda')[:, None] + Tk - Tq if causal else torch.full((Tq, 1), Tk - 1, device='cuda')
+    rows, head = torch.arange(B, device='cuda')[:, None, None], (torch.arange(H, device='cuda') // n)[None, None]
+    s = torch.matmul(k[:, :, 0].float(), k[:, :, 0].float().transpose(1, 2).contiguous()) * c
+    s.diagonal(dim1=1, dim2=2).fill_(-math.inf)
+    assert float(s.max()) < c * D - 20 - math.log(Tk)
+    rp = E * (32 + 8 * c * D)
+    for first in range(0, len(edges), Tq * n):
+        t = torch.minimum(edges[(first + slot) % len(edges)], sees)                                                # (Tq, H): the key of each query
+        t = t[None].expand(B, Tq, H)
+        q = (k[rows, t, head] * c).detach()
+        vv = v.detach().requires_grad_(True)
+        y = ot.attention(q, k, vv, causal=causal, scale=1.0)
+        (dv,) = torch.autograd.grad(y, vv, g)
+        want = v[rows, t, head].double()
+        close('y', y.detach(), want, (u + rp) * want.abs() + 1e-6)
+        sums = [torch.zeros((B, Tk, Hk, D), device='cuda', dtype=torch.float64).index_put_((rows.expand(B, Tq, H), t, head.expand(B, Tq, H)), x, accumulate=True)
+                for x in (g.double(), g.double().abs())]
+        close('dv', dv, sums[0], u * sums[0].abs() + (u + rp + 2 * Tq * n * E) * sums[1] + 1e-6)
+
+
+def attention_spread(q, k, v, g, causal, keep=None):
+    """float64 results and the variances of their errors in bf16: {name: (value, variance)}.  A value that is rounded is off by u / sqrt(3) of it at most in the mean square; the weights
+    are rounded before their product with v or g, the score gradients before theirs with k or q, and each result once.  keep (Tq, Tk): pairs that count."""
+    u2 = HALF[q.dtype] ** 2 / 3
+    B, Tq, H, D = q.shape
+    Tk, Hk = k.shape[1:3]
+    n, scale = H // Hk, 1.0 / math.sqrt(D)
+    q, g = q.double().transpose(1, 2), g.double().transpose(1, 2)
+    k, v = (t.double().transpose(1, 2).repeat_interleave(n, 1) for t in (k, v))
+    on = torch.ones((Tq, Tk), dtype=torch.bool, device=q.device).tril(Tk - Tq) if causal else torch.ones((Tq, Tk), dtype=torch.bool, device=q.device)
+    if keep is not None:
+        on = on & keep
+    T = lambda t: t.transpose(2, 3)  # noqa: E731
+    p = torch.softmax(((q @ T(k)) * scale).masked_fill(~on, -1e300), -1) * on
+    o = p @ v
+    ds = p * (g @ T(v) - (g * o).sum(-1, keepdim=True)) * scale
+    fold = lambda t: t.unflatten(1, (Hk, n)).sum(2)  # noqa: E731
+    out = {'y': (o, p ** 2 @ v ** 2), 'dq': (ds @ k, ds ** 2 @ k ** 2), 'dk': (fold(T(ds) @ q), fold(T(ds ** 2) @ q ** 2)),
+           'dv': (fold(T(p) @ g), fold(T(p ** 2) @ g ** 2))}
+    return {x: (a.transpose(1, 2), (u2 * (e + a ** 2)).transpose(1, 2)) for x, (a, e) in out.items()}
+
+
+def norm_ratio(got, want, var):
+    """the error's 2-norm, in twice its expected one: elements err one by one, and a share of the fp32 operations comes on top"""
+    return float((got.double() - want).norm() / (2 * var.sum().sqrt()))
+
+
+def long_inputs(B, Tq, Tk, H, Hk, D, device):
+    r = lambda *s: rand(s[:-1], torch.bfloat16, s[-1], device=device)  # noqa: E731
+    return r(B, Tq, H, D, 1), r(B, Tk, Hk, D, 2), r(B, Tk, Hk, D, 3), r(B, Tq, H, D, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('B,Tq,Tk,H,Hk,D,causal', LONG)
+def test_attention_long_axes_in_the_mean_square(ot, B, Tq, Tk, H, Hk, D, causal):
+    """bf16: worst-case bounds grow with the length and the results shrink with its root, so a lost tile would pass them"""
+    q, k, v, g = long_inputs(B, Tq, Tk, H, Hk, D, 'cuda')
+    want = attention_spread(q, k, v, g, causal)
+    q, k, v = (t.requires_grad_(True) for t in (q, k, v))
+    y = ot.attention(q, k, v, causal=causal)
+    for name, got in zip(('y', 'dq', 'dk', 'dv'), (y.detach(),) + torch.autograd.grad(y, (q, k, v), g)):
+        ratio = norm_ratio(got, *want[name])
+        print(f'{name}: {ratio:.3f} of its bound')
+        assert ratio <= 1.0, (name, ratio)
+
+
+@pytest.mark.parametrize('B,Tq,Tk,H,Hk,D,causal', [c for c in LONG if c[1] * c[2] < 500000])
+def test_the_mean_square_sees_a_lost_tile(B, Tq, Tk, H, Hk, D, causal):
+    """the same bounds on results (float64, CPU) that leave out a tile or the remainder of one"""
+    q, k, v, g = long_inputs(B, Tq, Tk, H, Hk, D, 'cpu')
+    want = attention_spread(q, k, v, g, causal)
+    for axis, T, names in ((1, Tk, ('y', 'dq')), (0, Tq, ('dk', 'dv'))):
+        if T < 64:
+            continue
+        for lost in ((0, 64), (T // 128 * 64, T // 128 * 64 + 64), (T // 32 * 32, T)):
+            if lost[0] >= T or lost[1] > T:
+                continue
+            at = torch.arange(T)
+            keep = (at < lost[0]) | (at >= lost[1])
+            bad = attention_spread(q, k, v, g, causal, (keep[None] if axis else keep[:, None]).expand(Tq, Tk))
+            for name in names:
+                assert norm_ratio(bad[name][0], *want[name]) > 1.0, (name, lost)
+
+
 # ------------------------------------------------------------------------------------------------ forward-mode derivatives
 @pytest.mark.gpu
 @pytest.mark.parametrize('grad', [False, True])
@@ -146,6 +247,66 @@ def test_forward_mode_is_refused(ot, grad):
                     with pytest.raises(NotImplementedError):
                         f(*args, **{k: forward_ad.make_dual(t, torch.ones_like(t))})
             assert torch.equal(want, f(*args, **kw))
+
+
+# ------------------------------------------------------------------------------------------------ in use
+@pytest.mark.gpu
+def test_block_along_its_own_gradient(ot):
+    """the derivative along the gradient is the gradient's norm: against the difference quotient, whose own deviation from the derivative float64 shows"""
+    p = block_parameters(64, 4, 2, torch.float32)
+    x = rand((1, 33, 64), torch.float32, 23).requires_grad_(True)
+    mask = torch.ones((1, 1, 33, 33), dtype=torch.bool, device='cuda').tril()
+    g = rand((1, 33, 64), torch.float32, 24)
+    (gx,) = torch.autograd.grad(block(ot, p, x, mask, 4, 2), x, g)
+    p64, x64 = {k: t.detach().double() for k, t in p.items()}, x.detach().double().requires_grad_(True)
+    (gx64,) = torch.autograd.grad(block64(p64, x64, mask, 4, 2), x64, g.double())
+    d, h = gx64 / gx64.norm(), 0.25
+    with torch.no_grad():
+        quotient = lambda f, at, d: (f(at + h * d) - f(at - h * d)) / (2 * h)  # noqa: E731
+        num = quotient(lambda t: float((block(ot, p, t, mask, 4, 2).double() * g.double()).sum()), x, d.float())
+        num64 = quotient(lambda t: float((block64(p64, t, mask, 4, 2) * g.double()).sum()), x64, d)
+    want = float(gx64.norm())
+    assert abs(num - want) <= abs(num64 - want) + 1e-3 * want, (num, num64, want)
+    assert abs(float((gx.double() * d).sum()) - want) <= 1e-5 * want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('bias', [False, True])
+@pytest.mark.parametrize('patch', [None, (2, 2, 2), (1, 2, 1)])
+def test_hartley_attention_with_softmax_parameter_gradients(patch, bias):
+    """every gradient against autograd's in float64; products of at most 192 terms and a softmax of scores below 32: some 500 E in the worst case"""
+    import functools
+
+    from multimodal_3d_image_segmentation_amd.nets.hartley_mha import HartleyMultiHeadAttention
+    from oracle import hno_oracle as O
+    torch.manual_seed(3)
+    op = HartleyMultiHeadAttention(12, 12, 4, (2, 3, 4), patch, attention_activation=functools.partial(torch.softmax, dim=-1), use_bias=bias, use_transform=False).cuda()
+    if bias:
+        with torch.no_grad():
+            for i, b in enumerate((op.bias_query, op.bias_key, op.bias_value, op.bias_out)):
+                b.copy_(rand(b.shape, torch.float32, 20 + i, 0.3))
+    x = rand((2, 12, 4, 6, 8), torch.float32, 4, 3.0).requires_grad_(True)
+    y = op(x)
+    g = rand(y.shape, torch.float32, 5)
+    grads = torch.autograd.grad(y, [x, *op.parameters()], g)
+    w = {n: t.detach().double().requires_grad_(True) for n, t in op.named_parameters()}
+    x64 = x.detach().double().requires_grad_(True)
+    q, k, v = (torch.einsum('zoi,bidhw->bzodhw', w['weight_' + n], x64) + (w['bias_' + n] if bias else 0.0) for n in ('query', 'key', 'value'))
+    if patch is not None:
+        q, k, v = (O._group3d(t, patch) for t in (q, k, v))
+    shape = q.shape[3:]
+    q, k, v = (t.flatten(3) for t in (q, k, v))
+    att = torch.softmax(torch.einsum('bzcq,bzck->bzqk', q, k) / math.sqrt(k.shape[2]), dim=-1)
+    out = torch.einsum('bzqk,bzck->bzcq', att, v).unflatten(3, shape)
+    if patch is not None:
+        out = O._ungroup3d(out, op.value_dim, patch)
+    want = torch.einsum('oi,bidhw->bodhw', w['weight_out'], out.flatten(1, 2)) + (w['bias_out'] if bias else 0.0)
+    wants = torch.autograd.grad(want, [x64, *w.values()], g.double())
+    for name, a, b in zip(['y', 'x', *w], [y.detach(), *grads], [want.detach(), *wants]):
+        assert a.shape == b.shape
+        err = float((a.double() - b).abs().max() / (b.abs().max() if name != 'bias_key' else grads[1].abs().max()))      # (a softmax does not see a shift: its gradient is 0)
+        print(f'{name}: {err / E:.1f} E')
+        assert err < 500 * E, (name, err)
 
 
 # ------------------------------------------------------------------------------------------------ refusals (no GPU)
