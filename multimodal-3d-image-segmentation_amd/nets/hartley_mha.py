@@ -86,8 +86,8 @@ class HartleyMultiHeadAttention(Module):
             self.patch_size = (self.patch_size,) * (ndim - 2)
         if isinstance(self.attention_activation, str):
             self.attention_activation = getattr(torch.nn.functional, self.attention_activation)
-        grouped = max(key_dim, self.value_dim) * int(np.prod(self.patch_size or 1))
-        if softmax_over_keys(self.attention_activation) and grouped > ops_tokens.MAX_HEAD:
+        grouped = max(key_dim, self.value_dim) * (1 if self.patch_size is None else int(np.prod(self.patch_size)))
+        if grouped > ops_tokens.MAX_HEAD and softmax_over_keys(self.attention_activation):
             raise ValueError(f'a softmax over the keys is provided for up to {ops_tokens.MAX_HEAD} grouped channels a head (channels x patch size), '
                              f'not for {grouped} grouped channels')
         self.weight_query = Parameter(torch.empty((num_heads, key_dim, self.in_channels), **fk))

@@ -337,5 +337,7 @@ def test_hartley_softmax_beyond_the_largest_head_is_refused_at_construction():
     assert make(torch.nn.Softmax(-1), 16)(x).shape == (1, 3, 32, 32, 32)           # 128: the largest
     op = lambda **kw: HartleyMultiHeadAttention(8, 8, 2, (2, 2, 2), (2, 2, 2), torch.nn.Softmax(-1), device='meta', **kw)  # noqa: E731
     op(value_dim=16)
+    import numpy as np
+    HartleyMultiHeadAttention(8, 32, 2, (2, 2, 2), np.array((2, 2, 2)), 'selu', device='meta')      # (a patch in any form)
     with pytest.raises(ValueError, match='136 grouped channels'):
         op(value_dim=17)
