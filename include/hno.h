@@ -614,6 +614,7 @@ int hno_affine_nearest(const float *x, float *out, const double *matrix12, float
  *   query is aligned with the last key), and mask[b, h, i, j] != 0 (NULL: all; strides of 0 broadcast).
  *   Rows of k and v from L on, and those that a mask without query and head axis hides, are not looked at: they may hold anything.  Other rows have to
  *   be finite, also where a mask hides them.  fp32 products are formed from three bf16 terms per value (errors as in fp32; an infinity becomes NaN).
+ *   The relative error of a weight is about 2^-24 of the row's largest score; scores from 2^20 on are not provided.
  *   For the backward pass: lse (B, Tq, H) fp32, +inf for an empty row, and out_res (bf16 only), the rounding error of out; both NULL otherwise.
  * hno_attn_bwd: dq, dk, dv (contiguous; dq or both of dk, dv may be NULL) from out, out_res, lse and dout (contiguous). */
 typedef struct hno_attn {

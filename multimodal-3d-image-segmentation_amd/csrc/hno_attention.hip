@@ -252,7 +252,8 @@ __device__ __forceinline__ void at_product2(tk16 &x, tk16 &y, const AtAddr<DP> &
                                    });
 }
 // acc[dt] += (32 tile rows)^T . w, w being a result over the same rows.  make(e) brings element e of w about: the second half's between the products of the
-// first.
+// first.  bf16: w (a probability or a score gradient) is rounded to the matrix instruction's operand type, the one rounding on the way to the fp32 sum; a
+// second bf16 term of it would cost a second product for less than the rounding of the result.
 template <typename T, int DP, int PLANE, typename M>
 __device__ __forceinline__ void at_accumulate(tk16 (&acc)[DP / 32], const AtAddr<DP> &at, int off, tk16 &w, M make) {
     constexpr int ND = DP / 32;
@@ -363,8 +364,8 @@ __device__ __forceinline__ int at_wave_min(int x) {
     for (int k = 16; k; k >>= 1) x = min(x, __shfl_xor(x, k));
     return __builtin_amdgcn_readfirstlane(x);
 }
-// the weights of 8 keys as an operand, and their sum as the product takes them: the weights of a row then add up to one whatever they
-// were rounded to
+// the weights of 8 keys as an operand (bf16: rounded once, as the matrix instruction takes them), and their sum as the product takes them: the weights of a row then
+// add up to one whatever they were rounded to.  With the rounding of the result the error is sqrt(2) of a rounding in the mean square (0.0024, 0.0017 for one).
 __device__ __forceinline__ void at_weights(TkFrag<tkh> &f, const tk16 &s, int t, float &l) {
     typedef __bf16 b2 __attribute__((ext_vector_type(2)));
     const b2 one = {(__bf16)1.f, (__bf16)1.f};

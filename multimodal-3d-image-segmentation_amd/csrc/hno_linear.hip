@@ -198,8 +198,9 @@ __device__ __forceinline__ void ln_finish(const LinArgs &a, int m, int n, float 
 }
 
 // DMA: two LDS buffers, the next step's tiles on their way while this one is multiplied.  Else the next step's tiles wait in registers: one buffer.
-// Bound by the matrix pipes: 8192 x 8192 x 2048 bf16 238 us = 1155 TFLOP/s (the library's product 222), with residual 257, with gelu 257, with bias, gelu and residual
-// 285 (LnMid: 330) -- the epilogue of a tile waits for its products, one workgroup a CU.  fp32 (six bf16 products each): 2000 x 512 x 512 27 us.
+// Bound by the matrix pipes: 8192 x 8192 x 2048 bf16, calls back to back, 250 us = 1100 TFLOP/s (the library's product 230), with residual 267, with gelu 272, with bias,
+// gelu and residual 300 (LnMid: 330) -- the epilogue of a tile waits for its products, one workgroup a CU.  The first dozen calls of a process take 273, 326 and
+// 349 (bare, gelu, everything).  fp32 (six bf16 products each): 2000 x 512 x 512 27 us.
 template <typename T, bool AX, bool BX, typename C, bool DMA, int ACT>
 __global__ __launch_bounds__(64 * ln_waves<C>(), 2) void linear_kernel(LinArgs a) {
     constexpr int TM = C::TM, TN = C::TN, KB = C::KB, P = tk_planes<T>(), WM = C::WM, WN = C::WN, NT = 64 * ln_waves<C>(), NB = DMA ? 2 : 1;
@@ -389,7 +390,8 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinArgs a) {
 }
 
 // Up to four rows: bound by reading the weight once, so no tiles.  A workgroup owns two columns, its lanes walk the contraction 8 elements at a time, every
-// product and sum in fp32; the lanes' sums meet in shuffles, the waves' in LDS; one launch.  bf16 4 x 2048 x 2048: 5.0 us (tiles in 32 runs 10.3), 4 x 16384 x 8192: 60 us =
+// product and sum in fp32; the lanes' sums meet in shuffles, the waves' in LDS; one launch.  4 x 2048 x 2048: bf16 5.7 us (tiles in 32 runs 10.3), fp32 8.3; bf16 4 x 8192 x 16384:
+// 45 us = 6.0 TB/s, the weight partly from the last-level cache; 4 x 16384 x 8192 60 us =
 // 4.5 TB/s (72), one row 43 us = 6.2 TB/s (72, the weight partly from the last-level cache).  Eight rows are quicker in tiles (8 x 8192 x 2048: 12.0 us, 30.8 here: every
 // workgroup reads all of x).
 constexpr int LN_ROWS = 4, LN_COLS = 2;
@@ -446,8 +448,10 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(LinArgs a) {
     ((T *)a.y)[at] = tk_down<T>(y);
 }
 
-// dz = dy act'(z) and the column sums of dz: a workgroup owns 256 columns (32 lanes of 8) of a run of rows and leaves one slab row per run; single columns a lane
-// took 16 us for 3920 x 1536 bf16 instead of 11.  dz == nullptr: act is none, dz is dy itself and only the sums are wanted.
+// dz = dy act'(z) and the column sums of dz.  dz is rounded to the operator's type, being an operand of two products (db adds it up before that); z was kept in that
+// type too: half the memory, for an error of the slope below dz's own rounding where |z| is of order one.
+// A workgroup owns 256 columns (32 lanes of 8) of a run of rows and leaves one slab row per run; single columns a lane took 16 us for 3920 x 1536 bf16 instead of 11.
+// dz == nullptr: act is none, dz is dy itself and only the sums are wanted.
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void linear_dz_kernel(const T *__restrict__ dy, const T *__restrict__ z, T *__restrict__ dz, float *__restrict__ slab,
                                                         int M, int N, int rows_per) {

@@ -2,8 +2,9 @@
 product with bias, activation and residual in its epilogue, and group norm with an activation -- on channels-last tokens, in fp32 or bf16, with
 their backward passes.
 
-Tensors are torch containers; nothing computes through ATen and there is no CPU path (meta tensors get shape inference only).  Parameters may
-stay fp32 next to bf16 activations: the matrix product then rounds its weight to bf16, as the bf16 convolutions do, and returns an fp32 gradient.
+Tensors are torch containers; no product, sum, norm or activation goes through ATen, and there is no CPU path (meta tensors get shape inference only).
+What ATen does beside allocations: copies of operands whose layout the kernels do not take, and conversions of lengths and norm parameters of another type.
+Parameters may stay fp32 next to bf16 activations: the matrix product then rounds its weight to bf16, as the bf16 convolutions do, and returns an fp32 gradient.
 Gradients of gradients and forward-mode derivatives are refused.
 """
 import ctypes
@@ -178,6 +179,7 @@ def attention(q, k, v, *, causal=False, mask=None, kv_lens=None, scale=None):
     Keys and values from L on, and those that a mask of shape (B, 1, 1, Tk) hides, may hold anything (inf, NaN); all others have to be finite, also
     where a mask hides them.  Additive (floating) masks are refused.  fp32 products are formed from three bf16 terms per value, so an
     infinity comes out as NaN.
+    The relative error of a weight is about 2^-24 of the row's largest |scale q k| (in bf16 beside its rounding), in both passes; scores from 2^20 on are not provided.
     Differentiable in q, k, v; the probabilities are recomputed in the backward pass, memory grows with Tq + Tk only."""
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError('attention: q, k, v must be (batch, tokens, heads, channels)')
@@ -370,7 +372,7 @@ class GroupNormClFn(torch.autograd.Function):
 def group_norm(x, num_groups, weight=None, bias=None, *, eps=1e-5, act=None):
     """act(gamma (x - mean) / sqrt(var + eps) + beta) on channels-last x (B, ..., C), fp32 or bf16, statistics per sample and group of
     C / num_groups neighbouring channels over all positions; weight, bias (C,) fp32 or x's type; at most 65535 samples.  ``act``: see ``act_id``.
-    Statistics are sums of differences from a value of the group, in fp32 and, over more than a few thousand values, joined in 64 bits.  Differentiable in x,
+    Statistics: means and squared distances from them, in fp32 and, over more than a few thousand values, joined in 64 bits.  Differentiable in x,
     weight, bias; the backward pass keeps x and the statistics."""
     a = act_id(act)
     num_groups, eps = int(num_groups), float(eps)

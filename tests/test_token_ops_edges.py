@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_token_ops import ACT64, DTYPES, E, HALF, block, block64, block_parameters, close, ot, rand, slope64  # noqa: F401
+from test_token_ops import ACT64, DTYPES, E, HALF, block, block64, block_parameters, check_attention, close, ot, rand, slope64  # noqa: F401
 
 
 # ------------------------------------------------------------------------------------------------ group norm
@@ -122,6 +122,15 @@ def test_attention_gradients_without_keys(ot, need, dtype):
     assert y.shape == (2, 5, 4, 24) and (y == 0).all()
     for x, g in zip(leaves, torch.autograd.grad(y, leaves, torch.ones_like(y))):
         assert g.shape == x.shape and (g == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('size', [30.0, 300.0])
+def test_attention_large_scores(ot, size, dtype):
+    """scores of 10^4 and 10^5: weights of 0 and 1 mostly, each operation on an exponent off by 2^-24 of it"""
+    q, k, v = rand((1, 66, 2, 64), dtype, 17, size), rand((1, 1300, 2, 64), dtype, 18, 40.0), rand((1, 1300, 2, 64), dtype, 19)
+    check_attention(ot, q, k, v, scale=1.0)
 
 
 # B, Tq, Tk, H, Hk, D, causal: long axes, cut into runs; remainders of a tile on either side
